@@ -8,7 +8,9 @@ Layout:
 * ``decls``     declarations of softmax, rmsnorm, layernorm, swiglu, rope, causal_attention,
                 fused_add_rms_norm, causal_attention_gqa, llama3_attention (RoPE on q, k
                 then grouped causal attention), cross_entropy, fused_linear_cross_entropy,
-                llama3_decoder_layer (one whole Llama-3 decoder layer)
+                llama3_decoder_layer (one whole Llama-3 decoder layer), and the operators of
+                packed batches: packed_attention, rotary (a position per token), block_norm
+                (the norms around a block with its gate and residual scale)
 * ``pairs``     one module per operator with the reference's
                 ``<op>_forward_with_saved`` / ``<op>_backward_from_saved`` functions
 * ``bind``      ``bind(op, module)`` -> a ``torch.autograd.Function``-backed callable
@@ -30,6 +32,9 @@ PAIR_MODULES = {
     "cross_entropy": "evograd_amd.pairs.cross_entropy",
     "fused_linear_cross_entropy": "evograd_amd.pairs.fused_linear_cross_entropy",
     "llama3_decoder_layer": "evograd_amd.pairs.llama3_decoder_layer",
+    "packed_attention": "evograd_amd.pairs.packed_attention",
+    "rotary": "evograd_amd.pairs.rotary",
+    "block_norm": "evograd_amd.pairs.block_norm",
 }
 
 # Small-shape programs and the shape dispatchers that route to them below the

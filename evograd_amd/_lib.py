@@ -20,7 +20,7 @@ import torch  # noqa: F401  (loads the HIP runtime first; see module docstring)
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libevograd_hip.so")
 
 EG_F32, EG_F16, EG_BF16 = 0, 1, 2
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 _DTYPE_TAG = {
     torch.float32: EG_F32,
@@ -84,6 +84,18 @@ SIGNATURES: dict[str, tuple] = {
     "eg_rmsnorm_bwd_small": (_i32, [_p, _p, _p, _p, _p, _p, _i64, _i64, _i32, _p]),
     "eg_layernorm_bwd_small": (_i32, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i32, _p]),
     "eg_silu_mul": (_i32, [_p, _p, _p, _i64, _i32, _p]),
+    "eg_packed_attn_fwd": (_i32, [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _f32,
+                                  _i32, _p]),
+    "eg_packed_attn_workspace_bytes": (_size, [_i64, _i64, _i64, _i64, _i64, _i32]),
+    "eg_packed_attn_bwd": (_i32, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64,
+                                  _i64, _i64, _p, _f32, _i32, _p]),
+    "eg_rotary": (_i32, [_p, _p, _p, _p, _p, _i32, _p, _i64, _i64, _i64, _i64, _i64, _p, _f32,
+                         _i32, _i32, _i32, _p]),
+    "eg_block_norm_fwd": (_i32, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i32, _f32, _f32,
+                                 _i32, _p]),
+    "eg_block_norm_workspace_bytes": (_size, [_i64, _i64]),
+    "eg_block_norm_bwd": (_i32, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64,
+                                 _i64, _i32, _f32, _i32, _p]),
     "eg_probe_mfma_bf16": (_i32, [_p, _p, _i32, _i32, _p]),
     "eg_probe_mfma_mix": (_i32, [_i32, _p, _p, _i32, _i32, _p]),
     "eg_gemm_segmented": (_i32, [_p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32,
@@ -141,6 +153,16 @@ def call(name: str, *args) -> None:
     if rc != 0:
         msg = load().eg_last_error()
         raise RuntimeError(f"{name} failed (rc={rc}): {msg.decode() if msg else ''}")
+
+
+def call_on(t: torch.Tensor, name: str, *args) -> None:
+    """``call`` with t's GPU as the current one, as a launch on its stream needs."""
+    index = t.get_device()
+    if index == torch._C._cuda_getDevice():
+        call(name, *args)
+    else:
+        with torch.cuda.device(index):
+            call(name, *args)
 
 
 def query(name: str, *args):

@@ -19,6 +19,9 @@ drop-in the reference's harness looks up:
   declared here the way an external ``--declaration path.py:op`` would be
   (src/evograd/opdecl/verify_cli.py:35-38).
 
+* packed_attention, rotary and block_norm, the operators of packed batches, have no
+  counterpart in the reference; they are declared the same way.
+
 Differences from the reference declarations, all deliberate:
 
 * Tolerances are the stricter gate of this build: fp32 (1e-5, 1e-5),
@@ -665,11 +668,158 @@ LLAMA3_DECODER_LAYER = declare_op(
     regime_split=LLAMA_REGIME_SPLIT,
 )
 
+# ------------------------------------------------------- operators of packed batches
+# Prompts of different lengths along one token axis: the attention of each by itself, rotary
+# positions per token, and the norms around a block. The oracle runs them in fp64, which the
+# angles of far positions need.
+def _packed(lengths, H, KVH, D, dtype, pad=0, label=""):
+    return Workload(dims=dict(T=sum(lengths) + pad, H=H, KVH=KVH, D=D, N1=len(lengths) + 1),
+                    dtype=dtype, label=label, extra={"lengths": tuple(lengths)})
+
+
+PACKED_ATTENTION = declare_op(
+    name="packed_attention",
+    forward="oracle.forward_refs:packed_attention_forward_ref",
+    dims=("T", "H", "KVH", "D", "N1"),
+    args=(
+        Active("q", "[T, H, D]"),
+        Active("k", "[T, KVH, D]"),
+        Active("v", "[T, KVH, D]"),
+        Inactive("cu_seqlens", "[N1]", dtype="int32",
+                 note="first row of each sequence, then the last sequence's end"),
+    ),
+    output=Active("o", "[T, H, D]"),
+    forward_semantics=(
+        "Every row attends to the rows of its own sequence up to itself, k and v shared by "
+        "groups of H/KVH query heads: o = softmax(q k^T / sqrt(D)) v; rows of no sequence "
+        "give zeros."
+    ),
+    backward_semantics=(
+        "Return dq, dk, dv; dk and dv summed over each query group; zero in rows of no "
+        "sequence; P is recomputed from the saved logsumexp."
+    ),
+    reference_dtype="float64",
+    correctness=tuple(
+        _packed(lengths, H, KVH, D, dt, pad)
+        for lengths, H, KVH, D, pad in (
+            ((1,), 2, 1, 64, 0),
+            ((17, 64, 1, 0, 46), 4, 2, 128, 0),
+            ((200, 129, 3), 8, 2, 64, 21),
+        )
+        for dt in ("bfloat16", "float16")
+    ) + (
+        _packed((33, 11, 33), 4, 1, 32, "float32"),
+        _packed((100, 0, 1, 70), 4, 2, 64, "float32", 5),
+        _packed((40, 30), 2, 2, 80, "bfloat16"),
+    ),
+    benchmark=(
+        _packed((4096, 1500, 900, 700, 411, 300, 180, 105), 32, 8, 128, "bfloat16",
+                label="llama3_8b_packed"),
+    ),
+    tolerances=TOLERANCES,
+    make_inputs="evograd_amd.inputs:make_packed_attention_inputs",
+    memory_inputs=("q", "k", "v"),
+    regime_feature=_tokens_feature,
+    regime_split=LLAMA_REGIME_SPLIT,
+)
+
+
+def _rotary(T, n_heads, head_dim, pairs, dtype, label="", **extra):
+    return Workload(dims=dict(T=T, n_heads=n_heads, head_dim=head_dim, pairs=pairs), dtype=dtype,
+                    label=label, extra=extra)
+
+
+ROTARY = declare_op(
+    name="rotary",
+    forward="oracle.forward_refs:rotary_forward_ref",
+    dims=("T", "n_heads", "head_dim", "pairs"),
+    args=(
+        Active("x", "[T, n_heads, head_dim]"),
+        Inactive("positions", "[T]", dtype="int32", note="each token's own position"),
+        Inactive("freqs", "[pairs]", dtype="float64", note="radians per position"),
+        Inactive("amplitude", default=1.0),
+        Inactive("interleaved", default=0, note="pairs (2i, 2i + 1), not (i, i + pairs)"),
+    ),
+    output=Active("y", "[T, n_heads, head_dim]"),
+    forward_semantics=(
+        "The first 2 * pairs columns of each head rotated by position * freqs (angles in "
+        "fp64) and scaled by amplitude, in fp32, cast back to x's dtype; the others copied."
+    ),
+    backward_semantics="The transpose: the rotation by the negative angles.",
+    reference_dtype="float64",
+    correctness=tuple(
+        _rotary(T, H, D, n, dt, interleaved=inter, amplitude=amp, far=far)
+        for T, H, D, n, inter, amp, far in (
+            (1, 4, 128, 64, 0, 1.0, 1 << 20),
+            (37, 6, 64, 16, 1, 1.0, 4096),
+            (129, 3, 80, 20, 0, 1.25, 131072),
+            (16, 5, 10, 3, 1, 0.5, 100),
+        )
+        for dt in ("float32", "float16", "bfloat16")
+    ),
+    benchmark=(
+        _rotary(8192, 32, 128, 64, "bfloat16", label="llama3_8b_packed", far=8192),
+    ),
+    tolerances=TOLERANCES,
+    make_inputs="evograd_amd.inputs:make_rotary_inputs",
+    memory_inputs=("x",),
+    regime_feature=_tokens_feature,
+    regime_split=LLAMA_REGIME_SPLIT,
+)
+
+
+def _block(rows, cols, gate, dtype, label="", scale=1.0):
+    return Workload(dims=dict(rows=rows, cols=cols), dtype=dtype, label=label,
+                    extra={"gate": gate, "scale": scale})
+
+
+BLOCK_NORM = declare_op(
+    name="block_norm",
+    forward="oracle.forward_refs:block_norm_forward_ref",
+    dims=("rows", "cols"),
+    args=(
+        Active("x", "[rows, cols]", note="the residual stream"),
+        Active("h", "[rows, cols]", note="the block's output"),
+        Active("post_weight", "[cols]"),
+        Active("gate", note="[cols], [rows, 1] or [rows, cols]"),
+        Active("pre_weight", "[cols]"),
+        Inactive("scale", default=1.0, note="residual scale"),
+        Inactive("eps", default=1e-6),
+    ),
+    output=Active("out", "[2, rows, cols]"),
+    forward_semantics=(
+        "out[0] = s = x + scale * gate * rmsnorm(h) * post_weight and out[1] = rmsnorm(s) * "
+        "pre_weight, in fp32 from the unrounded s, cast to x's dtype."
+    ),
+    backward_semantics=(
+        "Return dx, dh, dpost_weight, dgate (summed over the axes the gate was broadcast "
+        "along) and dpre_weight; fp32 accumulation."
+    ),
+    reference_dtype="float64",
+    correctness=(
+        _block(8, 64, "channel", "float32"),
+        _block(17, 127, "row", "float32"),
+        _block(17, 1000, "element", "bfloat16", scale=0.5),
+        _block(5, 6, "channel", "bfloat16"),
+        _block(64, 512, "row", "float16"),
+        _block(600, 4096, "channel", "bfloat16", scale=0.7071),
+        _block(33, 8192, "element", "bfloat16"),
+        _block(3, 20001, "channel", "float16"),
+    ),
+    benchmark=(
+        _block(16384, 4096, "channel", "bfloat16", label="llama3_8b"),
+    ),
+    tolerances=TOLERANCES,
+    make_inputs="evograd_amd.inputs:make_block_norm_inputs",
+    regime_feature=_rows_feature,
+    regime_split=LLAMA_REGIME_SPLIT,
+)
+
 OPS: dict[str, OpDecl] = {
     op.name: op
     for op in (SOFTMAX, RMSNORM, LAYERNORM, SWIGLU, ROPE, CAUSAL_ATTENTION, FUSED_ADD_RMS_NORM,
                CAUSAL_ATTENTION_GQA, LLAMA3_ATTENTION, CROSS_ENTROPY, FUSED_LINEAR_CROSS_ENTROPY,
-               LLAMA3_DECODER_LAYER)
+               LLAMA3_DECODER_LAYER, PACKED_ATTENTION, ROTARY, BLOCK_NORM)
 }
 
 

@@ -257,6 +257,65 @@ def make_llama3_decoder_layer_inputs(op, workload, device="cuda"):
     return out
 
 
+def make_packed_attention_inputs(op, workload, device="cuda"):
+    """Generic seed; q, do [T, H, D] and k, v [T, KVH, D] ~ N(0,1) drawn in the order q, k, v,
+    do; cu_seqlens int32 of ``extra["lengths"]`` (rows past their sum belong to none)."""
+    d = workload.dims
+    lengths = workload.extra["lengths"]
+    if len(lengths) + 1 != d["N1"] or sum(lengths) > d["T"]:
+        raise ValueError(f"lengths {lengths} do not fit N1={d['N1']}, T={d['T']}")
+    qs, ks = (d["T"], d["H"], d["D"]), (d["T"], d["KVH"], d["D"])
+    dt = resolve_dtype(workload.dtype)
+    torch.manual_seed(case_seed(workload))
+    q = torch.randn(qs, device=device, dtype=dt)
+    k = torch.randn(ks, device=device, dtype=dt)
+    v = torch.randn(ks, device=device, dtype=dt)
+    do = torch.randn(qs, device=device, dtype=dt)
+    cu = torch.zeros(len(lengths) + 1, dtype=torch.int64)
+    cu[1:] = torch.tensor(lengths, dtype=torch.int64).cumsum(0)
+    return {"q": q, "k": k, "v": v, "cu_seqlens": cu.to(device=device, dtype=torch.int32),
+            "do": do}
+
+
+def make_rotary_inputs(op, workload, device="cuda"):
+    """Generic seed; x = 0.5 N(0,1), positions uniform below ``extra["far"]`` (default 4096),
+    dy = 0.5 N(0,1), drawn in that order; freqs at Llama-3's theta; ``extra`` may set
+    interleaved and amplitude."""
+    d = workload.dims
+    dt = resolve_dtype(workload.dtype)
+    shape = (d["T"], d["n_heads"], d["head_dim"])
+    torch.manual_seed(case_seed(workload))
+    x = torch.randn(shape, device=device, dtype=dt) * 0.5
+    positions = torch.randint(0, int(workload.extra.get("far", 4096)), (d["T"],), device=device)
+    dy = torch.randn(shape, device=device, dtype=dt) * 0.5
+    i = torch.arange(d["pairs"], dtype=torch.float64, device=device)
+    freqs = LLAMA3_ROPE_THETA ** (-i / max(1, d["pairs"]))
+    return {"x": x, "positions": positions.to(torch.int32), "freqs": freqs,
+            "amplitude": float(workload.extra.get("amplitude", 1.0)),
+            "interleaved": int(workload.extra.get("interleaved", 0)), "dy": dy}
+
+
+def make_block_norm_inputs(op, workload, device="cuda"):
+    """Generic seed; x, h ~ N(0,1); both weights 1 + 0.1 N(0,1) and the gate 0.5 + 0.2 N(0,1)
+    drawn in fp32 then cast; dout ~ N(0,1); drawn in the order x, h, post_weight, gate,
+    pre_weight, dout. ``extra["gate"]``: "channel" (default), "row" or "element"."""
+    rows, cols = workload.dims["rows"], workload.dims["cols"]
+    dt = resolve_dtype(workload.dtype)
+    torch.manual_seed(case_seed(workload))
+
+    def around(mean, spread, *shape):
+        return (mean + spread * torch.randn(shape, device=device, dtype=torch.float32)).to(dt)
+
+    x, h = around(0.0, 1.0, rows, cols), around(0.0, 1.0, rows, cols)
+    shape = {"channel": (cols,), "row": (rows, 1), "element": (rows, cols)}
+    post = around(1.0, 0.1, cols)
+    gate = around(0.5, 0.2, *shape[workload.extra.get("gate", "channel")])
+    pre = around(1.0, 0.1, cols)
+    return {"x": x, "h": h, "post_weight": post, "gate": gate, "pre_weight": pre,
+            "scale": float(workload.extra.get("scale", 1.0)), "eps": 1e-6,
+            "dout": around(0.0, 1.0, 2, rows, cols)}
+
+
 RECIPES = {
     "make_softmax_inputs": make_softmax_inputs,
     "make_rmsnorm_inputs": make_rmsnorm_inputs,
@@ -270,6 +329,9 @@ RECIPES = {
     "make_cross_entropy_inputs": make_cross_entropy_inputs,
     "make_flce_inputs": make_flce_inputs,
     "make_llama3_decoder_layer_inputs": make_llama3_decoder_layer_inputs,
+    "make_packed_attention_inputs": make_packed_attention_inputs,
+    "make_rotary_inputs": make_rotary_inputs,
+    "make_block_norm_inputs": make_block_norm_inputs,
 }
 
 

@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from evograd_amd import _lib
@@ -23,3 +25,26 @@ def workspace(nbytes: int, device) -> torch.Tensor:
 
 
 tag = _lib.dtype_tag
+
+
+# The widest step between tokens or heads that the strided kernels address with 32-bit offsets.
+MAX_STRIDE = 1 << 24
+
+
+def head_rows(t: torch.Tensor) -> torch.Tensor:
+    """A [tokens, heads, head_dim] tensor as the strided kernels take it: itself when a head's
+    columns are contiguous and its steps are in range, else a contiguous copy."""
+    if t.stride(2) == 1 and all(n == 1 or s <= MAX_STRIDE for n, s in zip(t.shape[:2], t.stride())):
+        return t
+    return t.contiguous()
+
+
+def strides_arg(*tensors: torch.Tensor):
+    """Token and head strides of [tokens, heads, head_dim] tensors as a C array; an axis of one
+    element has the step of a contiguous tensor, whatever torch notes for it."""
+    steps = []
+    for t in tensors:
+        tokens, heads, dim = t.shape
+        steps.append(t.stride(0) if tokens > 1 else heads * dim)
+        steps.append(t.stride(1) if heads > 1 else dim)
+    return (ctypes.c_int64 * len(steps))(*steps)

@@ -452,6 +452,71 @@ int eg_add(const void* a, const void* b, void* c, int64_t n, int dtype, void* st
  * rounds silu first). Its backward is eg_swiglu_bwd's formula. */
 int eg_silu_mul(const void* gate, const void* up, void* out, int64_t n, int dtype, void* stream);
 
+/* ------------------------------------------------ operators of packed batches
+ * Sequences of different lengths, one behind the other along the token axis. */
+
+/* Causal grouped-query attention over packed sequences. q [tokens, heads, head_dim],
+ * k, v [tokens, kv_heads, head_dim]; sequence s holds the rows cu_seqlens[s] ..
+ * cu_seqlens[s + 1] - 1 (device int32 [seqs + 1], from 0, not decreasing, at most
+ * tokens; empty sequences allowed), and each row attends to its own sequence's rows
+ * up to itself:
+ *   o_i = sum_j p_ij v_j,  p_ij = exp(scale q_i . k_j - lse_i)
+ * `strides` (host, read during the call): token and head steps of q, of k and of v,
+ * in elements, at most 2^24; a head's columns are contiguous. o [tokens, heads,
+ * head_dim], lse fp32 [heads, tokens]. Rows that no sequence holds get o = 0 and are
+ * read into no result. The bounds are read on the device alone; ones that break the
+ * rules give undefined values but no access outside the tensors. fp32, bf16, fp16;
+ * even head_dim up to 128. Sizes: tokens <= 2^28, (tokens / 16 + seqs) * heads < 2^28. */
+int eg_packed_attn_fwd(const void* q, const void* k, const void* v, const int* cu_seqlens,
+                       void* o, float* lse, int64_t tokens, int64_t seqs, int64_t heads,
+                       int64_t kv_heads, int64_t head_dim, const int64_t* strides, float scale,
+                       int dtype, void* stream);
+
+/* Bytes of workspace eg_packed_attn_bwd needs: delta = rowsum(do * o), fp32 [heads,
+ * tokens] rounded up to 256 bytes, and, where the key blocks alone leave the GPU partly
+ * idle, the fp32 sums of the dK/dV walk's pieces. */
+size_t eg_packed_attn_workspace_bytes(int64_t tokens, int64_t seqs, int64_t heads,
+                                      int64_t kv_heads, int64_t head_dim, int dtype);
+
+/* Its backward: dout, dq [tokens, heads, head_dim]; dk, dv [tokens, kv_heads, head_dim],
+ * summed over each query group, all contiguous; zero in rows that no sequence holds. */
+int eg_packed_attn_bwd(const void* dout, const void* q, const void* k, const void* v,
+                       const int* cu_seqlens, const void* o, const float* lse, void* dq,
+                       void* dk, void* dv, void* workspace, int64_t tokens, int64_t seqs,
+                       int64_t heads, int64_t kv_heads, int64_t head_dim,
+                       const int64_t* strides, float scale, int dtype, void* stream);
+
+/* Rotary positions by a position per token: q [tokens, heads_q, head_dim] and k [tokens,
+ * heads_k, head_dim] (heads_k = 0: q alone) in one launch. With angle = position *
+ * freqs[i] (fp64, radians per position), pair i is (x[i], x[i + pairs]) or, interleaved,
+ * (x[2i], x[2i + 1]) and becomes amplitude * (x1 cos - x2 sin, x2 cos + x1 sin); columns
+ * from 2 * pairs on are copied. inverse: the transpose (the backward). positions: int32, or
+ * int64 with positions_64. `strides` (host): token and head steps of q and of k, in
+ * elements; a head's columns are contiguous; outputs are contiguous. */
+int eg_rotary(const void* q, const void* k, void* q_out, void* k_out, const void* positions,
+              int positions_64, const double* freqs, int64_t tokens, int64_t heads_q,
+              int64_t heads_k, int64_t head_dim, int64_t pairs, const int64_t* strides,
+              float amplitude, int interleaved, int inverse, int dtype, void* stream);
+
+/* The norms around a block with its gate, residual scale and residual, rows x cols:
+ *   s = x + alpha * gate * (h * rstd_h * post_weight),  y = s * rstd_s * pre_weight
+ * in fp32, y from the unrounded s; rstd fp32 [2, rows] (of h, of s; saved). gate_kind 0: no
+ * gate, 1: gate [cols], 2: [rows], 3: [rows, cols]. */
+int eg_block_norm_fwd(const void* x, const void* h, const void* post_weight, const void* gate,
+                      const void* pre_weight, void* s, void* y, float* rstd, int64_t rows,
+                      int64_t cols, int gate_kind, float alpha, float eps, int dtype,
+                      void* stream);
+
+/* Bytes of fp32 partial column sums that eg_block_norm_bwd keeps in its workspace. */
+size_t eg_block_norm_workspace_bytes(int64_t rows, int64_t cols);
+
+/* Its backward: dx, dh [rows, cols]; dpost_weight, dpre_weight [cols]; dgate like gate. */
+int eg_block_norm_bwd(const void* ds, const void* dy, const void* x, const void* h,
+                      const void* post_weight, const void* gate, const void* pre_weight,
+                      const float* rstd, void* dx, void* dh, void* dpost_weight, void* dgate,
+                      void* dpre_weight, void* workspace, int64_t rows, int64_t cols,
+                      int gate_kind, float alpha, int dtype, void* stream);
+
 /* ---- measurement aid (no counterpart in the reference) ---------------------
  * Sustained bf16 MFMA rate, for reading the roofline fractions of the MFMA-bound
  * kernels (bench.py reports it beside the published peak): `workgroups` 256-thread

@@ -243,6 +243,53 @@ def llama3_decoder_layer_runtime_ref(*args, **kwargs):
     return _llama3_decoder_layer(_layer_rms_norm_fused, *args, **kwargs)
 
 
+# ------------------------------------------------------- operators of packed batches
+def packed_attention_forward_ref(q, k, v, cu_seqlens):
+    """Causal softmax attention of each sequence's rows by itself, k and v repeated over each
+    query group (the attention of llama3_decoder_layer/forward_ref.py:101-107 one sequence at
+    a time); rows of no sequence are zero."""
+    group = q.shape[1] // k.shape[1]
+    bounds = cu_seqlens.tolist()
+    out = torch.zeros_like(q)
+    for a, b in zip(bounds[:-1], bounds[1:]):
+        if a == b:
+            continue
+        qs = q[a:b].transpose(0, 1)
+        ks = k[a:b].transpose(0, 1).repeat_interleave(group, dim=0)
+        vs = v[a:b].transpose(0, 1).repeat_interleave(group, dim=0)
+        scores = qs @ ks.transpose(1, 2).contiguous() / q.shape[2] ** 0.5
+        hidden = torch.ones(b - a, b - a, dtype=torch.bool, device=q.device).triu(1)
+        o = torch.softmax(scores.masked_fill(hidden, float("-inf")), dim=-1) @ vs
+        out = torch.cat((out[:a], o.transpose(0, 1), out[b:]))
+    return out
+
+
+def rotary_forward_ref(x, positions, freqs, amplitude: float = 1.0, interleaved: int = 0):
+    """The rotation of rope_forward_ref by angles formed in fp64 from a position per token,
+    over the first 2 * len(freqs) columns."""
+    angle = positions.double()[:, None, None] * freqs.double()
+    cos = (amplitude * angle.cos()).to(x.dtype)
+    sin = (amplitude * angle.sin()).to(x.dtype)
+    n = freqs.shape[0]
+    part, rest = x[..., :2 * n], x[..., 2 * n:]
+    x1, x2 = (part[..., 0::2], part[..., 1::2]) if interleaved else (part[..., :n], part[..., n:])
+    y1, y2 = x1 * cos - x2 * sin, x2 * cos + x1 * sin
+    part = torch.stack((y1, y2), dim=-1).flatten(-2) if interleaved else torch.cat((y1, y2), dim=-1)
+    return torch.cat((part, rest), dim=-1)
+
+
+def block_norm_forward_ref(x, h, post_weight, gate, pre_weight, scale: float = 1.0,
+                           eps: float = 1e-6):
+    """rmsnorm_forward_ref's norm of h, the gate and residual scale, the residual, and the same
+    norm of the sum: [2, rows, cols], the sum first."""
+    def norm(a, w):
+        return a * torch.rsqrt(a.pow(2).mean(dim=-1, keepdim=True) + eps) * w
+
+    branch = norm(h, post_weight)
+    s = x + scale * (branch if gate is None else gate * branch)
+    return torch.stack((s, norm(s, pre_weight)))
+
+
 FORWARDS = {
     "softmax_forward_ref": softmax_forward_ref,
     "rmsnorm_forward_ref": rmsnorm_forward_ref,
@@ -263,4 +310,7 @@ FORWARDS = {
     "fused_linear_cross_entropy_forward_ref": fused_linear_cross_entropy_forward_ref,
     "llama3_decoder_layer_forward_ref": llama3_decoder_layer_forward_ref,
     "llama3_decoder_layer_runtime_ref": llama3_decoder_layer_runtime_ref,
+    "packed_attention_forward_ref": packed_attention_forward_ref,
+    "rotary_forward_ref": rotary_forward_ref,
+    "block_norm_forward_ref": block_norm_forward_ref,
 }

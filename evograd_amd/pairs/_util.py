@@ -27,14 +27,19 @@ def workspace(nbytes: int, device) -> torch.Tensor:
 tag = _lib.dtype_tag
 
 
-# The widest step between tokens or heads that the strided kernels address with 32-bit offsets.
-MAX_STRIDE = 1 << 24
+# The widest steps between tokens, whose rows the strided kernels address with 32-bit offsets
+# inside a tile, and between heads.
+MAX_TOKEN_STRIDE, MAX_HEAD_STRIDE = 1 << 22, 1 << 40
 
 
 def head_rows(t: torch.Tensor) -> torch.Tensor:
     """A [tokens, heads, head_dim] tensor as the strided kernels take it: itself when a head's
-    columns are contiguous and its steps are in range, else a contiguous copy."""
-    if t.stride(2) == 1 and all(n == 1 or s <= MAX_STRIDE for n, s in zip(t.shape[:2], t.stride())):
+    columns are contiguous, its rows do not overlap and its steps are in range, else a
+    contiguous copy."""
+    tokens, heads, dim = t.shape
+    if ((dim == 1 or t.stride(2) == 1)
+            and (tokens <= 1 or dim <= t.stride(0) <= MAX_TOKEN_STRIDE)
+            and (heads <= 1 or t.stride(1) <= MAX_HEAD_STRIDE)):
         return t
     return t.contiguous()
 

@@ -462,7 +462,7 @@ int eg_silu_mul(const void* gate, const void* up, void* out, int64_t n, int dtyp
  * up to itself:
  *   o_i = sum_j p_ij v_j,  p_ij = exp(scale q_i . k_j - lse_i)
  * `strides` (host, read during the call): token and head steps of q, of k and of v,
- * in elements, at most 2^24; a head's columns are contiguous. o [tokens, heads,
+ * in elements, at most 2^22 and 2^40; a head's columns are contiguous. o [tokens, heads,
  * head_dim], lse fp32 [heads, tokens]. Rows that no sequence holds get o = 0 and are
  * read into no result. The bounds are read on the device alone; ones that break the
  * rules give undefined values but no access outside the tensors. fp32, bf16, fp16;

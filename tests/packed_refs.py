@@ -26,6 +26,8 @@ def attention64(q, k, v, do, lengths, mfma):
     c = D ** -0.5
     out = [[torch.zeros_like(t), torch.zeros_like(t)] for t in (q, q, k, v)]
     ur = u(dt) if mfma else 0.0
+    # below 2^-14 fp16 numbers lie 2^-24 apart, so a P or dS down there moves by up to 2^-25
+    us = 2.0 ** -25 if mfma and dt == torch.float16 else 0.0
     a = 0
     for n in lengths:
         r = slice(a, a + n)
@@ -46,16 +48,17 @@ def attention64(q, k, v, do, lengths, mfma):
             # an error of p itself, at most 2^-126
             ep = p * (es + (p * es).sum(-1, keepdim=True) + f) + torch.clamp(p, max=2.0 ** -126)
             o = p @ V
-            eo = (ur * p + ep) @ V.abs() + f * (p @ V.abs()) + u(dt) * o.abs()
+            seen = (~hidden).double()
+            eo = (ur * p + us * seen + ep) @ V.abs() + f * (p @ V.abs()) + u(dt) * o.abs()
             delta = (DO * o).sum(-1, keepdim=True)
             edelta = (DO.abs() * (eo + f * o.abs())).sum(-1, keepdim=True)
             dp = DO @ V.T
             edp = f * (DO.abs() @ V.abs().T)
             ds = p * (dp - delta)
-            eds = ep * (dp - delta).abs() + p * (edp + edelta) + (ur + f) * ds.abs()
+            eds = ep * (dp - delta).abs() + p * (edp + edelta) + (ur + f) * ds.abs() + us * seen
             dq, edq = c * (ds @ K), c * (eds @ K.abs() + f * (ds.abs() @ K.abs()))
             dk, edk = c * (ds.T @ Q), c * (eds.T @ Q.abs() + f * (ds.abs().T @ Q.abs()))
-            dv, edv = p.T @ DO, (ur * p + ep + f * p).T @ DO.abs()
+            dv, edv = p.T @ DO, (ur * p + us * seen + ep + f * p).T @ DO.abs()
             for i, (x, e, at) in enumerate(((o, eo, h), (dq, edq, h), (dk, edk, g), (dv, edv, g))):
                 out[i][0][r, at] += x
                 out[i][1][r, at] += e

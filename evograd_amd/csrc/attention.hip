@@ -94,9 +94,9 @@ __global__ __launch_bounds__(NW * KG * 64, 2) void attn_fwd_kernel(
   const int bh = query_head(vh, BH / group, group);
   const int q0 = (nqb - 1 - blk) * (32 * NW);  // longest rows first
   const int64_t own = (int64_t)bh * S * D, kv = (int64_t)(bh / group) * S * D;
-  attn_fwd_rows<T, D, NW, KG, ROPE, false>(q + own, D, k + kv, D, v + kv, D, o + own, D,
-                                           lse + (int64_t)bh * S, S, scale_log2, q0, rope_cos,
-                                           rope_sin);
+  attn_fwd_rows<T, D, NW, KG, 1, ROPE, false>(q + own, D, 0, k + kv, D, v + kv, D, o + own, D, 0,
+                                              lse + (int64_t)bh * S, 0, S, scale_log2, q0,
+                                              rope_cos, rope_sin);
 }
 
 // Workgroup (kv head, part of the walk, key block); with parts > 1 the walk is cut into
@@ -121,7 +121,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dkdv_kernel(
       q + heads, D, slice, k + own, D, v + own, D, dout + heads, D, slice, lse + rows, delta + rows,
       S, dk + own, dv + own, D, S, scale, scale_log2, kb * 32 * NW, group, rope_cos, rope_sin,
       parts, pi, part ? part + pi * slab + own : nullptr,
-      part ? part + (parts + pi) * slab + own : nullptr);
+      part ? part + (parts + pi) * slab + own : nullptr, D);
 }
 
 // dK, dV of a split walk: the parts' fp32 slabs ([2][parts][BHkv][S][D], dK slabs
@@ -164,10 +164,10 @@ __global__ __launch_bounds__(NW * KG * 64, 2) void attn_dq_kernel(
   const int bh = query_head(vh, BH / group, group);
   const int64_t own = (int64_t)bh * S * D, kv = (int64_t)(bh / group) * S * D;
   const int64_t row = (int64_t)bh * S;
-  attn_dq_rows<T, D, NW, KG, ROPE, false>(q + own, D, k + kv, D, v + kv, D, dout + own, D, o + own,
-                                          D, lse + row, delta + row, dq + own, D, S, scale,
-                                          scale_log2, (nqb - 1 - blk) * (32 * NW), rope_cos,
-                                          rope_sin);
+  attn_dq_rows<T, D, NW, KG, 1, ROPE, false>(q + own, D, 0, k + kv, D, v + kv, D, dout + own,
+                                             o + own, dq + own, D, 0, lse + row, delta + row, 0, S,
+                                             scale, scale_log2, (nqb - 1 - blk) * (32 * NW),
+                                             rope_cos, rope_sin);
 }
 
 // --------------------------------------------------------------- launchers

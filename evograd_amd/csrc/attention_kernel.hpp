@@ -306,16 +306,18 @@ __device__ __forceinline__ void add_seen(f32x16 (&acc)[D / 32], const uint16_t* 
 // turns, each with tile buffers, a reference max, sums and an output of its own; group 1
 // hands these to group 0 through LDS at the end. Halves the chain of tiles of a row block,
 // which is what bounds a grid that leaves the chip's SIMDs with one wave or less.
-// The workgroup's rows are those from q0 on of one head's sequence of S rows; rows of q, k, v
-// and o lie ldq, ldk, ldv and ldo elements apart. PACKED: see all_finite and TileLoader.
-template <typename T, int D, int NW, int KG, bool ROPE, bool PACKED>
+// The workgroup's rows are those from q0 on of HW heads' sequences of S rows; the heads share
+// their keys and values, the waves are dealt out over them, and the next head's q, o and lse
+// lie hq, ho and hl elements on. Rows of q, k, v and o lie ldq, ldk, ldv and ldo elements
+// apart. PACKED: see all_finite and TileLoader.
+template <typename T, int D, int NW, int KG, int HW, bool ROPE, bool PACKED>
 __device__ __forceinline__ void attn_fwd_rows(
-    const uint16_t* __restrict__ q, int64_t ldq, const uint16_t* __restrict__ kp, int ldk,
-    const uint16_t* __restrict__ vp, int ldv, uint16_t* __restrict__ o, int64_t ldo,
-    float* __restrict__ lse, int S, float scale_log2, int q0, const float* __restrict__ rope_cos,
-    const float* __restrict__ rope_sin) {
+    const uint16_t* __restrict__ q, int64_t ldq, int64_t hq, const uint16_t* __restrict__ kp,
+    int ldk, const uint16_t* __restrict__ vp, int ldv, uint16_t* __restrict__ o, int64_t ldo,
+    int64_t ho, float* __restrict__ lse, int64_t hl, int S, float scale_log2, int q0,
+    const float* __restrict__ rope_cos, const float* __restrict__ rope_sin) {
   using v8 = typename MM<T>::v8;
-  constexpr int BM = 32 * NW, BN = 64;
+  constexpr int HR = NW / HW, BM = 32 * HR, BN = 64;  // HR: waves of a head
   constexpr int KSTEPS = D / 16, DT = D / 32;
   // One __shared__ object per buffer (see the file comment): LDS reads of one
   // buffer never wait for the loads in flight into the other.
@@ -326,8 +328,14 @@ __device__ __forceinline__ void attn_fwd_rows(
   const int w = KG == 1 ? wave_id() : wave_id() % NW, kg = KG == 1 ? 0 : wave_id() / NW;
   const int kvo = kg * BN * D;  // this group's tile buffers
   const int l32 = lane & 31, hh = lane >> 5;
+  const int wr = HW == 1 ? w : w % HR;  // among the waves of its head
+  if constexpr (HW > 1) {
+    q += w / HR * hq;
+    o += w / HR * ho;
+    lse += w / HR * hl;
+  }
 
-  const int qrow = q0 + 32 * w + l32;
+  const int qrow = q0 + 32 * wr + l32;
   const int qrc = qrow < S ? qrow : S - 1;
   v8 qf[KSTEPS];
 #pragma unroll
@@ -359,7 +367,7 @@ __device__ __forceinline__ void attn_fwd_rows(
   const int kv_end = min(S, q0 + BM);
   const int ntiles = (kv_end + BN - 1) / BN;
   const int nturns = (ntiles + KG - 1) / KG;  // tile KG * j + kg in turn j
-  const int wave_first_row = q0 + 32 * w;
+  const int wave_first_row = q0 + 32 * wr;
 
   zero_lds<NW * KG * 64>(Ks0, sizeof(Ks0));
   zero_lds<NW * KG * 64>(Ks1, sizeof(Ks1));
@@ -589,8 +597,8 @@ __device__ __forceinline__ void attn_fwd_rows(
 // The workgroup's keys are those from k0 on of one kv head's sequence of S rows; q, dout, lse
 // and delta are those of its group's first query head, the next head's lie hq, hdo and hl
 // elements on, rows ldq, ldk, ldv and lddo apart. With parts > 1 the walk below is cut into
-// ranges of steps, and part pi's sums go to the fp32 rows pk, pv; else to dk, dv, both ldd
-// apart. PACKED: see all_finite and TileLoader.
+// ranges of steps, and part pi's sums go to the fp32 rows pk, pv, ldp apart; else to dk and dv,
+// ldd apart. PACKED: see all_finite and TileLoader.
 template <typename T, int D, int NW, int BQ, bool ROPE, bool PACKED>
 __device__ __forceinline__ void attn_dkdv_keys(
     const uint16_t* __restrict__ q, int ldq, int64_t hq, const uint16_t* __restrict__ k,
@@ -599,7 +607,7 @@ __device__ __forceinline__ void attn_dkdv_keys(
     int64_t hl, uint16_t* __restrict__ dk, uint16_t* __restrict__ dv, int64_t ldd, int S,
     float scale, float scale_log2, int k0, int group, const float* __restrict__ rope_cos,
     const float* __restrict__ rope_sin, int parts, int pi, float* __restrict__ pk,
-    float* __restrict__ pv) {
+    float* __restrict__ pv, int64_t ldp) {
   using v8 = typename MM<T>::v8;
   constexpr int BK = 32 * NW;
   constexpr int KSTEPS = D / 16, DT = D / 32;
@@ -865,8 +873,8 @@ __device__ __forceinline__ void attn_dkdv_keys(
     if (pk) {  // this part's sums, scaled (and unrotated) like the direct store
 #pragma unroll
       for (int t = 0; t < DT; ++t) {
-        store_rows_f32(pk + key * ldd, dka[t], t, hh, fk);
-        store_rows_f32(pv + key * ldd, dva[t], t, hh, 1.0f);
+        store_rows_f32(pk + key * ldp, dka[t], t, hh, fk);
+        store_rows_f32(pv + key * ldp, dva[t], t, hh, 1.0f);
       }
     } else {
 #pragma unroll
@@ -880,17 +888,17 @@ __device__ __forceinline__ void attn_dkdv_keys(
 
 // ------------------------------------------------------------------- dQ
 // KG as in the forward.
-// Rows as in attn_fwd_rows, those of dout and dq lddo and lddq apart.
-template <typename T, int D, int NW, int KG, bool ROPE, bool PACKED>
+// Rows and heads as in attn_fwd_rows; dout, o and dq share their steps, as lse and delta do.
+template <typename T, int D, int NW, int KG, int HW, bool ROPE, bool PACKED>
 __device__ __forceinline__ void attn_dq_rows(
-    const uint16_t* __restrict__ q, int64_t ldq, const uint16_t* __restrict__ kp, int ldk,
-    const uint16_t* __restrict__ vp, int ldv, const uint16_t* __restrict__ dout, int64_t lddo,
-    const uint16_t* __restrict__ o, int64_t ldo, const float* __restrict__ lse,
-    float* __restrict__ delta, uint16_t* __restrict__ dq, int64_t lddq, int S, float scale,
+    const uint16_t* __restrict__ q, int64_t ldq, int64_t hq, const uint16_t* __restrict__ kp,
+    int ldk, const uint16_t* __restrict__ vp, int ldv, const uint16_t* __restrict__ dout,
+    const uint16_t* __restrict__ o, uint16_t* __restrict__ dq, int64_t ldo, int64_t ho,
+    const float* __restrict__ lse, float* __restrict__ delta, int64_t hl, int S, float scale,
     float scale_log2, int q0, const float* __restrict__ rope_cos,
     const float* __restrict__ rope_sin) {
   using v8 = typename MM<T>::v8;
-  constexpr int BM = 32 * NW, BN = 64;
+  constexpr int HR = NW / HW, BM = 32 * HR, BN = 64;  // HR: waves of a head
   constexpr int KSTEPS = D / 16, DT = D / 32;
   // one object per buffer
   __shared__ __align__(16) uint16_t Ks0[KG * BN * D], Ks1[KG * BN * D];
@@ -900,8 +908,17 @@ __device__ __forceinline__ void attn_dq_rows(
   const int w = KG == 1 ? wave_id() : wave_id() % NW, kg = KG == 1 ? 0 : wave_id() / NW;
   const int kvo = kg * BN * D;  // this group's tile buffers
   const int l32 = lane & 31, hh = lane >> 5;
+  const int wr = HW == 1 ? w : w % HR;  // among the waves of its head
+  if constexpr (HW > 1) {
+    q += w / HR * hq;
+    dout += w / HR * ho;
+    o += w / HR * ho;
+    dq += w / HR * ho;
+    lse += w / HR * hl;
+    delta += w / HR * hl;
+  }
 
-  const int qrow = q0 + 32 * w + l32;
+  const int qrow = q0 + 32 * wr + l32;
   const int qrc = qrow < S ? qrow : S - 1;
   v8 qf[KSTEPS], df[KSTEPS];
   // delta = rowsum(do * o) for this row: the lane pair (l, l + 32) holds the
@@ -912,7 +929,7 @@ __device__ __forceinline__ void attn_dq_rows(
   for (int kk = 0; kk < KSTEPS; ++kk) {
     const int col = kk * 16 + 8 * hh;
     qf[kk] = *reinterpret_cast<const v8*>(q + qrc * ldq + col);
-    df[kk] = *reinterpret_cast<const v8*>(dout + qrc * lddo + col);
+    df[kk] = *reinterpret_cast<const v8*>(dout + qrc * ldo + col);
     const uint4 ou = *reinterpret_cast<const uint4*>(o + qrc * ldo + col);
     uint4 du;
     __builtin_memcpy(&du, &df[kk], 16);
@@ -935,7 +952,7 @@ __device__ __forceinline__ void attn_dq_rows(
   const int kv_end = min(S, q0 + BM);
   const int ntiles = (kv_end + BN - 1) / BN;
   const int nturns = (ntiles + KG - 1) / KG;
-  const int wave_first_row = q0 + 32 * w;
+  const int wave_first_row = q0 + 32 * wr;
 
   // Element offsets of this lane's operand reads inside a tile, computed once (as in
   // the forward): rows for S and dP (the K and V tiles share the layout), transposed
@@ -1108,7 +1125,7 @@ __device__ __forceinline__ void attn_dq_rows(
   }
 
   if (qrow < S) {
-    uint16_t* op = dq + qrow * lddq;
+    uint16_t* op = dq + qrow * ldo;
     float fq = scale;
     if constexpr (ROPE) {  // dq of the pre-rotation queries: the rotation's transpose
 #pragma unroll

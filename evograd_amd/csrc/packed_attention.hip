@@ -33,148 +33,162 @@ __device__ __forceinline__ void packed_coords(int slots, int& slot, int& rank) {
   }
 }
 
-// Slot v -> query head: the heads of a group have the same v % 8 when kv_heads is a
-// multiple of 8, so they share an XCD's L2.
+// HW heads of a group share a workgroup, its keys and its values (attn_fwd_rows). Slot v ->
+// first of them: the slots of a group have the same v % 8 when kv_heads is a multiple of
+// 8, so they share an XCD's L2.
+template <int HW>
 __device__ __forceinline__ int slot_head(const PackedAttn& a, int v) {
-  return (v % a.kv_heads) * (a.heads / a.kv_heads) + v / a.kv_heads;
+  return (v % a.kv_heads) * (a.heads / a.kv_heads) + v / a.kv_heads * HW;
 }
 
-template <typename T, int D, int NW, int KG>
-__global__ __launch_bounds__(NW * KG * 64, 2) void packed_fwd_kernel(PackedAttn a, int tiles,
+template <typename T, int D, int NW, int KG, int HW>
+__global__ __launch_bounds__(NW * KG * 64, 2) void packed_fwd_kernel(PackedAttn a, int ranks,
                                                                      float scale_log2) {
-  int slot, rank, spare;
-  packed_coords(a.heads, slot, rank);
-  const int h = slot_head(a, slot), kvh = h / (a.heads / a.kv_heads);
+  constexpr int ROWS = 32 * NW / HW;
+  int slot, rank;
+  packed_coords(a.heads / HW, slot, rank);
+  const int h = slot_head<HW>(a, slot), kvh = h / (a.heads / a.kv_heads);
   const int64_t ldo = (int64_t)a.heads * D;
   uint16_t* o = (uint16_t*)a.o + h * D;
   float* lse = a.lse + (int64_t)h * a.seqs.tokens;
   SeqTile t;
-  float walk;
-  if (!find_tile<32 * NW, false>(a.seqs, rank, t, spare, walk)) {
-    zero_unused_rows(a.seqs, spare, tiles - rank + spare, (T*)o, ldo, D);
-    zero_unused_rows(a.seqs, spare, tiles - rank + spare, lse, 1, 1);
+  if (!find_tile<ROWS, false>(a.seqs, rank, t)) {
+    zero_unused_rows(a.seqs, t, rank, ranks, (T*)o, ldo, HW * D);
+#pragma unroll
+    for (int i = 0; i < HW; ++i)
+      zero_unused_rows(a.seqs, t, rank, ranks, lse + i * (int64_t)a.seqs.tokens, 1, 1);
     return;
   }
-  attn_fwd_rows<T, D, NW, KG, false, true>(
-      (const uint16_t*)a.q + t.begin * a.q_token + h * a.q_head, a.q_token,
+  attn_fwd_rows<T, D, NW, KG, HW, false, true>(
+      (const uint16_t*)a.q + t.begin * a.q_token + h * a.q_head, a.q_token, a.q_head,
       (const uint16_t*)a.k + t.begin * a.k_token + kvh * a.k_head, (int)a.k_token,
       (const uint16_t*)a.v + t.begin * a.v_token + kvh * a.v_head, (int)a.v_token,
-      o + t.begin * ldo, ldo, lse + t.begin, t.len, scale_log2, t.tile * 32 * NW, nullptr, nullptr);
-}
-
-template <typename T, int D, int NW, int KG>
-__global__ __launch_bounds__(NW * KG * 64, 2) void packed_dq_kernel(PackedAttn a, int tiles,
-                                                                    float scale_log2) {
-  int slot, rank, spare;
-  packed_coords(a.heads, slot, rank);
-  const int h = slot_head(a, slot), kvh = h / (a.heads / a.kv_heads);
-  const int64_t ldo = (int64_t)a.heads * D;
-  uint16_t* dq = (uint16_t*)a.dq + h * D;
-  SeqTile t;
-  float walk;
-  if (!find_tile<32 * NW, false>(a.seqs, rank, t, spare, walk)) {
-    zero_unused_rows(a.seqs, spare, tiles - rank + spare, (T*)dq, ldo, D);
-    return;
-  }
-  const int64_t own = t.begin * ldo + h * D, row = (int64_t)h * a.seqs.tokens + t.begin;
-  attn_dq_rows<T, D, NW, KG, false, true>(
-      (const uint16_t*)a.q + t.begin * a.q_token + h * a.q_head, a.q_token,
-      (const uint16_t*)a.k + t.begin * a.k_token + kvh * a.k_head, (int)a.k_token,
-      (const uint16_t*)a.v + t.begin * a.v_token + kvh * a.v_head, (int)a.v_token,
-      (const uint16_t*)a.dout + own, ldo, (const uint16_t*)a.o + own, ldo, a.lse + row,
-      a.delta + row, dq + t.begin * ldo, ldo, t.len, a.scale, scale_log2, t.tile * 32 * NW,
+      o + t.begin * ldo, ldo, D, lse + t.begin, a.seqs.tokens, t.len, scale_log2, t.tile * ROWS,
       nullptr, nullptr);
 }
 
-// The dK/dV walk of a block of 128 keys, cut where it is long against the work of the whole
-// batch: into as many of at most `most` pieces as keep each near 1 / 512 of it (two
-// workgroups per CU), but no shorter than kMinSteps steps of 32 rows, about what a piece's
-// fp32 slabs cost to write and read.
-constexpr int kKeyWaves = 4, kKeys = 32 * kKeyWaves, kWalkRows = 32;
-constexpr float kMinSteps = 16.f;
-__device__ __forceinline__ int mfma_parts(const PackedAttn& a, const SeqTile& t, float walk,
-                                          int most) {
-  const float per_tile = (float)(a.heads / a.kv_heads) * (kKeys / kWalkRows);
-  const float each = fmaxf(walk * per_tile * a.kv_heads * (1.f / 512.f), kMinSteps);
-  return min(most, max(1, (int)(per_tile * (t.tile + 1) / each + 0.999f)));
+template <typename T, int D, int NW, int KG, int HW>
+__global__ __launch_bounds__(NW * KG * 64, 2) void packed_dq_kernel(PackedAttn a, int ranks,
+                                                                    float scale_log2) {
+  constexpr int ROWS = 32 * NW / HW;
+  int slot, rank;
+  packed_coords(a.heads / HW, slot, rank);
+  const int h = slot_head<HW>(a, slot), kvh = h / (a.heads / a.kv_heads);
+  const int64_t ldo = (int64_t)a.heads * D;
+  SeqTile t;
+  if (!find_tile<ROWS, false>(a.seqs, rank, t)) {
+    zero_unused_rows(a.seqs, t, rank, ranks, (T*)a.dq + h * D, ldo, HW * D);
+    return;
+  }
+  const int64_t own = t.begin * ldo + h * D, row = (int64_t)h * a.seqs.tokens + t.begin;
+  attn_dq_rows<T, D, NW, KG, HW, false, true>(
+      (const uint16_t*)a.q + t.begin * a.q_token + h * a.q_head, a.q_token, a.q_head,
+      (const uint16_t*)a.k + t.begin * a.k_token + kvh * a.k_head, (int)a.k_token,
+      (const uint16_t*)a.v + t.begin * a.v_token + kvh * a.v_head, (int)a.v_token,
+      (const uint16_t*)a.dout + own, (const uint16_t*)a.o + own, (uint16_t*)a.dq + own, ldo, D,
+      a.lse + row, a.delta + row, a.seqs.tokens, t.len, a.scale, scale_log2, t.tile * ROWS, nullptr,
+      nullptr);
 }
 
-// Key blocks are counted from the end of their sequence, so the longest walks come first.
-// Slabs: [most][tokens][kv_heads][D] fp32 of dK, then of dV.
-template <typename T, int D>
-__global__ __launch_bounds__(kKeyWaves * 64, 2) void packed_dkdv_kernel(PackedAttn a, int tiles,
-                                                                        int most,
-                                                                        float scale_log2) {
-  int slot, rank, spare;
-  packed_coords(a.kv_heads * most, slot, rank);
-  const int kvh = slot % a.kv_heads, pi = slot / a.kv_heads;
-  const int group = a.heads / a.kv_heads, h0 = kvh * group;
+// A workgroup's rows or keys lie in one sequence, so where sequences are shorter than a block
+// on the mean a narrower one leaves fewer waves without rows.
+constexpr int64_t kShort = 112;
+inline bool short_seqs(int64_t tokens, int64_t seqs) { return tokens < kShort * seqs; }
+
+// The dK/dV walk of a block of keys (32 a wave), cut where it is long against the work of the
+// whole batch: each piece is at most 1 / kTarget of it (two workgroups per CU), but no
+// shorter than kMinSteps steps of 32 rows, about what a piece's fp32 slab costs to write and
+// read.
+constexpr int kWalkRows = 32;
+constexpr int64_t kTarget = 512, kMinSteps = 8;
+
+struct WalkCut {
+  int least;        // find_tile's arguments
+  float share;
+  int ranks, slabs;  // pieces of a kv head at most; those of them that belong to cut walks
+  int waves;         // of 32 keys each
+};
+WalkCut walk_cut(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads) {
+  WalkCut c;
+  c.waves = short_seqs(tokens, seqs) ? 2 : 4;
+  const int64_t per_tile = heads / kv_heads * (32 * c.waves / kWalkRows);
+  c.least = (int)((kMinSteps + per_tile - 1) / per_tile);
+  c.share = (float)kv_heads / kTarget;
+  // a tile of index j makes at most 1 + j / m pieces, a cut one (j >= m) at most 2 j / m, and
+  // the sum of j / m over a kv head's tiles is at most kTarget / kv_heads
+  const int64_t more = (kTarget + kv_heads - 1) / kv_heads;
+  c.ranks = (int)(packed_tiles(tokens, seqs, 32 * c.waves) + more);
+  c.slabs = (int)std::min<int64_t>(c.ranks, 2 * more + 1);
+  return c;
+}
+
+// Key blocks are counted from the end of their sequence, so the longest walks come first, and
+// the pieces of cut walks before the others: slab [kv head][rank][2][keys][D], dK then dV.
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(NW * 64, 2) void packed_dkdv_kernel(PackedAttn a, WalkCut c,
+                                                                 float scale_log2) {
+  constexpr int kKeys = 32 * NW;
+  int kvh, rank;
+  packed_coords(a.kv_heads, kvh, rank);
+  const int h0 = kvh * (a.heads / a.kv_heads);
   const int64_t ldkv = (int64_t)a.kv_heads * D, ldo = (int64_t)a.heads * D;
   uint16_t *dk = (uint16_t*)a.dk + kvh * D, *dv = (uint16_t*)a.dv + kvh * D;
   SeqTile t;
-  float walk;
-  if (!find_tile<kKeys, true>(a.seqs, rank, t, spare, walk)) {
-    if (pi != 0) return;
-    zero_unused_rows(a.seqs, spare, tiles - rank + spare, (T*)dk, ldkv, D);
-    zero_unused_rows(a.seqs, spare, tiles - rank + spare, (T*)dv, ldkv, D);
+  if (!find_tile<kKeys, true>(a.seqs, rank, t, c.least, c.share)) {
+    zero_unused_rows(a.seqs, t, rank, c.ranks, (T*)dk, ldkv, D);
+    zero_unused_rows(a.seqs, t, rank, c.ranks, (T*)dv, ldkv, D);
     return;
   }
-  const int parts = mfma_parts(a, t, walk, most);
-  if (pi >= parts) return;
-  const int64_t own = t.begin * ldkv, slab = a.seqs.tokens * ldkv;
-  const int64_t row = (int64_t)h0 * a.seqs.tokens + t.begin;
-  float* part = parts > 1 ? a.part + pi * slab + own + kvh * D : nullptr;
-  attn_dkdv_keys<T, D, kKeyWaves, kWalkRows, false, true>(
+  const int k0 = (t.tiles - 1 - t.tile) * kKeys;
+  float* part = nullptr;
+  if (t.pieces > 1) {
+    if (rank >= c.slabs) return;  // no batch's: the bound is walk_cut's
+    part = a.part + ((int64_t)kvh * c.slabs + rank) * (2 * kKeys * D) - (int64_t)k0 * D;
+  }
+  const int64_t own = t.begin * ldkv, row = (int64_t)h0 * a.seqs.tokens + t.begin;
+  attn_dkdv_keys<T, D, NW, kWalkRows, false, true>(
       (const uint16_t*)a.q + t.begin * a.q_token + h0 * a.q_head, (int)a.q_token, a.q_head,
       (const uint16_t*)a.k + t.begin * a.k_token + kvh * a.k_head, a.k_token,
       (const uint16_t*)a.v + t.begin * a.v_token + kvh * a.v_head, (int)a.v_token,
       (const uint16_t*)a.dout + t.begin * ldo + h0 * D, (int)ldo, D, a.lse + row, a.delta + row,
-      a.seqs.tokens, dk + own, dv + own, ldkv, t.len, a.scale, scale_log2,
-      (t.tiles - 1 - t.tile) * kKeys, group, nullptr, nullptr, parts, pi, part,
-      part ? part + most * slab : nullptr);
+      a.seqs.tokens, dk + own, dv + own, ldkv, t.len, a.scale, scale_log2, k0,
+      a.heads / a.kv_heads, nullptr, nullptr, t.pieces, t.piece, part,
+      part ? part + kKeys * D : nullptr, D);
 }
 
-// dK and dV of the walks that were cut: their slabs in order, rounded once. Workgroup = the
-// 128 keys of a dK/dV workgroup.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void packed_reduce_kernel(PackedAttn a, int most) {
-  int kvh, rank, spare;
+// dK and dV of the walks that were cut: their slabs in order, rounded once. The workgroups of
+// a walk's pieces share its keys.
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(256) void packed_reduce_kernel(PackedAttn a, WalkCut c) {
+  constexpr int kKeys = 32 * NW;
+  int kvh, rank;
   packed_coords(a.kv_heads, kvh, rank);
   SeqTile t;
-  float walk;
-  if (!find_tile<kKeys, true>(a.seqs, rank, t, spare, walk)) return;
-  const int parts = mfma_parts(a, t, walk, most);
-  if (parts == 1) return;
+  if (!find_tile<kKeys, true>(a.seqs, rank, t, c.least, c.share)) return;
+  const int head = rank - t.piece;  // the walk's first piece
+  if (t.pieces == 1 || head + t.pieces > c.slabs) return;
   const int k0 = (t.tiles - 1 - t.tile) * kKeys, rows = min(kKeys, t.len - k0);
-  const int64_t ldkv = (int64_t)a.kv_heads * D, slab = a.seqs.tokens * ldkv;
-  for (int e = threadIdx.x; e < rows * (D / 4); e += 256) {
-    const int64_t at = (t.begin + k0 + e / (D / 4)) * ldkv + kvh * D + e % (D / 4) * 4;
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const float* p = a.part + which * most * slab + at;
-      float4 x = *reinterpret_cast<const float4*>(p);
-      for (int i = 1; i < parts; ++i) {
-        const float4 y = *reinterpret_cast<const float4*>(p + i * slab);
-        x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
-      }
-      uint2 u;
-      u.x = MM<T>::pack2(x.x, x.y);
-      u.y = MM<T>::pack2(x.z, x.w);
-      *reinterpret_cast<uint2*>((uint16_t*)(which ? a.dv : a.dk) + at) = u;
+  const float* part = a.part + ((int64_t)kvh * c.slabs + head) * (2 * kKeys * D);
+  const int64_t ldkv = (int64_t)a.kv_heads * D, first = (t.begin + k0) * ldkv + kvh * D;
+  for (int e = t.piece * 256 + threadIdx.x; e < 2 * rows * (D / 4); e += 256 * t.pieces) {
+    const int which = e >= rows * (D / 4), f = e - which * rows * (D / 4);
+    const float* p = part + which * (kKeys * D) + f * 4;
+    float4 x = *reinterpret_cast<const float4*>(p);
+    for (int i = 1; i < t.pieces; ++i) {
+      const float4 y = *reinterpret_cast<const float4*>(p + i * (2 * kKeys * D));
+      x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
     }
+    uint2 u;
+    u.x = MM<T>::pack2(x.x, x.y);
+    u.y = MM<T>::pack2(x.z, x.w);
+    *reinterpret_cast<uint2*>((uint16_t*)(which ? a.dv : a.dk) + first + f / (D / 4) * ldkv +
+                              f % (D / 4) * 4) = u;
   }
 }
 
-// The most pieces a walk is cut into, what the workspace holds slabs for: none where the
-// key blocks alone fill the chip several times over.
-int64_t most_parts(int64_t tokens, int64_t kv_heads) {
-  const int64_t blocks = kv_heads * ((tokens + kKeys - 1) / kKeys);
-  return std::max<int64_t>(1, std::min<int64_t>(8, (2048 + blocks - 1) / blocks));
-}
-
-size_t mfma_part_bytes(int64_t tokens, int64_t kv_heads, int64_t D) {
-  const int64_t most = most_parts(tokens, kv_heads);
-  return most > 1 ? (size_t)2 * most * tokens * kv_heads * D * 4 : 0;
+size_t mfma_part_bytes(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t D) {
+  const WalkCut c = walk_cut(tokens, seqs, heads, kv_heads);
+  return (size_t)kv_heads * c.slabs * 2 * (32 * c.waves) * D * 4;
 }
 
 bool mfma_sizes(int64_t D, int dtype) {
@@ -203,37 +217,72 @@ int by_type(const PackedAttn& a, int dtype, F&& f) {
   return a.head_dim == 128 ? f(f16_t{}, Int<128>{}) : f(f16_t{}, Int<64>{});
 }
 
+// Two key groups per workgroup (KG = 2), which halve a row block's chain of key tiles: for few
+// long walks.
+inline bool split_keys(const PackedAttn& a, bool dq) {
+  const int64_t grid = ((int64_t)a.seqs.tokens + 127) / 128 * a.heads;
+  if (short_seqs(a.seqs.tokens, a.seqs.n)) return false;
+  return dq ? a.head_dim == 64 && grid <= 384 : grid <= 512;
+}
+
+// Workgroups of the forward and dQ: f(HW, NW, KG).
+// HW heads of a group share their keys and values: their waves walk the same keys, where the
+// waves of one head's rows end one after the other, and short sequences fill a tile of 32
+// rows where 128 of one head would be mostly empty.
+template <int D, typename F>
+int by_rows(const PackedAttn& a, bool dq, F&& f) {
+  const int group = a.heads / a.kv_heads;
+  const bool split = split_keys(a, dq);
+  auto go = [&](auto hw) -> int {
+    constexpr int HW = decltype(hw)::value;
+    if (split) return f(hw, Int<4>{}, Int<2>{});
+    if constexpr (D == 64 && HW < 4) {
+      if (short_seqs(a.seqs.tokens, a.seqs.n)) return f(hw, Int<2>{}, Int<1>{});
+    }
+    return f(hw, Int<4>{}, Int<1>{});
+  };
+  if (group % 4 == 0) return go(Int<4>{});
+  if (group % 2 == 0) return go(Int<2>{});
+  return go(Int<1>{});
+}
+
 int mfma_fwd(const PackedAttn& a, int dtype, hipStream_t st) {
   return by_type(a, dtype, [&](auto tc, auto dc) {
     using T = decltype(tc);
     constexpr int D = decltype(dc)::value;
-    auto go = [&](auto nwc, auto kgc) {
-      constexpr int NW = decltype(nwc)::value, KG = decltype(kgc)::value;
-      const int64_t tiles = packed_tiles(a.seqs.tokens, a.seqs.n, 32 * NW);
-      EG_LAUNCH((packed_fwd_kernel<T, D, NW, KG>), dim3((unsigned)(tiles * a.heads)),
-                dim3(NW * KG * 64), 0, st, a, (int)tiles, a.scale * kLog2e);
+    return by_rows<D>(a, false, [&](auto hw, auto nw, auto kg) {
+      constexpr int HW = decltype(hw)::value, NW = decltype(nw)::value, KG = decltype(kg)::value;
+      const int64_t ranks = packed_tiles(a.seqs.tokens, a.seqs.n, 32 * NW / HW);
+      EG_LAUNCH((packed_fwd_kernel<T, D, NW, KG, HW>), dim3((unsigned)(ranks * (a.heads / HW))),
+                dim3(NW * KG * 64), 0, st, a, (int)ranks, a.scale * kLog2e);
       return check_launch("eg_packed_attn_fwd");
-    };
-    return go(Int<4>{}, Int<1>{});
+    });
   });
 }
 
 int mfma_bwd(const PackedAttn& a, int dtype, hipStream_t st) {
-  const int64_t tiles = packed_tiles(a.seqs.tokens, a.seqs.n, kKeys);
-  const int most = (int)most_parts(a.seqs.tokens, a.kv_heads);
+  const WalkCut cut = walk_cut(a.seqs.tokens, a.seqs.n, a.heads, a.kv_heads);
   return by_type(a, dtype, [&](auto tc, auto dc) {
     using T = decltype(tc);
     constexpr int D = decltype(dc)::value;
-    EG_LAUNCH((packed_dq_kernel<T, D, 4, 1>), dim3((unsigned)(tiles * a.heads)), dim3(256), 0, st,
-              a, (int)tiles, a.scale * kLog2e);
-    if (int e = check_launch("eg_packed_attn_bwd(dq)")) return e;
-    EG_LAUNCH((packed_dkdv_kernel<T, D>), dim3((unsigned)(tiles * a.kv_heads * most)),
-              dim3(kKeyWaves * 64), 0, st, a, (int)tiles, most, a.scale * kLog2e);
-    if (int e = check_launch("eg_packed_attn_bwd(dkdv)")) return e;
-    if (most == 1) return 0;
-    EG_LAUNCH((packed_reduce_kernel<T, D>), dim3((unsigned)(tiles * a.kv_heads)), dim3(256), 0, st,
-              a, most);
-    return check_launch("eg_packed_attn_bwd(dkdv reduce)");
+    const int rc = by_rows<D>(a, true, [&](auto hw, auto nw, auto kg) {
+      constexpr int HW = decltype(hw)::value, NW = decltype(nw)::value, KG = decltype(kg)::value;
+      const int64_t ranks = packed_tiles(a.seqs.tokens, a.seqs.n, 32 * NW / HW);
+      EG_LAUNCH((packed_dq_kernel<T, D, NW, KG, HW>), dim3((unsigned)(ranks * (a.heads / HW))),
+                dim3(NW * KG * 64), 0, st, a, (int)ranks, a.scale * kLog2e);
+      return check_launch("eg_packed_attn_bwd(dq)");
+    });
+    if (rc) return rc;
+    auto keys = [&](auto nwc) {
+      constexpr int NW = decltype(nwc)::value;
+      EG_LAUNCH((packed_dkdv_kernel<T, D, NW>), dim3((unsigned)(cut.ranks * a.kv_heads)),
+                dim3(NW * 64), 0, st, a, cut, a.scale * kLog2e);
+      if (int e = check_launch("eg_packed_attn_bwd(dkdv)")) return e;
+      EG_LAUNCH((packed_reduce_kernel<T, D, NW>), dim3((unsigned)(cut.slabs * a.kv_heads)),
+                dim3(256), 0, st, a, cut);
+      return check_launch("eg_packed_attn_bwd(dkdv reduce)");
+    };
+    return cut.waves == 2 ? keys(Int<2>{}) : keys(Int<4>{});
   });
 }
 
@@ -278,11 +327,11 @@ int check_packed(const char* name, const PackedAttn& a, int64_t tokens, int64_t 
       set_error("%s: head strides must be at least 0 and at most 2^40 elements", name);
       return 1;
     }
-  // tiles of 16 rows times heads and walk pieces index one grid
+  // tiles of 16 rows (and pieces of walks) times heads index one grid
   if (tokens > kMaxTokens || seqs > kMaxSeqs || heads > 4096 ||
-      packed_tiles(tokens, seqs, 16) * heads * 8 > 0x7fffffffLL) {
+      packed_tiles(tokens, seqs, 16) * heads > ((int64_t)1 << 30)) {
     set_error("%s: size out of range (tokens <= 268435456, sequences <= 16777216, heads <= 4096, "
-              "(tokens / 16 + sequences) * heads < 2^28)", name);
+              "(tokens / 16 + sequences) * heads < 2^30)", name);
     return 1;
   }
   return 0;
@@ -306,11 +355,13 @@ PackedAttn describe(const void* q, const void* k, const void* v, const int* cu, 
 
 extern "C" size_t eg_packed_attn_workspace_bytes(int64_t tokens, int64_t seqs, int64_t heads,
                                                  int64_t kv_heads, int64_t head_dim, int dtype) {
-  if (tokens <= 0 || seqs < 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 0;
-  const size_t generic = packed_generic_part_bytes(tokens, kv_heads, head_dim);
+  if (tokens <= 0 || seqs < 0 || heads <= 0 || kv_heads <= 0 || heads < kv_heads || head_dim <= 0)
+    return 0;
+  const size_t generic = packed_generic_part_bytes(tokens, seqs, heads, kv_heads, head_dim);
   // rows of any alignment may come: the larger of the two where both kernels may run
   return delta_bytes(tokens, heads) +
-         (mfma_sizes(head_dim, dtype) ? std::max(generic, mfma_part_bytes(tokens, kv_heads, head_dim))
+         (mfma_sizes(head_dim, dtype) ? std::max(generic,
+                                               mfma_part_bytes(tokens, seqs, heads, kv_heads, head_dim))
                                       : generic);
 }
 

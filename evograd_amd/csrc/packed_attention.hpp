@@ -22,7 +22,8 @@ struct PackedAttn {
 };
 
 // packed_attn_generic.hip: any type, even head size up to 128 and strides.
-size_t packed_generic_part_bytes(int64_t tokens, int64_t kv_heads, int64_t head_dim);
+size_t packed_generic_part_bytes(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads,
+                                 int64_t head_dim);
 int packed_generic_fwd(const PackedAttn& a, int dtype, hipStream_t st);
 int packed_generic_bwd(const PackedAttn& a, int dtype, hipStream_t st);
 

@@ -66,6 +66,7 @@ LENGTHS = {
     "ones": [1] * 40,
     "long_and_short": [700, 1, 2, 3, 90],
     "past_a_wave": [3, 0, 17] * 23 + [140],
+    "past_its_registers": [2, 0, 5, 1] * 70 + [150, 33],
 }
 
 

@@ -167,7 +167,7 @@ def test_entry_points_check_their_arguments():
                       ("out of range", dict(tokens=1 << 29)),
                       ("out of range", dict(seqs=1 << 25)),
                       ("out of range", dict(heads=8192, kv=1)),
-                      ("out of range", dict(tokens=1 << 28, heads=64, kv=64)),
+                      ("out of range", dict(tokens=1 << 28, heads=128, kv=128)),
                       ("null pointer", dict(q=None))):
         with pytest.raises(RuntimeError, match=words):
             attention(**kw)
@@ -209,8 +209,12 @@ def test_entry_points_check_their_arguments():
 def test_workspaces():
     al = lambda n: (n + 255) // 256 * 256
     assert _lib.query("eg_packed_attn_workspace_bytes", 0, 1, 2, 2, 64, _lib.EG_F32) == 0
-    # 100 blocks of 16 keys of 2 kv heads: at most 5 pieces of a walk
+    # fp32, 2 kv heads: the slabs (16 keys) of 512 cut pieces at most, or of every piece there is
     got = _lib.query("eg_packed_attn_workspace_bytes", 1600, 3, 8, 2, 32, _lib.EG_F32)
-    assert got == al(1600 * 8 * 4) + 2 * 5 * 1600 * 2 * 32 * 4
+    assert got == al(1600 * 8 * 4) + 2 * min((1600 + 3 * 15) // 16 + 1 + 256, 513) * 2 * 16 * 32 * 4
+    # bf16 on MFMA (128 keys): does not grow with the tokens but for delta
+    mfma = lambda T: _lib.query("eg_packed_attn_workspace_bytes", T, 7, 32, 8, 128, _lib.EG_BF16)
+    assert mfma(1 << 20) - mfma(1 << 17) == ((1 << 20) - (1 << 17)) * 32 * 4
+    assert mfma(1 << 17) - al((1 << 17) * 32 * 4) == 8 * 129 * 2 * 128 * 128 * 4
     assert _lib.query("eg_block_norm_workspace_bytes", 0, 64) == 0
     assert _lib.query("eg_block_norm_workspace_bytes", 3, 64) == 3 * 2 * 64 * 4

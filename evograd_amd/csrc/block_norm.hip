@@ -21,6 +21,7 @@
 // partial row each, which a second kernel adds in order (no atomics).
 #include "eg_common.hpp"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace eg {
@@ -78,6 +79,20 @@ struct RowPack {
   }
 };
 
+// Sum over the workgroup, in wave order. One barrier: a kernel gives each of its sums a buffer
+// of its own, and another sum's barrier lies between two uses of one.
+template <int BLOCK>
+__device__ __forceinline__ float row_sum(float v, float* lds) {
+  v = wave_reduce(v, SumOp());
+  if constexpr (BLOCK == 64) return v;
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  float r = lds[0];
+#pragma unroll
+  for (int w = 1; w < BLOCK / 64; ++w) r += lds[w];
+  return r;
+}
+
 template <typename T>
 __device__ __forceinline__ const void* row_of(const void* p, int64_t row, int cols) {
   return (const T*)p + row * cols;
@@ -87,145 +102,135 @@ __device__ __forceinline__ void* row_of(void* p, int64_t row, int cols) {
   return (T*)p + row * cols;
 }
 
-// Workgroup of BLOCK threads per row, PPT packs per thread.
-template <typename T, int VEC, int BLOCK, int PPT, bool RAG, int GATE>
+// Workgroup of BLOCK threads per row, a pack per thread.
+template <typename T, int VEC, int BLOCK, bool RAG, int GATE>
 __global__ __launch_bounds__(BLOCK) void block_norm_fwd_kernel(NormArgs a) {
-  __shared__ float red[BLOCK / 64];
+  __shared__ float red[2][BLOCK / 64];
   const int64_t row = blockIdx.x;
   const int cols = a.cols;
-  RowPack<T, VEC, RAG> at[PPT];
-  float h[PPT][VEC], x[PPT][VEC];
-#pragma unroll
-  for (int p = 0; p < PPT; ++p) {
-    at[p].set(threadIdx.x + p * BLOCK, cols);
-    at[p].load(row_of<T>(a.h, row, cols), h[p]);
-  }
-#pragma unroll
-  for (int p = 0; p < PPT; ++p) at[p].load(row_of<T>(a.x, row, cols), x[p]);
-  float sum = 0.f;
-#pragma unroll
-  for (int p = 0; p < PPT; ++p)
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) sum += h[p][i] * h[p][i];
-  const float rh = rsqrtf(block_reduce<BLOCK>(sum, SumOp(), red) / cols + a.eps);
+  RowPack<T, VEC, RAG> at;
+  at.set(threadIdx.x, cols);
+  float h[VEC], x[VEC], w[VEC], g[VEC], w2[VEC];
+  at.load(row_of<T>(a.h, row, cols), h);
+  at.load(row_of<T>(a.x, row, cols), x);
+  at.load(a.w1, w);
+  if (GATE == kChannel) at.load(a.gate, g);
+  if (GATE == kElement) at.load(row_of<T>(a.gate, row, cols), g);
+  at.load(a.w2, w2);
   float scale = a.alpha;
   if (GATE == kRow) scale *= to_f32(((const T*)a.gate)[row]);
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) sum += h[i] * h[i];
+  const float rh = rsqrtf(row_sum<BLOCK>(sum, red[0]) / cols + a.eps);
   sum = 0.f;
 #pragma unroll
-  for (int p = 0; p < PPT; ++p) {
-    float w[VEC], g[VEC];
-    at[p].load(a.w1, w);
-    if (GATE == kChannel) at[p].load(a.gate, g);
-    if (GATE == kElement) at[p].load(row_of<T>(a.gate, row, cols), g);
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const float n = h[p][i] * rh * w[i];
-      x[p][i] += GATE == kChannel || GATE == kElement ? scale * g[i] * n : scale * n;
-      sum += x[p][i] * x[p][i];
-    }
-    at[p].store(row_of<T>(a.s, row, cols), x[p]);
+  for (int i = 0; i < VEC; ++i) {
+    const float n = h[i] * rh * w[i];
+    x[i] += GATE == kChannel || GATE == kElement ? scale * g[i] * n : scale * n;
+    sum += x[i] * x[i];
   }
-  const float rs = rsqrtf(block_reduce<BLOCK>(sum, SumOp(), red) / cols + a.eps);
+  at.store(row_of<T>(a.s, row, cols), x);
+  const float rs = rsqrtf(row_sum<BLOCK>(sum, red[1]) / cols + a.eps);
 #pragma unroll
-  for (int p = 0; p < PPT; ++p) {
-    float w[VEC];
-    at[p].load(a.w2, w);
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) x[p][i] = x[p][i] * rs * w[i];
-    at[p].store(row_of<T>(a.y, row, cols), x[p]);
-  }
+  for (int i = 0; i < VEC; ++i) x[i] = x[i] * rs * w2[i];
+  at.store(row_of<T>(a.y, row, cols), x);
   if (threadIdx.x == 0) {
     a.rstd[row] = rh;
     a.rstd[a.rows + row] = rs;
   }
 }
 
-template <typename T, int VEC, int BLOCK, int PPT, bool RAG, int GATE>
-__global__ __launch_bounds__(BLOCK) void block_norm_bwd_kernel(NormArgs a) {
-  __shared__ float red[BLOCK / 64];
-  const int cols = a.cols;
-  RowPack<T, VEC, RAG> at[PPT];
-  float acc1[PPT][VEC], acc2[PPT][VEC];
-#pragma unroll
-  for (int p = 0; p < PPT; ++p) {
-    at[p].set(threadIdx.x + p * BLOCK, cols);
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) acc1[p][i] = acc2[p][i] = 0.f;
+// A row's packs as they lie in memory: the backward loads the next row's while it works on
+// this one's, in a quarter (16-bit types: half) of the registers that fp32 values take.
+template <typename T, int VEC, bool RAG>
+struct RawPack {
+  Pack<T, VEC> v;
+  __device__ __forceinline__ void load(const RowPack<T, VEC, RAG>& at, const void* row) {
+    if (!at.in) return;
+    if constexpr (RAG) v = load_ragged_raw<T, VEC, false>((const T*)row + at.c);
+    else v = *reinterpret_cast<const Pack<T, VEC>*>((const T*)row + at.c);
   }
+  __device__ __forceinline__ void get(const RowPack<T, VEC, RAG>& at, float (&f)[VEC]) const {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) f[i] = at.in && i >= at.lo ? to_f32(v.v[i]) : 0.f;
+  }
+};
+
+template <typename T, int VEC, int BLOCK, bool RAG, int GATE>
+__global__ __launch_bounds__(BLOCK) void block_norm_bwd_kernel(NormArgs a) {
+  __shared__ float red[3][BLOCK / 64];
+  const int cols = a.cols;
+  RowPack<T, VEC, RAG> at;
+  at.set(threadIdx.x, cols);
+  RawPack<T, VEC, RAG> w1, w2, gate, rh_, rx, rdy, rds;
+  w1.load(at, a.w1);
+  w2.load(at, a.w2);
+  if (GATE == kChannel) gate.load(at, a.gate);
+  auto fetch = [&](int64_t row) {
+    rh_.load(at, row_of<T>(a.h, row, cols));
+    rx.load(at, row_of<T>(a.x, row, cols));
+    rdy.load(at, row_of<T>(a.dy, row, cols));
+    rds.load(at, row_of<T>(a.ds, row, cols));
+    if (GATE == kElement) gate.load(at, row_of<T>(a.gate, row, cols));
+  };
+  float acc1[VEC], acc2[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) acc1[i] = acc2[i] = 0.f;
+  fetch(blockIdx.x);
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const float rh = a.rstd[row], rs = a.rstd[a.rows + row];
     const float grow = GATE == kRow ? to_f32(((const T*)a.gate)[row]) : 1.f;
-    float hhat[PPT][VEC], shat[PPT][VEC], e[PPT][VEC], dyw[PPT][VEC];
+    float hhat[VEC], shat[VEC], e[VEC], dyw[VEC], g[VEC];
+    rh_.get(at, hhat);
+    rx.get(at, shat);
+    rdy.get(at, dyw);
+    rds.get(at, e);
+    if (GATE == kElement) gate.get(at, g);
+    if (row + gridDim.x < a.rows) fetch(row + gridDim.x);
+    if (GATE == kChannel) gate.get(at, g);
+    float w[VEC], v[VEC], sum = 0.f;
+    w1.get(at, w);
+    w2.get(at, v);
 #pragma unroll
-    for (int p = 0; p < PPT; ++p) {
-      at[p].load(row_of<T>(a.h, row, cols), hhat[p]);
-      at[p].load(row_of<T>(a.x, row, cols), shat[p]);
-      at[p].load(row_of<T>(a.dy, row, cols), dyw[p]);
-      at[p].load(row_of<T>(a.ds, row, cols), e[p]);
+    for (int i = 0; i < VEC; ++i) {
+      hhat[i] *= rh;
+      if (GATE != kChannel && GATE != kElement) g[i] = grow;
+      shat[i] = (shat[i] + a.alpha * g[i] * (hhat[i] * w[i])) * rs;
+      acc2[i] += dyw[i] * shat[i];
+      dyw[i] *= v[i];
+      sum += dyw[i] * shat[i];
     }
-    float sum = 0.f;
+    const float m1 = row_sum<BLOCK>(sum, red[0]) / cols;
+    float dot = 0.f, dgrow = 0.f, dg[VEC];
 #pragma unroll
-    for (int p = 0; p < PPT; ++p) {
-      float w[VEC], g[VEC], v[VEC];
-      at[p].load(a.w1, w);
-      at[p].load(a.w2, v);
-      if (GATE == kChannel) at[p].load(a.gate, g);
-      if (GATE == kElement) at[p].load(row_of<T>(a.gate, row, cols), g);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        hhat[p][i] *= rh;
-        const float n = hhat[p][i] * w[i];
-        const float gate = GATE == kChannel || GATE == kElement ? g[i] : grow;
-        shat[p][i] = (shat[p][i] + a.alpha * gate * n) * rs;
-        acc2[p][i] += dyw[p][i] * shat[p][i];
-        dyw[p][i] *= v[i];
-        sum += dyw[p][i] * shat[p][i];
-      }
+    for (int i = 0; i < VEC; ++i) {
+      e[i] += rs * (dyw[i] - shat[i] * m1);
+      const float ae = a.alpha * e[i];
+      dyw[i] = g[i] * ae * w[i];  // dn w1 from here on
+      dot += dyw[i] * hhat[i];
+      acc1[i] += (GATE == kChannel ? ae : g[i] * ae) * hhat[i];
+      dg[i] = ae * (hhat[i] * w[i]);
+      dgrow += dg[i];
     }
-    const float m1 = block_reduce<BLOCK>(sum, SumOp(), red) / cols;
-    float dot = 0.f, dgrow = 0.f;
-#pragma unroll
-    for (int p = 0; p < PPT; ++p) {
-      float w[VEC], g[VEC], dg[VEC];
-      at[p].load(a.w1, w);
-      if (GATE == kChannel) at[p].load(a.gate, g);
-      if (GATE == kElement) at[p].load(row_of<T>(a.gate, row, cols), g);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        e[p][i] += rs * (dyw[p][i] - shat[p][i] * m1);
-        const float ae = a.alpha * e[p][i];
-        const float gate = GATE == kChannel || GATE == kElement ? g[i] : grow;
-        // dn w1, in dyw's registers
-        dyw[p][i] = gate * ae * w[i];
-        dot += dyw[p][i] * hhat[p][i];
-        acc1[p][i] += (GATE == kChannel ? ae : gate * ae) * hhat[p][i];
-        if (GATE == kRow) dgrow += ae * (hhat[p][i] * w[i]);
-        if (GATE == kElement) dg[i] = ae * (hhat[p][i] * w[i]);
-      }
-      at[p].store(row_of<T>(a.dx, row, cols), e[p]);
-      if (GATE == kElement) at[p].store(row_of<T>(a.dgate, row, cols), dg);
-    }
+    at.store(row_of<T>(a.dx, row, cols), e);
+    if (GATE == kElement) at.store(row_of<T>(a.dgate, row, cols), dg);
     if (GATE == kRow) {
-      dgrow = block_reduce<BLOCK>(dgrow, SumOp(), red);
+      dgrow = row_sum<BLOCK>(dgrow, red[2]);
       if (threadIdx.x == 0) ((T*)a.dgate)[row] = from_f32<T>(dgrow);
     }
-    const float m2 = block_reduce<BLOCK>(dot, SumOp(), red) / cols;
+    const float m2 = row_sum<BLOCK>(dot, red[1]) / cols;
 #pragma unroll
-    for (int p = 0; p < PPT; ++p) {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) dyw[p][i] = rh * (dyw[p][i] - hhat[p][i] * m2);
-      at[p].store(row_of<T>(a.dh, row, cols), dyw[p]);
-    }
+    for (int i = 0; i < VEC; ++i) dyw[i] = rh * (dyw[i] - hhat[i] * m2);
+    at.store(row_of<T>(a.dh, row, cols), dyw);
   }
   float* part = a.part + (int64_t)blockIdx.x * 2 * cols;
-#pragma unroll
-  for (int p = 0; p < PPT; ++p) {
-    if (!at[p].in) continue;
+  if (at.in) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i)
-      if (i >= at[p].lo) {
-        part[at[p].c + i] = acc1[p][i];
-        part[cols + at[p].c + i] = acc2[p][i];
+      if (i >= at.lo) {
+        part[at.c + i] = acc1[i];
+        part[cols + at.c + i] = acc2[i];
       }
   }
 }
@@ -375,28 +380,36 @@ __global__ __launch_bounds__(kWideBlock) void block_norm_bwd_wide_kernel(NormArg
   }
 }
 
-// dw1, dw2 and a channel gate's gradient from the workgroups' partial rows: 64 columns per
-// workgroup, its rows dealt to 16 lanes of adders whose sums are added in order.
+// dw1, dw2 and a channel gate's gradient from the workgroups' partial rows: 16 columns (a
+// 64-byte run of each row) per workgroup, its rows dealt to 64 adders whose sums are added
+// in order.
+constexpr int kSumCols = 16, kSumRows = 64;
 template <typename T, int GATE>
-__global__ __launch_bounds__(1024) void block_norm_sum_kernel(NormArgs a, int parts) {
-  __shared__ float sums[2][16][64];
-  const int lane = threadIdx.x & 63, lane_row = threadIdx.x >> 6;
-  const int c = blockIdx.x * 64 + lane;
+__global__ __launch_bounds__(kSumCols * kSumRows) void block_norm_sum_kernel(NormArgs a, int parts) {
+  __shared__ float sums[2][kSumRows][kSumCols];
+  const int lane = threadIdx.x % kSumCols, adder = threadIdx.x / kSumCols;
+  const int c = blockIdx.x * kSumCols + lane;
   float s1 = 0.f, s2 = 0.f;
-  if (c < a.cols)
-    for (int p = lane_row; p < parts; p += 16) {
-      s1 += a.part[(int64_t)p * 2 * a.cols + c];
-      s2 += a.part[((int64_t)p * 2 + 1) * a.cols + c];
+  if (c < a.cols) {
+    const float* p = a.part + c;
+#pragma unroll 4
+    for (int r = adder; r < parts; r += kSumRows) {
+      s1 += p[(int64_t)r * 2 * a.cols];
+      s2 += p[((int64_t)r * 2 + 1) * a.cols];
     }
-  sums[0][lane_row][lane] = s1;
-  sums[1][lane_row][lane] = s2;
-  __syncthreads();
-  if (lane_row != 0 || c >= a.cols) return;
-#pragma unroll
-  for (int r = 1; r < 16; ++r) {
-    s1 += sums[0][r][lane];
-    s2 += sums[1][r][lane];
   }
+  sums[0][adder][lane] = s1;
+  sums[1][adder][lane] = s2;
+  __syncthreads();
+#pragma unroll
+  for (int n = kSumRows / 2; n >= 1; n /= 2) {
+    if (adder < n) {
+      sums[0][adder][lane] = s1 += sums[0][adder + n][lane];
+      sums[1][adder][lane] = s2 += sums[1][adder + n][lane];
+    }
+    __syncthreads();
+  }
+  if (adder != 0 || c >= a.cols) return;
   if (GATE == kChannel) {
     ((T*)a.dgate)[c] = from_f32<T>(s1 * to_f32(((const T*)a.w1)[c]));
     s1 *= to_f32(((const T*)a.gate)[c]);
@@ -406,32 +419,44 @@ __global__ __launch_bounds__(1024) void block_norm_sum_kernel(NormArgs a, int pa
 }
 
 constexpr int64_t kMaxCols = (int64_t)1 << 24;
-constexpr int64_t kWorkgroups = 512;
 
-int64_t parts_of(int64_t rows) { return rows < kWorkgroups ? rows : kWorkgroups; }
+// Threads of a row's workgroup: as many as packs (up to 1024 packs: 8192 16-bit columns, 4096
+// fp32), 0 where the row is too wide.
+int block_of(int64_t cols, int vec) {
+  const int64_t packs = (cols + vec - 1) / vec;
+  for (int b = 64; b <= 1024; b *= 2)
+    if (packs <= b) return b;
+  return 0;
+}
+// Workgroups of the backward, a partial row each: about 16 waves per CU, 2048 at most, whose
+// partial rows the sum kernel reads in a few us.
+int64_t parts_for(int64_t rows, int64_t cols, int vec) {
+  const int block = block_of(cols, vec);
+  const int64_t most = block ? std::min<int64_t>(2048, 256 * 1024 / block) : 512;
+  return std::min(rows, most);
+}
 
-// go(VEC, BLOCK, PPT, RAG) for a row that a workgroup's registers hold (up to 1024 packs: 8192
-// 16-bit columns, 4096 fp32), else wide(VEC).
+// go(VEC, BLOCK, RAG) for a row that a workgroup's registers hold, else wide(VEC).
 template <typename T, typename F, typename W>
 int by_shape(const NormArgs& a, F&& go, W&& wide) {
   using std::integral_constant;
   constexpr int V = 16 / (int)sizeof(T);
-  integral_constant<int, 1> one;
-  integral_constant<int, 64> wave;
-  integral_constant<int, 256> four;
-  if (a.cols < V) return go(one, wave, one, std::false_type{});
+  if (a.cols < V)
+    return go(integral_constant<int, 1>{}, integral_constant<int, 64>{}, std::false_type{});
   bool aligned = a.cols % V == 0;
   for (const void* p : {a.x, a.h, a.w1, a.gate, a.w2, (const void*)a.s, (const void*)a.y, a.ds, a.dy,
                         (const void*)a.dx, (const void*)a.dh, (const void*)a.dgate})
     aligned = aligned && aligned16(p);
   const integral_constant<int, V> vec;
-  const int packs = (a.cols + V - 1) / V;
-  if (packs > 1024) return wide(vec);
   auto by_row = [&](auto rag) -> int {
-    if (packs <= 64) return go(vec, wave, one, rag);
-    if (packs <= 256) return go(vec, four, one, rag);
-    if (packs <= 512) return go(vec, four, integral_constant<int, 2>{}, rag);
-    return go(vec, four, integral_constant<int, 4>{}, rag);
+    switch (block_of(a.cols, V)) {
+      case 64: return go(vec, integral_constant<int, 64>{}, rag);
+      case 128: return go(vec, integral_constant<int, 128>{}, rag);
+      case 256: return go(vec, integral_constant<int, 256>{}, rag);
+      case 512: return go(vec, integral_constant<int, 512>{}, rag);
+      case 1024: return go(vec, integral_constant<int, 1024>{}, rag);
+      default: return wide(vec);
+    }
   };
   return aligned ? by_row(std::false_type{}) : by_row(std::true_type{});
 }
@@ -464,7 +489,9 @@ using namespace eg;
 
 extern "C" size_t eg_block_norm_workspace_bytes(int64_t rows, int64_t cols) {
   if (rows <= 0 || cols <= 0) return 0;
-  return (size_t)parts_of(rows) * 2 * cols * sizeof(float);
+  // the narrower packs (fp32) of the dtype not known here have the wider workgroups
+  return (size_t)std::max(parts_for(rows, cols, 4), parts_for(rows, cols, 8)) * 2 * cols *
+         sizeof(float);
 }
 
 extern "C" int eg_block_norm_fwd(const void* x, const void* h, const void* post_weight,
@@ -485,10 +512,9 @@ extern "C" int eg_block_norm_fwd(const void* x, const void* h, const void* post_
   a.rows = rows, a.cols = (int)cols, a.alpha = alpha, a.eps = eps;
   return EG_DISPATCH_FLOAT(dtype, name, [&]() -> int {
     return by_gate(gate_kind, [&](auto g) {
-      return by_shape<scalar_t>(a, [&](auto vec, auto block, auto ppt, auto rag) {
-        constexpr int V = decltype(vec)::value, B = decltype(block)::value,
-                      P = decltype(ppt)::value, G = decltype(g)::value;
-        EG_LAUNCH((block_norm_fwd_kernel<scalar_t, V, B, P, decltype(rag)::value, G>),
+      return by_shape<scalar_t>(a, [&](auto vec, auto block, auto rag) {
+        constexpr int V = decltype(vec)::value, B = decltype(block)::value, G = decltype(g)::value;
+        EG_LAUNCH((block_norm_fwd_kernel<scalar_t, V, B, decltype(rag)::value, G>),
                   dim3((unsigned)rows), dim3(B), 0, as_stream(stream), a);
         return check_launch(name);
       }, [&](auto vec) {
@@ -527,15 +553,14 @@ extern "C" int eg_block_norm_bwd(const void* ds, const void* dy, const void* x, 
   a.dx = dx, a.dh = dh, a.dw1 = dpost_weight, a.dgate = dgate, a.dw2 = dpre_weight;
   a.part = (float*)workspace;
   a.rows = rows, a.cols = (int)cols, a.alpha = alpha;
-  const int parts = (int)parts_of(rows);
   return EG_DISPATCH_FLOAT(dtype, name, [&]() -> int {
+    const int parts = (int)parts_for(rows, cols, 16 / (int)sizeof(scalar_t));
     return by_gate(gate_kind, [&](auto g) -> int {
       constexpr int G = decltype(g)::value;
       if (rows > 0) {
-        const int rc = by_shape<scalar_t>(a, [&](auto vec, auto block, auto ppt, auto rag) {
-          constexpr int V = decltype(vec)::value, B = decltype(block)::value,
-                        P = decltype(ppt)::value;
-          EG_LAUNCH((block_norm_bwd_kernel<scalar_t, V, B, P, decltype(rag)::value, G>),
+        const int rc = by_shape<scalar_t>(a, [&](auto vec, auto block, auto rag) {
+          constexpr int V = decltype(vec)::value, B = decltype(block)::value;
+          EG_LAUNCH((block_norm_bwd_kernel<scalar_t, V, B, decltype(rag)::value, G>),
                     dim3((unsigned)parts), dim3(B), 0, as_stream(stream), a);
           return check_launch(name);
         }, [&](auto vec) {
@@ -545,8 +570,8 @@ extern "C" int eg_block_norm_bwd(const void* ds, const void* dy, const void* x, 
         });
         if (rc) return rc;
       }
-      EG_LAUNCH((block_norm_sum_kernel<scalar_t, G>), dim3((unsigned)((cols + 63) / 64)),
-                dim3(1024), 0, as_stream(stream), a, parts);
+      EG_LAUNCH((block_norm_sum_kernel<scalar_t, G>), dim3((unsigned)((cols + kSumCols - 1) / kSumCols)),
+                dim3(kSumCols * kSumRows), 0, as_stream(stream), a, parts);
       return check_launch(name);
     });
   });

@@ -74,22 +74,21 @@ struct RowPack {
   }
   __device__ __forceinline__ void store(void* row, const float (&v)[VEC]) const {
     if (!in) return;
-    if constexpr (RAG) store_ragged<T, VEC, false>((T*)row + c, lo, v);
-    else store_f32<T, VEC>((T*)row + c, v);
+    if constexpr (RAG) store_ragged<T, VEC, true>((T*)row + c, lo, v);
+    else store_vec<T, VEC, true>((T*)row + c, v);
   }
 };
 
 // Sum over the workgroup, in wave order. One barrier: a kernel gives each of its sums a buffer
 // of its own, and another sum's barrier lies between two uses of one.
-template <int BLOCK>
 __device__ __forceinline__ float row_sum(float v, float* lds) {
   v = wave_reduce(v, SumOp());
-  if constexpr (BLOCK == 64) return v;
+  const int waves = blockDim.x / 64;
+  if (waves == 1) return v;
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
   float r = lds[0];
-#pragma unroll
-  for (int w = 1; w < BLOCK / 64; ++w) r += lds[w];
+  for (int w = 1; w < waves; ++w) r += lds[w];
   return r;
 }
 
@@ -102,39 +101,55 @@ __device__ __forceinline__ void* row_of(void* p, int64_t row, int cols) {
   return (T*)p + row * cols;
 }
 
-// Workgroup of BLOCK threads per row, a pack per thread.
-template <typename T, int VEC, int BLOCK, bool RAG, int GATE>
-__global__ __launch_bounds__(BLOCK) void block_norm_fwd_kernel(NormArgs a) {
-  __shared__ float red[2][BLOCK / 64];
+// A workgroup per row, PPT packs per thread: pack p of thread t is p * threads + t.
+constexpr int kFwdThreads = 256, kBwdThreads = 512;
+
+template <typename T, int VEC, int PPT, bool RAG, int GATE>
+__global__ __launch_bounds__(kFwdThreads) void block_norm_fwd_kernel(NormArgs a) {
+  __shared__ float red[2][kFwdThreads / 64];
   const int64_t row = blockIdx.x;
   const int cols = a.cols;
-  RowPack<T, VEC, RAG> at;
-  at.set(threadIdx.x, cols);
-  float h[VEC], x[VEC], w[VEC], g[VEC], w2[VEC];
-  at.load(row_of<T>(a.h, row, cols), h);
-  at.load(row_of<T>(a.x, row, cols), x);
-  at.load(a.w1, w);
-  if (GATE == kChannel) at.load(a.gate, g);
-  if (GATE == kElement) at.load(row_of<T>(a.gate, row, cols), g);
-  at.load(a.w2, w2);
+  RowPack<T, VEC, RAG> at[PPT];
+  float h[PPT][VEC], x[PPT][VEC];
+#pragma unroll
+  for (int p = 0; p < PPT; ++p) {
+    at[p].set(threadIdx.x + p * blockDim.x, cols);
+    at[p].load(row_of<T>(a.h, row, cols), h[p]);
+  }
+#pragma unroll
+  for (int p = 0; p < PPT; ++p) at[p].load(row_of<T>(a.x, row, cols), x[p]);
   float scale = a.alpha;
   if (GATE == kRow) scale *= to_f32(((const T*)a.gate)[row]);
   float sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) sum += h[i] * h[i];
-  const float rh = rsqrtf(row_sum<BLOCK>(sum, red[0]) / cols + a.eps);
+  for (int p = 0; p < PPT; ++p)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) sum += h[p][i] * h[p][i];
+  const float rh = rsqrtf(row_sum(sum, red[0]) / cols + a.eps);
   sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    const float n = h[i] * rh * w[i];
-    x[i] += GATE == kChannel || GATE == kElement ? scale * g[i] * n : scale * n;
-    sum += x[i] * x[i];
-  }
-  at.store(row_of<T>(a.s, row, cols), x);
-  const float rs = rsqrtf(row_sum<BLOCK>(sum, red[1]) / cols + a.eps);
+  for (int p = 0; p < PPT; ++p) {
+    float w[VEC], g[VEC];
+    at[p].load(a.w1, w);
+    if (GATE == kChannel) at[p].load(a.gate, g);
+    if (GATE == kElement) at[p].load(row_of<T>(a.gate, row, cols), g);
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) x[i] = x[i] * rs * w2[i];
-  at.store(row_of<T>(a.y, row, cols), x);
+    for (int i = 0; i < VEC; ++i) {
+      const float n = h[p][i] * rh * w[i];
+      x[p][i] += GATE == kChannel || GATE == kElement ? scale * g[i] * n : scale * n;
+      sum += x[p][i] * x[p][i];
+    }
+    at[p].store(row_of<T>(a.s, row, cols), x[p]);
+  }
+  const float rs = rsqrtf(row_sum(sum, red[1]) / cols + a.eps);
+#pragma unroll
+  for (int p = 0; p < PPT; ++p) {
+    float w[VEC];
+    at[p].load(a.w2, w);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) x[p][i] = x[p][i] * rs * w[i];
+    at[p].store(row_of<T>(a.y, row, cols), x[p]);
+  }
   if (threadIdx.x == 0) {
     a.rstd[row] = rh;
     a.rstd[a.rows + row] = rs;
@@ -142,95 +157,135 @@ __global__ __launch_bounds__(BLOCK) void block_norm_fwd_kernel(NormArgs a) {
 }
 
 // A row's packs as they lie in memory: the backward loads the next row's while it works on
-// this one's, in a quarter (16-bit types: half) of the registers that fp32 values take.
-template <typename T, int VEC, bool RAG>
-struct RawPack {
-  Pack<T, VEC> v;
-  __device__ __forceinline__ void load(const RowPack<T, VEC, RAG>& at, const void* row) {
-    if (!at.in) return;
-    if constexpr (RAG) v = load_ragged_raw<T, VEC, false>((const T*)row + at.c);
-    else v = *reinterpret_cast<const Pack<T, VEC>*>((const T*)row + at.c);
-  }
-  __device__ __forceinline__ void get(const RowPack<T, VEC, RAG>& at, float (&f)[VEC]) const {
+// this one's, in half the registers (16-bit types) that fp32 values take.
+template <typename T, int VEC, int PPT, bool RAG, bool NT>
+struct RawRow {
+  Pack<T, VEC> v[PPT];
+  __device__ __forceinline__ void load(const RowPack<T, VEC, RAG> (&at)[PPT], const void* row) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) f[i] = at.in && i >= at.lo ? to_f32(v.v[i]) : 0.f;
+    for (int p = 0; p < PPT; ++p) {
+      if (!at[p].in) continue;
+      if constexpr (RAG || NT) v[p] = load_ragged_raw<T, VEC, NT>((const T*)row + at[p].c);
+      else v[p] = *reinterpret_cast<const Pack<T, VEC>*>((const T*)row + at[p].c);
+    }
+  }
+  __device__ __forceinline__ void get(const RowPack<T, VEC, RAG> (&at)[PPT], int p,
+                                      float (&f)[VEC]) const {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) f[i] = at[p].in && i >= at[p].lo ? to_f32(v[p].v[i]) : 0.f;
   }
 };
 
-template <typename T, int VEC, int BLOCK, bool RAG, int GATE>
-__global__ __launch_bounds__(BLOCK) void block_norm_bwd_kernel(NormArgs a) {
-  __shared__ float red[3][BLOCK / 64];
+// One pack per thread up to 256 packs, then two, on up to 512 threads: a CU's registers hold
+// the values of three or four rows, and of the rows after them, either way.
+template <typename T, int VEC, int PPT, bool RAG, bool NT, int GATE>
+__global__ __launch_bounds__(PPT == 1 ? kBwdThreads / 2 : kBwdThreads,
+                             PPT == 2 ? 2 : RAG ? 3 : 4) void block_norm_bwd_kernel(NormArgs a) {
+  __shared__ float red[3][kBwdThreads / 64];
   const int cols = a.cols;
-  RowPack<T, VEC, RAG> at;
-  at.set(threadIdx.x, cols);
-  RawPack<T, VEC, RAG> w1, w2, gate, rh_, rx, rdy, rds;
+  RowPack<T, VEC, RAG> at[PPT];
+#pragma unroll
+  for (int p = 0; p < PPT; ++p) at[p].set(threadIdx.x + p * blockDim.x, cols);
+  RawRow<T, VEC, PPT, RAG, false> w1, w2, gate;
+  RawRow<T, VEC, PPT, RAG, NT> rawg, rawh, rawx, rawdy, rawds;
   w1.load(at, a.w1);
   w2.load(at, a.w2);
   if (GATE == kChannel) gate.load(at, a.gate);
   auto fetch = [&](int64_t row) {
-    rh_.load(at, row_of<T>(a.h, row, cols));
-    rx.load(at, row_of<T>(a.x, row, cols));
-    rdy.load(at, row_of<T>(a.dy, row, cols));
-    rds.load(at, row_of<T>(a.ds, row, cols));
-    if (GATE == kElement) gate.load(at, row_of<T>(a.gate, row, cols));
+    rawh.load(at, row_of<T>(a.h, row, cols));
+    rawx.load(at, row_of<T>(a.x, row, cols));
+    rawdy.load(at, row_of<T>(a.dy, row, cols));
+    rawds.load(at, row_of<T>(a.ds, row, cols));
+    if (GATE == kElement) rawg.load(at, row_of<T>(a.gate, row, cols));
   };
-  float acc1[VEC], acc2[VEC];
+  // the gate of a pack's columns in the present row
+  auto gates = [&](int p, float grow, float (&g)[VEC]) {
+    if constexpr (GATE == kChannel || GATE == kElement) {
+      gate.get(at, p, g);
+    } else {
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) acc1[i] = acc2[i] = 0.f;
+      for (int i = 0; i < VEC; ++i) g[i] = grow;
+    }
+  };
+  float acc1[PPT][VEC], acc2[PPT][VEC];
+#pragma unroll
+  for (int p = 0; p < PPT; ++p)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) acc1[p][i] = acc2[p][i] = 0.f;
   fetch(blockIdx.x);
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const float rh = a.rstd[row], rs = a.rstd[a.rows + row];
     const float grow = GATE == kRow ? to_f32(((const T*)a.gate)[row]) : 1.f;
-    float hhat[VEC], shat[VEC], e[VEC], dyw[VEC], g[VEC];
-    rh_.get(at, hhat);
-    rx.get(at, shat);
-    rdy.get(at, dyw);
-    rds.get(at, e);
-    if (GATE == kElement) gate.get(at, g);
+    float hhat[PPT][VEC], shat[PPT][VEC], e[PPT][VEC], dyw[PPT][VEC];
+#pragma unroll
+    for (int p = 0; p < PPT; ++p) {
+      rawh.get(at, p, hhat[p]);
+      rawx.get(at, p, shat[p]);
+      rawdy.get(at, p, dyw[p]);
+      rawds.get(at, p, e[p]);
+    }
+    if constexpr (GATE == kElement) {
+#pragma unroll
+      for (int p = 0; p < PPT; ++p) gate.v[p] = rawg.v[p];
+    }
     if (row + gridDim.x < a.rows) fetch(row + gridDim.x);
-    if (GATE == kChannel) gate.get(at, g);
-    float w[VEC], v[VEC], sum = 0.f;
-    w1.get(at, w);
-    w2.get(at, v);
+    float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      hhat[i] *= rh;
-      if (GATE != kChannel && GATE != kElement) g[i] = grow;
-      shat[i] = (shat[i] + a.alpha * g[i] * (hhat[i] * w[i])) * rs;
-      acc2[i] += dyw[i] * shat[i];
-      dyw[i] *= v[i];
-      sum += dyw[i] * shat[i];
-    }
-    const float m1 = row_sum<BLOCK>(sum, red[0]) / cols;
-    float dot = 0.f, dgrow = 0.f, dg[VEC];
+    for (int p = 0; p < PPT; ++p) {
+      float w[VEC], v[VEC], g[VEC];
+      w1.get(at, p, w);
+      w2.get(at, p, v);
+      gates(p, grow, g);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      e[i] += rs * (dyw[i] - shat[i] * m1);
-      const float ae = a.alpha * e[i];
-      dyw[i] = g[i] * ae * w[i];  // dn w1 from here on
-      dot += dyw[i] * hhat[i];
-      acc1[i] += (GATE == kChannel ? ae : g[i] * ae) * hhat[i];
-      dg[i] = ae * (hhat[i] * w[i]);
-      dgrow += dg[i];
+      for (int i = 0; i < VEC; ++i) {
+        hhat[p][i] *= rh;
+        shat[p][i] = (shat[p][i] + a.alpha * g[i] * (hhat[p][i] * w[i])) * rs;
+        acc2[p][i] += dyw[p][i] * shat[p][i];
+        dyw[p][i] *= v[i];
+        sum += dyw[p][i] * shat[p][i];
+      }
     }
-    at.store(row_of<T>(a.dx, row, cols), e);
-    if (GATE == kElement) at.store(row_of<T>(a.dgate, row, cols), dg);
+    const float m1 = row_sum(sum, red[0]) / cols;
+    float dot = 0.f, dgrow = 0.f;
+#pragma unroll
+    for (int p = 0; p < PPT; ++p) {
+      float w[VEC], g[VEC], dg[VEC];
+      w1.get(at, p, w);
+      gates(p, grow, g);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        e[p][i] += rs * (dyw[p][i] - shat[p][i] * m1);
+        const float ae = a.alpha * e[p][i];
+        dyw[p][i] = g[i] * ae * w[i];  // dn w1 from here on
+        dot += dyw[p][i] * hhat[p][i];
+        acc1[p][i] += (GATE == kChannel ? ae : g[i] * ae) * hhat[p][i];
+        dg[i] = ae * (hhat[p][i] * w[i]);
+        dgrow += dg[i];
+      }
+      at[p].store(row_of<T>(a.dx, row, cols), e[p]);
+      if (GATE == kElement) at[p].store(row_of<T>(a.dgate, row, cols), dg);
+    }
     if (GATE == kRow) {
-      dgrow = row_sum<BLOCK>(dgrow, red[2]);
+      dgrow = row_sum(dgrow, red[2]);
       if (threadIdx.x == 0) ((T*)a.dgate)[row] = from_f32<T>(dgrow);
     }
-    const float m2 = row_sum<BLOCK>(dot, red[1]) / cols;
+    const float m2 = row_sum(dot, red[1]) / cols;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) dyw[i] = rh * (dyw[i] - hhat[i] * m2);
-    at.store(row_of<T>(a.dh, row, cols), dyw);
+    for (int p = 0; p < PPT; ++p) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) dyw[p][i] = rh * (dyw[p][i] - hhat[p][i] * m2);
+      at[p].store(row_of<T>(a.dh, row, cols), dyw[p]);
+    }
   }
   float* part = a.part + (int64_t)blockIdx.x * 2 * cols;
-  if (at.in) {
+#pragma unroll
+  for (int p = 0; p < PPT; ++p) {
+    if (!at[p].in) continue;
 #pragma unroll
     for (int i = 0; i < VEC; ++i)
-      if (i >= at.lo) {
-        part[at.c + i] = acc1[i];
-        part[cols + at.c + i] = acc2[i];
+      if (i >= at[p].lo) {
+        part[at[p].c + i] = acc1[p][i];
+        part[cols + at[p].c + i] = acc2[p][i];
       }
   }
 }
@@ -420,45 +475,42 @@ __global__ __launch_bounds__(kSumCols * kSumRows) void block_norm_sum_kernel(Nor
 
 constexpr int64_t kMaxCols = (int64_t)1 << 24;
 
-// Threads of a row's workgroup: as many as packs (up to 1024 packs: 8192 16-bit columns, 4096
-// fp32), 0 where the row is too wide.
-int block_of(int64_t cols, int vec) {
+// Packs per thread and threads of a row's workgroup, whole waves. Rows of more than 1024 packs (8192 16-bit columns, 4096 fp32) take the wide kernels.
+constexpr int64_t kRowPacks = 1024;
+struct RowShape {
+  int ppt, threads;
+};
+RowShape row_shape(int64_t cols, int vec, bool backward) {
   const int64_t packs = (cols + vec - 1) / vec;
-  for (int b = 64; b <= 1024; b *= 2)
-    if (packs <= b) return b;
-  return 0;
+  RowShape r = {packs <= 256 ? 1 : backward || packs <= 512 ? 2 : 4, 0};
+  r.threads = (int)((packs + 64 * r.ppt - 1) / (64 * r.ppt)) * 64;
+  return r;
 }
-// Workgroups of the backward, a partial row each: about 16 waves per CU, 2048 at most, whose
-// partial rows the sum kernel reads in a few us.
+// Past this size of one tensor its six do not fit the 256 MB last-level cache twice over, and
+// the backward reads them with the non-temporal hint: bf16 [16384, 4096] step 261 -> 248 us,
+// [8192, 8192] 307 -> 294; fp16 [8192, 5000] would go 222 -> 240.
+constexpr int64_t kStreamBytes = 96 << 20;
+// Workgroups of the backward, a partial row each: about 16 waves per CU, 2048 workgroups at
+// most, whose partial rows the sum kernel reads in a few us.
 int64_t parts_for(int64_t rows, int64_t cols, int vec) {
-  const int block = block_of(cols, vec);
-  const int64_t most = block ? std::min<int64_t>(2048, 256 * 1024 / block) : 512;
-  return std::min(rows, most);
+  if (cols > kRowPacks * vec) return std::min<int64_t>(rows, 512);
+  const RowShape r = row_shape(cols, vec, true);
+  return std::min<int64_t>({rows, 2048, 256 * 1024 / r.threads / r.ppt});
 }
 
-// go(VEC, BLOCK, RAG) for a row that a workgroup's registers hold, else wide(VEC).
+// go(VEC, RAG) for a row that a workgroup's registers hold, else wide(VEC).
 template <typename T, typename F, typename W>
 int by_shape(const NormArgs& a, F&& go, W&& wide) {
   using std::integral_constant;
   constexpr int V = 16 / (int)sizeof(T);
-  if (a.cols < V)
-    return go(integral_constant<int, 1>{}, integral_constant<int, 64>{}, std::false_type{});
+  if (a.cols < V) return go(integral_constant<int, 1>{}, std::false_type{});
   bool aligned = a.cols % V == 0;
   for (const void* p : {a.x, a.h, a.w1, a.gate, a.w2, (const void*)a.s, (const void*)a.y, a.ds, a.dy,
                         (const void*)a.dx, (const void*)a.dh, (const void*)a.dgate})
     aligned = aligned && aligned16(p);
   const integral_constant<int, V> vec;
-  auto by_row = [&](auto rag) -> int {
-    switch (block_of(a.cols, V)) {
-      case 64: return go(vec, integral_constant<int, 64>{}, rag);
-      case 128: return go(vec, integral_constant<int, 128>{}, rag);
-      case 256: return go(vec, integral_constant<int, 256>{}, rag);
-      case 512: return go(vec, integral_constant<int, 512>{}, rag);
-      case 1024: return go(vec, integral_constant<int, 1024>{}, rag);
-      default: return wide(vec);
-    }
-  };
-  return aligned ? by_row(std::false_type{}) : by_row(std::true_type{});
+  if (a.cols > kRowPacks * V) return wide(vec);
+  return aligned ? go(vec, std::false_type{}) : go(vec, std::true_type{});
 }
 
 template <typename F>
@@ -512,11 +564,19 @@ extern "C" int eg_block_norm_fwd(const void* x, const void* h, const void* post_
   a.rows = rows, a.cols = (int)cols, a.alpha = alpha, a.eps = eps;
   return EG_DISPATCH_FLOAT(dtype, name, [&]() -> int {
     return by_gate(gate_kind, [&](auto g) {
-      return by_shape<scalar_t>(a, [&](auto vec, auto block, auto rag) {
-        constexpr int V = decltype(vec)::value, B = decltype(block)::value, G = decltype(g)::value;
-        EG_LAUNCH((block_norm_fwd_kernel<scalar_t, V, B, decltype(rag)::value, G>),
-                  dim3((unsigned)rows), dim3(B), 0, as_stream(stream), a);
-        return check_launch(name);
+      return by_shape<scalar_t>(a, [&](auto vec, auto rag) {
+        constexpr int V = decltype(vec)::value, G = decltype(g)::value;
+        const RowShape r = row_shape(cols, V, false);
+        auto go = [&](auto ppt) {
+          EG_LAUNCH((block_norm_fwd_kernel<scalar_t, V, decltype(ppt)::value, decltype(rag)::value, G>),
+                    dim3((unsigned)rows), dim3(r.threads), 0, as_stream(stream), a);
+          return check_launch(name);
+        };
+        if constexpr (V > 1) {
+          if (r.ppt == 4) return go(std::integral_constant<int, 4>{});
+          if (r.ppt == 2) return go(std::integral_constant<int, 2>{});
+        }
+        return go(std::integral_constant<int, 1>{});
       }, [&](auto vec) {
         constexpr int V = decltype(vec)::value, G = decltype(g)::value;
         EG_LAUNCH((block_norm_fwd_wide_kernel<scalar_t, V, G>), dim3((unsigned)rows),
@@ -558,11 +618,21 @@ extern "C" int eg_block_norm_bwd(const void* ds, const void* dy, const void* x, 
     return by_gate(gate_kind, [&](auto g) -> int {
       constexpr int G = decltype(g)::value;
       if (rows > 0) {
-        const int rc = by_shape<scalar_t>(a, [&](auto vec, auto block, auto rag) {
-          constexpr int V = decltype(vec)::value, B = decltype(block)::value;
-          EG_LAUNCH((block_norm_bwd_kernel<scalar_t, V, B, decltype(rag)::value, G>),
-                    dim3((unsigned)parts), dim3(B), 0, as_stream(stream), a);
-          return check_launch(name);
+        const int rc = by_shape<scalar_t>(a, [&](auto vec, auto rag) {
+          constexpr int V = decltype(vec)::value;
+          const RowShape r = row_shape(cols, V, true);
+          auto go = [&](auto ppt, auto nt) {
+            EG_LAUNCH((block_norm_bwd_kernel<scalar_t, V, decltype(ppt)::value,
+                                             decltype(rag)::value, decltype(nt)::value, G>),
+                      dim3((unsigned)parts), dim3(r.threads), 0, as_stream(stream), a);
+            return check_launch(name);
+          };
+          if constexpr (V > 1) {
+            if (r.ppt == 2 && rows * cols * (int64_t)sizeof(scalar_t) > kStreamBytes)
+              return go(std::integral_constant<int, 2>{}, std::true_type{});
+            if (r.ppt == 2) return go(std::integral_constant<int, 2>{}, std::false_type{});
+          }
+          return go(std::integral_constant<int, 1>{}, std::false_type{});
         }, [&](auto vec) {
           EG_LAUNCH((block_norm_bwd_wide_kernel<scalar_t, decltype(vec)::value, G>),
                     dim3((unsigned)parts), dim3(kWideBlock), 0, as_stream(stream), a);

@@ -13,16 +13,21 @@
 // it for all of its heads, so no table is stored, gathered or read.
 //
 // Layout: q [tokens, heads_q, head_dim] and k [tokens, heads_k, head_dim], head_dim
-// contiguous, other strides free; outputs contiguous. A thread owns a (token, chunk of VEC
-// pairs) and serves groups of four heads, the group's loads issued together; the heads'
-// groups are dealt out along grid y as far as that fills the chip.
+// contiguous, other strides free; outputs contiguous. A thread owns a chunk of VEC pairs of one
+// token in HPT heads, `lanes` apart in the list of q's heads and then k's, so neighbouring
+// threads read neighbouring heads of a token, and all of a thread's loads are issued before
+// its sines. (With neighbouring threads on neighbouring tokens instead, a wave's load is
+// eight runs of 128 bytes a token's 8 KB apart: q and k of 32768 tokens, 32 + 8 heads of 128,
+// forward and backward 304 us against @US@.)
 #include "eg_common.hpp"
+
+#include <algorithm>
+#include <type_traits>
 
 namespace eg {
 namespace {
 
 constexpr int kBlock = 256;
-constexpr int kHeads = 4;  // heads whose loads are in flight together
 
 struct RotaryArgs {
   const void *q, *k;
@@ -31,85 +36,119 @@ struct RotaryArgs {
   const double* freq;
   int64_t tokens, q_token, q_head, k_token, k_head;
   int heads_q, heads_k, head_dim, pairs, pos64;
+  int lanes, per_block;  // threads along the heads; tokens of a workgroup
   float amp, sign;
 };
 
+template <typename T, int VEC>
+__device__ __forceinline__ Pack<T, VEC> read(const T* p) {
+  return *reinterpret_cast<const Pack<T, VEC>*>(p);
+}
+// Results are written past the caches (whole 16-byte packs): each is touched once.
+template <typename T, int VEC>
+__device__ __forceinline__ void write(T* p, const Pack<T, VEC>& v) {
+  if constexpr (sizeof(T) * VEC == 16) {
+    typedef unsigned int words __attribute__((ext_vector_type(4)));
+    words raw;
+    __builtin_memcpy(&raw, &v, 16);
+    __builtin_nontemporal_store(raw, reinterpret_cast<words*>(p));
+  } else {
+    *reinterpret_cast<Pack<T, VEC>*>(p) = v;
+  }
+}
+
 // Chunks of a head: pairs / VEC of them rotate 2 VEC columns, the rest copy VEC each.
-template <typename T, int VEC, bool INTER>
+template <typename T, int VEC, int HPT, bool INTER>
 __global__ __launch_bounds__(kBlock) void rotary_kernel(RotaryArgs a) {
-  const int turned = a.pairs / VEC, chunks = turned + (a.head_dim - 2 * a.pairs) / VEC;
-  const int64_t idx = (int64_t)blockIdx.x * kBlock + threadIdx.x;
-  const int64_t t = idx / chunks;
-  if (t >= a.tokens) return;
-  const int ch = (int)(idx - t * chunks);
-  const bool turn = ch < turned;
+  const unsigned turned = a.pairs / VEC, chunks = turned + (a.head_dim - 2 * a.pairs) / VEC;
+  const unsigned per = chunks * a.lanes;  // threads of a token
+  const unsigned e = blockIdx.y * kBlock + threadIdx.x, tl = e / per, in = e - tl * per;
+  const int64_t t = (int64_t)blockIdx.x * a.per_block + tl;
+  if ((int)tl >= a.per_block || t >= a.tokens) return;
+  const int hl = in / chunks, ch = in - hl * chunks;
+  const bool turn = ch < (int)turned;
   // columns of the chunk's two packs (a copying chunk has the first alone)
-  const int c1 = !turn ? 2 * a.pairs + (ch - turned) * VEC : INTER ? 2 * ch * VEC : ch * VEC;
+  const int c1 = !turn ? 2 * a.pairs + (ch - (int)turned) * VEC : INTER ? 2 * ch * VEC : ch * VEC;
   const int c2 = !turn ? c1 : INTER ? c1 + VEC : c1 + a.pairs;
+  Pack<T, VEC> x1[HPT], x2[HPT];
+  T* dst[HPT];
+#pragma unroll
+  for (int j = 0; j < HPT; ++j) {
+    const int h = hl + j * a.lanes, hk = h - a.heads_q;
+    const bool isq = hk < 0;
+    dst[j] = nullptr;
+    if (hk >= a.heads_k) continue;
+    const T* src = isq ? (const T*)a.q + t * a.q_token + h * a.q_head
+                       : (const T*)a.k + t * a.k_token + hk * a.k_head;
+    dst[j] = isq ? (T*)a.qo + (t * a.heads_q + h) * a.head_dim
+                 : (T*)a.ko + (t * a.heads_k + hk) * a.head_dim;
+    x1[j] = read<T, VEC>(src + c1);
+    if (turn) x2[j] = read<T, VEC>(src + c2);
+  }
+  if (!turn) {
+#pragma unroll
+    for (int j = 0; j < HPT; ++j)
+      if (dst[j]) write(dst[j] + c1, x1[j]);
+    return;
+  }
   float cs[VEC], sn[VEC];
-  if (turn) {
-    const double pos = a.pos64 ? (double)((const int64_t*)a.pos)[t] : (double)((const int*)a.pos)[t];
+  const double pos = a.pos64 ? (double)((const int64_t*)a.pos)[t] : (double)((const int*)a.pos)[t];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    // explicit fma, here and below: every width of packs gives the same bits
+    const double f = a.freq[ch * VEC + i] * 0.15915494309189533577;
+    const double rest = __builtin_fma(pos, f, -rint(pos * f)), quarter = rint(4.0 * rest);
+    float s0, c0;
+    sincospif(2.f * (float)__builtin_fma(-0.25, quarter, rest), &s0, &c0);
+    const int n = (int)quarter & 3;  // s0, c0 turned by n quarters
+    const float s1 = n & 1 ? c0 : s0, c1 = n & 1 ? s0 : c0;
+    cs[i] = a.amp * ((n + 1) & 2 ? -c1 : c1);
+    sn[i] = a.amp * a.sign * (n & 2 ? -s1 : s1);
+  }
+#pragma unroll
+  for (int j = 0; j < HPT; ++j) {
+    if (!dst[j]) continue;
+    Pack<T, VEC> y1, y2;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      const double turns = pos * (a.freq[ch * VEC + i] * 0.15915494309189533577);
-      const double rest = turns - rint(turns), quarter = rint(4.0 * rest);
-      float s0, c0;
-      sincospif(2.f * (float)(rest - 0.25 * quarter), &s0, &c0);
-      const int n = (int)quarter & 3;  // s0, c0 turned by n quarters
-      const float s1 = n & 1 ? c0 : s0, c1 = n & 1 ? s0 : c0;
-      cs[i] = a.amp * ((n + 1) & 2 ? -c1 : c1);
-      sn[i] = a.amp * a.sign * (n & 2 ? -s1 : s1);
+      // pair i: elements i of the two packs, or 2i and 2i + 1 of the two as one run
+      const int p = INTER ? 2 * i : i, r = INTER ? 2 * i + 1 : i;
+      const float u = to_f32(INTER && p >= VEC ? x2[j].v[p % VEC] : x1[j].v[p % VEC]);
+      const float v = to_f32(!INTER || r >= VEC ? x2[j].v[r % VEC] : x1[j].v[r % VEC]);
+      float fu = __builtin_fmaf(u, cs[i], -(v * sn[i])), fv = __builtin_fmaf(v, cs[i], u * sn[i]);
+      // fp32 values: not to be merged with the conversion into v_fma_mix, which rounds once
+      asm("" : "+v"(fu), "+v"(fv));
+      const T yu = from_f32<T>(fu), yv = from_f32<T>(fv);
+      if (INTER && p >= VEC) y2.v[p % VEC] = yu; else y1.v[p % VEC] = yu;
+      if (!INTER || r >= VEC) y2.v[r % VEC] = yv; else y1.v[r % VEC] = yv;
     }
-  }
-  const int groups_q = (a.heads_q + kHeads - 1) / kHeads;
-  const int groups = groups_q + (a.heads_k + kHeads - 1) / kHeads;
-  for (int g = blockIdx.y; g < groups; g += gridDim.y) {
-    const bool isq = g < groups_q;
-    const int heads = isq ? a.heads_q : a.heads_k, h0 = (isq ? g : g - groups_q) * kHeads;
-    const int64_t step = isq ? a.q_head : a.k_head;
-    const T* src = (const T*)(isq ? a.q : a.k) + t * (isq ? a.q_token : a.k_token) + h0 * step;
-    T* dst = (T*)(isq ? a.qo : a.ko) + (t * heads + h0) * a.head_dim;
-    Pack<T, VEC> x1[kHeads], x2[kHeads];
-#pragma unroll
-    for (int j = 0; j < kHeads; ++j)
-      if (h0 + j < heads) {
-        x1[j] = *reinterpret_cast<const Pack<T, VEC>*>(src + j * step + c1);
-        if (turn) x2[j] = *reinterpret_cast<const Pack<T, VEC>*>(src + j * step + c2);
-      }
-#pragma unroll
-    for (int j = 0; j < kHeads; ++j) {
-      if (h0 + j >= heads) continue;
-      T* row = dst + (int64_t)j * a.head_dim;
-      if (turn) {
-        Pack<T, VEC> y1, y2;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          // pair i: elements i of the two packs, or 2i and 2i + 1 of the two as one run
-          const int e = INTER ? 2 * i : i, f = INTER ? 2 * i + 1 : i;
-          const float u = to_f32(INTER && e >= VEC ? x2[j].v[e % VEC] : x1[j].v[e % VEC]);
-          const float v = to_f32(!INTER || f >= VEC ? x2[j].v[f % VEC] : x1[j].v[f % VEC]);
-          const T yu = from_f32<T>(u * cs[i] - v * sn[i]), yv = from_f32<T>(v * cs[i] + u * sn[i]);
-          if (INTER && e >= VEC) y2.v[e % VEC] = yu; else y1.v[e % VEC] = yu;
-          if (!INTER || f >= VEC) y2.v[f % VEC] = yv; else y1.v[f % VEC] = yv;
-        }
-        *reinterpret_cast<Pack<T, VEC>*>(row + c1) = y1;
-        *reinterpret_cast<Pack<T, VEC>*>(row + c2) = y2;
-      } else {
-        *reinterpret_cast<Pack<T, VEC>*>(row + c1) = x1[j];
-      }
-    }
+    write(dst[j] + c1, y1);
+    write(dst[j] + c2, y2);
   }
 }
 
 template <typename T, int VEC, bool INTER>
-int launch(const RotaryArgs& a, hipStream_t st) {
+int launch(RotaryArgs a, hipStream_t st) {
   const int64_t chunks = a.pairs / VEC + (a.head_dim - 2 * a.pairs) / VEC;
-  const int64_t gx = (a.tokens * chunks + kBlock - 1) / kBlock;
-  const int64_t groups = (a.heads_q + kHeads - 1) / kHeads + (a.heads_k + kHeads - 1) / kHeads;
-  if (gx > 0x7fffffffLL) { set_error("eg_rotary: grid too large"); return 1; }
-  EG_LAUNCH((rotary_kernel<T, VEC, INTER>), dim3((unsigned)gx, (unsigned)groups), dim3(kBlock), 0,
-            st, a);
-  return check_launch("eg_rotary");
+  const int64_t heads = a.heads_q + a.heads_k;
+  auto go = [&](auto hpt) {
+    constexpr int HPT = decltype(hpt)::value;
+    a.lanes = (int)((heads + HPT - 1) / HPT);
+    const int64_t per = chunks * a.lanes;
+    a.per_block = (int)std::max<int64_t>(1, kBlock / per);
+    const int64_t gx = (a.tokens + a.per_block - 1) / a.per_block, gy = (per + kBlock - 1) / kBlock;
+    if (gx > 0x7fffffffLL || gy > 65535) {
+      set_error("eg_rotary: grid too large");
+      return 1;
+    }
+    EG_LAUNCH((rotary_kernel<T, VEC, HPT, INTER>), dim3((unsigned)gx, (unsigned)gy), dim3(kBlock), 0,
+              st, a);
+    return check_launch("eg_rotary");
+  };
+  // Four heads per sine where that still leaves a thread for every lane of the chip's 1024
+  // SIMDs twice over, one where tokens are few.
+  if (a.tokens * chunks * ((heads + 3) / 4) < 131072) return go(std::integral_constant<int, 1>{});
+  return go(std::integral_constant<int, 4>{});
 }
 
 // The widest pack (at most 16 bytes) that divides the halves, the copied columns and every

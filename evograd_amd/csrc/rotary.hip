@@ -9,16 +9,15 @@
 // Angles: a position of a long context times a frequency leaves few bits of an fp32 product
 // behind its whole turns (at position 131072 an fp32 angle is off by 0.004), so the turns
 // pos * freq / 2 pi are formed in fp64 and reduced there to an eighth of a turn; only that
-// remainder is rounded to fp32 for the sine and cosine. A thread does that once for its pairs of a token and uses
-// it for all of its heads, so no table is stored, gathered or read.
+// remainder is rounded to fp32 for the sine and cosine. A workgroup forms them once for its
+// tokens, into LDS, while its loads are on their way, and uses them for every head.
 //
 // Layout: q [tokens, heads_q, head_dim] and k [tokens, heads_k, head_dim], head_dim
 // contiguous, other strides free; outputs contiguous. A thread owns a chunk of VEC pairs of one
 // token in HPT heads, `lanes` apart in the list of q's heads and then k's, so neighbouring
-// threads read neighbouring heads of a token, and all of a thread's loads are issued before
-// its sines. (With neighbouring threads on neighbouring tokens instead, a wave's load is
+// threads read neighbouring heads of a token. (With neighbouring threads on neighbouring tokens instead, a wave's load is
 // eight runs of 128 bytes a token's 8 KB apart: q and k of 32768 tokens, 32 + 8 heads of 128,
-// forward and backward 304 us against @US@.)
+// forward and backward 304 us against 254.)
 #include "eg_common.hpp"
 
 #include <algorithm>
@@ -27,7 +26,7 @@
 namespace eg {
 namespace {
 
-constexpr int kBlock = 256;
+constexpr int kMostThreads = 512;
 
 struct RotaryArgs {
   const void *q, *k;
@@ -57,19 +56,29 @@ __device__ __forceinline__ void write(T* p, const Pack<T, VEC>& v) {
   }
 }
 
-// Chunks of a head: pairs / VEC of them rotate 2 VEC columns, the rest copy VEC each.
+// Chunks of a head: pairs / VEC of them rotate two packs of VEC columns, the rest copy one
+// 16-byte pack or two narrower ones.
+template <typename T, int VEC> constexpr int kCopies = VEC * sizeof(T) == 16 ? 1 : 2;
+template <typename T, int VEC>
+__host__ __device__ inline int chunks_of(int head_dim, int pairs) {
+  constexpr int COPY = kCopies<T, VEC> * VEC;
+  return pairs / VEC + (head_dim - 2 * pairs + COPY - 1) / COPY;
+}
 template <typename T, int VEC, int HPT, bool INTER>
-__global__ __launch_bounds__(kBlock) void rotary_kernel(RotaryArgs a) {
-  const unsigned turned = a.pairs / VEC, chunks = turned + (a.head_dim - 2 * a.pairs) / VEC;
+__global__ __launch_bounds__(kMostThreads) void rotary_kernel(RotaryArgs a) {
+  const unsigned turned = a.pairs / VEC, chunks = chunks_of<T, VEC>(a.head_dim, a.pairs);
   const unsigned per = chunks * a.lanes;  // threads of a token
-  const unsigned e = blockIdx.y * kBlock + threadIdx.x, tl = e / per, in = e - tl * per;
+  const unsigned e = blockIdx.y * blockDim.x + threadIdx.x, tl = e / per, in = e - tl * per;
   const int64_t t = (int64_t)blockIdx.x * a.per_block + tl;
-  if ((int)tl >= a.per_block || t >= a.tokens) return;
+  const bool live = (int)tl < a.per_block && t < a.tokens;
   const int hl = in / chunks, ch = in - hl * chunks;
   const bool turn = ch < (int)turned;
-  // columns of the chunk's two packs (a copying chunk has the first alone)
-  const int c1 = !turn ? 2 * a.pairs + (ch - (int)turned) * VEC : INTER ? 2 * ch * VEC : ch * VEC;
-  const int c2 = !turn ? c1 : INTER ? c1 + VEC : c1 + a.pairs;
+  // columns of the chunk's packs
+  const int c1 = !turn   ? 2 * a.pairs + (ch - (int)turned) * (kCopies<T, VEC> * VEC)
+                 : INTER ? 2 * ch * VEC
+                         : ch * VEC;
+  const int c2 = turn && !INTER ? c1 + a.pairs : c1 + VEC;
+  const bool two = turn || (kCopies<T, VEC> == 2 && c2 < a.head_dim);
   Pack<T, VEC> x1[HPT], x2[HPT];
   T* dst[HPT];
 #pragma unroll
@@ -77,33 +86,47 @@ __global__ __launch_bounds__(kBlock) void rotary_kernel(RotaryArgs a) {
     const int h = hl + j * a.lanes, hk = h - a.heads_q;
     const bool isq = hk < 0;
     dst[j] = nullptr;
-    if (hk >= a.heads_k) continue;
+    if (!live || hk >= a.heads_k) continue;
     const T* src = isq ? (const T*)a.q + t * a.q_token + h * a.q_head
                        : (const T*)a.k + t * a.k_token + hk * a.k_head;
     dst[j] = isq ? (T*)a.qo + (t * a.heads_q + h) * a.head_dim
                  : (T*)a.ko + (t * a.heads_k + hk) * a.head_dim;
     x1[j] = read<T, VEC>(src + c1);
-    if (turn) x2[j] = read<T, VEC>(src + c2);
+    if (two) x2[j] = read<T, VEC>(src + c2);
   }
-  if (!turn) {
-#pragma unroll
-    for (int j = 0; j < HPT; ++j)
-      if (dst[j]) write(dst[j] + c1, x1[j]);
-    return;
-  }
-  float cs[VEC], sn[VEC];
-  const double pos = a.pos64 ? (double)((const int64_t*)a.pos)[t] : (double)((const int*)a.pos)[t];
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) {
+  // (cos, sin) of the workgroup's tokens, while the packs are on their way
+  extern __shared__ float2 table[];
+  const int64_t t0 = (int64_t)blockIdx.x * a.per_block;
+  for (int i = threadIdx.x; i < a.per_block * a.pairs; i += blockDim.x) {
+    const int64_t tok = min(t0 + i / a.pairs, a.tokens - 1);
+    const double pos =
+        a.pos64 ? (double)((const int64_t*)a.pos)[tok] : (double)((const int*)a.pos)[tok];
     // explicit fma, here and below: every width of packs gives the same bits
-    const double f = a.freq[ch * VEC + i] * 0.15915494309189533577;
+    const double f = a.freq[i % a.pairs] * 0.15915494309189533577;
     const double rest = __builtin_fma(pos, f, -rint(pos * f)), quarter = rint(4.0 * rest);
     float s0, c0;
     sincospif(2.f * (float)__builtin_fma(-0.25, quarter, rest), &s0, &c0);
     const int n = (int)quarter & 3;  // s0, c0 turned by n quarters
     const float s1 = n & 1 ? c0 : s0, c1 = n & 1 ? s0 : c0;
-    cs[i] = a.amp * ((n + 1) & 2 ? -c1 : c1);
-    sn[i] = a.amp * a.sign * (n & 2 ? -s1 : s1);
+    table[i] = make_float2(a.amp * ((n + 1) & 2 ? -c1 : c1), a.amp * a.sign * (n & 2 ? -s1 : s1));
+  }
+  __syncthreads();
+  if (!live) return;
+  if (!turn) {
+#pragma unroll
+    for (int j = 0; j < HPT; ++j) {
+      if (!dst[j]) continue;
+      write(dst[j] + c1, x1[j]);
+      if (two) write(dst[j] + c2, x2[j]);
+    }
+    return;
+  }
+  float cs[VEC], sn[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    const float2 e = table[tl * a.pairs + ch * VEC + i];
+    cs[i] = e.x;
+    sn[i] = e.y;
   }
 #pragma unroll
   for (int j = 0; j < HPT; ++j) {
@@ -129,26 +152,35 @@ __global__ __launch_bounds__(kBlock) void rotary_kernel(RotaryArgs a) {
 
 template <typename T, int VEC, bool INTER>
 int launch(RotaryArgs a, hipStream_t st) {
-  const int64_t chunks = a.pairs / VEC + (a.head_dim - 2 * a.pairs) / VEC;
+  const int64_t chunks = chunks_of<T, VEC>(a.head_dim, a.pairs);
   const int64_t heads = a.heads_q + a.heads_k;
   auto go = [&](auto hpt) {
     constexpr int HPT = decltype(hpt)::value;
     a.lanes = (int)((heads + HPT - 1) / HPT);
+    // As many whole tokens as fill the waves of a workgroup best, from 256 threads on; a token
+    // of more than 512 threads lies over several workgroups.
     const int64_t per = chunks * a.lanes;
-    a.per_block = (int)std::max<int64_t>(1, kBlock / per);
-    const int64_t gx = (a.tokens + a.per_block - 1) / a.per_block, gy = (per + kBlock - 1) / kBlock;
+    int64_t best = std::max<int64_t>(1, 256 / per), unused = 64;
+    for (int64_t n = best; n * per <= kMostThreads; ++n) {
+      const int64_t idle = (64 - n * per % 64) % 64;
+      if (idle < unused) best = n, unused = idle;
+    }
+    a.per_block = (int)best;
+    const int64_t used = best * per, gy = (used + kMostThreads - 1) / kMostThreads;
+    const int threads = (int)((used + 64 * gy - 1) / (64 * gy)) * 64;
+    const int64_t gx = (a.tokens + a.per_block - 1) / a.per_block;
     if (gx > 0x7fffffffLL || gy > 65535) {
       set_error("eg_rotary: grid too large");
       return 1;
     }
-    EG_LAUNCH((rotary_kernel<T, VEC, HPT, INTER>), dim3((unsigned)gx, (unsigned)gy), dim3(kBlock), 0,
-              st, a);
+    EG_LAUNCH((rotary_kernel<T, VEC, HPT, INTER>), dim3((unsigned)gx, (unsigned)gy), dim3(threads),
+              a.per_block * a.pairs * sizeof(float2), st, a);
     return check_launch("eg_rotary");
   };
-  // Four heads per sine where that still leaves a thread for every lane of the chip's 1024
-  // SIMDs twice over, one where tokens are few.
-  if (a.tokens * chunks * ((heads + 3) / 4) < 131072) return go(std::integral_constant<int, 1>{});
-  return go(std::integral_constant<int, 4>{});
+  // Two heads a thread (q and k of 32768 tokens, 32 + 8 heads of 128, forward and backward: one
+  // 270 us, two 230, four 233, eight 254), one where tokens are few.
+  if (a.tokens * chunks * ((heads + 1) / 2) < 65536) return go(std::integral_constant<int, 1>{});
+  return go(std::integral_constant<int, 2>{});
 }
 
 // The widest pack (at most 16 bytes) that divides the halves, the copied columns and every
@@ -186,9 +218,9 @@ extern "C" int eg_rotary(const void* q, const void* k, void* q_out, void* k_out,
               (long long)head_dim);
     return 1;
   }
-  if (heads_q > (1 << 16) || heads_k > (1 << 16) || head_dim > (1 << 16) ||
+  if (heads_q > (1 << 16) || heads_k > (1 << 16) || head_dim > (1 << 13) ||
       tokens > ((int64_t)1 << 32)) {
-    set_error("%s: size out of range (heads and head_dim <= 65536, tokens <= 2^32)", name);
+    set_error("%s: size out of range (heads <= 65536, head_dim <= 8192, tokens <= 2^32)", name);
     return 1;
   }
   if (!strides) { set_error("%s: null strides", name); return 1; }

@@ -6,7 +6,7 @@
 //
 // A 16-row block is a workgroup of four waves. The dK/dV walk of a key block is cut where it
 // is long against the work of the whole batch: each piece is at most 1 / kGenTarget of it (two
-// workgroups per CU), but no shorter than two steps per wave; a last kernel adds the pieces'
+// workgroups per CU), but no shorter than eight steps per wave; a last kernel adds the pieces'
 // fp32 slabs in order. No atomics: every sum has a fixed order.
 #include "attn_generic_kernel.hpp"
 #include "packed_attention.hpp"
@@ -24,7 +24,7 @@ struct WalkCut {
   int ranks, slabs;  // pieces of a kv head at most; those of them that belong to cut walks
 };
 WalkCut walk_cut(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads) {
-  const int64_t group = heads / kv_heads, steps = 2 * kGenWaves;
+  const int64_t group = heads / kv_heads, steps = 8 * kGenWaves;
   WalkCut c;
   c.least = (int)((steps + group - 1) / group);
   c.share = (float)kv_heads / kGenTarget;

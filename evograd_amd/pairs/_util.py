@@ -2,7 +2,7 @@
 
 from __future__ import annotations
 
-import ctypes
+import struct
 
 import torch
 
@@ -44,12 +44,18 @@ def head_rows(t: torch.Tensor) -> torch.Tensor:
     return t.contiguous()
 
 
-def strides_arg(*tensors: torch.Tensor):
-    """Token and head strides of [tokens, heads, head_dim] tensors as a C array; an axis of one
-    element has the step of a contiguous tensor, whatever torch notes for it."""
+def strides_arg(*tensors: torch.Tensor) -> bytes:
+    """Token and head strides of [tokens, heads, head_dim] tensors as a C array of int64; an axis
+    of one element has the step of a contiguous tensor, whatever torch notes for it."""
     steps = []
     for t in tensors:
         tokens, heads, dim = t.shape
-        steps.append(t.stride(0) if tokens > 1 else heads * dim)
-        steps.append(t.stride(1) if heads > 1 else dim)
-    return (ctypes.c_int64 * len(steps))(*steps)
+        token, head, _ = t.stride()
+        steps += (token if tokens > 1 else heads * dim, head if heads > 1 else dim)
+    return struct.pack(f"{len(steps)}q", *steps)
+
+
+def contiguous_like(t: torch.Tensor) -> torch.Tensor:
+    """An uninitialised contiguous tensor of t's shape, dtype and device (empty_like would keep
+    a strided tensor's order of axes)."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)

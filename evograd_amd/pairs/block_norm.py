@@ -68,7 +68,7 @@ def _check(x, h, post_weight, gate, pre_weight):
 def _forward(s, y, x, h, post_weight, gate, pre_weight, scale, eps):
     rows, cols = x.shape
     kind = _gate_kind(gate, rows, cols)
-    rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+    rstd = x.new_empty((2, rows), dtype=torch.float32)
     _lib.call_on(x, "eg_block_norm_fwd", _lib.ptr(x), _lib.ptr(h), _lib.ptr(post_weight),
               _lib.ptr(gate), _lib.ptr(pre_weight), _lib.ptr(s), _lib.ptr(y), _lib.ptr(rstd),
               rows, cols, kind, float(scale), float(eps), tag(x.dtype), _lib.stream_of(x))
@@ -88,7 +88,7 @@ def block_norm_forward_with_saved(x: torch.Tensor, h: torch.Tensor, post_weight:
                                   gate: torch.Tensor | None, pre_weight: torch.Tensor,
                                   scale: float = 1.0, eps: float = 1e-6):
     args = _prepare("block_norm_forward_with_saved", x, h, post_weight, gate, pre_weight)
-    out = torch.empty((2, *x.shape), dtype=x.dtype, device=x.device)
+    out = x.new_empty((2, *x.shape))
     return out, _forward(out[0], out[1], *args, scale, eps)
 
 

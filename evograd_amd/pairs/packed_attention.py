@@ -36,7 +36,8 @@ import math
 import torch
 
 from evograd_amd import _lib
-from evograd_amd.pairs._util import as_contiguous, check_same, head_rows, strides_arg, tag, workspace
+from evograd_amd.pairs._util import (as_contiguous, check_same, contiguous_like, head_rows,
+                                     strides_arg, tag, workspace)
 
 
 def _check(q, k, v, cu_seqlens):
@@ -68,8 +69,8 @@ def packed_attention_forward_with_saved(q: torch.Tensor, k: torch.Tensor, v: tor
     q, k, v = head_rows(q), head_rows(k), head_rows(v)
     cu_seqlens = as_contiguous("cu_seqlens", cu_seqlens)
     T, H, D = q.shape
-    o = torch.empty((T, H, D), dtype=q.dtype, device=q.device)
-    lse = torch.empty((H, T), dtype=torch.float32, device=q.device)
+    o = contiguous_like(q)
+    lse = q.new_empty((H, T), dtype=torch.float32)
     _lib.call_on(q, "eg_packed_attn_fwd", _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(cu_seqlens),
               _lib.ptr(o), _lib.ptr(lse), T, cu_seqlens.shape[0] - 1, H, k.shape[1], D,
               strides_arg(q, k, v), 1.0 / math.sqrt(D), tag(q.dtype), _lib.stream_of(q))
@@ -84,9 +85,7 @@ def packed_attention_backward_from_saved(do: torch.Tensor, saved):
     do = as_contiguous("do", do)
     T, H, D = q.shape
     KVH, N = k.shape[1], cu_seqlens.shape[0] - 1
-    dq = torch.empty((T, H, D), dtype=q.dtype, device=q.device)
-    dk = torch.empty((T, KVH, D), dtype=q.dtype, device=q.device)
-    dv = torch.empty((T, KVH, D), dtype=q.dtype, device=q.device)
+    dq, dk, dv = contiguous_like(q), contiguous_like(k), contiguous_like(v)
     ws = workspace(_lib.query("eg_packed_attn_workspace_bytes", T, N, H, KVH, D, tag(q.dtype)),
                    q.device)
     _lib.call_on(q, "eg_packed_attn_bwd", _lib.ptr(do), _lib.ptr(q), _lib.ptr(k), _lib.ptr(v),

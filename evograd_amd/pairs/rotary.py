@@ -34,7 +34,7 @@ import math
 import torch
 
 from evograd_amd import _lib
-from evograd_amd.pairs._util import as_contiguous, head_rows, strides_arg, tag
+from evograd_amd.pairs._util import as_contiguous, contiguous_like, head_rows, strides_arg, tag
 
 
 def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: dict | None = None,
@@ -99,25 +99,29 @@ def _check(name, x, positions, freqs):
 
 
 def _turn(name, q, k, positions, freqs, amplitude, interleaved, inverse):
-    """Rotate q, and k unless it is None."""
-    tensors = (q,) if k is None else (q, k)
-    _lib.require_gpu(name, *tensors, positions, freqs)
-    for t in tensors:
-        _check(name, t, positions, freqs)
-    if k is not None and (k.shape[2] != q.shape[2] or k.dtype != q.dtype):
-        raise ValueError(f"{name}: q and k must share head_dim and dtype")
-    tensors = tuple(head_rows(t) for t in tensors)
+    """q, and k unless it is None, rotated."""
+    if k is None:
+        _lib.require_gpu(name, q, positions, freqs)
+        _check(name, q, positions, freqs)
+    else:
+        _lib.require_gpu(name, q, k, positions, freqs)
+        _check(name, q, positions, freqs)
+        _check(name, k, positions, freqs)
+        if k.shape[2] != q.shape[2] or k.dtype != q.dtype:
+            raise ValueError(f"{name}: q and k must share head_dim and dtype")
+        k = head_rows(k)
+        ko = contiguous_like(k)
+    q = head_rows(q)
+    qo = contiguous_like(q)
     positions, freqs = as_contiguous("positions", positions), as_contiguous("freqs", freqs)
-    outs = tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in tensors)
     T, H, D = q.shape
-    two = k is not None
-    _lib.call_on(q, "eg_rotary", _lib.ptr(tensors[0]), _lib.ptr(tensors[1]) if two else None,
-              _lib.ptr(outs[0]), _lib.ptr(outs[1]) if two else None, _lib.ptr(positions),
-              int(positions.dtype == torch.int64), _lib.ptr(freqs), T, H,
-              k.shape[1] if two else 0, D, freqs.shape[0], strides_arg(*(tensors * 2)[:2]),
-              float(amplitude), int(bool(interleaved)), int(inverse), tag(q.dtype),
-              _lib.stream_of(q))
-    return outs, (positions, freqs)
+    _lib.call_on(q, "eg_rotary", q.data_ptr(), _lib.ptr(k), qo.data_ptr(),
+                 None if k is None else ko.data_ptr(), positions.data_ptr(),
+                 positions.dtype == torch.int64, freqs.data_ptr(), T, H,
+                 0 if k is None else k.shape[1], D, freqs.shape[0],
+                 strides_arg(q, q if k is None else k), amplitude, bool(interleaved), inverse,
+                 tag(q.dtype), _lib.stream_of(q))
+    return (qo,) if k is None else (qo, ko), (positions, freqs)
 
 
 def rotary_forward_with_saved(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor,

@@ -84,7 +84,8 @@ SIGNATURES: dict[str, tuple] = {
     "eg_rmsnorm_bwd_small": (_i32, [_p, _p, _p, _p, _p, _p, _i64, _i64, _i32, _p]),
     "eg_layernorm_bwd_small": (_i32, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i32, _p]),
     "eg_silu_mul": (_i32, [_p, _p, _p, _i64, _i32, _p]),
-    "eg_packed_attn_fwd": (_i32, [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _f32,
+    "eg_packed_attn_fwd_workspace_bytes": (_size, [_i64]),
+    "eg_packed_attn_fwd": (_i32, [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _f32,
                                   _i32, _p]),
     "eg_packed_attn_workspace_bytes": (_size, [_i64, _i64, _i64, _i64, _i64, _i32]),
     "eg_packed_attn_bwd": (_i32, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64,

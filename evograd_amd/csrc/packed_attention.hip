@@ -111,6 +111,11 @@ struct WalkCut {
 WalkCut walk_cut(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads) {
   WalkCut c;
   c.waves = short_seqs(tokens, seqs) ? 2 : 4;
+  if (seqs > kSearchSeqs) {  // walks are not cut
+    c.least = 1, c.share = 1.f, c.slabs = 0;
+    c.ranks = (int)packed_tiles(tokens, seqs, 32 * c.waves);
+    return c;
+  }
   const int64_t per_tile = heads / kv_heads * (32 * c.waves / kWalkRows);
   c.least = (int)((kMinSteps + per_tile - 1) / per_tile);
   c.share = (float)kv_heads / kTarget;
@@ -253,8 +258,11 @@ int mfma_fwd(const PackedAttn& a, int dtype, hipStream_t st) {
     return by_rows<D>(a, false, [&](auto hw, auto nw, auto kg) {
       constexpr int HW = decltype(hw)::value, NW = decltype(nw)::value, KG = decltype(kg)::value;
       const int64_t ranks = packed_tiles(a.seqs.tokens, a.seqs.n, 32 * NW / HW);
+      const int rows = 32 * NW / HW;
+      PackedAttn b = a;
+      if (int e = packed_plan(a.seqs, 1, &rows, a.plan, &b.seqs, st)) return e;
       EG_LAUNCH((packed_fwd_kernel<T, D, NW, KG, HW>), dim3((unsigned)(ranks * (a.heads / HW))),
-                dim3(NW * KG * 64), 0, st, a, (int)ranks, a.scale * kLog2e);
+                dim3(NW * KG * 64), 0, st, b, (int)ranks, a.scale * kLog2e);
       return check_launch("eg_packed_attn_fwd");
     });
   });
@@ -265,28 +273,108 @@ int mfma_bwd(const PackedAttn& a, int dtype, hipStream_t st) {
   return by_type(a, dtype, [&](auto tc, auto dc) {
     using T = decltype(tc);
     constexpr int D = decltype(dc)::value;
+    PackedAttn keys_of = a;
     const int rc = by_rows<D>(a, true, [&](auto hw, auto nw, auto kg) {
       constexpr int HW = decltype(hw)::value, NW = decltype(nw)::value, KG = decltype(kg)::value;
       const int64_t ranks = packed_tiles(a.seqs.tokens, a.seqs.n, 32 * NW / HW);
+      const int rows[2] = {32 * NW / HW, 32 * cut.waves};
+      PackedSeqs seqs[2];
+      if (int e = packed_plan(a.seqs, 2, rows, a.plan, seqs, st)) return e;
+      PackedAttn b = a;
+      b.seqs = seqs[0];
+      keys_of.seqs = seqs[1];
       EG_LAUNCH((packed_dq_kernel<T, D, NW, KG, HW>), dim3((unsigned)(ranks * (a.heads / HW))),
-                dim3(NW * KG * 64), 0, st, a, (int)ranks, a.scale * kLog2e);
+                dim3(NW * KG * 64), 0, st, b, (int)ranks, a.scale * kLog2e);
       return check_launch("eg_packed_attn_bwd(dq)");
     });
     if (rc) return rc;
     auto keys = [&](auto nwc) {
       constexpr int NW = decltype(nwc)::value;
       EG_LAUNCH((packed_dkdv_kernel<T, D, NW>), dim3((unsigned)(cut.ranks * a.kv_heads)),
-                dim3(NW * 64), 0, st, a, cut, a.scale * kLog2e);
+                dim3(NW * 64), 0, st, keys_of, cut, a.scale * kLog2e);
       if (int e = check_launch("eg_packed_attn_bwd(dkdv)")) return e;
+      if (cut.slabs == 0) return 0;
       EG_LAUNCH((packed_reduce_kernel<T, D, NW>), dim3((unsigned)(cut.slabs * a.kv_heads)),
-                dim3(256), 0, st, a, cut);
+                dim3(256), 0, st, keys_of, cut);
       return check_launch("eg_packed_attn_bwd(dkdv reduce)");
     };
     return cut.waves == 2 ? keys(Int<2>{}) : keys(Int<4>{});
   });
 }
 
+// One workgroup per table. Sequences go into classes by the bits of their tile count, the
+// largest class first; where a sequence stands inside its class is left to the order in which
+// the atomics come and moves no result, only which workgroup finds it.
+constexpr int kPlanThreads = 1024, kClasses = 32;
+struct PlanJob {
+  int rows[2];
+  int* table[2];
+};
+__global__ __launch_bounds__(kPlanThreads) void packed_plan_kernel(PackedSeqs p, PlanJob job) {
+  __shared__ int at[kClasses], sums[kPlanThreads / 64];
+  const int rows = job.rows[blockIdx.x], tid = threadIdx.x, lane = tid & 63;
+  int *order = job.table[blockIdx.x], *start = order + p.n;
+  auto tiles = [&](int s) {
+    int b, len;
+    seq_bounds(p, s, b, len);
+    return (int)(((unsigned)len + rows - 1) / rows);
+  };
+  auto size_class = [](int nt) { return nt ? 32 - __builtin_clz(nt) : 0; };
+  if (tid < kClasses) at[tid] = 0;
+  __syncthreads();
+  for (int s = tid; s < p.n; s += kPlanThreads) atomicAdd(&at[size_class(tiles(s))], 1);
+  __syncthreads();
+  if (tid == 0) {
+    int before = 0;
+    for (int c = kClasses - 1; c >= 0; --c) {
+      const int n = at[c];
+      at[c] = before;
+      before += n;
+    }
+  }
+  __syncthreads();
+  for (int s = tid; s < p.n; s += kPlanThreads) order[atomicAdd(&at[size_class(tiles(s))], 1)] = s;
+  __syncthreads();
+  // running count of tiles: a run of slots per thread
+  const int run = (p.n + kPlanThreads - 1) / kPlanThreads;
+  const int first = min(p.n, tid * run), last = min(p.n, first + run);
+  int mine = 0;
+  for (int i = first; i < last; ++i) mine += tiles(order[i]);
+  int upto = mine;  // inclusive over the wave
+#pragma unroll
+  for (int off = 1; off < 64; off *= 2) {
+    const int x = __shfl_up(upto, off, 64);
+    if (lane >= off) upto += x;
+  }
+  if (lane == 63) sums[tid >> 6] = upto;
+  __syncthreads();
+  int count = upto - mine;
+  for (int w = 0; w < (tid >> 6); ++w) count += sums[w];
+  for (int i = first; i < last; ++i) {
+    start[i] = count;
+    count += tiles(order[i]);
+  }
+  if (tid == kPlanThreads - 1) start[p.n] = count;
+}
+
 }  // namespace
+
+int packed_plan(const PackedSeqs& seqs, int tables, const int* rows, void* const* table,
+                PackedSeqs* out, hipStream_t st) {
+  PlanJob job = {};
+  for (int i = 0; i < tables; ++i) {
+    out[i] = seqs;
+    if (seqs.n <= kSearchSeqs) continue;
+    job.rows[i] = rows[i];
+    job.table[i] = (int*)table[i];
+    out[i].order = job.table[i];
+    out[i].start = job.table[i] + seqs.n;
+  }
+  if (seqs.n <= kSearchSeqs) return 0;
+  EG_LAUNCH(packed_plan_kernel, dim3((unsigned)tables), dim3(kPlanThreads), 0, st, seqs, job);
+  return check_launch("eg_packed_attn(plan)");
+}
+
 }  // namespace eg
 
 using namespace eg;
@@ -341,7 +429,7 @@ PackedAttn describe(const void* q, const void* k, const void* v, const int* cu, 
                     int64_t seqs, int64_t heads, int64_t kv_heads, int64_t D,
                     const int64_t* strides, float scale) {
   PackedAttn a = {};
-  a.seqs = {cu, (int)seqs, (int)tokens};
+  a.seqs = {cu, (int)seqs, (int)tokens, nullptr, nullptr};
   a.q = q, a.k = k, a.v = v;
   a.q_token = strides[0], a.q_head = strides[1];
   a.k_token = strides[2], a.k_head = strides[3];
@@ -359,16 +447,20 @@ extern "C" size_t eg_packed_attn_workspace_bytes(int64_t tokens, int64_t seqs, i
     return 0;
   const size_t generic = packed_generic_part_bytes(tokens, seqs, heads, kv_heads, head_dim);
   // rows of any alignment may come: the larger of the two where both kernels may run
-  return delta_bytes(tokens, heads) +
+  return delta_bytes(tokens, heads) + 2 * plan_bytes(seqs) +
          (mfma_sizes(head_dim, dtype) ? std::max(generic,
                                                mfma_part_bytes(tokens, seqs, heads, kv_heads, head_dim))
                                       : generic);
 }
 
+extern "C" size_t eg_packed_attn_fwd_workspace_bytes(int64_t seqs) {
+  return seqs > 0 ? plan_bytes(seqs) : 0;
+}
+
 extern "C" int eg_packed_attn_fwd(const void* q, const void* k, const void* v, const int* cu_seqlens,
-                                  void* o, float* lse, int64_t tokens, int64_t seqs, int64_t heads,
-                                  int64_t kv_heads, int64_t head_dim, const int64_t* strides,
-                                  float scale, int dtype, void* stream) {
+                                  void* o, float* lse, void* workspace, int64_t tokens,
+                                  int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                  const int64_t* strides, float scale, int dtype, void* stream) {
   static const char* name = "eg_packed_attn_fwd";
   clear_error();
   if (!strides) { set_error("%s: null strides", name); return 1; }
@@ -376,8 +468,12 @@ extern "C" int eg_packed_attn_fwd(const void* q, const void* k, const void* v, c
                           scale);
   if (check_packed(name, a, tokens, seqs, heads, kv_heads, head_dim, dtype)) return 1;
   if (tokens == 0 || heads == 0) return 0;
-  if (!q || !k || !v || !cu_seqlens || !o || !lse) { set_error("%s: null pointer", name); return 1; }
+  if (!q || !k || !v || !cu_seqlens || !o || !lse || (plan_bytes(seqs) && !workspace)) {
+    set_error("%s: null pointer", name);
+    return 1;
+  }
   a.o = o, a.lse = lse;
+  a.plan[0] = workspace;
   if (mfma_sizes(head_dim, dtype) && mfma_rows(a)) return mfma_fwd(a, dtype, as_stream(stream));
   return packed_generic_fwd(a, dtype, as_stream(stream));
 }
@@ -400,8 +496,11 @@ extern "C" int eg_packed_attn_bwd(const void* dout, const void* q, const void* k
   }
   a.o = const_cast<void*>(o), a.lse = const_cast<float*>(lse);
   a.dout = dout, a.dq = dq, a.dk = dk, a.dv = dv;
-  a.delta = (float*)workspace;
-  a.part = (float*)((char*)workspace + delta_bytes(tokens, heads));
+  char* ws = (char*)workspace;
+  a.delta = (float*)ws;
+  a.plan[0] = ws += delta_bytes(tokens, heads);
+  a.plan[1] = ws += plan_bytes(seqs);
+  a.part = (float*)(ws + plan_bytes(seqs));
   if (mfma_sizes(head_dim, dtype) && mfma_rows(a)) return mfma_bwd(a, dtype, as_stream(stream));
   return packed_generic_bwd(a, dtype, as_stream(stream));
 }

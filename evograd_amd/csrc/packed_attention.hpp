@@ -17,9 +17,19 @@ struct PackedAttn {
   const void* dout;
   void *dq, *dk, *dv;
   float *delta, *part;  // workspace
+  void* plan[2];        // plan_bytes each: for query tiles, for key tiles
   int heads, kv_heads, head_dim;
   float scale;
 };
+
+// Orders the sequences for tiles of `rows` rows into `table` (plan_bytes(n) bytes), where there
+// are so many that the kernels search a plan (packed_attention.hip), and returns seqs with it;
+// rc gets a launch error. Both tables of a backward pass in one launch.
+inline size_t plan_bytes(int64_t n) {
+  return n > kSearchSeqs ? ((size_t)(2 * n + 1) * 4 + 255) / 256 * 256 : 0;
+}
+int packed_plan(const PackedSeqs& seqs, int tables, const int* rows, void* const* table,
+                PackedSeqs* out, hipStream_t st);
 
 // packed_attn_generic.hip: any type, even head size up to 128 and strides.
 size_t packed_generic_part_bytes(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads,

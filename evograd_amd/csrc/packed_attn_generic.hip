@@ -26,6 +26,11 @@ struct WalkCut {
 WalkCut walk_cut(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads) {
   const int64_t group = heads / kv_heads, steps = 8 * kGenWaves;
   WalkCut c;
+  if (seqs > kSearchSeqs) {  // walks are not cut
+    c.least = 1, c.share = 1.f, c.slabs = 0;
+    c.ranks = (int)packed_tiles(tokens, seqs, kRows);
+    return c;
+  }
   c.least = (int)((steps + group - 1) / group);
   c.share = (float)kv_heads / kGenTarget;
   // a tile of index j makes at most 1 + j / m pieces, a cut one (j >= m) at most 2 j / m, and
@@ -160,7 +165,9 @@ size_t packed_generic_part_bytes(int64_t tokens, int64_t seqs, int64_t heads, in
          sizeof(float);
 }
 
-int packed_generic_fwd(const PackedAttn& a, int dtype, hipStream_t st) {
+int packed_generic_fwd(const PackedAttn& given, int dtype, hipStream_t st) {
+  PackedAttn a = given;
+  if (int e = packed_plan(given.seqs, 1, &kRows, given.plan, &a.seqs, st)) return e;
   const int64_t ranks = packed_tiles(a.seqs.tokens, a.seqs.n, kRows);
   return dispatch(a, dtype, false, "eg_packed_attn_fwd", [&](auto tag, auto dm, auto vec) {
     EG_LAUNCH((packed_gen_fwd_kernel<decltype(tag), decltype(dm)::value, decltype(vec)::value>),
@@ -170,7 +177,9 @@ int packed_generic_fwd(const PackedAttn& a, int dtype, hipStream_t st) {
   });
 }
 
-int packed_generic_bwd(const PackedAttn& a, int dtype, hipStream_t st) {
+int packed_generic_bwd(const PackedAttn& given, int dtype, hipStream_t st) {
+  PackedAttn a = given;  // query and key tiles are of one size: one plan
+  if (int e = packed_plan(given.seqs, 1, &kRows, given.plan, &a.seqs, st)) return e;
   const int64_t ranks = packed_tiles(a.seqs.tokens, a.seqs.n, kRows);
   const WalkCut cut = walk_cut(a.seqs.tokens, a.seqs.n, a.heads, a.kv_heads);
   return dispatch(a, dtype, true, "eg_packed_attn_bwd", [&](auto tag, auto dm, auto vec) {
@@ -183,6 +192,7 @@ int packed_generic_bwd(const PackedAttn& a, int dtype, hipStream_t st) {
     EG_LAUNCH((packed_gen_dkdv_kernel<T, DM, VEC>), dim3((unsigned)(cut.ranks * a.kv_heads)),
               dim3(kGenThreads), 0, st, a, cut);
     if (int e = check_launch("eg_packed_attn_bwd(generic dkdv)")) return e;
+    if (cut.slabs == 0) return 0;
     EG_LAUNCH((packed_gen_reduce_kernel<T>), dim3((unsigned)(cut.slabs * a.kv_heads)),
               dim3(kGenThreads), 0, st, a, cut);
     return check_launch("eg_packed_attn_bwd(generic dkdv reduce)");

@@ -14,18 +14,33 @@
 // being the same for all, so the pieces of the tiles below index j of a sequence have a
 // closed form too (Cut::below) and the search is the same.
 //
-// What it costs: two dependent loads (the bounds, from L2) and about 30 instructions a
-// halving. Up to 256 sequences the bounds stay in registers, four per lane.
+// What it costs: the bounds' load (from L2) and about 30 instructions a halving; up to
+// kSearchSeqs sequences the bounds stay in registers, four per lane. Past that every halving
+// would read them again (1024 sequences: 15 us a workgroup), so there one workgroup orders the
+// sequences by size class first (packed_plan_kernel, packed_attention.hip) and a workgroup
+// searches the running count of their tiles, 64 entries a step; walks are not cut then.
 #pragma once
 
 #include "eg_common.hpp"
 
 namespace eg {
 
+constexpr int kSearchSeqs = 256;
+
 struct PackedSeqs {
   const int* cu;  // [n + 1]
   int n, tokens;
+  // past kSearchSeqs sequences: their order [n], and the tiles before each in it [n + 1]
+  const int *order, *start;
 };
+
+// First row and length of sequence s (none for s >= n). Every bound is clamped to the tensors'
+// rows, so whatever cu holds no access leaves them.
+__device__ __forceinline__ void seq_bounds(const PackedSeqs& p, int s, int& begin, int& len) {
+  const int b = p.cu[min(s, p.n)], e = p.cu[min(s + 1, p.n)];
+  begin = min(max(b, 0), p.tokens);
+  len = min(max(e, begin), p.tokens) - begin;
+}
 
 // Tiles of `rows` rows that n sequences of `tokens` rows have at most, and one workgroup at
 // least for the rows that no sequence holds.
@@ -93,20 +108,42 @@ struct SeqTile {
   int spare;          // no tile: index past the last piece, or -1 (bounds that are no sequence's)
 };
 
+// The tile of rank `rank` by the plan: the sequences in its order, each one's tiles from its
+// last on. Wave-uniform; the search narrows [lo, hi) to a 64th a step.
+template <int ROWS>
+__device__ __forceinline__ bool find_planned(const PackedSeqs& p, int rank, SeqTile& t) {
+  const int lane = threadIdx.x & 63;
+  const int all = p.start[p.n];
+  t.piece = 0;
+  t.pieces = 1;
+  t.tile = t.tiles = 0;
+  t.spare = rank - all;
+  if (rank >= all) return false;
+  int lo = 0, hi = p.n;  // start[lo] <= rank < start[hi]
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 63) / 64, at = lo + (lane + 1) * step;
+    const bool before = at < hi && p.start[min(at, hi)] <= rank;
+    const int n = __builtin_popcountll(__builtin_amdgcn_ballot_w64(before));
+    hi = min(hi, lo + (n + 1) * step);
+    lo += n * step;
+  }
+  t.spare = -1;
+  seq_bounds(p, p.order[lo], t.begin, t.len);
+  t.tiles = (int)(((unsigned)t.len + ROWS - 1) / ROWS);
+  t.tile = t.tiles - 1 - (rank - p.start[lo]);
+  return t.tile >= 0 && t.tile < t.tiles;  // false: bounds that are no sequences'
+}
+
 // The piece of rank `rank`, or false. Called by whole waves; every lane gets the result.
 // CUT: with the batch's work known, W = the sum over all tiles of (index + 1), walks are cut
 // with m = max(least, ceil(W * share)); pass least and share > 0.
 template <int ROWS, bool CUT>
 __device__ __forceinline__ bool find_tile(const PackedSeqs& p, int rank, SeqTile& t, int least = 0,
                                           float share = 0.f) {
-  constexpr int KEEP = 4;
+  constexpr int KEEP = kSearchSeqs / 64;
   const int lane = threadIdx.x & 63;
-  // Every bound is clamped to the tensors' rows, so whatever cu holds no access leaves them.
-  auto bounds = [&](int s, int& begin, int& len) {
-    const int b = p.cu[min(s, p.n)], e = p.cu[min(s + 1, p.n)];
-    begin = min(max(b, 0), p.tokens);
-    len = min(max(e, begin), p.tokens) - begin;
-  };
+  if (p.n > kSearchSeqs) return find_planned<ROWS>(p, rank, t);
+  auto bounds = [&](int s, int& begin, int& len) { seq_bounds(p, s, begin, len); };
   auto tiles_of = [](int len) { return (int)(((unsigned)len + ROWS - 1) / ROWS); };
   int begin[KEEP], len[KEEP];
   bounds(lane, begin[0], len[0]);
@@ -122,11 +159,6 @@ __device__ __forceinline__ bool find_tile(const PackedSeqs& p, int rank, SeqTile
     if (p.n > 64) {
 #pragma unroll
       for (int c = 1; c < KEEP; ++c) f(tiles_of(len[c]));
-      for (int s0 = 64 * KEEP; s0 < p.n; s0 += 64) {
-        int b, l;
-        bounds(s0 + lane, b, l);
-        f(tiles_of(l));
-      }
     }
   };
   Cut cut{0, 0.f};
@@ -192,11 +224,6 @@ __device__ __forceinline__ bool find_tile(const PackedSeqs& p, int rank, SeqTile
 #pragma unroll
   for (int c = 1; c < KEEP; ++c)
     if (!found && 64 * c < p.n) look(begin[c], len[c]);
-  for (int s0 = 64 * KEEP; s0 < p.n && !found; s0 += 64) {
-    int b, l;
-    bounds(s0 + lane, b, l);
-    look(b, l);
-  }
   t.tiles = found ? tiles_of(t.len) : 0;
   return found;
 }

@@ -70,8 +70,8 @@ def _forward(s, y, x, h, post_weight, gate, pre_weight, scale, eps):
     kind = _gate_kind(gate, rows, cols)
     rstd = x.new_empty((2, rows), dtype=torch.float32)
     _lib.call_on(x, "eg_block_norm_fwd", _lib.ptr(x), _lib.ptr(h), _lib.ptr(post_weight),
-              _lib.ptr(gate), _lib.ptr(pre_weight), _lib.ptr(s), _lib.ptr(y), _lib.ptr(rstd),
-              rows, cols, kind, float(scale), float(eps), tag(x.dtype), _lib.stream_of(x))
+                 _lib.ptr(gate), _lib.ptr(pre_weight), _lib.ptr(s), _lib.ptr(y), _lib.ptr(rstd),
+                 rows, cols, kind, float(scale), float(eps), tag(x.dtype), _lib.stream_of(x))
     return x, h, post_weight, gate, pre_weight, rstd
 
 
@@ -111,10 +111,10 @@ def block_norm_backward_from_saved(dout, saved, scale: float = 1.0):
     dgate = None if gate is None else torch.empty_like(gate)
     ws = workspace(_lib.query("eg_block_norm_workspace_bytes", rows, cols), x.device)
     _lib.call_on(x, "eg_block_norm_bwd", _lib.ptr(ds), _lib.ptr(dy), _lib.ptr(x), _lib.ptr(h),
-              _lib.ptr(post_weight), _lib.ptr(gate), _lib.ptr(pre_weight), _lib.ptr(rstd),
-              _lib.ptr(dx), _lib.ptr(dh), _lib.ptr(dpost), _lib.ptr(dgate), _lib.ptr(dpre),
-              _lib.ptr(ws), rows, cols, _gate_kind(gate, rows, cols), float(scale), tag(x.dtype),
-              _lib.stream_of(x))
+                 _lib.ptr(post_weight), _lib.ptr(gate), _lib.ptr(pre_weight), _lib.ptr(rstd),
+                 _lib.ptr(dx), _lib.ptr(dh), _lib.ptr(dpost), _lib.ptr(dgate), _lib.ptr(dpre),
+                 _lib.ptr(ws), rows, cols, _gate_kind(gate, rows, cols), float(scale), tag(x.dtype),
+                 _lib.stream_of(x))
     return dx, dh, dpost, dgate, dpre
 
 

@@ -69,11 +69,14 @@ def packed_attention_forward_with_saved(q: torch.Tensor, k: torch.Tensor, v: tor
     q, k, v = head_rows(q), head_rows(k), head_rows(v)
     cu_seqlens = as_contiguous("cu_seqlens", cu_seqlens)
     T, H, D = q.shape
+    N = cu_seqlens.shape[0] - 1
+    nbytes = _lib.query("eg_packed_attn_fwd_workspace_bytes", N)
+    ws = workspace(nbytes, q.device) if nbytes else None
     o = contiguous_like(q)
     lse = q.new_empty((H, T), dtype=torch.float32)
-    _lib.call_on(q, "eg_packed_attn_fwd", _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(cu_seqlens),
-              _lib.ptr(o), _lib.ptr(lse), T, cu_seqlens.shape[0] - 1, H, k.shape[1], D,
-              strides_arg(q, k, v), 1.0 / math.sqrt(D), tag(q.dtype), _lib.stream_of(q))
+    _lib.call_on(q, "eg_packed_attn_fwd", _lib.ptr(q), _lib.ptr(k), _lib.ptr(v),
+                 _lib.ptr(cu_seqlens), _lib.ptr(o), _lib.ptr(lse), _lib.ptr(ws), T, N, H, k.shape[1],
+                 D, strides_arg(q, k, v), 1.0 / math.sqrt(D), tag(q.dtype), _lib.stream_of(q))
     return o, (q, k, v, o, lse, cu_seqlens)
 
 
@@ -89,7 +92,7 @@ def packed_attention_backward_from_saved(do: torch.Tensor, saved):
     ws = workspace(_lib.query("eg_packed_attn_workspace_bytes", T, N, H, KVH, D, tag(q.dtype)),
                    q.device)
     _lib.call_on(q, "eg_packed_attn_bwd", _lib.ptr(do), _lib.ptr(q), _lib.ptr(k), _lib.ptr(v),
-              _lib.ptr(cu_seqlens), _lib.ptr(o), _lib.ptr(lse), _lib.ptr(dq), _lib.ptr(dk),
-              _lib.ptr(dv), _lib.ptr(ws), T, N, H, KVH, D, strides_arg(q, k, v),
-              1.0 / math.sqrt(D), tag(q.dtype), _lib.stream_of(q))
+                 _lib.ptr(cu_seqlens), _lib.ptr(o), _lib.ptr(lse), _lib.ptr(dq), _lib.ptr(dk),
+                 _lib.ptr(dv), _lib.ptr(ws), T, N, H, KVH, D, strides_arg(q, k, v),
+                 1.0 / math.sqrt(D), tag(q.dtype), _lib.stream_of(q))
     return dq, dk, dv

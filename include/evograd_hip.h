@@ -466,15 +466,17 @@ int eg_silu_mul(const void* gate, const void* up, void* out, int64_t n, int dtyp
  * head_dim], lse fp32 [heads, tokens]. Rows that no sequence holds get o = 0 and are
  * read into no result. The bounds are read on the device alone; ones that break the
  * rules give undefined values but no access outside the tensors. fp32, bf16, fp16;
- * even head_dim up to 128. Sizes: tokens <= 2^28, (tokens / 16 + seqs) * heads < 2^30. */
+ * even head_dim up to 128. Sizes: tokens <= 2^28, (tokens / 16 + seqs) * heads < 2^30.
+ * workspace: eg_packed_attn_fwd_workspace_bytes(seqs), which is 0 up to 256 sequences. */
+size_t eg_packed_attn_fwd_workspace_bytes(int64_t seqs);
 int eg_packed_attn_fwd(const void* q, const void* k, const void* v, const int* cu_seqlens,
-                       void* o, float* lse, int64_t tokens, int64_t seqs, int64_t heads,
+                       void* o, float* lse, void* workspace, int64_t tokens, int64_t seqs, int64_t heads,
                        int64_t kv_heads, int64_t head_dim, const int64_t* strides, float scale,
                        int dtype, void* stream);
 
 /* Bytes of workspace eg_packed_attn_bwd needs: delta = rowsum(do * o), fp32 [heads,
  * tokens] rounded up to 256 bytes, and the fp32 sums of the pieces that long dK/dV walks
- * are cut into. */
+ * are cut into or, past 256 sequences, two tables of their order. */
 size_t eg_packed_attn_workspace_bytes(int64_t tokens, int64_t seqs, int64_t heads,
                                       int64_t kv_heads, int64_t head_dim, int dtype);
 

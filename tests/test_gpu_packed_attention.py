@@ -79,6 +79,12 @@ def test_batches(name, H, KVH, D, dtype):
     check(LENGTHS[name], H, KVH, D, dtype, pad=7 if name != "equal" else 0)
 
 
+@pytest.mark.parametrize("dtype,D", ((BF16, 128), (F16, 64), (F32, 32)))
+def test_thousands_of_sequences(dtype, D):
+    """Empty, one-token and longer ones, ordered by a plan on the GPU."""
+    check([1, 0, 3] * 500 + [200] + [17, 2] * 30 + [0, 0, 70], 2, 1, D, dtype, pad=11)
+
+
 @pytest.mark.parametrize("dtype,D", ((BF16, 128), (BF16, 64), (F32, 64)))
 @pytest.mark.parametrize("lengths,H,KVH", (
     ([1500], 8, 1), ([1200, 30, 600], 8, 8), ([2100, 100], 2, 1), ([900, 800, 20], 32, 8)))
@@ -227,8 +233,12 @@ def test_same_bits_on_every_run_and_on_another_stream(D, dtype):
 
 
 @pytest.mark.parametrize("D,dtype", ((128, BF16), (64, F32)))
-def test_a_captured_graph_replays_with_other_lengths(D, dtype):
+@pytest.mark.parametrize("many", (False, True))
+def test_a_captured_graph_replays_with_other_lengths(many, D, dtype):
     sets = ([100, 60, 40], [1, 199, 0], [0, 0, 150], [64, 64, 72])
+    if many:  # past what the kernels search themselves
+        sets = ([1] * 150 + [0] * 150, [0] * 299 + [200], [0, 1] * 100 + [99] + [0] * 99,
+                [150] + [0, 0] * 149 + [50])
     T = 200
     t = make([T], 4, 2, D, dtype)
     cu = bounds(sets[0])

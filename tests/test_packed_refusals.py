@@ -153,8 +153,9 @@ def test_block_norm_arguments(no_device_check):
 def test_entry_points_check_their_arguments():
     steps = (ctypes.c_int64 * 6)(16, 8, 16, 8, 16, 8)
 
-    def attention(tokens=4, seqs=1, heads=2, kv=2, dim=8, strides=steps, dtype=_lib.EG_F32, q=P):
-        _lib.call("eg_packed_attn_fwd", q, P, P, P, P, P, tokens, seqs, heads, kv, dim, strides,
+    def attention(tokens=4, seqs=1, heads=2, kv=2, dim=8, strides=steps, dtype=_lib.EG_F32, q=P,
+                  ws=None):
+        _lib.call("eg_packed_attn_fwd", q, P, P, P, P, P, ws, tokens, seqs, heads, kv, dim, strides,
                   1.0, dtype, None)
 
     for words, kw in (("negative", dict(tokens=-1)), ("negative", dict(seqs=-1)),
@@ -168,7 +169,8 @@ def test_entry_points_check_their_arguments():
                       ("out of range", dict(seqs=1 << 25)),
                       ("out of range", dict(heads=8192, kv=1)),
                       ("out of range", dict(tokens=1 << 28, heads=128, kv=128)),
-                      ("null pointer", dict(q=None))):
+                      ("null pointer", dict(q=None)),
+                      ("null pointer", dict(tokens=400, seqs=257))):
         with pytest.raises(RuntimeError, match=words):
             attention(**kw)
     attention(tokens=0, q=None)  # nothing to do is no error
@@ -216,5 +218,10 @@ def test_workspaces():
     mfma = lambda T: _lib.query("eg_packed_attn_workspace_bytes", T, 7, 32, 8, 128, _lib.EG_BF16)
     assert mfma(1 << 20) - mfma(1 << 17) == ((1 << 20) - (1 << 17)) * 32 * 4
     assert mfma(1 << 17) - al((1 << 17) * 32 * 4) == 8 * 129 * 2 * 128 * 128 * 4
+    # past 256 sequences: tables of their order, and no pieces
+    assert _lib.query("eg_packed_attn_fwd_workspace_bytes", 256) == 0
+    assert _lib.query("eg_packed_attn_fwd_workspace_bytes", 257) == al(4 * 515)
+    many = _lib.query("eg_packed_attn_workspace_bytes", 9000, 300, 8, 2, 128, _lib.EG_BF16)
+    assert many == al(9000 * 8 * 4) + 2 * al(4 * 601)
     assert _lib.query("eg_block_norm_workspace_bytes", 0, 64) == 0
     assert _lib.query("eg_block_norm_workspace_bytes", 3, 64) == 3 * 2 * 64 * 4

@@ -38,6 +38,8 @@ WalkCut walk_cut(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads) 
   const int64_t more = (kGenTarget + kv_heads - 1) / kv_heads;
   c.ranks = (int)(packed_tiles(tokens, seqs, kRows) + more);
   c.slabs = (int)std::min<int64_t>(c.ranks, 2 * more + 1);
+  // no sequence has a tile of index `least`: nothing is cut
+  if ((tokens + kRows - 1) / kRows <= c.least) c.slabs = 0;
   return c;
 }
 

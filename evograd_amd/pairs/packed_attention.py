@@ -51,7 +51,7 @@ def _check(q, k, v, cu_seqlens):
     if k.shape != v.shape or k.shape[0] != T or k.shape[2] != D:
         raise ValueError(f"{name}: k and v must be [tokens, kv_heads, head_dim] matching q "
                          f"{tuple(q.shape)}; got {tuple(k.shape)}, {tuple(v.shape)}")
-    if k.shape[1] == 0 or H % k.shape[1]:
+    if k.shape[1] == 0 or H == 0 or H % k.shape[1]:
         raise ValueError(f"{name}: {H} query heads are not a multiple of {k.shape[1]} kv heads")
     if D < 2 or D > 128 or D % 2:
         raise ValueError(f"{name}: head_dim must be even and at most 128, got {D}")

@@ -166,16 +166,16 @@ def test_values_behind_the_last_sequence_are_read_into_nothing(D, dtype, bad):
         assert torch.equal(x, y)
 
 
-@pytest.mark.parametrize("D,dtype", ((128, BF16), (64, F16), (64, F32)))
-@pytest.mark.parametrize("bad", (float("nan"), float("inf"), float("-inf")))
-@pytest.mark.parametrize("row", (0, 3, 70, 129))
-def test_a_non_finite_row_reaches_only_the_rows_that_see_it(D, dtype, bad, row):
-    lengths, at = [40, 130, 9], 40 + row
-    clean = make(lengths, 4, 2, D, dtype, seed=2)
+def reaches_only_the_rows_that_see_it(lengths, row, bad, H, KVH, D, dtype):
+    """A value of `row` of the second sequence's k, v, q and do is `bad`: everything that does
+    not depend on it is what it is without it."""
+    first, own_end, T = lengths[0], sum(lengths[:2]), sum(lengths)
+    at = first + row
+    clean = make(lengths, H, KVH, D, dtype, seed=2)
     cu = bounds(lengths)
     o_, dq_, dk_, dv_ = attention64(*clean, lengths, takes_mfma(*clean[:3]))
-    before, own, after = slice(40, at), slice(at, 170), slice(at + 1, 170)
-    others = torch.cat((torch.arange(40), torch.arange(170, 179))).cuda()
+    before, own, after = slice(first, at), slice(at, own_end), slice(at + 1, own_end)
+    others = torch.cat((torch.arange(first), torch.arange(own_end, T))).cuda()
 
     def clean_values(name, x, want, rows, cols=slice(None)):
         assert_within(name, x[rows][..., cols], want[0][rows][..., cols], want[1][rows][..., cols])
@@ -214,6 +214,21 @@ def test_a_non_finite_row_reaches_only_the_rows_that_see_it(D, dtype, bad, row):
     for rows in (after, others):
         clean_values("dk", dk, dk_, rows)
         clean_values("dv", dv, dv_, rows)
+
+
+@pytest.mark.parametrize("D,dtype", ((128, BF16), (64, F16), (64, F32)))
+@pytest.mark.parametrize("bad", (float("nan"), float("inf"), float("-inf")))
+@pytest.mark.parametrize("row", (0, 3, 70, 129))
+def test_a_non_finite_row_reaches_only_the_rows_that_see_it(D, dtype, bad, row):
+    reaches_only_the_rows_that_see_it([40, 130, 9], row, bad, 4, 2, D, dtype)
+
+
+@pytest.mark.parametrize("D,dtype", ((128, BF16), (64, BF16), (64, F32)))
+@pytest.mark.parametrize("bad", (float("nan"), float("inf")))
+@pytest.mark.parametrize("H,KVH", ((4, 1), (3, 3), (48, 12)))
+def test_a_non_finite_row_of_long_sequences(H, KVH, bad, D, dtype):
+    """Two key groups, whole and cut walks, groups of four heads and none."""
+    reaches_only_the_rows_that_see_it([350, 900, 20], 333, bad, H, KVH, D, dtype)
 
 
 @pytest.mark.parametrize("D,dtype", ((128, BF16), (64, F16), (32, F32)))

@@ -39,6 +39,7 @@ CU = torch.tensor([0, 4], dtype=torch.int32)
     ((4, 8), (4, 8), (4, 8), CU, ValueError, "tokens, heads, head_dim"),
     ((4, 4, 8), (4, 3, 8), (4, 3, 8), CU, ValueError, "not a multiple"),
     ((4, 4, 8), (4, 0, 8), (4, 0, 8), CU, ValueError, "not a multiple"),
+    ((4, 0, 8), (4, 2, 8), (4, 2, 8), CU, ValueError, "not a multiple"),
     ((4, 4, 8), (5, 2, 8), (5, 2, 8), CU, ValueError, "matching q"),
     ((4, 4, 8), (4, 2, 8), (4, 4, 8), CU, ValueError, "matching q"),
     ((4, 4, 9), (4, 2, 9), (4, 2, 9), CU, ValueError, "even"),
@@ -177,6 +178,11 @@ def test_entry_points_check_their_arguments():
     with pytest.raises(RuntimeError, match="null pointer"):
         _lib.call("eg_packed_attn_bwd", P, P, P, P, P, P, P, P, P, P, None, 4, 1, 2, 2, 8, steps,
                   1.0, _lib.EG_F32, None)
+    with pytest.raises(RuntimeError, match="16-byte aligned"):
+        _lib.call("eg_packed_attn_bwd", P, P, P, P, P, P, P, P, P, P, P + 4, 4, 1, 2, 2, 8, steps,
+                  1.0, _lib.EG_F32, None)
+    with pytest.raises(RuntimeError, match="positive multiple"):
+        attention(heads=0)
 
     def turn(tokens=4, hq=2, hk=2, dim=8, pairs=4, strides=steps, dtype=_lib.EG_F32, q=P):
         _lib.call("eg_rotary", q, P, P, P, P, 0, P, tokens, hq, hk, dim, pairs, strides, 1.0, 0, 0,
@@ -218,6 +224,9 @@ def test_workspaces():
     mfma = lambda T: _lib.query("eg_packed_attn_workspace_bytes", T, 7, 32, 8, 128, _lib.EG_BF16)
     assert mfma(1 << 20) - mfma(1 << 17) == ((1 << 20) - (1 << 17)) * 32 * 4
     assert mfma(1 << 17) - al((1 << 17) * 32 * 4) == 8 * 129 * 2 * 128 * 128 * 4
+    # no tile of index 8 (fp32, groups of 4 heads) or 1 (bf16 on MFMA): nothing to cut
+    assert _lib.query("eg_packed_attn_workspace_bytes", 128, 3, 8, 2, 32, _lib.EG_F32) == 128 * 8 * 4
+    assert _lib.query("eg_packed_attn_workspace_bytes", 128, 1, 8, 2, 128, _lib.EG_BF16) == 128 * 8 * 4
     # past 256 sequences: tables of their order, and no pieces
     assert _lib.query("eg_packed_attn_fwd_workspace_bytes", 256) == 0
     assert _lib.query("eg_packed_attn_fwd_workspace_bytes", 257) == al(4 * 515)

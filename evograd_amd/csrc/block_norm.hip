@@ -19,6 +19,13 @@
 // reductions, so each element is moved once. The backward's workgroups walk the rows in
 // steps of the grid and keep the column sums of their rows in registers; they leave one
 // partial row each, which a second kernel adds in order (no atomics).
+//
+// Kernel times, forward + backward + column sums: bf16 [16384, 4096] with a gate per channel
+// 100 + 148 + 8 us, the backward at 5.4 TB/s, behind two dependent row sums; bf16 [4099, 1538]
+// with a gate per element 14.5 + 32 + 7.4 us, the backward at 3.2 TB/s on unaligned packs; fp32
+// [64, 768] 3.8 + 4.2 + 3.4 us, launches. Without the backward's loads of the next row under
+// the present one the first took 393 us a step instead of 273, before the non-temporal
+// accesses (240 with them).
 #include "eg_common.hpp"
 
 #include <algorithm>

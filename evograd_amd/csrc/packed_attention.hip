@@ -14,7 +14,7 @@
 // Rounding: scores, softmax statistics, dP and every sum are fp32. P and dS are rounded to the
 // tensors' 16 bits before their products, which take both operands in one type (splitting
 // dS into two parts would add two products to the backward's seven), and delta is formed
-// from the stored o. Of the norm of dq and dk that leaves 0.25% in bf16 where a single
+// from the stored o. Of the norm of dq and dk that leaves 0.25 to 0.28% in bf16 where a single
 // rounding of the result leaves 0.17% (0.032% and 0.021% in fp16), with o and dv between.
 //
 // What bounds it, kernel times at 32 query and 8 kv heads of 128, bf16 (forward + dQ + dK/dV):

@@ -15,9 +15,14 @@
 // Layout: q [tokens, heads_q, head_dim] and k [tokens, heads_k, head_dim], head_dim
 // contiguous, other strides free; outputs contiguous. A thread owns a chunk of VEC pairs of one
 // token in HPT heads, `lanes` apart in the list of q's heads and then k's, so neighbouring
-// threads read neighbouring heads of a token. (With neighbouring threads on neighbouring tokens instead, a wave's load is
-// eight runs of 128 bytes a token's 8 KB apart: q and k of 32768 tokens, 32 + 8 heads of 128,
-// forward and backward 304 us against 254.)
+// threads read neighbouring heads of a token. (With neighbouring threads on neighbouring
+// tokens instead, a wave's load is eight runs of 128 bytes a token's 8 KB apart: q and k of
+// 32768 tokens, 32 + 8 heads of 128, forward and backward 304 us against 254, both with sines
+// formed per thread; 226 with the sines in LDS.)
+//
+// Memory-bound: each element is read and written once. bf16 32768 tokens, 32 + 8 heads of 128:
+// 115 us each way, 5.9 TB/s; fp16 5003 tokens, 16 + 16 heads of 96, 64 columns interleaved:
+// 13 us each way; 32 tokens 4 us, a launch.
 #include "eg_common.hpp"
 
 #include <algorithm>

@@ -16,6 +16,7 @@ The reference's arithmetic lives in PyTorch (a third-party dependency, unpinned 
 the reference's pyproject.toml:13-17; installed here as torch 2.10.0+rocm7.0), so
 the oracle is a torch restatement rather than a C one. How each function is pinned
 (closed forms, invariants, fp64 finite differences, brute force on tiny inputs)
-is recorded in tests/test_oracle_pins.py; no function of this package is left
+is recorded in tests/test_oracle_pins.py and, for the operators of packed batches, in
+tests/test_oracle_pins_packed.py; no function of this package is left
 unpinned.
 """

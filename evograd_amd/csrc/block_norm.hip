@@ -574,6 +574,7 @@ extern "C" int eg_block_norm_fwd(const void* x, const void* h, const void* post_
       return by_shape<scalar_t>(a, [&](auto vec, auto rag) {
         constexpr int V = decltype(vec)::value, G = decltype(g)::value;
         const RowShape r = row_shape(cols, V, false);
+        if (check_grid(name, rows, r.threads)) return 1;
         auto go = [&](auto ppt) {
           EG_LAUNCH((block_norm_fwd_kernel<scalar_t, V, decltype(ppt)::value, decltype(rag)::value, G>),
                     dim3((unsigned)rows), dim3(r.threads), 0, as_stream(stream), a);
@@ -586,6 +587,7 @@ extern "C" int eg_block_norm_fwd(const void* x, const void* h, const void* post_
         return go(std::integral_constant<int, 1>{});
       }, [&](auto vec) {
         constexpr int V = decltype(vec)::value, G = decltype(g)::value;
+        if (check_grid(name, rows, kWideBlock)) return 1;
         EG_LAUNCH((block_norm_fwd_wide_kernel<scalar_t, V, G>), dim3((unsigned)rows),
                   dim3(kWideBlock), 0, as_stream(stream), a);
         return check_launch(name);

@@ -25,6 +25,14 @@ void clear_error();
 // runtime's sticky launch error.
 int check_launch(const char* what);
 
+// 0, or 1 with an error: a grid has fewer than 2^32 threads along an axis.
+inline int check_grid(const char* name, int64_t blocks, int64_t threads) {
+  if (blocks * threads < ((int64_t)1 << 32)) return 0;
+  set_error("%s: grid too large (%lld workgroups of %lld threads)", name, (long long)blocks,
+            (long long)threads);
+  return 1;
+}
+
 // ------------------------------------------------------------ dtype tags
 struct bf16_t { uint16_t bits; };
 typedef _Float16 f16_t;

@@ -187,7 +187,7 @@ __global__ __launch_bounds__(256) void packed_reduce_kernel(PackedAttn a, WalkCu
   SeqTile t;
   if (!find_tile<kKeys, true>(a.seqs, rank, t, c.least, c.share)) return;
   const int head = rank - t.piece;  // the walk's first piece
-  if (t.pieces == 1 || head + t.pieces > c.slabs) return;
+  if (t.pieces == 1 || head < 0 || head + t.pieces > c.slabs) return;
   const int k0 = (t.tiles - 1 - t.tile) * kKeys, rows = min(kKeys, t.len - k0);
   const float* part = a.part + ((int64_t)kvh * c.slabs + head) * (2 * kKeys * D);
   const int64_t ldkv = (int64_t)a.kv_heads * D, first = (t.begin + k0) * ldkv + kvh * D;
@@ -276,6 +276,7 @@ int mfma_fwd(const PackedAttn& a, int dtype, hipStream_t st) {
       const int64_t ranks = packed_tiles(a.seqs.tokens, a.seqs.n, 32 * NW / HW);
       const int rows = 32 * NW / HW;
       PackedAttn b = a;
+      if (check_grid("eg_packed_attn_fwd", ranks * (a.heads / HW), NW * KG * 64)) return 1;
       if (int e = packed_plan(a.seqs, 1, &rows, a.plan, &b.seqs, st)) return e;
       EG_LAUNCH((packed_fwd_kernel<T, D, NW, KG, HW>), dim3((unsigned)(ranks * (a.heads / HW))),
                 dim3(NW * KG * 64), 0, st, b, (int)ranks, a.scale * kLog2e);
@@ -295,6 +296,9 @@ int mfma_bwd(const PackedAttn& a, int dtype, hipStream_t st) {
       const int64_t ranks = packed_tiles(a.seqs.tokens, a.seqs.n, 32 * NW / HW);
       const int rows[2] = {32 * NW / HW, 32 * cut.waves};
       PackedSeqs seqs[2];
+      if (check_grid("eg_packed_attn_bwd", ranks * (a.heads / HW), NW * KG * 64) ||
+          check_grid("eg_packed_attn_bwd", (int64_t)cut.ranks * a.kv_heads, cut.waves * 64))
+        return 1;
       if (int e = packed_plan(a.seqs, 2, rows, a.plan, seqs, st)) return e;
       PackedAttn b = a;
       b.seqs = seqs[0];

@@ -131,7 +131,7 @@ __global__ __launch_bounds__(kGenThreads) void packed_gen_reduce_kernel(PackedAt
   SeqTile t;
   if (!find_tile<kRows, true>(a.seqs, rank, t, c.least, c.share)) return;
   const int head = rank - t.piece;  // the walk's first piece
-  if (t.pieces == 1 || head + t.pieces > c.slabs) return;
+  if (t.pieces == 1 || head < 0 || head + t.pieces > c.slabs) return;
   const int k0 = (t.tiles - 1 - t.tile) * kRows, n = min(kRows, t.len - k0), D = a.head_dim;
   const float* part = a.part + ((int64_t)kvh * c.slabs + head) * (2 * kRows * D);
   const int64_t ldkv = (int64_t)a.kv_heads * D, first = (t.begin + k0) * ldkv + kvh * D;
@@ -169,8 +169,9 @@ size_t packed_generic_part_bytes(int64_t tokens, int64_t seqs, int64_t heads, in
 
 int packed_generic_fwd(const PackedAttn& given, int dtype, hipStream_t st) {
   PackedAttn a = given;
-  if (int e = packed_plan(given.seqs, 1, &kRows, given.plan, &a.seqs, st)) return e;
   const int64_t ranks = packed_tiles(a.seqs.tokens, a.seqs.n, kRows);
+  if (check_grid("eg_packed_attn_fwd", ranks * a.heads, kGenThreads)) return 1;
+  if (int e = packed_plan(given.seqs, 1, &kRows, given.plan, &a.seqs, st)) return e;
   return dispatch(a, dtype, false, "eg_packed_attn_fwd", [&](auto tag, auto dm, auto vec) {
     EG_LAUNCH((packed_gen_fwd_kernel<decltype(tag), decltype(dm)::value, decltype(vec)::value>),
               dim3((unsigned)(ranks * a.heads)), dim3(kGenThreads), 0, st, a, (int)ranks,
@@ -181,9 +182,12 @@ int packed_generic_fwd(const PackedAttn& given, int dtype, hipStream_t st) {
 
 int packed_generic_bwd(const PackedAttn& given, int dtype, hipStream_t st) {
   PackedAttn a = given;  // query and key tiles are of one size: one plan
-  if (int e = packed_plan(given.seqs, 1, &kRows, given.plan, &a.seqs, st)) return e;
   const int64_t ranks = packed_tiles(a.seqs.tokens, a.seqs.n, kRows);
   const WalkCut cut = walk_cut(a.seqs.tokens, a.seqs.n, a.heads, a.kv_heads);
+  if (check_grid("eg_packed_attn_bwd", std::max(ranks * a.heads, (int64_t)cut.ranks * a.kv_heads),
+                 kGenThreads))
+    return 1;
+  if (int e = packed_plan(given.seqs, 1, &kRows, given.plan, &a.seqs, st)) return e;
   return dispatch(a, dtype, true, "eg_packed_attn_bwd", [&](auto tag, auto dm, auto vec) {
     using T = decltype(tag);
     constexpr int DM = decltype(dm)::value;

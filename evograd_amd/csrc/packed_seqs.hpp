@@ -113,7 +113,7 @@ struct SeqTile {
 template <int ROWS>
 __device__ __forceinline__ bool find_planned(const PackedSeqs& p, int rank, SeqTile& t) {
   const int lane = threadIdx.x & 63;
-  const int all = p.start[p.n];
+  const int all = max(p.start[p.n], 0);  // a count past 2^31 is no sequences'
   t.piece = 0;
   t.pieces = 1;
   t.tile = t.tiles = 0;
@@ -182,7 +182,7 @@ __device__ __forceinline__ bool find_tile(const PackedSeqs& p, int rank, SeqTile
     each([&](int nt) { c += nt > j ? cut.below(nt) - under : 0; });
     return wave_sum(c);
   };
-  const int all = count(0);
+  const int all = max(count(0), 0);  // a count past 2^31 is no sequences'
   if (rank >= all) {
     t.spare = rank - all;
     return false;

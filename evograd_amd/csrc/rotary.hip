@@ -178,6 +178,7 @@ int launch(RotaryArgs a, hipStream_t st) {
       set_error("eg_rotary: grid too large");
       return 1;
     }
+    if (check_grid("eg_rotary", gx, threads)) return 1;
     EG_LAUNCH((rotary_kernel<T, VEC, HPT, INTER>), dim3((unsigned)gx, (unsigned)gy), dim3(threads),
               a.per_block * a.pairs * sizeof(float2), st, a);
     return check_launch("eg_rotary");

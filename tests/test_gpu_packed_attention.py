@@ -6,9 +6,11 @@ import sys
 import pytest
 import torch
 
+from evograd_amd import _lib
 from evograd_amd.bind import bind
 from evograd_amd.decls import PACKED_ATTENTION
 from evograd_amd.pairs import packed_attention as pair
+from evograd_amd.pairs._util import strides_arg
 from tests.packed_refs import assert_within, attention64
 
 pytestmark = pytest.mark.gpu
@@ -272,6 +274,58 @@ def test_a_captured_graph_replays_with_other_lengths(many, D, dtype):
         got = [x.clone() for x in out]
         for x, y in zip(got, run(*fresh, bounds(lengths))):
             assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("D,dtype", ((128, BF16), (64, F16), (64, F32)))
+@pytest.mark.parametrize("many", (False, True))
+def test_bounds_that_are_no_sequences_stay_inside_the_tensors(many, D, dtype):
+    """Decreasing, negative, overlapping and far bounds give undefined rows; every tensor lies
+    between guards, which stay as they were, and a sound call on the same memory afterwards is
+    right."""
+    H, KVH, guard = 8, 2, 4096
+    lengths = [1] * 260 + [140] if many else [100, 0, 60, 40]
+    T = sum(lengths)
+    n = len(lengths)
+    held = []
+
+    def guarded(shape, dt):
+        count = torch.Size(shape).numel()
+        whole = torch.full((count + 2 * guard,), 7.0, device="cuda", dtype=dt)
+        held.append((whole, count))
+        return whole[guard:guard + count].view(shape)
+
+    src = make([T], H, KVH, D, dtype)
+    q, k, v, do = [guarded(t.shape, dtype).copy_(t) for t in src]
+    o, dq = guarded(q.shape, dtype), guarded(q.shape, dtype)
+    dk, dv = guarded(k.shape, dtype), guarded(k.shape, dtype)
+    lse = guarded((H, T), F32)
+    fwd_bytes = _lib.query("eg_packed_attn_fwd_workspace_bytes", n)
+    bwd_bytes = _lib.query("eg_packed_attn_workspace_bytes", T, n, H, KVH, D, _lib.dtype_tag(dtype))
+    fws, bws = guarded((fwd_bytes // 4 + 1,), F32), guarded((bwd_bytes // 4 + 1,), F32)
+    steps = strides_arg(q, k, v)
+    common = (T, n, H, KVH, D, steps, D ** -0.5, _lib.dtype_tag(dtype), _lib.stream_of(q))
+
+    def step(cu):
+        _lib.call("eg_packed_attn_fwd", *map(_lib.ptr, (q, k, v, cu, o, lse, fws)), *common)
+        _lib.call("eg_packed_attn_bwd",
+                  *map(_lib.ptr, (do, q, k, v, cu, o, lse, dq, dk, dv, bws)), *common)
+        torch.cuda.synchronize()
+
+    far = (1 << 31) - 1
+    g = torch.Generator().manual_seed(3)
+    for bad in ([T, 0] * n, [0, T] * n, [-5, far] * n, [far] * (2 * n), [-far] * (2 * n),
+                torch.randint(-T, 3 * T, (2 * n,), generator=g).tolist()):
+        cu = torch.tensor(bad[:n + 1], dtype=torch.int32, device="cuda")
+        print(f"\n[gpu-packed] bad bounds {bad[:4]} x {n} D={D} {dtype}", flush=True)
+        step(cu)
+        for whole, count in held:
+            assert bool((whole[:guard] == 7).all()) and bool((whole[guard + count:] == 7).all())
+        for x, y in zip((q, k, v, do), src):
+            assert torch.equal(x, y)
+    cu = bounds(lengths)
+    step(cu)
+    for x, y in zip((o, dq, dk, dv), run(*src, cu)):
+        assert torch.equal(x, y)
 
 
 def test_gradient_against_differences_of_the_definition():

@@ -214,6 +214,29 @@ def test_entry_points_check_their_arguments():
 
 
 @built
+def test_grids_past_32_bits_are_refused():
+    """Sizes within every other limit whose grid would have 2^32 threads or more."""
+    steps = (ctypes.c_int64 * 6)(1 << 14, 256, 1 << 14, 256, 1 << 14, 256)
+    many = 1 << 24
+    for dim, dtype in ((8, _lib.EG_F32), (128, _lib.EG_BF16)):
+        with pytest.raises(RuntimeError, match="grid too large"):
+            _lib.call("eg_packed_attn_fwd", P, P, P, P, P, P, P, 4, many, 64, 64, dim, steps, 1.0,
+                      dtype, None)
+        with pytest.raises(RuntimeError, match="grid too large"):
+            _lib.call("eg_packed_attn_bwd", P, P, P, P, P, P, P, P, P, P, P, 4, many, 64, 64, dim,
+                      steps, 1.0, dtype, None)
+    with pytest.raises(RuntimeError, match="grid too large"):
+        _lib.call("eg_rotary", P, P, P, P, P, 0, P, 1 << 32, 1, 1, 8, 4,
+                  (ctypes.c_int64 * 4)(8, 8, 8, 8), 1.0, 0, 0, _lib.EG_F32, None)
+    with pytest.raises(RuntimeError, match="grid too large"):
+        _lib.call("eg_block_norm_fwd", P, P, P, None, P, P, P, P, 1 << 30, 64, 0, 1.0, 1e-6,
+                  _lib.EG_BF16, None)
+    with pytest.raises(RuntimeError, match="grid too large"):
+        _lib.call("eg_block_norm_fwd", P, P, P, None, P, P, P, P, 1 << 26, 40000, 0, 1.0, 1e-6,
+                  _lib.EG_BF16, None)
+
+
+@built
 def test_workspaces():
     al = lambda n: (n + 255) // 256 * 256
     assert _lib.query("eg_packed_attn_workspace_bytes", 0, 1, 2, 2, 64, _lib.EG_F32) == 0

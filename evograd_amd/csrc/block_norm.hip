@@ -25,7 +25,7 @@
 // with a gate per element 14.5 + 32 + 7.4 us, the backward at 3.2 TB/s on unaligned packs; fp32
 // [64, 768] 3.8 + 4.2 + 3.4 us, launches. Without the backward's loads of the next row under
 // the present one the first took 393 us a step instead of 273, before the non-temporal
-// accesses (240 with them).
+// accesses (240 to 244 with them).
 #include "eg_common.hpp"
 
 #include <algorithm>

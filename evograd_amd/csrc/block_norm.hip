@@ -22,8 +22,8 @@
 //
 // Kernel times, forward + backward + column sums: bf16 [16384, 4096] with a gate per channel
 // 100 + 148 + 8 us, the backward at 5.4 TB/s, behind two dependent row sums; bf16 [4099, 1538]
-// with a gate per element 14.5 + 32 + 7.4 us, the backward at 3.2 TB/s on unaligned packs; fp32
-// [64, 768] 3.8 + 4.2 + 3.4 us, launches. Without the backward's loads of the next row under
+// with a gate per element 14.4 + 26.5 + 5.9 us, the backward at 3.8 TB/s on unaligned packs; fp32
+// [64, 768] 3.8 + 4.3 + 3.3 us, launches. Without the backward's loads of the next row under
 // the present one the first took 393 us a step instead of 273, before the non-temporal
 // accesses (240 to 244 with them).
 #include "eg_common.hpp"
@@ -497,12 +497,19 @@ RowShape row_shape(int64_t cols, int vec, bool backward) {
 // the backward reads them with the non-temporal hint: bf16 [16384, 4096] step 261 -> 248 us,
 // [8192, 8192] 307 -> 294; fp16 [8192, 5000] would go 222 -> 240.
 constexpr int64_t kStreamBytes = 96 << 20;
-// Workgroups of the backward, a partial row each: about 16 waves per CU, 2048 workgroups at
-// most, whose partial rows the sum kernel reads in a few us.
+// Workgroups of the backward, a partial row each: as many whole ones as are resident at once, for
+// they walk the rows in steps of the grid and a second round of a few would leave the others'
+// CUs idle. The 16-bit kernels' registers allow three waves per SIMD with one pack a thread
+// (four without RAG and an element's gate, which gain nothing) and two with two packs: 12 and 8
+// per CU. Against 16 and 8 without counting whole workgroups (step times, bf16): [4099, 1538] 54
+// -> 47 us, [2048, 2050] 57 -> 45, [6000, 6001] 336 -> 273, [8192, 1024] fp16 70 -> 62,
+// [16384, 4096] the same; fp32 [5000, 1027] 50 -> 52. At most 2048, whose partial rows the sum
+// kernel reads in a few us.
 int64_t parts_for(int64_t rows, int64_t cols, int vec) {
   if (cols > kRowPacks * vec) return std::min<int64_t>(rows, 512);
   const RowShape r = row_shape(cols, vec, true);
-  return std::min<int64_t>({rows, 2048, 256 * 1024 / r.threads / r.ppt});
+  const int64_t resident = (r.ppt == 1 ? 12 : 8) / (r.threads / 64);
+  return std::min<int64_t>({rows, 2048, 256 * std::max<int64_t>(resident, 1)});
 }
 
 // go(VEC, RAG) for a row that a workgroup's registers hold, else wide(VEC).

@@ -952,8 +952,9 @@ __device__ __forceinline__ void attn_dq_rows(
   dsum += __shfl_xor(dsum, 32, 64);
   const float lraw = lse[qrc];
   const float l2 = qrow < S ? lraw * kLog2e : INFINITY;
-  const float dl = qrow < S ? dsum : 0.f;
-  if (qrow < S && hh == 0 && kg == 0) delta[qrow] = dsum;
+  float dl = qrow < S ? dsum : 0.f;
+  if constexpr (!PACKED)
+    if (qrow < S && hh == 0 && kg == 0) delta[qrow] = dsum;
 
   f32x16 acc[DT];
 #pragma unroll
@@ -1049,6 +1050,26 @@ __device__ __forceinline__ void attn_dq_rows(
           if (kkey > qrow) s[T2][r] = 0.f;
         }
     }
+    if constexpr (PACKED) {
+      // Rows whose keys are this tile's: delta = sum p dp / sum p, from fp32 registers. The
+      // stored o's rounding enters dS by p times its part of delta, which for rows of few keys,
+      // and peaked ones, is most of what dq and dk are off by (at 4 keys bf16 0.34 -> 0.24% of
+      // their norm). Rows of one key get dS = 0 exactly.
+      if (k0 == 0 && wave_first_row < BN) {
+        float pd = 0.f, ps = 0.f;
+#pragma unroll
+        for (int T2 = 0; T2 < 2; ++T2)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int kkey = 32 * T2 + (r >> 2) * 8 + 4 * hh + (r & 3);
+            pd += kkey > qrow ? 0.f : s[T2][r] * dp[T2][r];
+            ps += s[T2][r];
+          }
+        pd += __shfl_xor(pd, 32, 64);
+        ps += __shfl_xor(ps, 32, 64);
+        dl = qrow < S ? pd / ps : 0.f;
+      }
+    }
 #pragma unroll
     for (int T2 = 0; T2 < 2; ++T2)
 #pragma unroll
@@ -1074,6 +1095,7 @@ __device__ __forceinline__ void attn_dq_rows(
     if (j + 1 < nturns) tile(std::integral_constant<int, 1>{}, j + 1);
   }
   if constexpr (PACKED) {
+    if (qrow < S && hh == 0 && kg == 0) delta[qrow] = dl;
     if (__syncthreads_or(qrow < S && !all_finite<DT>(acc))) {
 #pragma unroll
       for (int t = 0; t < DT; ++t) acc[t] = f32x16{};

@@ -91,9 +91,9 @@ __global__ __launch_bounds__(kGenThreads, DM > 64 ? 1 : 2) void attn_gen_dq_kern
   if (blk >= nqb) return;
   const int q0 = (nqb - 1 - walk_order<(DM <= 64)>(blk, nqb)) * 16;
   const int64_t slice = (int64_t)S * D, own = bh * slice, kv = (bh / group) * slice;
-  attn_gen_dq_rows<T, DM, VEC>(q + own, D, k + kv, D, v + kv, D, dout + own, D, o + own, D,
-                               lse + (int64_t)bh * S, delta + (int64_t)bh * S, dq + own, D, S, D,
-                               q0, scale);
+  attn_gen_dq_rows<T, DM, VEC, false>(q + own, D, k + kv, D, v + kv, D, dout + own, D, o + own, D,
+                                      lse + (int64_t)bh * S, delta + (int64_t)bh * S, dq + own, D,
+                                      S, D, q0, scale);
 }
 
 // dK, dV: workgroup = 16 keys of one kv head, part pi of `parts`. With parts > 1 the sums go

@@ -13,9 +13,14 @@
 //
 // Rounding: scores, softmax statistics, dP and every sum are fp32. P and dS are rounded to the
 // tensors' 16 bits before their products, which take both operands in one type (splitting
-// dS into two parts would add two products to the backward's seven), and delta is formed
-// from the stored o. Of the norm of dq and dk that leaves 0.25 to 0.28% in bf16 where a single
-// rounding of the result leaves 0.17% (0.032% and 0.021% in fp16), with o and dv between.
+// dS into two parts would add two products to the backward's seven). delta is formed in fp32
+// from a tile's own P and dP for a sequence's first 64 rows, whose keys are that tile, and from
+// the stored o for the others. Of the norm of dq and dk that leaves, with standard normal
+// inputs and 4 to 1000 tokens a sequence, 0.23 to 0.24% in bf16 where a single rounding of the
+// result leaves 0.17% (0.030% and 0.021% in fp16), with o and dv between. Where scores are
+// peaked (of a spread of 4), o's rounding in delta shows past the first 64 rows: 0.23% at 4 to 64
+// tokens, 0.31% at 120, 0.37% at 1000 (0.030, 0.039 and 0.046% in fp16). Leaving it out there
+// would take a fourth product in dQ (sum p k).
 //
 // What bounds it, kernel times at 32 query and 8 kv heads of 128, bf16 (forward + dQ + dK/dV):
 // 32768 tokens in 7 sequences 2.46 + 3.47 + 5.39 ms, 1107, 1175 and 1011 TFLOP/s of the 4, 6

@@ -78,12 +78,12 @@ __global__ __launch_bounds__(kGenThreads, DM > 64 ? 1 : 2) void packed_gen_dq_ke
   const int kvh = h / (a.heads / a.kv_heads);
   const int64_t own = t.begin * ldo + h * a.head_dim;
   const int64_t row = (int64_t)h * a.seqs.tokens + t.begin;
-  attn_gen_dq_rows<T, DM, VEC>((const T*)a.q + t.begin * a.q_token + h * a.q_head, a.q_token,
-                               (const T*)a.k + t.begin * a.k_token + kvh * a.k_head, a.k_token,
-                               (const T*)a.v + t.begin * a.v_token + kvh * a.v_head, a.v_token,
-                               (const T*)a.dout + own, ldo, (const T*)a.o + own, ldo, a.lse + row,
-                               a.delta + row, dqs + t.begin * ldo, ldo, t.len, a.head_dim,
-                               t.tile * kRows, a.scale);
+  attn_gen_dq_rows<T, DM, VEC, true>(
+      (const T*)a.q + t.begin * a.q_token + h * a.q_head, a.q_token,
+      (const T*)a.k + t.begin * a.k_token + kvh * a.k_head, a.k_token,
+      (const T*)a.v + t.begin * a.v_token + kvh * a.v_head, a.v_token, (const T*)a.dout + own, ldo,
+      (const T*)a.o + own, ldo, a.lse + row, a.delta + row, dqs + t.begin * ldo, ldo, t.len,
+      a.head_dim, t.tile * kRows, a.scale);
 }
 
 // Workgroup = 16 keys of one kv head, one piece of their walk; key blocks are counted from

@@ -1,0 +1,74 @@
+"""Packed attention where its arithmetic has an edge: scores of -inf, values that no row sees,
+rows of few keys, upstream gradients past fp16's range, rows that share their memory. Against
+the definition in 64 bits (tests/packed_edge_refs.py)."""
+
+import pytest
+import torch
+
+from evograd_amd.pairs import packed_attention as pair
+from tests.packed_edge_refs import attention64
+from tests.packed_refs import assert_within
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+FAR = 1.0e4  # a finite stand-in for inf: its scores weigh exp(-FAR / sqrt(D)), which is zero
+
+
+def bounds(lengths):
+    cu = torch.zeros(len(lengths) + 1, dtype=torch.int32)
+    cu[1:] = torch.tensor(lengths, dtype=torch.int32).cumsum(0)
+    return cu.cuda()
+
+
+def make(lengths, H, KVH, D, dtype, seed=0, scale=1.0):
+    print(f"\n[gpu-packed-edges] {lengths[:6]}x{len(lengths)} {H}/{KVH} D={D} {dtype}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    T = sum(lengths)
+    shapes = ((T, H, D), (T, KVH, D), (T, KVH, D), (T, H, D))
+    return [(torch.randn(s, generator=g, device="cuda") * scale).to(dtype) for s in shapes]
+
+
+def run(q, k, v, do, cu):
+    o, saved = pair.packed_attention_forward_with_saved(q, k, v, cu)
+    dq, dk, dv = pair.packed_attention_backward_from_saved(do, saved)
+    return {"o": o, "dq": dq, "dk": dk, "dv": dv, "lse": saved[4]}
+
+
+KINDS = ((128, BF16), (64, BF16), (64, F16), (64, F32), (96, BF16))
+
+
+# ------------------------------------------------------------- rows of few keys
+@pytest.mark.parametrize("scale", (1.0, 2.0))
+@pytest.mark.parametrize("lengths", ([2], [4] * 9, [1, 3, 16, 7, 12], [26] * 3, [64, 63, 33]))
+@pytest.mark.parametrize("H,KVH,D,dtype", (
+    (8, 2, 128, BF16), (3, 1, 64, BF16), (4, 4, 128, F16), (4, 2, 64, F16), (2, 1, 64, F32),
+    (4, 2, 96, BF16), (2, 1, 80, F16), (4, 2, 32, F16)))
+def test_rows_of_few_keys_have_delta_in_32_bits(H, KVH, D, dtype, lengths, scale):
+    """Where a row's keys fit one tile, delta = sum p dp takes no rounding of o in, which for peaked
+    rows would be most of the error of dq and dk."""
+    q, k, v, do = make(lengths, H, KVH, D, dtype, seed=3, scale=scale)
+    want, _ = attention64(q, k, v, do, lengths)
+    got = run(q, k, v, do, bounds(lengths))
+    for name in got:
+        assert_within(name, got[name], *want[name])
+
+
+@pytest.mark.parametrize("H,KVH,D,dtype", ((8, 2, 128, BF16), (4, 4, 64, F16), (2, 1, 64, BF16)))
+@pytest.mark.parametrize("lengths", ([700, 300], [66, 90, 70] * 4))
+def test_the_first_rows_of_longer_sequences(lengths, H, KVH, D, dtype):
+    q, k, v, do = make(lengths, H, KVH, D, dtype, seed=4, scale=2.0)
+    want, _ = attention64(q, k, v, do, lengths)
+    got = run(q, k, v, do, bounds(lengths))
+    first = torch.cat([torch.arange(64) + sum(lengths[:i]) for i in range(len(lengths))]).cuda()
+    assert_within("dq", got["dq"][first], *(x[first] for x in want["dq"]))
+
+
+@pytest.mark.parametrize("D,dtype", KINDS)
+def test_a_row_of_one_key_has_no_gradient_through_its_weight(D, dtype):
+    """p is one whatever the score, so dS is zero: exactly, not to rounding."""
+    lengths = [1] * 20
+    q, k, v, do = make(lengths, 4, 2, D, dtype, seed=5, scale=3.0)
+    got = run(q, k, v, do, bounds(lengths))
+    for name in ("dq", "dk"):
+        assert int(torch.count_nonzero(got[name])) == 0, name

@@ -545,11 +545,13 @@ __device__ __forceinline__ void attn_fwd_rows(
 #pragma unroll
         for (int t = 0; t < DT; ++t) acc[t] *= alpha;
         m = m_new;
+        // every score so far may be -inf: weights of zero, not -inf + inf
+        const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
         for (int T2 = 0; T2 < 2; ++T2)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            s[T2][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[T2][r], scale_log2, -m));
+            s[T2][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[T2][r], scale_log2, -ref));
             lsum += s[T2][r];
           }
 #pragma unroll

@@ -72,3 +72,33 @@ def test_a_row_of_one_key_has_no_gradient_through_its_weight(D, dtype):
     got = run(q, k, v, do, bounds(lengths))
     for name in ("dq", "dk"):
         assert int(torch.count_nonzero(got[name])) == 0, name
+
+
+# ------------------------------------------------------------------ scores of -inf
+@pytest.mark.parametrize("D,dtype", KINDS)
+@pytest.mark.parametrize("lengths,H,KVH", (([200], 2, 1), ([200], 4, 1), ([150, 1, 1, 1, 9], 4, 2)))
+@pytest.mark.parametrize("first,last", ((64, 65), (0, 64)))
+@pytest.mark.parametrize("spoilt", (None, 70))
+def test_a_first_tile_of_hidden_and_infinitely_low_scores(spoilt, first, last, lengths, H, KVH, D,
+                                                          dtype):
+    """Keys first .. last - 1 score -inf against every row, and a row whose keys so far all do has
+    no maximum yet: its later (or other group's) keys alone decide it, whether or not another row
+    of its workgroup is NaN."""
+    q, k, v, do = make(lengths, H, KVH, D, dtype, seed=1)
+    q[..., 5] = -1.0
+    k[first:last, :, 5] = FAR
+    want, _ = attention64(q, k, v, do, lengths)
+    k[first:last, :, 5] = float("inf")
+    n = lengths[0]
+    rows = torch.arange(last if first == 0 else 0, n, device="cuda")
+    if spoilt is not None:
+        q[spoilt, :, 5] = 1.0  # its scores against those keys are +inf: the row is NaN
+        rows = rows[rows != spoilt]
+    got = run(q, k, v, do, bounds(lengths))
+    assert_within("o", got["o"][rows], *(x[rows] for x in want["o"]))
+    assert_within("lse", got["lse"][:, rows], *(x[:, rows] for x in want["lse"]))
+    if first > 0:  # dq's column 5 is 0 times inf
+        keep = [i for i in range(D) if i != 5]
+        assert_within("dq", got["dq"][rows][..., keep], *(x[rows][..., keep] for x in want["dq"]))
+    else:  # the first rows see nothing else
+        assert bool(torch.isnan(got["o"][:last]).all())

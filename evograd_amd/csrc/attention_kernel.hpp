@@ -854,7 +854,8 @@ __device__ __forceinline__ void attn_dkdv_keys(
           dp = MM<T>::mma(*reinterpret_cast<const v8*>(Ds0 + at),
                           *reinterpret_cast<const v8*>(Vw + at), dp);
         }
-        auto seen = [&](int r) { return qi0 + r >= key; };
+        // (rows past S are zeros, which an infinite key turns into a NaN score)
+        auto seen = [&](int r) { return qi0 + r >= key && qi0 + r < S; };
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int row = (r >> 2) * 8 + 4 * hh + (r & 3);

@@ -102,3 +102,23 @@ def test_a_first_tile_of_hidden_and_infinitely_low_scores(spoilt, first, last, l
         assert_within("dq", got["dq"][rows][..., keep], *(x[rows][..., keep] for x in want["dq"]))
     else:  # the first rows see nothing else
         assert bool(torch.isnan(got["o"][:last]).all())
+
+
+# ------------------------------------------------- rows past the end see no key
+@pytest.mark.parametrize("D,dtype", KINDS)
+@pytest.mark.parametrize("n", (64, 65, 95, 130, 450))
+@pytest.mark.parametrize("H,KVH", ((2, 2), (8, 2)))
+def test_an_infinite_key_that_weighs_nothing_has_the_gradients_of_one(H, KVH, n, D, dtype):
+    """The last key of a sequence scores -inf against its only row. What a tile holds past the
+    sequence's end takes no part in its gradients, whether or not the tile is full."""
+    lengths = [n, 40]
+    q, k, v, do = make(lengths, H, KVH, D, dtype, seed=n)
+    q[n - 1, :, 5] = -1.0
+    k[n - 1, :, 5] = FAR
+    want, _ = attention64(q, k, v, do, lengths)
+    k[n - 1, :, 5] = float("inf")
+    got = run(q, k, v, do, bounds(lengths))
+    for name in ("o", "dk", "dv"):
+        assert_within(name, got[name], *want[name])
+    keep = [i for i in range(D) if i != 5]  # of that row, dq's column 5 is 0 times inf
+    assert_within("dq", got["dq"][..., keep], *(x[..., keep] for x in want["dq"]))

@@ -262,7 +262,10 @@ __device__ __forceinline__ void zero_lds(void* p, int bytes) {
 // PACKED variants look at the finished sums (a few instructions per workgroup, nothing in the
 // loops): where one is not finite, the walk is done again with the masked pairs left out
 // of the products (add_seen), so that such values reach the rows that see them and no
-// others.
+// others. The second walk also takes what fp16 cannot hold: a dS past 65504 (the gradients of a
+// scaled loss) is infinite as an operand though dq and dk may be well in range, so there each
+// tile's dS is rounded as a multiple of a power of two (half_range). It is slow, a product per
+// row: with one NaN in q, bf16 8192 tokens in 11 sequences 150 + 463 -> 204 + 2098 us.
 template <int DT>
 __device__ __forceinline__ bool all_finite(const f32x16 (&acc)[DT]) {
   float z = 0.f;
@@ -273,13 +276,33 @@ __device__ __forceinline__ bool all_finite(const f32x16 (&acc)[DT]) {
   return z == 0.f;
 }
 
-// acc += (16 tile rows, transposed)^T w for the rows that this lane's column sees: a product
+// fp16: scales w by the power of two that brings its largest finite value in the wave below 2^15,
+// if it is not, and returns that power's inverse.
+template <typename T>
+__device__ __forceinline__ float half_range(f32x16& w) {
+  if constexpr (!std::is_same_v<T, f16_t>) return 1.f;
+  float most = 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const float x = __builtin_fabsf(w[r]);
+    most = x < INFINITY ? fmaxf(most, x) : most;
+  }
+  most = wave_reduce(most, MaxOp());
+  const int over = max(0, __builtin_amdgcn_frexp_expf(most) - 15);  // most < 2^(over + 15)
+  const float back = ldexpf(1.f, over), to = ldexpf(1.f, -over);
+#pragma unroll
+  for (int r = 0; r < 16; ++r) w[r] *= to;
+  return back;
+}
+
+// acc += back * (16 tile rows, transposed)^T w for the rows that this lane's column sees: a product
 // per row, of the row's operand elements alone, whose result a lane takes or leaves. The
 // row's element: rows 4hh + 0..3 are elements 0..3 of half hh's lanes, rows 8 + 4hh + 0..3
 // elements 4..7.
 template <typename T, int D, typename Seen>
 __device__ __forceinline__ void add_seen(f32x16 (&acc)[D / 32], const uint16_t* rows,
-                                         typename MM<T>::v8 w, int lane, Seen seen) {
+                                         typename MM<T>::v8 w, int lane, Seen seen,
+                                         float back = 1.f) {
   using v8 = typename MM<T>::v8;
   const int hh = lane >> 5;
   uint32_t ww[4];
@@ -305,7 +328,8 @@ __device__ __forceinline__ void add_seen(f32x16 (&acc)[D / 32], const uint16_t* 
       __builtin_memcpy(x, &a, 16);
       const f32x16 one = MM<T>::mma(alone(x), wr, f32x16{});
 #pragma unroll
-      for (int i = 0; i < 16; ++i) acc[t][i] = in ? acc[t][i] + one[i] : acc[t][i];
+      for (int i = 0; i < 16; ++i)
+        acc[t][i] = in ? __builtin_fmaf(back, one[i], acc[t][i]) : acc[t][i];
     }
   }
 }
@@ -863,11 +887,12 @@ __device__ __forceinline__ void attn_dkdv_keys(
           s[r] = seen(row) ? p : 0.f;
           dp[r] = seen(row) ? p * (dp[r] - Es[0][row]) : 0.f;
         }
+        const float back = half_range<T>(dp);
 #pragma unroll
         for (int ms = 0; ms < BQ / 16; ++ms) {
           auto seen16 = [&](int r) { return seen(16 * ms + r); };
           add_seen<T, D>(dva, Ds0 + 16 * D * ms, pack8<T>(s, 8 * ms), lane, seen16);
-          add_seen<T, D>(dka, Qs0 + 16 * D * ms, pack8<T>(dp, 8 * ms), lane, seen16);
+          add_seen<T, D>(dka, Qs0 + 16 * D * ms, pack8<T>(dp, 8 * ms), lane, seen16, back);
         }
       }
     }
@@ -1127,10 +1152,11 @@ __device__ __forceinline__ void attn_dq_rows(
             const bool in = k0 + 32 * T2 + (r >> 2) * 8 + 4 * hh + (r & 3) <= qrow;
             dp[r] = in ? p * (dp[r] - dl) : 0.f;
           }
+          const float back = half_range<T>(dp);
 #pragma unroll
           for (int ms = 0; ms < 2; ++ms)
             add_seen<T, D>(acc, Ks0 + kvo + 16 * D * (2 * T2 + ms), pack8<T>(dp, 8 * ms), lane,
-                           [&](int r) { return k0 + 32 * T2 + 16 * ms + r <= qrow; });
+                           [&](int r) { return k0 + 32 * T2 + 16 * ms + r <= qrow; }, back);
         }
       }
     }

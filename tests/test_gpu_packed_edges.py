@@ -122,3 +122,25 @@ def test_an_infinite_key_that_weighs_nothing_has_the_gradients_of_one(H, KVH, n,
         assert_within(name, got[name], *want[name])
     keep = [i for i in range(D) if i != 5]  # of that row, dq's column 5 is 0 times inf
     assert_within("dq", got["dq"][..., keep], *(x[..., keep] for x in want["dq"]))
+
+
+# -------------------------------------------------------------- fp16's range of dS
+@pytest.mark.parametrize("D", (64, 128))
+@pytest.mark.parametrize("lengths,H,KVH", (([2, 3, 5, 9, 1], 2, 2), ([40, 64, 17], 4, 4),
+                                           ([300, 5], 2, 2), ([2] * 300, 2, 1)))
+@pytest.mark.parametrize("spoilt", (None, 1))
+def test_gradients_whose_products_pass_the_half_range(spoilt, lengths, H, KVH, D):
+    """Upstream gradients of a scaled loss: dS passes 65504 where dq and dk are well inside it."""
+    q, k, v, do = make(lengths, H, KVH, D, F16, seed=6)
+    q, k = (0.25 * q.float()).half(), (0.25 * k.float()).half()
+    v = (3.0 * v.float()).half()
+    do = (1.2e4 * torch.sign(do.float())).half()
+    want, largest = attention64(q, k, v, do, lengths, half_range=True)
+    assert largest > 65504 and all(float(x.abs().max()) < 60000 for x, _ in want.values())
+    keep = torch.ones(sum(lengths), dtype=torch.bool, device="cuda")
+    if spoilt is not None:  # a NaN row of the first sequence: the others are what they were
+        q[spoilt] = float("nan")
+        keep[:lengths[0]] = False
+    got = run(q, k, v, do, bounds(lengths))
+    for name in ("o", "dq", "dk", "dv"):
+        assert_within(name, got[name][keep], *(x[keep] for x in want[name]))

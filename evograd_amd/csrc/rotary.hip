@@ -230,11 +230,14 @@ extern "C" int eg_rotary(const void* q, const void* k, void* q_out, void* k_out,
     return 1;
   }
   if (!strides) { set_error("%s: null strides", name); return 1; }
-  for (int i = 0; i < 4; ++i)
-    if (strides[i] < 0 || strides[i] > ((int64_t)1 << 32)) {
-      set_error("%s: strides must be at least 0 and at most 2^32 elements", name);
+  for (int i = 0; i < 4; ++i) {  // token steps and head steps
+    const int bits = i % 2 ? 40 : 32;
+    if (strides[i] < 0 || strides[i] > ((int64_t)1 << bits)) {
+      set_error("%s: strides must be at least 0 and at most 2^32 (tokens) or 2^40 (heads) elements",
+                name);
       return 1;
     }
+  }
   if (tokens == 0 || head_dim == 0 || heads_q + heads_k == 0) return 0;
   if ((heads_q && (!q || !q_out)) || (heads_k && (!k || !k_out)) || !positions ||
       (pairs && !freqs)) {

@@ -493,8 +493,11 @@ int eg_packed_attn_bwd(const void* dout, const void* q, const void* k, const voi
  * freqs[i] (fp64, radians per position), pair i is (x[i], x[i + pairs]) or, interleaved,
  * (x[2i], x[2i + 1]) and becomes amplitude * (x1 cos - x2 sin, x2 cos + x1 sin); columns
  * from 2 * pairs on are copied. inverse: the transpose (the backward). positions: int32, or
- * int64 with positions_64. `strides` (host): token and head steps of q and of k, in
- * elements; a head's columns are contiguous; outputs are contiguous. */
+ * int64 with positions_64. `strides` (host, read during the call): token and head steps of
+ * q and of k, in elements, at most 2^32 and 2^40; a head's columns are contiguous; outputs are
+ * contiguous. fp32, bf16, fp16. Sizes: tokens <= 2^32, heads_q and heads_k <= 2^16 each,
+ * head_dim <= 2^13, and a grid of fewer than 2^32 threads (tokens * (heads_q + heads_k) *
+ * head_dim <= 2^31 is within it). */
 int eg_rotary(const void* q, const void* k, void* q_out, void* k_out, const void* positions,
               int positions_64, const double* freqs, int64_t tokens, int64_t heads_q,
               int64_t heads_k, int64_t head_dim, int64_t pairs, const int64_t* strides,

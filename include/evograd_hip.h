@@ -466,7 +466,9 @@ int eg_silu_mul(const void* gate, const void* up, void* out, int64_t n, int dtyp
  * head_dim], lse fp32 [heads, tokens]. Rows that no sequence holds get o = 0 and are
  * read into no result. The bounds are read on the device alone; ones that break the
  * rules give undefined values but no access outside the tensors. fp32, bf16, fp16;
- * even head_dim up to 128. Sizes: tokens <= 2^28, (tokens / 16 + seqs) * heads < 2^30.
+ * even head_dim up to 128. Sizes: tokens <= 2^28, seqs <= 2^24, heads <= 4096 and, in both
+ * directions, grids of fewer than 2^32 threads, for which (tokens / 16 + seqs + 1) * heads < 2^24
+ * is enough (bf16 and fp16 heads of 64 and 128 go further).
  * workspace: eg_packed_attn_fwd_workspace_bytes(seqs), which is 0 up to 256 sequences. */
 size_t eg_packed_attn_fwd_workspace_bytes(int64_t seqs);
 int eg_packed_attn_fwd(const void* q, const void* k, const void* v, const int* cu_seqlens,
@@ -506,7 +508,9 @@ int eg_rotary(const void* q, const void* k, void* q_out, void* k_out, const void
 /* The norms around a block with its gate, residual scale and residual, rows x cols:
  *   s = x + alpha * gate * (h * rstd_h * post_weight),  y = s * rstd_s * pre_weight
  * in fp32, y from the unrounded s; rstd fp32 [2, rows] (of h, of s; saved). gate_kind 0: no
- * gate, 1: gate [cols], 2: [rows], 3: [rows, cols]. */
+ * gate, 1: gate [cols], 2: [rows], 3: [rows, cols]. fp32, bf16, fp16. Sizes: cols <= 2^24,
+ * rows <= 2^30 and, in the forward, fewer than 2^32 threads, of which a row takes 64 to 256, or
+ * 1024 past 8192 columns (fp32: 4096): rows < 2^24 or 2^22 are enough. */
 int eg_block_norm_fwd(const void* x, const void* h, const void* post_weight, const void* gate,
                       const void* pre_weight, void* s, void* y, float* rstd, int64_t rows,
                       int64_t cols, int gate_kind, float alpha, float eps, int dtype,

@@ -32,6 +32,7 @@ if not __package__:
         _sys.path.insert(0, _ROOT)
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from evograd_amd import _lib
 from evograd_amd.pairs._util import as_contiguous, check_same, tag, workspace
@@ -132,6 +133,7 @@ class BlockNorm(torch.autograd.Function):
         return s, y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, ds, dy):
         saved = ctx.saved_tensors
         if not ctx.has_gate:

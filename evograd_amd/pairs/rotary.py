@@ -32,6 +32,7 @@ if not __package__:
 import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from evograd_amd import _lib
 from evograd_amd.pairs._util import as_contiguous, contiguous_like, head_rows, strides_arg, tag
@@ -163,6 +164,7 @@ class RotaryQK(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dq_out, dk_out):
         dq, dk = rotary_qk_backward_from_saved((dq_out, dk_out), ctx.saved_tensors, *ctx.scalars)
         return dq, dk, None, None, None, None

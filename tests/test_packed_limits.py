@@ -9,6 +9,8 @@ import torch
 
 from evograd_amd import _lib
 from evograd_amd.pairs._util import MAX_HEAD_STRIDE, MAX_TOKEN_STRIDE, head_rows
+from evograd_amd.pairs.block_norm import BlockNorm
+from evograd_amd.pairs.rotary import RotaryQK
 
 built = pytest.mark.skipif(not os.path.exists(_lib.LIB_PATH), reason="library not built")
 P = 1 << 20  # an address no refused call reads
@@ -43,3 +45,36 @@ def test_head_rows_keeps_steps_up_to_the_limits():
     for token, head in ((MAX_TOKEN_STRIDE + 1, 64), (64, MAX_HEAD_STRIDE + 1), (63, 64), (0, 64)):
         t = view(2, 2, 64, token, head)
         assert head_rows(t) is not t and head_rows(t).is_contiguous()
+
+
+@pytest.fixture
+def no_kernels(monkeypatch):
+    """The pairs on CPU tensors with every launch left out (results are not looked at)."""
+    for name in ("require_gpu", "call_on"):
+        monkeypatch.setattr(_lib, name, lambda *a: None)
+    monkeypatch.setattr(_lib, "stream_of", lambda t: 0)
+    monkeypatch.setattr(_lib, "query", lambda *a: 16)
+
+
+def test_gradients_of_gradients_are_refused(no_kernels):
+    """The backward kernels have no backward of their own: a second differentiation through the
+    nodes raises, where it would leave their part out."""
+    def leaf(*shape):
+        return torch.zeros(shape, requires_grad=True)
+
+    x, h, w1, w2 = leaf(4, 8), leaf(4, 8), leaf(8), leaf(8)
+    s, y = BlockNorm.apply(x, h, w1, None, w2, 1.0, 1e-6)
+    norm_grads = torch.autograd.grad((s * s).sum() + (y * y).sum(), (x, h), create_graph=True)
+    q, k = leaf(4, 2, 8), leaf(4, 1, 8)
+    a, b = RotaryQK.apply(q, k, torch.arange(4), torch.ones(4, dtype=torch.float64))
+    turn_grads = torch.autograd.grad((a * a).sum() + (b * b).sum(), (q, k), create_graph=True)
+    for g, other in ((norm_grads[0], x), (norm_grads[1], h), (turn_grads[0], q), (turn_grads[1], k)):
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            (g.sum() + other.sum()).backward(retain_graph=True)
+
+
+def test_first_gradients_need_no_second(no_kernels):
+    x, h, w1, w2 = (torch.zeros(s, requires_grad=True) for s in ((4, 8), (4, 8), 8, 8))
+    s, _ = BlockNorm.apply(x, h, w1, None, w2, 1.0, 1e-6)
+    s.sum().backward()
+    assert all(t.grad is not None and t.grad.shape == t.shape for t in (x, h, w1, w2))

@@ -245,23 +245,26 @@ int by_type(const PackedAttn& a, int dtype, F&& f) {
 
 // Two key groups per workgroup (KG = 2), which halve a row block's chain of key tiles: for few
 // long walks.
-inline bool split_keys(const PackedAttn& a, bool dq) {
+template <int D, bool DQ>
+inline bool split_keys(const PackedAttn& a) {
+  if (DQ && D != 64) return false;
   const int64_t grid = ((int64_t)a.seqs.tokens + 127) / 128 * a.heads;
-  if (short_seqs(a.seqs.tokens, a.seqs.n)) return false;
-  return dq ? a.head_dim == 64 && grid <= 384 : grid <= 512;
+  return !short_seqs(a.seqs.tokens, a.seqs.n) && grid <= (DQ ? 384 : 512);
 }
 
 // Workgroups of the forward and dQ: f(HW, NW, KG).
 // HW heads of a group share their keys and values: their waves walk the same keys, where the
 // waves of one head's rows end one after the other, and short sequences fill a tile of 32
 // rows where 128 of one head would be mostly empty.
-template <int D, typename F>
-int by_rows(const PackedAttn& a, bool dq, F&& f) {
+template <int D, bool DQ, typename F>
+int by_rows(const PackedAttn& a, F&& f) {
   const int group = a.heads / a.kv_heads;
-  const bool split = split_keys(a, dq);
+  const bool split = split_keys<D, DQ>(a);
   auto go = [&](auto hw) -> int {
     constexpr int HW = decltype(hw)::value;
-    if (split) return f(hw, Int<4>{}, Int<2>{});
+    if constexpr (!DQ || D == 64) {
+      if (split) return f(hw, Int<4>{}, Int<2>{});
+    }
     if constexpr (D == 64 && HW < 4) {
       if (short_seqs(a.seqs.tokens, a.seqs.n)) return f(hw, Int<2>{}, Int<1>{});
     }
@@ -276,7 +279,7 @@ int mfma_fwd(const PackedAttn& a, int dtype, hipStream_t st) {
   return by_type(a, dtype, [&](auto tc, auto dc) {
     using T = decltype(tc);
     constexpr int D = decltype(dc)::value;
-    return by_rows<D>(a, false, [&](auto hw, auto nw, auto kg) {
+    return by_rows<D, false>(a, [&](auto hw, auto nw, auto kg) {
       constexpr int HW = decltype(hw)::value, NW = decltype(nw)::value, KG = decltype(kg)::value;
       const int64_t ranks = packed_tiles(a.seqs.tokens, a.seqs.n, 32 * NW / HW);
       const int rows = 32 * NW / HW;
@@ -296,7 +299,7 @@ int mfma_bwd(const PackedAttn& a, int dtype, hipStream_t st) {
     using T = decltype(tc);
     constexpr int D = decltype(dc)::value;
     PackedAttn keys_of = a;
-    const int rc = by_rows<D>(a, true, [&](auto hw, auto nw, auto kg) {
+    const int rc = by_rows<D, true>(a, [&](auto hw, auto nw, auto kg) {
       constexpr int HW = decltype(hw)::value, NW = decltype(nw)::value, KG = decltype(kg)::value;
       const int64_t ranks = packed_tiles(a.seqs.tokens, a.seqs.n, 32 * NW / HW);
       const int rows[2] = {32 * NW / HW, 32 * cut.waves};

@@ -237,7 +237,9 @@ struct TileLoader {
     // Where the rows of a lane's loads are 16 apart or a multiple, their swizzles agree and the
     // later offsets follow from the first. Packed tiles at D = 128 form them so: with two row
     // steps in a loop registers are short there (packed dK/dV held in scratch what the loop
-    // needs; bf16 32768 tokens, 32 / 8 heads, forward and backward 11.8 -> 11.4 ms).
+    // needs; bf16 32768 tokens, 32 / 8 heads, forward and backward 11.8 -> 11.4 ms. The 22 registers
+    // a lane that it still spills belong to the second walk; of the two-wave form's 35, three are
+    // read again in every step).
     constexpr int STEP = 64 * NW / CPR;
     constexpr bool FORM = PACKED && D == 128 && STEP % 16 == 0;
     int base = voff[0];

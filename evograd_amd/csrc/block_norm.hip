@@ -184,7 +184,10 @@ struct RawRow {
 };
 
 // One pack per thread up to 256 packs, then two, on up to 512 threads: a CU's registers hold
-// the values of three or four rows, and of the rows after them, either way.
+// the values of three or four rows, and of the rows after them, either way. Whole 16-bit packs,
+// one a thread, are held to four waves per SIMD's registers, which spills 7 of them with a channel
+// gate, 1 to 3 with a row's and 16 with an element's. At three waves (bf16, backward): [8192, 2048]
+// 53 -> 48 us, 50 -> 49 and 63 -> 51, but [4099, 1536] 32 -> 34, 30 -> 37 and 36 -> 35.
 template <typename T, int VEC, int PPT, bool RAG, bool NT, int GATE>
 __global__ __launch_bounds__(PPT == 1 ? kBwdThreads / 2 : kBwdThreads,
                              PPT == 2 ? 2 : RAG ? 3 : 4) void block_norm_bwd_kernel(NormArgs a) {
@@ -299,7 +302,9 @@ __global__ __launch_bounds__(PPT == 1 ? kBwdThreads / 2 : kBwdThreads,
 
 // Rows too wide for a workgroup's registers: the row is read again for every reduction (from
 // L2: a workgroup's row is at most a few hundred KB), and the backward's column sums are kept
-// in the workgroup's partial row, where each column belongs to one thread.
+// in the workgroup's partial row, where each column belongs to one thread. With a gate per channel
+// fp32 [8192, 8192] takes 240 us forward and 753 backward, bf16 [8192, 16384] 292 and 1519, where the
+// bytes take 174 and 261.
 constexpr int kWideBlock = 1024;
 
 template <typename T, int VEC, int GATE>
@@ -482,7 +487,8 @@ __global__ __launch_bounds__(kSumCols * kSumRows) void block_norm_sum_kernel(Nor
 
 constexpr int64_t kMaxCols = (int64_t)1 << 24;
 
-// Packs per thread and threads of a row's workgroup, whole waves. Rows of more than 1024 packs (8192 16-bit columns, 4096 fp32) take the wide kernels.
+// Packs per thread and threads of a row's workgroup, whole waves. Rows of more than 1024 packs
+// (8192 16-bit columns, 4096 fp32) take the wide kernels.
 constexpr int64_t kRowPacks = 1024;
 struct RowShape {
   int ppt, threads;
@@ -501,8 +507,8 @@ constexpr int64_t kStreamBytes = 96 << 20;
 // they walk the rows in steps of the grid and a second round of a few would leave the others'
 // CUs idle. The 16-bit kernels' registers allow three waves per SIMD with one pack a thread
 // (four without RAG and an element's gate, which gain nothing) and two with two packs: 12 and 8
-// per CU. Against 16 and 8 without counting whole workgroups (step times, bf16): [4099, 1538] 54
-// -> 47 us, [2048, 2050] 57 -> 45, [6000, 6001] 336 -> 273, [8192, 1024] fp16 70 -> 62,
+// per CU. Against 16 and 8 without counting whole workgroups (step times, bf16): [4099, 1538] 51
+// -> 44 us, [2048, 2050] 57 -> 45, [6000, 6001] 336 -> 273, [8192, 1024] fp16 70 -> 62,
 // [16384, 4096] the same; fp32 [5000, 1027] 50 -> 52. At most 2048, whose partial rows the sum
 // kernel reads in a few us.
 int64_t parts_for(int64_t rows, int64_t cols, int vec) {

@@ -110,14 +110,20 @@ __global__ __launch_bounds__(NW * KG * 64, 2) void packed_dq_kernel(PackedAttn a
 }
 
 // A workgroup's rows or keys lie in one sequence, so where sequences are shorter than a block
-// on the mean a narrower one leaves fewer waves without rows.
+// on the mean a narrower one leaves fewer waves without rows: key blocks of two waves instead of
+// four, and at D = 64 row blocks of two for one or two heads a workgroup. Backward, four waves
+// (with dQ's key groups, below 128 tokens) against two, bf16: 12 heads of 64, 160 prompts of 24
+// tokens 90 / 40 us, 50 of 96 48 / 42, 40 of 128 46 / 41; 32 / 8 heads of 64, 100 of 48 73 / 61, 40
+// of 128 the same; 32 / 8 heads of 128, 160 of 24 97 / 92, but 100 of 48 104 / 109 and 40 of 128
+// 104 / 115. One limit lies between them.
 constexpr int64_t kShort = 112;
 inline bool short_seqs(int64_t tokens, int64_t seqs) { return tokens < kShort * seqs; }
 
 // The dK/dV walk of a block of keys (32 a wave), cut where it is long against the work of the
 // whole batch: each piece is at most 1 / kTarget of it (two workgroups per CU), but no
 // shorter than kMinSteps steps of 32 rows, about what a piece's fp32 slab costs to write and
-// read.
+// read (4, 8 and 16 steps, backward: 12 heads of 64, 4 prompts of 256 tokens 31.7, 32.4 and 32.7
+// us, 2 of 512 41.1, 39.9 and 43.1; 32 / 8 heads of 128 within 0.3%).
 constexpr int kWalkRows = 32;
 constexpr int64_t kTarget = 512, kMinSteps = 8;
 
@@ -130,7 +136,10 @@ struct WalkCut {
 WalkCut walk_cut(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads) {
   WalkCut c;
   c.waves = short_seqs(tokens, seqs) ? 2 : 4;
-  if (seqs > kSearchSeqs) {  // walks are not cut
+  // Walks are not cut: a document among many prompts then has its first keys' walk as a tail (32
+  // / 8 heads of 128, 301 sequences, one of 4096 of 7096 tokens, backward 1101 us, against 829
+  // with 251; with one of 8192 of 12288 tokens 2754 and 2767).
+  if (seqs > kSearchSeqs) {
     c.least = 1, c.share = 1.f, c.slabs = 0;
     c.ranks = (int)packed_tiles(tokens, seqs, 32 * c.waves);
     return c;
@@ -244,7 +253,15 @@ int by_type(const PackedAttn& a, int dtype, F&& f) {
 }
 
 // Two key groups per workgroup (KG = 2), which halve a row block's chain of key tiles: for few
-// long walks.
+// long walks. Forward, one group against two, bf16, by the grid (blocks of 128 rows times
+// heads): 128 heads of 128, one sequence of 2048 39 / 32 us; 256, one of 1024 25.6 / 23.2, 4 of 1024
+// 30.0 / 25.5; 384, 2 of 768 28.5 / 28.0; 512, one of 2048 50 / 52. Below 512 tokens a sequence it
+// costs more than it gives, most where the grid fills the CUs: 128, 4 of 128 10.8 / 12.3; 512, 4
+// of 512 25 / 36, 16 of 128 22 / 30. The host knows the mean length alone, which does not tell such
+// a batch from one long sequence among short ones (12 heads of 64, one of 1111 and 7 of 250 19.6 /
+// 16.7, one of 1024 and 7 of 120 16.8 / 14.8), so both take it. dQ at D = 64, backward: 128, one of
+// 2048 79 / 76; 256, 4 of 1024 67.6 / 65.0; 384, 2 of 768 65.5 / 67.5; 128, 4 of 128 38.3 / 39.8. dQ
+// at D = 128 loses throughout (3 to 8 us).
 template <int D, bool DQ>
 inline bool split_keys(const PackedAttn& a) {
   if (DQ && D != 64) return false;

@@ -22,9 +22,9 @@ struct PackedAttn {
   float scale;
 };
 
-// Orders the sequences for tiles of `rows` rows into `table` (plan_bytes(n) bytes), where there
-// are so many that the kernels search a plan (packed_attention.hip), and returns seqs with it;
-// rc gets a launch error. Both tables of a backward pass in one launch.
+// Where there are so many sequences that the kernels search a plan (packed_attention.hip), orders
+// them for tiles of rows[i] rows into table[i] (plan_bytes(n) bytes each), all in one launch; out[i]
+// is seqs with that plan, or seqs as it is. Returns 0 or a launch error.
 inline size_t plan_bytes(int64_t n) {
   return n > kSearchSeqs ? ((size_t)(2 * n + 1) * 4 + 255) / 256 * 256 : 0;
 }

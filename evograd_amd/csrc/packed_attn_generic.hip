@@ -26,7 +26,9 @@ struct WalkCut {
 WalkCut walk_cut(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads) {
   const int64_t group = heads / kv_heads, steps = 8 * kGenWaves;
   WalkCut c;
-  if (seqs > kSearchSeqs) {  // walks are not cut
+  // walks are not cut (8 / 2 heads of 64, fp32, one sequence of 2048 of 3548 tokens, backward: 301
+  // sequences 379 us, 251 305)
+  if (seqs > kSearchSeqs) {
     c.least = 1, c.share = 1.f, c.slabs = 0;
     c.ranks = (int)packed_tiles(tokens, seqs, kRows);
     return c;

@@ -618,7 +618,14 @@ extern "C" int eg_block_norm_bwd(const void* ds, const void* dy, const void* x, 
   static const char* name = "eg_block_norm_bwd";
   clear_error();
   if (check(name, rows, cols, gate_kind)) return 1;
-  if (cols == 0) return 0;
+  if (cols == 0) {  // nothing but a row gate's gradient, a sum over no columns
+    if (gate_kind != kRow) return 0;
+    if (dtype != EG_F32 && dtype != EG_F16 && dtype != EG_BF16) {
+      set_error("%s: unsupported dtype %d", name, dtype);
+      return 1;
+    }
+    return zero_fill(dgate, (size_t)rows * (dtype == EG_F32 ? 4 : 2), as_stream(stream), name);
+  }
   // without rows the weights' gradients (and a channel gate's) are zero, and nothing is read
   const bool gated = gate_kind == kChannel || (gate_kind && rows > 0);
   if (!dpost_weight || !dpre_weight || !post_weight || !pre_weight || (gated && (!gate || !dgate))) {

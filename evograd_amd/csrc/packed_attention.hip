@@ -253,9 +253,9 @@ int by_type(const PackedAttn& a, int dtype, F&& f) {
 }
 
 // Two key groups per workgroup (KG = 2), which halve a row block's chain of key tiles: for few
-// long walks. Forward, one group against two, bf16, by the grid (blocks of 128 rows times
-// heads): 128 heads of 128, one sequence of 2048 39 / 32 us; 256, one of 1024 25.6 / 23.2, 4 of 1024
-// 30.0 / 25.5; 384, 2 of 768 28.5 / 28.0; 512, one of 2048 50 / 52. Below 512 tokens a sequence it
+// long walks. Forward, one group against two, bf16, 8 and 32 heads of 128, by the grid (blocks of
+// 128 rows times heads): 128, one sequence of 2048 39 / 32 us; 256, one of 1024 25.6 / 23.2, 4 of
+// 1024 30.0 / 25.5; 384, 2 of 768 28.5 / 28.0; 512, one of 2048 50 / 52. Below 512 tokens a sequence it
 // costs more than it gives, most where the grid fills the CUs: 128, 4 of 128 10.8 / 12.3; 512, 4
 // of 512 25 / 36, 16 of 128 22 / 30. The host knows the mean length alone, which does not tell such
 // a batch from one long sequence among short ones (12 heads of 64, one of 1111 and 7 of 250 19.6 /

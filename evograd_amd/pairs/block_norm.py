@@ -16,7 +16,8 @@ bytes as reading a saved s.
 
 The backward takes ``dout`` as a [2, rows, cols] tensor or as the pair ``(ds, dy)``.
 ``BlockNorm.apply(x, h, post_weight, gate, pre_weight, scale, eps)`` -> ``(s, y)`` is the same
-pair as an autograd node with two outputs, whose gradients arrive separately.
+pair as an autograd node with two outputs, whose gradients arrive separately; it can be
+differentiated once.
 """
 
 from __future__ import annotations

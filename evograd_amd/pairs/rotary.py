@@ -154,7 +154,8 @@ def rotary_qk_backward_from_saved(grads, saved, amplitude: float = 1.0, interlea
 
 class RotaryQK(torch.autograd.Function):
     """The joint q/k pair as an autograd node: ``RotaryQK.apply(q, k, positions, freqs,
-    amplitude, interleaved)`` -> ``(q', k')``; positions and frequencies get no gradient."""
+    amplitude, interleaved)`` -> ``(q', k')``; positions and frequencies get no gradient, and
+    the node can be differentiated once."""
 
     @staticmethod
     def forward(ctx, q, k, positions, freqs, amplitude=1.0, interleaved=0):

@@ -265,8 +265,8 @@ __device__ __forceinline__ void zero_lds(void* p, int bytes) {
 // loops): where one is not finite, the walk is done again with the masked pairs left out
 // of the products (add_seen), so that such values reach the rows that see them and no
 // others. The second walk also takes what fp16 cannot hold: a dS past 65504 (the gradients of a
-// scaled loss) is infinite as an operand though dq and dk may be well in range, so there each
-// tile's dS is rounded as a multiple of a power of two (half_range). It is slow, a product per
+// scaled loss) is infinite as an operand though dq and dk may be well in range, so there a
+// row's or key's dS of a tile is rounded as a multiple of a power of two (half_range). It is slow, a product per
 // row: with one NaN in q, bf16 8192 tokens in 11 sequences 150 + 463 -> 204 + 2098 us.
 template <int DT>
 __device__ __forceinline__ bool all_finite(const f32x16 (&acc)[DT]) {
@@ -278,8 +278,9 @@ __device__ __forceinline__ bool all_finite(const f32x16 (&acc)[DT]) {
   return z == 0.f;
 }
 
-// fp16: scales w by the power of two that brings its largest finite value in the wave below 2^15,
-// if it is not, and returns that power's inverse.
+// fp16: scales the values of this lane's column (its own and those of the lane 32 on) by the power
+// of two that brings the largest finite one below 2^15, if it is not, and returns that power's
+// inverse. The product's column is this lane's too, so no other row's (dQ) or key's (dK) share it.
 template <typename T>
 __device__ __forceinline__ float half_range(f32x16& w) {
   if constexpr (!std::is_same_v<T, f16_t>) return 1.f;
@@ -289,7 +290,7 @@ __device__ __forceinline__ float half_range(f32x16& w) {
     const float x = __builtin_fabsf(w[r]);
     most = x < INFINITY ? fmaxf(most, x) : most;
   }
-  most = wave_reduce(most, MaxOp());
+  most = fmaxf(most, __shfl_xor(most, 32, 64));
   const int over = max(0, __builtin_amdgcn_frexp_expf(most) - 15);  // most < 2^(over + 15)
   const float back = ldexpf(1.f, over), to = ldexpf(1.f, -over);
 #pragma unroll

@@ -14,9 +14,9 @@ def takes_mfma(dtype, D):
 def attention64(q, k, v, do, lengths, half_range=False):
     """({name: (value, bound)} of o, dq, dk, dv, lse, the largest |dS|). The MFMA kernels round P and
     dS to the tensors' type before their products. delta of a sequence's first rows, whose keys fit
-    one tile, is sum p dp in fp32; the others' takes the stored o. ``half_range``: dS of a tile past
-    2^15 is rounded to fp16 as a multiple of the power of two that brings the tile's largest below
-    2^15."""
+    one tile, is sum p dp in fp32; the others' takes the stored o. ``half_range``: a row's or a key's
+    dS of a tile, past 2^15, is rounded to fp16 as a multiple of the power of two that brings the
+    largest below 2^15."""
     dt, mfma = q.dtype, takes_mfma(q.dtype, q.shape[2])
     tile = 64 if mfma else 32 if q.shape[2] <= 64 else 16
     q, k, v, do = (t.double() for t in (q, k, v, do))

@@ -144,3 +144,20 @@ def test_gradients_whose_products_pass_the_half_range(spoilt, lengths, H, KVH, D
     got = run(q, k, v, do, bounds(lengths))
     for name in ("o", "dq", "dk", "dv"):
         assert_within(name, got[name][keep], *(x[keep] for x in want[name]))
+
+
+@pytest.mark.parametrize("D", (64, 128))
+@pytest.mark.parametrize("lengths,row", (([50, 30], 20), ([200], 100)))
+def test_a_row_past_the_half_range_leaves_its_neighbours_theirs(lengths, row, D):
+    """Upstream gradients of one row far above the others', whose dS are small normal numbers."""
+    q, k, v, do = make(lengths, 2, 2, D, F16, seed=7)
+    v = (8.0 * v.float()).half()
+    do = (1e-5 * do.float()).half()
+    want, _ = attention64(q, k, v, do, lengths)
+    others = torch.arange(sum(lengths), device="cuda") != row
+    later = torch.arange(sum(lengths), device="cuda") > row  # keys that the row does not see
+    do[row] = 6e4
+    got = run(q, k, v, do, bounds(lengths))
+    assert_within("dq", got["dq"][others], *(x[others] for x in want["dq"]))
+    for name in ("dk", "dv"):
+        assert_within(name, got[name][later], *(x[later] for x in want[name]))

@@ -266,8 +266,9 @@ __device__ __forceinline__ void zero_lds(void* p, int bytes) {
 // of the products (add_seen), so that such values reach the rows that see them and no
 // others. The second walk also takes what fp16 cannot hold: a dS past 65504 (the gradients of a
 // scaled loss) is infinite as an operand though dq and dk may be well in range, so there a
-// row's or key's dS of a tile is rounded as a multiple of a power of two (half_range). It is slow, a product per
-// row: with one NaN in q, bf16 8192 tokens in 11 sequences 150 + 463 -> 204 + 2098 us.
+// row's or key's dS of a tile is rounded as a multiple of a power of two (half_range). It is
+// slow, a product per row: with one NaN in q, bf16 8192 tokens in 11 sequences 150 + 461 -> 203 +
+// 2063 us.
 template <int DT>
 __device__ __forceinline__ bool all_finite(const f32x16 (&acc)[DT]) {
   float z = 0.f;

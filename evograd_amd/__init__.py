@@ -10,7 +10,9 @@ Layout:
                 then grouped causal attention), cross_entropy, fused_linear_cross_entropy,
                 llama3_decoder_layer (one whole Llama-3 decoder layer), and the operators of
                 packed batches: packed_attention, rotary (a position per token), block_norm
-                (the norms around a block with its gate and residual scale)
+                (the norms around a block with its gate and residual scale), embedding,
+                norm_rotary (norms per head with the rotation) and topk_distillation (the
+                loss against a teacher's top logits)
 * ``pairs``     one module per operator with the reference's
                 ``<op>_forward_with_saved`` / ``<op>_backward_from_saved`` functions
 * ``bind``      ``bind(op, module)`` -> a ``torch.autograd.Function``-backed callable
@@ -35,6 +37,9 @@ PAIR_MODULES = {
     "packed_attention": "evograd_amd.pairs.packed_attention",
     "rotary": "evograd_amd.pairs.rotary",
     "block_norm": "evograd_amd.pairs.block_norm",
+    "embedding": "evograd_amd.pairs.embedding",
+    "norm_rotary": "evograd_amd.pairs.norm_rotary",
+    "topk_distillation": "evograd_amd.pairs.topk_distillation",
 }
 
 # Small-shape programs and the shape dispatchers that route to them below the

@@ -20,7 +20,7 @@ import torch  # noqa: F401  (loads the HIP runtime first; see module docstring)
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libevograd_hip.so")
 
 EG_F32, EG_F16, EG_BF16 = 0, 1, 2
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 _DTYPE_TAG = {
     torch.float32: EG_F32,
@@ -97,6 +97,19 @@ SIGNATURES: dict[str, tuple] = {
     "eg_block_norm_workspace_bytes": (_size, [_i64, _i64]),
     "eg_block_norm_bwd": (_i32, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64,
                                  _i64, _i32, _f32, _i32, _p]),
+    "eg_embedding_fwd": (_i32, [_p, _p, _i32, _p, _i64, _i64, _i64, _f32, _i64, _i32, _p]),
+    "eg_embedding_workspace_bytes": (_size, [_i64, _i64, _i64]),
+    "eg_embedding_bwd": (_i32, [_p, _p, _i32, _p, _p, _i64, _i64, _i64, _f32, _i64, _i32, _i32, _p]),
+    "eg_norm_rotary_fwd": (_i32, [_p, _p, _p, _p, _p, _p, _p, _i32, _p, _i64, _i64, _i64, _i64,
+                                  _i64, _p, _f32, _f32, _i32, _i32, _p]),
+    "eg_norm_rotary_workspace_bytes": (_size, [_i64, _i64, _i64, _i64]),
+    "eg_norm_rotary_bwd": (_i32, [_p, _p, _p, _p, _p, _p, _p, _i32, _p, _p, _p, _p, _p, _p, _i64,
+                                  _i64, _i64, _i64, _i64, _p, _f32, _f32, _i32, _i32, _p]),
+    "eg_topk_distill_workspace_bytes": (_size, [_i64, _i64]),
+    "eg_topk_distill_fwd": (_i32, [_p, _p, _p, _i32, _p, _i32, _p, _p, _p, _p, _p, _i64, _i64, _i64,
+                                   _f32, _f32, _f32, _i64, _i32, _p]),
+    "eg_topk_distill_bwd": (_i32, [_p, _p, _p, _p, _i32, _p, _p, _p, _p, _i64, _i64, _i64, _f32,
+                                   _f32, _f32, _i64, _i32, _p]),
     "eg_probe_mfma_bf16": (_i32, [_p, _p, _i32, _i32, _p]),
     "eg_probe_mfma_mix": (_i32, [_i32, _p, _p, _i32, _i32, _p]),
     "eg_gemm_segmented": (_i32, [_p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32,

@@ -1,0 +1,617 @@
+// Norms of queries and keys for each head with the position rotation behind them, for gfx950.
+//
+//   n = x rstd w,  rstd = rsqrt(mean(x^2) + eps) over a head's columns
+//   y = rotation of n by position * freq (amp (n1 c - n2 s, n2 c + n1 s)); columns past
+//       2 * pairs are n itself
+// in fp32, rounded once. Backward, with dn the transposed rotation of dy and xhat = x rstd:
+//   dx = rstd (dn w - xhat mean(dn w xhat)),  dw = sum over tokens and heads of dn xhat
+// rstd is formed again from x, which the backward reads anyway: its two sums over a head,
+// x^2 and dn w x, do not wait for one another.
+//
+// Layout: q [tokens, heads_q, head_dim] and k [tokens, heads_k, head_dim], head_dim contiguous,
+// other strides free, each with its own weight [head_dim]; outputs contiguous. A head lies in
+// `group` neighbouring lanes (a power of two), each with two packs of VEC columns: the two
+// halves of VEC pairs, or neighbours where pairs are interleaved or columns are not turned.
+// Neighbouring groups take neighbouring heads of a token, q's and then k's. Sines are formed
+// once for a workgroup's tokens, into LDS.
+//
+// Memory-bound: the forward reads x and writes y, the backward reads x and dy and writes dx.
+// The backward's workgroups walk the tokens, keep the sums for dw of their heads in registers
+// and leave one partial row each of q's and k's, which a second kernel adds in order.
+#include "rotary_angles.hpp"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace eg {
+namespace {
+
+constexpr int kMostThreads = 512;
+
+struct HeadArgs {
+  const void *q, *k, *dqo, *dko, *qw, *kw;
+  void *qo, *ko;  // y, or dx
+  void *dqw, *dkw;
+  float* part;  // [workgroups][2][head_dim]
+  const void* pos;
+  const double* freq;
+  int64_t tokens, q_token, q_head, k_token, k_head, dq_token, dq_head, dk_token, dk_head;
+  int heads_q, heads_k, head_dim, pairs, pos64;
+  int group, lanes, per_block;  // lanes of a head; heads along a token's threads; tokens
+  float amp, eps;
+};
+
+template <typename T, int VEC>
+__device__ __forceinline__ void get(const T* p, bool in, Pack<T, VEC>& v) {
+  if (in) v = *reinterpret_cast<const Pack<T, VEC>*>(p);
+}
+
+// Sum over the `group` lanes of a head, the same bits in each.
+__device__ __forceinline__ float group_sum(float v, int group) {
+  for (int off = 1; off < group; off <<= 1) v += __shfl_xor(v, off);
+  return v;
+}
+
+// A thread's place: token of the workgroup, first head, columns.
+template <int VEC, bool INTER>
+struct Place {
+  int tl, hl, c1, c2;
+  bool in, turn, one, two;  // of the workgroup's tokens; turned columns; has each of the packs
+  int pair;                 // first pair
+  __device__ __forceinline__ Place(const HeadArgs& a) {
+    const unsigned per = a.lanes * a.group;  // threads of a token
+    const unsigned e = blockIdx.y * blockDim.x + threadIdx.x;
+    tl = e / per;
+    const unsigned r = e - tl * per;
+    hl = r / a.group;
+    const int ch = r - hl * a.group, turned = a.pairs / VEC;
+    in = tl < a.per_block;
+    turn = ch < turned;
+    pair = ch * VEC;
+    c1 = !turn ? 2 * a.pairs + (ch - turned) * 2 * VEC : INTER ? 2 * ch * VEC : ch * VEC;
+    c2 = turn && !INTER ? c1 + a.pairs : c1 + VEC;
+    one = in && c1 < a.head_dim;
+    two = in && c2 < a.head_dim;
+  }
+};
+
+// The rows of head h (q's heads, then k's).
+struct Head {
+  bool isq, in;
+  int at;
+  __device__ __forceinline__ Head(const HeadArgs& a, int h) {
+    isq = h < a.heads_q;
+    at = isq ? h : h - a.heads_q;
+    in = isq || at < a.heads_k;
+  }
+  template <typename T>
+  __device__ __forceinline__ const T* x(const HeadArgs& a, int64_t t) const {
+    return isq ? (const T*)a.q + t * a.q_token + at * a.q_head
+               : (const T*)a.k + t * a.k_token + at * a.k_head;
+  }
+  template <typename T>
+  __device__ __forceinline__ const T* dy(const HeadArgs& a, int64_t t) const {
+    return isq ? (const T*)a.dqo + t * a.dq_token + at * a.dq_head
+               : (const T*)a.dko + t * a.dk_token + at * a.dk_head;
+  }
+  template <typename T>
+  __device__ __forceinline__ T* out(const HeadArgs& a, int64_t t) const {
+    return isq ? (T*)a.qo + (t * a.heads_q + at) * a.head_dim
+               : (T*)a.ko + (t * a.heads_k + at) * a.head_dim;
+  }
+  template <typename T>
+  __device__ __forceinline__ const T* weight(const HeadArgs& a) const {
+    return (const T*)(isq ? a.qw : a.kw);
+  }
+};
+
+// (cos, sin) of per_block tokens from t0 on.
+__device__ __forceinline__ void form_table(const HeadArgs& a, int64_t t0, float sign, float2* table) {
+  for (int i = threadIdx.x; i < a.per_block * a.pairs; i += blockDim.x) {
+    const int64_t t = min(t0 + i / a.pairs, a.tokens - 1);
+    table[i] = rotary_turn(rotary_position(a.pos, a.pos64, t), a.freq[i % a.pairs], a.amp, sign);
+  }
+}
+
+// Elements of pair i of a thread's two packs.
+template <int VEC, bool INTER>
+struct PairAt {
+  int u, v;  // of the 2 * VEC elements
+  __device__ __forceinline__ PairAt(int i) : u(INTER ? 2 * i : i), v(INTER ? 2 * i + 1 : VEC + i) {}
+};
+
+// Turns the packs in place.
+template <int VEC, bool INTER>
+__device__ __forceinline__ void turn_packs(const float2* table, float (&n)[2 * VEC]) {
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    const PairAt<VEC, INTER> p(i);
+    const float2 cs = table[i];
+    const float a = n[p.u], b = n[p.v];
+    n[p.u] = __builtin_fmaf(a, cs.x, -(b * cs.y));
+    n[p.v] = __builtin_fmaf(b, cs.x, a * cs.y);
+  }
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void widen(const Pack<T, VEC> (&raw)[2], bool one, bool two,
+                                      float (&f)[2 * VEC]) {
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    f[i] = one ? to_f32(raw[0].v[i]) : 0.f;
+    f[VEC + i] = two ? to_f32(raw[1].v[i]) : 0.f;
+  }
+}
+
+template <typename T, int VEC, bool INTER>
+__device__ __forceinline__ void put(T* row, const Place<VEC, INTER>& at, const float (&f)[2 * VEC]) {
+  float v[VEC];
+  if (at.one) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = f[i];
+    store_vec<T, VEC, true>(row + at.c1, v);
+  }
+  if (at.two) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = f[VEC + i];
+    store_vec<T, VEC, true>(row + at.c2, v);
+  }
+}
+
+template <typename T, int VEC, int HPT, bool INTER>
+__global__ __launch_bounds__(kMostThreads) void norm_rotary_fwd_kernel(HeadArgs a) {
+  const Place<VEC, INTER> at(a);
+  const int64_t t0 = (int64_t)blockIdx.x * a.per_block, t = t0 + at.tl;
+  const bool live = at.in && t < a.tokens;
+  Pack<T, VEC> raw[HPT][2], w[HPT][2];
+#pragma unroll
+  for (int j = 0; j < HPT; ++j) {
+    const Head h(a, at.hl + j * a.lanes);
+    if (!live || !h.in) continue;
+    const T* x = h.x<T>(a, t);
+    const T* g = h.weight<T>(a);
+    get<T, VEC>(x + at.c1, at.one, raw[j][0]);
+    get<T, VEC>(x + at.c2, at.two, raw[j][1]);
+    get<T, VEC>(g + at.c1, at.one, w[j][0]);
+    get<T, VEC>(g + at.c2, at.two, w[j][1]);
+  }
+  extern __shared__ float2 table[];
+  form_table(a, t0, 1.f, table);
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < HPT; ++j) {
+    const Head h(a, at.hl + j * a.lanes);
+    if (!live || !h.in) continue;
+    float x[2 * VEC], g[2 * VEC];
+    widen<T, VEC>(raw[j], at.one, at.two, x);
+    widen<T, VEC>(w[j], at.one, at.two, g);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2 * VEC; ++i) sum += x[i] * x[i];
+    const float rstd = rsqrtf(group_sum(sum, a.group) / a.head_dim + a.eps);
+#pragma unroll
+    for (int i = 0; i < 2 * VEC; ++i) x[i] = x[i] * rstd * g[i];
+    if (at.turn) turn_packs<VEC, INTER>(table + at.tl * a.pairs + at.pair, x);
+    put<T, VEC, INTER>(h.out<T>(a, t), at, x);
+  }
+}
+
+template <typename T, int VEC, int HPT, bool INTER>
+__global__ __launch_bounds__(kMostThreads) void norm_rotary_bwd_kernel(HeadArgs a) {
+  extern __shared__ float2 table[];  // of this step's tokens and the next's; sums at the end
+  const Place<VEC, INTER> at(a);
+  const int64_t stride = (int64_t)gridDim.x * a.per_block;
+  float acc[HPT][2 * VEC];
+#pragma unroll
+  for (int j = 0; j < HPT; ++j)
+#pragma unroll
+    for (int i = 0; i < 2 * VEC; ++i) acc[j][i] = 0.f;
+  Pack<T, VEC> rawx[HPT][2], rawd[HPT][2];
+  auto fetch = [&](int64_t t) {
+#pragma unroll
+    for (int j = 0; j < HPT; ++j) {
+      const Head h(a, at.hl + j * a.lanes);
+      if (t >= a.tokens || !h.in) continue;
+      const T *x = h.x<T>(a, t), *d = h.dy<T>(a, t);
+      get<T, VEC>(x + at.c1, at.one, rawx[j][0]);
+      get<T, VEC>(x + at.c2, at.two, rawx[j][1]);
+      get<T, VEC>(d + at.c1, at.one, rawd[j][0]);
+      get<T, VEC>(d + at.c2, at.two, rawd[j][1]);
+    }
+  };
+  int64_t t0 = (int64_t)blockIdx.x * a.per_block;
+  fetch(t0 + at.tl);
+  form_table(a, t0, -1.f, table);
+  __syncthreads();
+  for (int side = 0; t0 < a.tokens; t0 += stride, side ^= 1) {
+    const int64_t t = t0 + at.tl, next = t0 + stride;
+    const float2* turns = table + side * a.per_block * a.pairs + at.tl * a.pairs + at.pair;
+    float x[HPT][2 * VEC], d[HPT][2 * VEC];
+#pragma unroll
+    for (int j = 0; j < HPT; ++j) {
+      widen<T, VEC>(rawx[j], at.one, at.two, x[j]);
+      widen<T, VEC>(rawd[j], at.one, at.two, d[j]);
+    }
+    if (next < a.tokens) {
+      fetch(next + at.tl);
+      form_table(a, next, -1.f, table + (side ^ 1) * a.per_block * a.pairs);
+    }
+    if (at.in && t < a.tokens) {
+#pragma unroll
+      for (int j = 0; j < HPT; ++j) {
+        const Head h(a, at.hl + j * a.lanes);
+        if (!h.in) continue;
+        if (at.turn) turn_packs<VEC, INTER>(turns, d[j]);  // dn
+        Pack<T, VEC> w[2];
+        float g[2 * VEC], squares = 0.f, dot = 0.f;
+        get<T, VEC>(h.weight<T>(a) + at.c1, at.one, w[0]);
+        get<T, VEC>(h.weight<T>(a) + at.c2, at.two, w[1]);
+        widen<T, VEC>(w, at.one, at.two, g);
+#pragma unroll
+        for (int i = 0; i < 2 * VEC; ++i) {
+          squares += x[j][i] * x[j][i];
+          g[i] *= d[j][i];
+          dot += g[i] * x[j][i];
+        }
+        squares = group_sum(squares, a.group);
+        dot = group_sum(dot, a.group);
+        const float rstd = rsqrtf(squares / a.head_dim + a.eps), mean = dot * rstd / a.head_dim;
+#pragma unroll
+        for (int i = 0; i < 2 * VEC; ++i) {
+          const float xhat = x[j][i] * rstd;
+          acc[j][i] += d[j][i] * xhat;
+          g[i] = rstd * (g[i] - xhat * mean);
+        }
+        put<T, VEC, INTER>(h.out<T>(a, t), at, g);
+      }
+    }
+    __syncthreads();
+  }
+  // this workgroup's sums: the heads' rows, one after the other
+  float* rows = (float*)table;
+  const int heads = blockDim.x / a.group, me = threadIdx.x / a.group;
+  float* part = a.part + ((int64_t)blockIdx.x * gridDim.y + blockIdx.y) * 2 * a.head_dim;
+  const int per = a.lanes * a.group;
+  float sum[2] = {0.f, 0.f};
+  // column by column of the partial rows; head_dim may pass the workgroup's threads
+  for (int c0 = 0; c0 < a.head_dim; c0 += blockDim.x) {
+    sum[0] = sum[1] = 0.f;
+    const int c = c0 + threadIdx.x;
+#pragma unroll
+    for (int j = 0; j < HPT; ++j) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        if (at.one) rows[me * a.head_dim + at.c1 + i] = acc[j][i];
+        if (at.two) rows[me * a.head_dim + at.c2 + i] = acc[j][VEC + i];
+      }
+      __syncthreads();
+      if (c < a.head_dim)
+        for (int m = 0; m < heads; ++m) {
+          const int e = blockIdx.y * blockDim.x + m * a.group;
+          const Head h(a, e % per / a.group + j * a.lanes);
+          if (e / per < a.per_block && h.in) sum[!h.isq] += rows[m * a.head_dim + c];
+        }
+    }
+    if (c < a.head_dim) {
+      part[c] = sum[0];
+      part[a.head_dim + c] = sum[1];
+    }
+  }
+}
+
+// Heads of more than 64 lanes' packs (single columns of wide heads): a wave per head, which reads
+// its columns again for every step and forms its own sines. Column sums lie in LDS, each
+// column with the lane that works on it.
+constexpr int kWideWaves = 2048;
+
+template <typename T, bool INTER, bool BACK>
+__global__ __launch_bounds__(kWave) void norm_rotary_wide_kernel(HeadArgs a) {
+  extern __shared__ float2 table[];
+  float* sums = (float*)table;  // [2][head_dim]
+  const int lane = threadIdx.x;
+  const int64_t heads = a.heads_q + a.heads_k, items = a.tokens * heads;
+  if (BACK)
+    for (int c = lane; c < 2 * a.head_dim; c += kWave) sums[c] = 0.f;
+  __syncthreads();
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int64_t t = item / heads;
+    const Head h(a, (int)(item - t * heads));
+    const T *x = h.x<T>(a, t), *w = h.weight<T>(a), *d = BACK ? h.dy<T>(a, t) : nullptr;
+    T* out = h.out<T>(a, t);
+    const double pos = rotary_position(a.pos, a.pos64, t);
+    // f(first column, second or -1, the columns' dn) for every pair and single column
+    auto columns = [&](auto f) {
+      for (int p = lane; p < a.pairs; p += kWave) {
+        const int u = INTER ? 2 * p : p, v = INTER ? 2 * p + 1 : p + a.pairs;
+        const float2 cs = rotary_turn(pos, a.freq[p], a.amp, BACK ? -1.f : 1.f);
+        f(u, v, cs);
+      }
+      for (int c = 2 * a.pairs + lane; c < a.head_dim; c += kWave) f(c, -1, make_float2(1.f, 0.f));
+    };
+    // the two columns' dn
+    auto upstream = [&](int u, int v, float2 cs, float& du, float& dv) {
+      const float p = to_f32(d[u]), r = v < 0 ? 0.f : to_f32(d[v]);
+      du = __builtin_fmaf(p, cs.x, -(r * cs.y));
+      dv = __builtin_fmaf(r, cs.x, p * cs.y);
+    };
+    float squares = 0.f, dot = 0.f;
+    columns([&](int u, int v, float2 cs) {
+      const float xu = to_f32(x[u]), xv = v < 0 ? 0.f : to_f32(x[v]);
+      squares += xu * xu + xv * xv;
+      if constexpr (BACK) {
+        float du, dv;
+        upstream(u, v, cs, du, dv);
+        dot += du * to_f32(w[u]) * xu;
+        if (v >= 0) dot += dv * to_f32(w[v]) * xv;
+      }
+    });
+    const float rstd = rsqrtf(wave_reduce(squares, SumOp()) / a.head_dim + a.eps);
+    const float mean = BACK ? wave_reduce(dot, SumOp()) * rstd / a.head_dim : 0.f;
+    float* sum = sums + (h.isq ? 0 : a.head_dim);
+    columns([&](int u, int v, float2 cs) {
+      const float xu = to_f32(x[u]) * rstd, xv = v < 0 ? 0.f : to_f32(x[v]) * rstd;
+      const float wu = to_f32(w[u]), wv = v < 0 ? 0.f : to_f32(w[v]);
+      if constexpr (BACK) {
+        float du, dv;
+        upstream(u, v, cs, du, dv);
+        sum[u] += du * xu;
+        out[u] = from_f32<T>(rstd * (du * wu - xu * mean));
+        if (v >= 0) {
+          sum[v] += dv * xv;
+          out[v] = from_f32<T>(rstd * (dv * wv - xv * mean));
+        }
+      } else {
+        const float p = xu * wu, r = xv * wv;
+        out[u] = from_f32<T>(__builtin_fmaf(p, cs.x, -(r * cs.y)));
+        if (v >= 0) out[v] = from_f32<T>(__builtin_fmaf(r, cs.x, p * cs.y));
+      }
+    });
+  }
+  if (BACK) {
+    __syncthreads();
+    float* part = a.part + (int64_t)blockIdx.x * 2 * a.head_dim;
+    for (int c = lane; c < 2 * a.head_dim; c += kWave) part[c] = sums[c];
+  }
+}
+
+// The weights' gradients from the partial rows: 16 columns a workgroup, its rows dealt to 64
+// adders whose sums are added in order.
+constexpr int kSumCols = 16, kSumRows = 64;
+template <typename T>
+__global__ __launch_bounds__(kSumCols* kSumRows) void norm_rotary_sum_kernel(HeadArgs a, int parts) {
+  __shared__ float sums[kSumRows][kSumCols];
+  const int lane = threadIdx.x % kSumCols, adder = threadIdx.x / kSumCols;
+  const int c = blockIdx.x * kSumCols + lane, cols = 2 * a.head_dim;
+  float s = 0.f;
+  if (c < cols) {
+#pragma unroll 4
+    for (int r = adder; r < parts; r += kSumRows) s += a.part[(int64_t)r * cols + c];
+  }
+  sums[adder][lane] = s;
+  __syncthreads();
+#pragma unroll
+  for (int n = kSumRows / 2; n >= 1; n /= 2) {
+    if (adder < n) sums[adder][lane] = s += sums[adder + n][lane];
+    __syncthreads();
+  }
+  if (adder != 0 || c >= cols) return;
+  if (c < a.head_dim) ((T*)a.dqw)[c] = from_f32<T>(s);
+  else if (a.dkw) ((T*)a.dkw)[c - a.head_dim] = from_f32<T>(s);
+}
+
+// The backward's workgroups, a partial row each: as many as a card holds at once, or as many as
+// one token's heads take.
+constexpr int64_t kBackBlocks = 1024;
+
+// How a call's heads lie on threads: 0 lanes if a head does not fit a wave.
+struct Shape {
+  int group, lanes, per_block, threads;
+  int64_t gx, gy;
+};
+Shape shape_of(const HeadArgs& a, int vec, int hpt) {
+  Shape s = {};
+  const int64_t heads = a.heads_q + a.heads_k;
+  const int chunks = a.pairs / vec + (a.head_dim - 2 * a.pairs + 2 * vec - 1) / (2 * vec);
+  s.group = 1;
+  while (s.group < chunks) s.group *= 2;
+  if (s.group > kWave) return s;
+  s.lanes = (int)((heads + hpt - 1) / hpt);
+  // As many whole tokens as fill the waves of a workgroup best, from 256 threads on; a token of
+  // more than 512 threads lies over several workgroups.
+  const int64_t per = (int64_t)s.group * s.lanes;
+  int64_t best = std::max<int64_t>(1, 256 / per), unused = 64;
+  for (int64_t n = best; n * per <= kMostThreads; ++n) {
+    const int64_t idle = (64 - n * per % 64) % 64;
+    if (idle < unused) best = n, unused = idle;
+  }
+  s.per_block = (int)best;
+  const int64_t used = best * per;
+  s.gy = (used + kMostThreads - 1) / kMostThreads;
+  s.threads = (int)((used + 64 * s.gy - 1) / (64 * s.gy)) * 64;
+  s.gx = (a.tokens + s.per_block - 1) / s.per_block;
+  return s;
+}
+
+// go(VEC) with the widest pack (at most 16 bytes) that divides the halves, the head and every
+// stride, and to which the tensors are aligned.
+template <typename T, int VEC, typename F>
+int by_width(const HeadArgs& a, F&& go) {
+  if constexpr (VEC > 1) {
+    bool fits = a.pairs % VEC == 0 && a.head_dim % VEC == 0;
+    for (int64_t s : {a.q_token, a.q_head, a.k_token, a.k_head, a.dq_token, a.dq_head, a.dk_token,
+                      a.dk_head})
+      fits = fits && s % VEC == 0;
+    for (const void* p : {a.q, a.k, a.dqo, a.dko, a.qw, a.kw, (const void*)a.qo, (const void*)a.ko})
+      fits = fits && (uintptr_t)p % (VEC * sizeof(T)) == 0;
+    if (!fits) return by_width<T, VEC / 2>(a, go);
+  }
+  return go(std::integral_constant<int, VEC>{});
+}
+
+template <typename F>
+int by_layout(bool interleaved, F&& f) {
+  return interleaved ? f(std::true_type{}) : f(std::false_type{});
+}
+
+int check(const char* name, int64_t tokens, int64_t heads_q, int64_t heads_k, int64_t head_dim,
+          int64_t pairs, const int64_t* strides, int n) {
+  if (tokens < 0 || heads_q < 0 || heads_k < 0 || head_dim < 0) {
+    set_error("%s: negative size", name);
+    return 1;
+  }
+  if (pairs < 0 || 2 * pairs > head_dim) {
+    set_error("%s: %lld pairs do not fit head_dim %lld", name, (long long)pairs,
+              (long long)head_dim);
+    return 1;
+  }
+  if (heads_q > (1 << 16) || heads_k > (1 << 16) || head_dim > (1 << 13) ||
+      tokens > ((int64_t)1 << 32)) {
+    set_error("%s: size out of range (heads <= 65536, head_dim <= 8192, tokens <= 2^32)", name);
+    return 1;
+  }
+  if (!strides) { set_error("%s: null strides", name); return 1; }
+  for (int i = 0; i < n; ++i) {  // token steps and head steps
+    const int bits = i % 2 ? 40 : 32;
+    if (strides[i] < 0 || strides[i] > ((int64_t)1 << bits)) {
+      set_error("%s: strides must be at least 0 and at most 2^32 (tokens) or 2^40 (heads) elements",
+                name);
+      return 1;
+    }
+  }
+  return 0;
+}
+
+int64_t part_rows(int64_t tokens, int64_t heads) {
+  // a token of more than 512 threads (64 lanes a head at most) takes several workgroups
+  return tokens ? std::max<int64_t>({kBackBlocks, (heads * kWave + kMostThreads - 1) / kMostThreads,
+                                     kWideWaves})
+                : 0;
+}
+
+}  // namespace
+}  // namespace eg
+
+using namespace eg;
+
+extern "C" int eg_norm_rotary_fwd(const void* q, const void* k, const void* q_weight,
+                                  const void* k_weight, void* q_out, void* k_out,
+                                  const void* positions, int positions_64, const double* freqs,
+                                  int64_t tokens, int64_t heads_q, int64_t heads_k,
+                                  int64_t head_dim, int64_t pairs, const int64_t* strides,
+                                  float eps, float amplitude, int interleaved, int dtype,
+                                  void* stream) {
+  static const char* name = "eg_norm_rotary_fwd";
+  clear_error();
+  if (check(name, tokens, heads_q, heads_k, head_dim, pairs, strides, 4)) return 1;
+  if (tokens == 0 || head_dim == 0 || heads_q + heads_k == 0) return 0;
+  if ((heads_q && (!q || !q_weight || !q_out)) || (heads_k && (!k || !k_weight || !k_out)) ||
+      !positions || (pairs && !freqs)) {
+    set_error("%s: null pointer", name);
+    return 1;
+  }
+  HeadArgs a = {};
+  a.q = q, a.k = heads_k ? k : nullptr, a.qw = q_weight, a.kw = heads_k ? k_weight : nullptr;
+  a.qo = q_out, a.ko = heads_k ? k_out : nullptr, a.pos = positions, a.freq = freqs;
+  a.tokens = tokens;
+  a.q_token = strides[0], a.q_head = strides[1], a.k_token = strides[2], a.k_head = strides[3];
+  a.heads_q = (int)heads_q, a.heads_k = (int)heads_k, a.head_dim = (int)head_dim;
+  a.pairs = (int)pairs, a.pos64 = positions_64, a.amp = amplitude, a.eps = eps;
+  return EG_DISPATCH_FLOAT(dtype, name, [&]() -> int {
+    using T = scalar_t;
+    return by_layout(interleaved, [&](auto inter) -> int {
+      constexpr bool I = decltype(inter)::value;
+      return by_width<T, 16 / (int)sizeof(T)>(a, [&](auto vec) -> int {
+        constexpr int V = decltype(vec)::value;
+        auto go = [&](auto hpt) -> int {
+          constexpr int N = decltype(hpt)::value;
+          const Shape s = shape_of(a, V, N);
+          a.group = s.group, a.lanes = s.lanes, a.per_block = s.per_block;
+          if (s.gx > 0x7fffffffLL || s.gy > 65535 || check_grid(name, s.gx, s.threads)) {
+            set_error("%s: grid too large", name);
+            return 1;
+          }
+          EG_LAUNCH((norm_rotary_fwd_kernel<T, V, N, I>), dim3((unsigned)s.gx, (unsigned)s.gy),
+                    dim3(s.threads), a.per_block * a.pairs * sizeof(float2), as_stream(stream), a);
+          return check_launch(name);
+        };
+        if (shape_of(a, V, 1).lanes == 0) {
+          const int64_t waves = std::min<int64_t>(tokens * (heads_q + heads_k), kWideWaves);
+          EG_LAUNCH((norm_rotary_wide_kernel<T, I, false>), dim3((unsigned)waves), dim3(kWave), 0,
+                    as_stream(stream), a);
+          return check_launch(name);
+        }
+        return go(std::integral_constant<int, 1>{});
+      });
+    });
+  });
+}
+
+extern "C" size_t eg_norm_rotary_workspace_bytes(int64_t tokens, int64_t heads_q, int64_t heads_k,
+                                                 int64_t head_dim) {
+  if (tokens <= 0 || heads_q < 0 || heads_k < 0 || head_dim <= 0) return 0;
+  return (size_t)part_rows(tokens, heads_q + heads_k) * 2 * head_dim * sizeof(float);
+}
+
+extern "C" int eg_norm_rotary_bwd(const void* dq_out, const void* dk_out, const void* q,
+                                  const void* k, const void* q_weight, const void* k_weight,
+                                  const void* positions, int positions_64, const double* freqs,
+                                  void* dq, void* dk, void* dq_weight, void* dk_weight,
+                                  void* workspace, int64_t tokens, int64_t heads_q,
+                                  int64_t heads_k, int64_t head_dim, int64_t pairs,
+                                  const int64_t* strides, float eps, float amplitude,
+                                  int interleaved, int dtype, void* stream) {
+  static const char* name = "eg_norm_rotary_bwd";
+  clear_error();
+  if (check(name, tokens, heads_q, heads_k, head_dim, pairs, strides, 8)) return 1;
+  if (head_dim == 0) return 0;
+  const bool some = tokens > 0 && heads_q + heads_k > 0;
+  if (!dq_weight || (heads_k && !dk_weight) ||
+      (some && (!positions || (pairs && !freqs) || !workspace)) ||
+      (some && heads_q && (!dq_out || !q || !q_weight || !dq)) ||
+      (some && heads_k && (!dk_out || !k || !k_weight || !dk))) {
+    set_error("%s: null pointer", name);
+    return 1;
+  }
+  HeadArgs a = {};
+  a.dqo = dq_out, a.q = q, a.qw = q_weight, a.qo = dq, a.dqw = dq_weight;
+  a.dkw = dk_weight;  // of no heads: zeros
+  if (heads_k) a.dko = dk_out, a.k = k, a.kw = k_weight, a.ko = dk;
+  a.part = (float*)workspace, a.pos = positions, a.freq = freqs, a.tokens = tokens;
+  a.q_token = strides[0], a.q_head = strides[1], a.k_token = strides[2], a.k_head = strides[3];
+  a.dq_token = strides[4], a.dq_head = strides[5], a.dk_token = strides[6], a.dk_head = strides[7];
+  a.heads_q = (int)heads_q, a.heads_k = (int)heads_k, a.head_dim = (int)head_dim;
+  a.pairs = (int)pairs, a.pos64 = positions_64, a.amp = amplitude, a.eps = eps;
+  return EG_DISPATCH_FLOAT(dtype, name, [&]() -> int {
+    using T = scalar_t;
+    int parts = 0;
+    if (some) {
+      const int rc = by_layout(interleaved, [&](auto inter) -> int {
+        constexpr bool I = decltype(inter)::value;
+        return by_width<T, 16 / (int)sizeof(T)>(a, [&](auto vec) -> int {
+          constexpr int V = decltype(vec)::value;
+          Shape s = shape_of(a, V, 1);
+          if (s.lanes == 0) {
+            parts = (int)std::min<int64_t>(tokens * (heads_q + heads_k), kWideWaves);
+            EG_LAUNCH((norm_rotary_wide_kernel<T, I, true>), dim3((unsigned)parts), dim3(kWave),
+                      2 * head_dim * sizeof(float), as_stream(stream), a);
+            return check_launch(name);
+          }
+          a.group = s.group, a.lanes = s.lanes, a.per_block = s.per_block;
+          s.gx = std::min(s.gx, std::max<int64_t>(1, kBackBlocks / s.gy));
+          if (s.gy > 65535) { set_error("%s: grid too large", name); return 1; }
+          parts = (int)(s.gx * s.gy);
+          const size_t lds = std::max<size_t>(2 * a.per_block * a.pairs * sizeof(float2),
+                                              (size_t)s.threads / s.group * head_dim * sizeof(float));
+          EG_LAUNCH((norm_rotary_bwd_kernel<T, V, 1, I>), dim3((unsigned)s.gx, (unsigned)s.gy),
+                    dim3(s.threads), lds, as_stream(stream), a);
+          return check_launch(name);
+        });
+      });
+      if (rc) return rc;
+    }
+    EG_LAUNCH((norm_rotary_sum_kernel<T>), dim3((unsigned)((2 * head_dim + kSumCols - 1) / kSumCols)),
+              dim3(kSumCols * kSumRows), 0, as_stream(stream), a, parts);
+    return check_launch(name);
+  });
+}

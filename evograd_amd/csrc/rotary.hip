@@ -6,11 +6,8 @@
 // interleaved one; columns past 2 * pairs are copied. The backward is the transpose,
 // amp (dy1 c + dy2 s, dy2 c - dy1 s).
 //
-// Angles: a position of a long context times a frequency leaves few bits of an fp32 product
-// behind its whole turns (at position 131072 an fp32 angle is off by 0.004), so the turns
-// pos * freq / 2 pi are formed in fp64 and reduced there to an eighth of a turn; only that
-// remainder is rounded to fp32 for the sine and cosine. A workgroup forms them once for its
-// tokens, into LDS, while its loads are on their way, and uses them for every head.
+// Angles are formed and reduced in fp64 (rotary_angles.hpp). A workgroup forms the sines once for
+// its tokens, into LDS, while its loads are on their way, and uses them for every head.
 //
 // Layout: q [tokens, heads_q, head_dim] and k [tokens, heads_k, head_dim], head_dim
 // contiguous, other strides free; outputs contiguous. A thread owns a chunk of VEC pairs of one
@@ -23,7 +20,7 @@
 // Memory-bound: each element is read and written once. bf16 32768 tokens, 32 + 8 heads of 128:
 // 115 us each way, 5.9 TB/s; fp16 5003 tokens, 16 + 16 heads of 96, 64 columns interleaved:
 // 13 us each way; 32 tokens 4 us, a launch.
-#include "eg_common.hpp"
+#include "rotary_angles.hpp"
 
 #include <algorithm>
 #include <type_traits>
@@ -104,16 +101,7 @@ __global__ __launch_bounds__(kMostThreads) void rotary_kernel(RotaryArgs a) {
   const int64_t t0 = (int64_t)blockIdx.x * a.per_block;
   for (int i = threadIdx.x; i < a.per_block * a.pairs; i += blockDim.x) {
     const int64_t tok = min(t0 + i / a.pairs, a.tokens - 1);
-    const double pos =
-        a.pos64 ? (double)((const int64_t*)a.pos)[tok] : (double)((const int*)a.pos)[tok];
-    // explicit fma, here and below: every width of packs gives the same bits
-    const double f = a.freq[i % a.pairs] * 0.15915494309189533577;
-    const double rest = __builtin_fma(pos, f, -rint(pos * f)), quarter = rint(4.0 * rest);
-    float s0, c0;
-    sincospif(2.f * (float)__builtin_fma(-0.25, quarter, rest), &s0, &c0);
-    const int n = (int)quarter & 3;  // s0, c0 turned by n quarters
-    const float s1 = n & 1 ? c0 : s0, c1 = n & 1 ? s0 : c0;
-    table[i] = make_float2(a.amp * ((n + 1) & 2 ? -c1 : c1), a.amp * a.sign * (n & 2 ? -s1 : s1));
+    table[i] = rotary_turn(rotary_position(a.pos, a.pos64, tok), a.freq[i % a.pairs], a.amp, a.sign);
   }
   __syncthreads();
   if (!live) return;

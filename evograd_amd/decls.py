@@ -19,8 +19,9 @@ drop-in the reference's harness looks up:
   declared here the way an external ``--declaration path.py:op`` would be
   (src/evograd/opdecl/verify_cli.py:35-38).
 
-* packed_attention, rotary and block_norm, the operators of packed batches, have no
-  counterpart in the reference; they are declared the same way.
+* packed_attention, rotary and block_norm, the operators of packed batches, and embedding,
+  norm_rotary and topk_distillation, those of a distillation step, have no counterpart in the
+  reference; they are declared the same way.
 
 Differences from the reference declarations, all deliberate:
 
@@ -815,11 +816,148 @@ BLOCK_NORM = declare_op(
     regime_split=LLAMA_REGIME_SPLIT,
 )
 
+# ------------------------------------------------- operators of a distillation step
+# From tokens to the loss against a teacher's stored top logits; oracle in fp64.
+def _embed(T, vocab, hidden, dtype, label="", **extra):
+    return Workload(dims=dict(T=T, vocab=vocab, hidden=hidden), dtype=dtype, label=label, extra=extra)
+
+
+EMBEDDING = declare_op(
+    name="embedding",
+    forward="oracle.forward_refs:embedding_forward_ref",
+    dims=("T", "vocab", "hidden"),
+    args=(
+        Active("weight", "[vocab, hidden]"),
+        Inactive("ids", "[T]", dtype="int32"),
+        Inactive("scale", default=1.0),
+        Inactive("ignore_index", default=-100),
+    ),
+    output=Active("out", "[T, hidden]"),
+    forward_semantics=(
+        "out[t] = scale * weight[ids[t]], rounded once; zeros where ids[t] is ignore_index, NaN "
+        "where it is otherwise outside [0, vocab)."
+    ),
+    backward_semantics=(
+        "dweight[v] = scale * sum of dout[t] over the tokens with ids[t] == v, fp32 accumulation "
+        "in a fixed order; every row is written."
+    ),
+    reference_dtype="float64",
+    correctness=tuple(
+        _embed(T, vocab, hidden, dt, **extra)
+        for T, vocab, hidden, extra in (
+            (1, 5, 8, {}),
+            (77, 100, 64, {"scale": 8.0}),
+            (300, 1000, 127, {"ignore_every": 7}),
+            (2000, 37, 96, {"same": 3}),
+        )
+        for dt in ("float32", "float16", "bfloat16")
+    ),
+    benchmark=(
+        _embed(16384, 128256, 4096, "bfloat16", label="llama3_8b"),
+    ),
+    tolerances=TOLERANCES,
+    make_inputs="evograd_amd.inputs:make_embedding_inputs",
+    memory_inputs=("weight",),
+    regime_feature=_tokens_feature,
+    regime_split=LLAMA_REGIME_SPLIT,
+)
+
+NORM_ROTARY = declare_op(
+    name="norm_rotary",
+    forward="oracle.forward_refs:norm_rotary_forward_ref",
+    dims=("T", "n_heads", "head_dim", "pairs"),
+    args=(
+        Active("x", "[T, n_heads, head_dim]"),
+        Active("weight", "[head_dim]"),
+        Inactive("positions", "[T]", dtype="int32", note="each token's own position"),
+        Inactive("freqs", "[pairs]", dtype="float64", note="radians per position"),
+        Inactive("eps", default=1e-6),
+        Inactive("amplitude", default=1.0),
+        Inactive("interleaved", default=0, note="pairs (2i, 2i + 1), not (i, i + pairs)"),
+    ),
+    output=Active("y", "[T, n_heads, head_dim]"),
+    forward_semantics=(
+        "n = x * rsqrt(mean(x^2) + eps) * weight over each head's columns, then rotary of n, in "
+        "fp32, cast back once."
+    ),
+    backward_semantics="Return dx and dweight, summed over tokens and heads in fp32.",
+    reference_dtype="float64",
+    correctness=tuple(
+        _rotary(T, H, D, n, dt, interleaved=inter, amplitude=amp, far=far)
+        for T, H, D, n, inter, amp, far in (
+            (1, 4, 128, 64, 0, 1.0, 1 << 20),
+            (37, 6, 64, 16, 1, 1.0, 4096),
+            (129, 3, 80, 20, 0, 1.25, 131072),
+            (16, 5, 10, 3, 1, 0.5, 100),
+        )
+        for dt in ("float32", "float16", "bfloat16")
+    ),
+    benchmark=(
+        _rotary(8192, 32, 128, 64, "bfloat16", label="llama3_8b_packed", far=8192),
+    ),
+    tolerances=TOLERANCES,
+    make_inputs="evograd_amd.inputs:make_norm_rotary_inputs",
+    memory_inputs=("x",),
+    regime_feature=_tokens_feature,
+    regime_split=LLAMA_REGIME_SPLIT,
+)
+
+
+def _distill(rows, cols, entries, dtype, label="", **extra):
+    return Workload(dims=dict(rows=rows, cols=cols, entries=entries), dtype=dtype, label=label,
+                    extra=extra)
+
+
+TOPK_DISTILLATION = declare_op(
+    name="topk_distillation",
+    forward="oracle.forward_refs:topk_distillation_forward_ref",
+    dims=("rows", "cols", "entries"),
+    args=(
+        Active("logits", "[rows, cols]"),
+        Inactive("target", "[rows]", dtype="int64"),
+        Inactive("teacher_logits", "[rows, entries]", dtype="float32"),
+        Inactive("teacher_ids", "[rows, entries]", dtype="int32"),
+        Inactive("temperature", default=1.0),
+        Inactive("soft_weight", default=1.0),
+        Inactive("hard_weight", default=0.0),
+        Inactive("ignore_index", default=-100),
+    ),
+    output=Active("loss", "[]"),
+    forward_semantics=(
+        "Mean over rows whose target is not ignore_index of soft_weight * tau^2 * sum p (log p - "
+        "log q[ids]) + hard_weight * (logsumexp(logits) - logits[target]), p the softmax of the "
+        "teacher's entries / tau (negative ids are none), q that of logits / tau; fp32 loss."
+    ),
+    backward_semantics=(
+        "dlogits = dloss / n_valid * (hard_weight (softmax(logits) - onehot(target)) + soft_weight "
+        "tau (q - sum of p at their tokens)), zero on ignored rows."
+    ),
+    reference_dtype="float64",
+    correctness=(
+        _distill(8, 512, 4, "float32"),
+        _distill(16, 1000, 33, "float32", temperature=2.0, hard=0.5),
+        _distill(32, 4099, 64, "float16", temperature=2.0, hard=0.5, cut=True),
+        _distill(64, 2048, 16, "bfloat16", temperature=0.7, ignore_every=3),
+        _distill(3, 50257, 20, "bfloat16", hard=1.0),
+        _distill(4, 128256, 64, "bfloat16", temperature=4.0, hard=0.1),
+        _distill(5, 127, 127, "float32", temperature=1.5, cut=True),
+    ),
+    benchmark=(
+        _distill(8192, 128256, 64, "bfloat16", label="llama3_8b", temperature=2.0, hard=0.5),
+    ),
+    tolerances=TOLERANCES,
+    make_inputs="evograd_amd.inputs:make_topk_distillation_inputs",
+    memory_inputs=("logits",),
+    regime_feature=_rows_feature,
+    regime_split=LLAMA_VOCAB_REGIME_SPLIT,
+)
+
 OPS: dict[str, OpDecl] = {
     op.name: op
     for op in (SOFTMAX, RMSNORM, LAYERNORM, SWIGLU, ROPE, CAUSAL_ATTENTION, FUSED_ADD_RMS_NORM,
                CAUSAL_ATTENTION_GQA, LLAMA3_ATTENTION, CROSS_ENTROPY, FUSED_LINEAR_CROSS_ENTROPY,
-               LLAMA3_DECODER_LAYER, PACKED_ATTENTION, ROTARY, BLOCK_NORM)
+               LLAMA3_DECODER_LAYER, PACKED_ATTENTION, ROTARY, BLOCK_NORM, EMBEDDING, NORM_ROTARY,
+               TOPK_DISTILLATION)
 }
 
 

@@ -316,6 +316,58 @@ def make_block_norm_inputs(op, workload, device="cuda"):
             "dout": around(0.0, 1.0, 2, rows, cols)}
 
 
+def make_embedding_inputs(op, workload, device="cuda"):
+    """Generic seed; weight ~ N(0,1), ids uniform in [0, vocab), dout ~ N(0,1), drawn in that
+    order. ``extra``: scale; ``ignore_every`` k sets tokens 0, k, 2k, ... to -100; ``same`` k
+    sets every k-th token to vocab // 2."""
+    d = workload.dims
+    dt = resolve_dtype(workload.dtype)
+    torch.manual_seed(case_seed(workload))
+    weight = torch.randn((d["vocab"], d["hidden"]), device=device, dtype=dt)
+    ids = torch.randint(0, d["vocab"], (d["T"],), device=device, dtype=torch.int32)
+    dout = torch.randn((d["T"], d["hidden"]), device=device, dtype=dt)
+    if workload.extra.get("same"):
+        ids[::int(workload.extra["same"])] = d["vocab"] // 2
+    if workload.extra.get("ignore_every"):
+        ids[::int(workload.extra["ignore_every"])] = -100
+    return {"weight": weight, "ids": ids, "scale": float(workload.extra.get("scale", 1.0)),
+            "ignore_index": -100, "dout": dout}
+
+
+def make_norm_rotary_inputs(op, workload, device="cuda"):
+    """make_rotary_inputs with a weight 1 + 0.1 N(0,1) [head_dim], drawn last in fp32 then cast."""
+    out = make_rotary_inputs(op, workload, device)
+    dt = resolve_dtype(workload.dtype)
+    weight = 1.0 + 0.1 * torch.randn((workload.dims["head_dim"],), device=device)
+    return {**out, "weight": weight.to(dt), "eps": 1e-6}
+
+
+def make_topk_distillation_inputs(op, workload, device="cuda"):
+    """Generic seed; logits ~ N(0,1), targets uniform, teacher logits 2 N(0,1) and as many distinct
+    columns a row in ascending order, dloss = 1; drawn in that order. ``extra``: temperature, hard
+    (hard_weight, soft_weight being 1), ``cut``: row r keeps its first r % (entries + 1) entries,
+    ``ignore_every`` k sets targets 0, k, 2k, ... to -100."""
+    d, extra = workload.dims, workload.extra
+    rows, cols, entries = d["rows"], d["cols"], d["entries"]
+    dt = resolve_dtype(workload.dtype)
+    torch.manual_seed(case_seed(workload))
+    logits = torch.randn((rows, cols), device=device, dtype=dt)
+    target = torch.randint(0, cols, (rows,), device=device, dtype=torch.int64)
+    teacher = 2.0 * torch.randn((rows, entries), device=device)
+    ids = torch.randint(0, cols - entries + 1, (rows, entries), device=device).sort(1).values
+    ids += torch.arange(entries, device=device)
+    if extra.get("cut"):
+        kept = torch.arange(rows, device=device) % (entries + 1)
+        ids[torch.arange(entries, device=device) >= kept[:, None]] = -1
+    if extra.get("ignore_every"):
+        target[::int(extra["ignore_every"])] = -100
+    return {"logits": logits, "target": target, "teacher_logits": teacher,
+            "teacher_ids": ids.to(torch.int32),
+            "temperature": float(extra.get("temperature", 1.0)), "soft_weight": 1.0,
+            "hard_weight": float(extra.get("hard", 0.0)), "ignore_index": -100,
+            "dloss": torch.ones((), device=device)}
+
+
 RECIPES = {
     "make_softmax_inputs": make_softmax_inputs,
     "make_rmsnorm_inputs": make_rmsnorm_inputs,
@@ -332,6 +384,9 @@ RECIPES = {
     "make_packed_attention_inputs": make_packed_attention_inputs,
     "make_rotary_inputs": make_rotary_inputs,
     "make_block_norm_inputs": make_block_norm_inputs,
+    "make_embedding_inputs": make_embedding_inputs,
+    "make_norm_rotary_inputs": make_norm_rotary_inputs,
+    "make_topk_distillation_inputs": make_topk_distillation_inputs,
 }
 
 

@@ -1,0 +1,158 @@
+"""Norms of queries and keys for each head with the position rotation behind them, on gfx950.
+
+x is [tokens, heads, head_dim], ``weight`` [head_dim] and ``positions`` [tokens] each token's own
+position. Per head, in one pass:
+
+    n = x * rsqrt(mean(x^2) + eps) * weight
+    y = n rotated by position * freqs over the first 2 * len(freqs) columns
+
+with the rotation, pairs and ``freqs`` of the ``rotary`` pair (fp64, from
+``rotary.rotary_frequencies``), whose ``amplitude`` scales the rotated columns alone. Sums and
+angles as there; y is rounded once. Saved state: ``(x, weight, positions, freqs)``, the caller's
+tensors: the backward forms the norms again from x, which it reads anyway, and so takes eps.
+
+``norm_rotary_qk_forward_with_saved`` / ``norm_rotary_qk_backward_from_saved`` take the query and
+key tensors of a layer, each with its weight, in one launch. x, q, k and the upstream gradients may
+be strided as long as a head's columns are contiguous; the results are contiguous.
+"""
+
+from __future__ import annotations
+
+if not __package__:
+    # Loaded from this file's path as a top-level candidate module (evograd's verify
+    # and bench commands load a program that way): put the package root on sys.path.
+    import pathlib as _pathlib
+    import sys as _sys
+
+    _ROOT = str(_pathlib.Path(__file__).resolve().parents[2])
+    if _ROOT not in _sys.path:
+        _sys.path.insert(0, _ROOT)
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from evograd_amd import _lib
+from evograd_amd.pairs._util import (as_contiguous, check_same, contiguous_like, head_rows,
+                                     strides_arg, tag, workspace)
+from evograd_amd.pairs.rotary import _check as _check_positions
+
+
+def _check(name, x, weight, positions, freqs):
+    _check_positions(name, x, positions, freqs)
+    if weight.dim() != 1 or weight.shape[0] != x.shape[2]:
+        raise ValueError(f"{name}: the weight must be [head_dim]={x.shape[2]}, got "
+                         f"{tuple(weight.shape)}")
+    check_same(name, x, weight)
+
+
+def _check_qk(name, q, k, q_weight, k_weight, positions, freqs):
+    """k and k_weight may be None."""
+    given = (q, q_weight) if k is None else (q, k, q_weight, k_weight)
+    _lib.require_gpu(name, *given, positions, freqs)
+    _check(name, q, q_weight, positions, freqs)
+    if k is not None:
+        _check(name, k, k_weight, positions, freqs)
+        if k.shape[2] != q.shape[2] or k.dtype != q.dtype:
+            raise ValueError(f"{name}: q and k must share head_dim and dtype")
+
+
+def _forward(name, q, k, q_weight, k_weight, positions, freqs, eps, amplitude, interleaved):
+    """y of q, and of k unless it is None, and the tensors as the kernels take them."""
+    _check_qk(name, q, k, q_weight, k_weight, positions, freqs)
+    q, q_weight = head_rows(q), as_contiguous("q_weight", q_weight)
+    qo, ko = contiguous_like(q), None
+    if k is not None:
+        k, k_weight = head_rows(k), as_contiguous("k_weight", k_weight)
+        ko = contiguous_like(k)
+    positions, freqs = as_contiguous("positions", positions), as_contiguous("freqs", freqs)
+    T, H, D = q.shape
+    _lib.call_on(q, "eg_norm_rotary_fwd", q.data_ptr(), _lib.ptr(k), q_weight.data_ptr(),
+                 _lib.ptr(k_weight), qo.data_ptr(), _lib.ptr(ko), positions.data_ptr(),
+                 positions.dtype == torch.int64, freqs.data_ptr(), T, H,
+                 0 if k is None else k.shape[1], D, freqs.shape[0],
+                 strides_arg(q, q if k is None else k), eps, amplitude, bool(interleaved),
+                 tag(q.dtype), _lib.stream_of(q))
+    return qo, ko, (q, k, q_weight, k_weight, positions, freqs)
+
+
+def _backward(name, dq_out, dk_out, q, k, q_weight, k_weight, positions, freqs, eps, amplitude,
+              interleaved):
+    _lib.require_gpu(name, *(t for t in (dq_out, dk_out) if t is not None))
+    _check_qk(name, q, k, q_weight, k_weight, positions, freqs)
+    for d, x in ((dq_out, q), (dk_out, k)):
+        if x is not None and (d.shape != x.shape or d.dtype != x.dtype):
+            raise ValueError(f"{name}: the upstream gradients must match q and k in shape and dtype")
+    q, dq_out = head_rows(q), head_rows(dq_out)
+    q_weight = as_contiguous("q_weight", q_weight)
+    dq, dqw, dk, dkw = contiguous_like(q), torch.empty_like(q_weight), None, None
+    if k is not None:
+        k, dk_out = head_rows(k), head_rows(dk_out)
+        k_weight = as_contiguous("k_weight", k_weight)
+        dk, dkw = contiguous_like(k), torch.empty_like(k_weight)
+    positions, freqs = as_contiguous("positions", positions), as_contiguous("freqs", freqs)
+    T, H, D = q.shape
+    heads_k = 0 if k is None else k.shape[1]
+    ws = workspace(_lib.query("eg_norm_rotary_workspace_bytes", T, H, heads_k, D), q.device)
+    steps = (q, q, dq_out, dq_out) if k is None else (q, k, dq_out, dk_out)
+    _lib.call_on(q, "eg_norm_rotary_bwd", dq_out.data_ptr(), _lib.ptr(dk_out), q.data_ptr(),
+                 _lib.ptr(k), q_weight.data_ptr(), _lib.ptr(k_weight), positions.data_ptr(),
+                 positions.dtype == torch.int64, freqs.data_ptr(), dq.data_ptr(), _lib.ptr(dk),
+                 dqw.data_ptr(), _lib.ptr(dkw), ws.data_ptr(), T, H, heads_k, D, freqs.shape[0],
+                 strides_arg(*steps), eps, amplitude, bool(interleaved), tag(q.dtype),
+                 _lib.stream_of(q))
+    return dq, dk, dqw, dkw
+
+
+def norm_rotary_forward_with_saved(x: torch.Tensor, weight: torch.Tensor, positions: torch.Tensor,
+                                   freqs: torch.Tensor, eps: float = 1e-6, amplitude: float = 1.0,
+                                   interleaved: int = 0):
+    y, _, saved = _forward("norm_rotary_forward_with_saved", x, None, weight, None, positions,
+                           freqs, eps, amplitude, interleaved)
+    return y, (saved[0], saved[2], *saved[4:])
+
+
+def norm_rotary_backward_from_saved(dy: torch.Tensor, saved, eps: float = 1e-6,
+                                    amplitude: float = 1.0, interleaved: int = 0):
+    x, weight, positions, freqs = saved
+    dx, _, dweight, _ = _backward("norm_rotary_backward_from_saved", dy, None, x, None, weight,
+                                  None, positions, freqs, eps, amplitude, interleaved)
+    return dx, dweight
+
+
+def norm_rotary_qk_forward_with_saved(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
+                                      k_weight: torch.Tensor, positions: torch.Tensor,
+                                      freqs: torch.Tensor, eps: float = 1e-6,
+                                      amplitude: float = 1.0, interleaved: int = 0):
+    qo, ko, saved = _forward("norm_rotary_qk_forward_with_saved", q, k, q_weight, k_weight,
+                             positions, freqs, eps, amplitude, interleaved)
+    return (qo, ko), saved
+
+
+def norm_rotary_qk_backward_from_saved(grads, saved, eps: float = 1e-6, amplitude: float = 1.0,
+                                       interleaved: int = 0):
+    """``(dq, dk, dq_weight, dk_weight)`` from the pair of upstream gradients."""
+    dq_out, dk_out = grads
+    return _backward("norm_rotary_qk_backward_from_saved", dq_out, dk_out, *saved, eps, amplitude,
+                     interleaved)
+
+
+class NormRotaryQK(torch.autograd.Function):
+    """The joint q/k pair as an autograd node: ``NormRotaryQK.apply(q, k, q_weight, k_weight,
+    positions, freqs, eps, amplitude, interleaved)`` -> ``(q', k')``; positions and frequencies
+    get no gradient, and the node can be differentiated once."""
+
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, positions, freqs, eps=1e-6, amplitude=1.0,
+                interleaved=0):
+        out, saved = norm_rotary_qk_forward_with_saved(q, k, q_weight, k_weight, positions, freqs,
+                                                       eps, amplitude, interleaved)
+        ctx.save_for_backward(*saved)
+        ctx.scalars = (eps, amplitude, interleaved)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq_out, dk_out):
+        grads = norm_rotary_qk_backward_from_saved((dq_out, dk_out), ctx.saved_tensors,
+                                                   *ctx.scalars)
+        return (*grads, None, None, None, None, None)

@@ -526,6 +526,84 @@ int eg_block_norm_bwd(const void* ds, const void* dy, const void* x, const void*
                       void* dpre_weight, void* workspace, int64_t rows, int64_t cols,
                       int gate_kind, float alpha, int dtype, void* stream);
 
+/* ------------------------------------------------ a distillation step's operators */
+
+/* Embedding lookup: out[t] = scale * weight[ids[t]] (fp32, rounded once), weight [vocab,
+ * hidden], ids [tokens] int32, or int64 with ids_64. A token equal to ignore_index gives zeros,
+ * any other one outside [0, vocab) NaN; neither is used as an index. fp32, bf16, fp16. Sizes:
+ * tokens and vocab <= 2^30, hidden <= 2^20, fewer than 2^32 threads (tokens < 2^24 is enough). */
+int eg_embedding_fwd(const void* weight, const void* ids, int ids_64, void* out, int64_t tokens,
+                     int64_t vocab, int64_t hidden, float scale, int64_t ignore_index, int dtype,
+                     void* stream);
+
+/* Bytes of workspace eg_embedding_bwd needs: the tokens' order, a bound for every id, and two
+ * fp32 partial rows per 32 tokens. */
+size_t eg_embedding_workspace_bytes(int64_t tokens, int64_t vocab, int64_t hidden);
+
+/* Its gradient: dweight[v] = scale * sum of dout[t] over the tokens with ids[t] == v, fp32 sums in
+ * an order that depends on the ids alone, one rounding; every row is written. accumulate: added
+ * to dweight instead, where the rows of ids without a token are neither read nor written. The
+ * workspace is 16-byte aligned. */
+int eg_embedding_bwd(const void* dout, const void* ids, int ids_64, void* dweight,
+                     void* workspace, int64_t tokens, int64_t vocab, int64_t hidden, float scale,
+                     int64_t ignore_index, int accumulate, int dtype, void* stream);
+
+/* RMSNorm of every head with the rotation of eg_rotary behind it: n = x * rsqrt(mean(x^2) + eps)
+ * * weight over a head's columns, then pairs of n rotated and scaled by amplitude as there, the
+ * columns from 2 * pairs on left as n. q [tokens, heads_q, head_dim] with q_weight [head_dim], k
+ * [tokens, heads_k, head_dim] with k_weight (heads_k = 0: q alone), one launch; strides, positions,
+ * freqs and sizes as for eg_rotary. fp32 arithmetic, one rounding. */
+int eg_norm_rotary_fwd(const void* q, const void* k, const void* q_weight, const void* k_weight,
+                       void* q_out, void* k_out, const void* positions, int positions_64,
+                       const double* freqs, int64_t tokens, int64_t heads_q, int64_t heads_k,
+                       int64_t head_dim, int64_t pairs, const int64_t* strides, float eps,
+                       float amplitude, int interleaved, int dtype, void* stream);
+
+/* Bytes of fp32 partial rows of the weights' gradients that eg_norm_rotary_bwd keeps. */
+size_t eg_norm_rotary_workspace_bytes(int64_t tokens, int64_t heads_q, int64_t heads_k,
+                                      int64_t head_dim);
+
+/* Its backward: dq, dk like q, k but contiguous; dq_weight, dk_weight [head_dim], summed over
+ * tokens and heads (fp32, a fixed order). `strides`: token and head steps of q, k, dq_out and
+ * dk_out. */
+int eg_norm_rotary_bwd(const void* dq_out, const void* dk_out, const void* q, const void* k,
+                       const void* q_weight, const void* k_weight, const void* positions,
+                       int positions_64, const double* freqs, void* dq, void* dk, void* dq_weight,
+                       void* dk_weight, void* workspace, int64_t tokens, int64_t heads_q,
+                       int64_t heads_k, int64_t head_dim, int64_t pairs, const int64_t* strides,
+                       float eps, float amplitude, int interleaved, int dtype, void* stream);
+
+/* Bytes of workspace eg_topk_distill_fwd needs. */
+size_t eg_topk_distill_workspace_bytes(int64_t rows, int64_t cols);
+
+/* Distillation from a teacher's top logits with a share of hard-label cross entropy: over the
+ * rows whose target is not ignore_index, n_valid of them,
+ *   loss = mean(soft_weight * tau^2 * sum_k p_k (log p_k - log q[ids_k])
+ *               + hard_weight * (logsumexp(logits) - logits[target])),
+ * p = softmax(teacher / tau) over the row's entries, q = softmax(logits / tau) over cols.
+ * logits [rows, cols] (dtype); teacher [rows, entries] (teacher_dtype) at the columns teacher_ids
+ * [rows, entries] int32, or int64 with ids_64; a negative id is no entry, several entries of one
+ * column all count, a row without entries has no soft part. An id >= cols, and with hard_weight
+ * != 0 a target outside [0, cols), makes the row's loss and gradient NaN. loss and n_valid: one
+ * fp32 each. Saved: stats fp32 [rows, 4], probs fp32 [rows, entries]. tau > 0; entries <= 1024,
+ * rows < 2^22, cols <= 2^30. */
+int eg_topk_distill_fwd(const void* logits, const int64_t* target, const void* teacher,
+                        int teacher_dtype, const void* teacher_ids, int ids_64, float* loss,
+                        float* stats, float* probs, float* n_valid, void* workspace, int64_t rows,
+                        int64_t cols, int64_t entries, float temperature, float soft_weight,
+                        float hard_weight, int64_t ignore_index, int dtype, void* stream);
+
+/* Its backward, with dloss one fp32 in device memory:
+ *   dlogits = dloss / n_valid * (hard_weight (softmax(logits) - onehot(target))
+ *             + soft_weight tau (q - sum of p at their columns)),
+ * zero in ignored rows. dlogits [rows, cols] (dtype) does not overlap logits; fewer than 2^33
+ * packs of 16 bytes. */
+int eg_topk_distill_bwd(const float* dloss, const void* logits, const int64_t* target,
+                        const void* teacher_ids, int ids_64, const float* stats,
+                        const float* probs, const float* n_valid, void* dlogits, int64_t rows,
+                        int64_t cols, int64_t entries, float temperature, float soft_weight,
+                        float hard_weight, int64_t ignore_index, int dtype, void* stream);
+
 /* ---- measurement aid (no counterpart in the reference) ---------------------
  * Sustained bf16 MFMA rate, for reading the roofline fractions of the MFMA-bound
  * kernels (bench.py reports it beside the published peak): `workgroups` 256-thread

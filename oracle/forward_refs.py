@@ -290,6 +290,42 @@ def block_norm_forward_ref(x, h, post_weight, gate, pre_weight, scale: float = 1
     return torch.stack((s, norm(s, pre_weight)))
 
 
+def embedding_forward_ref(weight, ids, scale: float = 1.0, ignore_index: int = -100):
+    """Rows of the table times the scale; zeros for ignored tokens, NaN for others outside it."""
+    ids = ids.long()
+    inside = (ids >= 0) & (ids < weight.shape[0])
+    rows = scale * weight[torch.where(inside, ids, 0)]
+    fill = torch.where(ids == ignore_index, 0.0, float("nan")).to(weight.dtype)
+    return torch.where((inside & (ids != ignore_index))[..., None], rows, fill[..., None])
+
+
+def norm_rotary_forward_ref(x, weight, positions, freqs, eps: float = 1e-6,
+                            amplitude: float = 1.0, interleaved: int = 0):
+    """rmsnorm_forward_ref's norm of each head, then rotary_forward_ref."""
+    n = x * torch.rsqrt(x.pow(2).mean(dim=-1, keepdim=True) + eps) * weight
+    return rotary_forward_ref(n, positions, freqs, amplitude, interleaved)
+
+
+def topk_distillation_forward_ref(logits, target, teacher_logits, teacher_ids,
+                                  temperature: float = 1.0, soft_weight: float = 1.0,
+                                  hard_weight: float = 0.0, ignore_index: int = -100):
+    """Row by row: the divergence of the teacher's distribution over its entries from the
+    student's, and the cross entropy of cross_entropy_forward_ref; the mean over counted rows."""
+    total, count = logits.new_zeros(()), 0
+    for r in range(logits.shape[0]):
+        if int(target[r]) == ignore_index:
+            continue
+        count += 1
+        if hard_weight:
+            total = total + hard_weight * (torch.logsumexp(logits[r], 0) - logits[r, target[r]])
+        kept = teacher_ids[r] >= 0
+        if soft_weight and bool(kept.any()):
+            p = torch.softmax(teacher_logits[r][kept] / temperature, 0)
+            logq = torch.log_softmax(logits[r] / temperature, 0)[teacher_ids[r][kept].long()]
+            total = total + soft_weight * temperature ** 2 * (torch.xlogy(p, p) - p * logq).sum()
+    return total / count
+
+
 FORWARDS = {
     "softmax_forward_ref": softmax_forward_ref,
     "rmsnorm_forward_ref": rmsnorm_forward_ref,
@@ -313,4 +349,7 @@ FORWARDS = {
     "packed_attention_forward_ref": packed_attention_forward_ref,
     "rotary_forward_ref": rotary_forward_ref,
     "block_norm_forward_ref": block_norm_forward_ref,
+    "embedding_forward_ref": embedding_forward_ref,
+    "norm_rotary_forward_ref": norm_rotary_forward_ref,
+    "topk_distillation_forward_ref": topk_distillation_forward_ref,
 }

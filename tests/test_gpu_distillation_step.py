@@ -1,0 +1,113 @@
+"""The operators of a distillation step together, over a packed batch: tokens to rows, the norm
+before the block, one projection to q, k and v, the norms per head with the rotation, attention
+over the packed sequences, the output projection with the next norms, the head (the embedding's
+own table) and the loss against the teacher's top logits; and back to every weight."""
+
+import pytest
+import torch
+
+from evograd_amd.bind import bind
+from evograd_amd.decls import EMBEDDING, PACKED_ATTENTION, TOPK_DISTILLATION
+from evograd_amd.pairs import embedding, packed_attention, rotary, topk_distillation
+from evograd_amd.pairs.block_norm import BlockNorm
+from evograd_amd.pairs.norm_rotary import NormRotaryQK
+from oracle import forward_refs as fr
+
+pytestmark = pytest.mark.gpu
+
+EPS = 1e-6
+TAU, SOFT, HARD = 2.0, 0.7, 0.3
+
+
+def model(ops, p, batch, H, KVH, D):
+    embed, norms, turn, attend, distill = ops
+    x = embed(p["table"], batch["ids"])
+    T = x.shape[0]
+    s, y = norms(x, x, p["post1"], p["pre1"])
+    qkv = (y @ p["wqkv"].T).view(T, H + 2 * KVH, D)
+    q, k, v = qkv.split((H, KVH, KVH), 1)
+    q, k = turn(q, k, p["qw"], p["kw"])
+    o = attend(q, k, v).reshape(T, H * D) @ p["wo"].T
+    _, y = norms(s, o, p["post2"], p["pre2"])
+    return distill(y @ p["table"].T)
+
+
+@pytest.mark.parametrize("dtype,D,tol", (
+    # fp32: twelve composed operators, sums of up to 500 terms (2^-24 * 500 each) there and back
+    (torch.float32, 32, 3e-4),
+    # bf16: about 25 stored tensors on the way, each rounded to 2^-8 of its value; independent
+    # errors, 2^-8 * sqrt(25) = 0.02 of a tensor's norm, twice for the way back
+    (torch.bfloat16, 64, 0.04)))
+def test_a_step_from_tokens_to_the_loss(dtype, D, tol):
+    H, KVH, lengths, V, C, K = 4, 2, [37, 1, 90, 5], 500, 256, 12
+    T = sum(lengths)
+    g = torch.Generator().manual_seed(0)
+
+    def normal(scale, *shape):
+        return (scale * torch.randn(shape, generator=g)).to("cuda", dtype)
+
+    p = {"table": normal(C ** -0.5, V, C), "wqkv": normal(C ** -0.5, (H + 2 * KVH) * D, C),
+         "wo": normal((H * D) ** -0.5, C, H * D), "qw": 1 + normal(0.1, D), "kw": 1 + normal(0.1, D)}
+    for i in "12":
+        p["post" + i], p["pre" + i] = 1 + normal(0.1, C), 1 + normal(0.1, C)
+    ids = torch.randint(0, V, (T,), generator=g).to(torch.int32)
+    target = torch.randint(0, V, (T,), generator=g)
+    target[:20] = -100
+    tids = torch.rand(T, V, generator=g).topk(K).indices.to(torch.int32)
+    tids[40:60, 5:] = -1
+    batch = {"ids": ids.cuda(), "target": target.cuda(), "tids": tids.cuda(),
+             "teacher": (3 * torch.randn(T, K, generator=g)).cuda()}
+    positions = torch.cat([torch.arange(n) for n in lengths]).to("cuda", torch.int32)
+    freqs = rotary.rotary_frequencies(D, device="cuda")
+    cu = torch.tensor([0, *torch.tensor(lengths).cumsum(0).tolist()], dtype=torch.int32, device="cuda")
+    loss_args = (batch["target"], batch["teacher"], batch["tids"], TAU, SOFT, HARD)
+
+    table, attend = bind(EMBEDDING, embedding), bind(PACKED_ATTENTION, packed_attention)
+    distill = bind(TOPK_DISTILLATION, topk_distillation)
+    mine = (lambda w, i: table(w, i, scale=C ** 0.5),
+            lambda x, h, w1, w2: BlockNorm.apply(x, h, w1, None, w2, 0.5, EPS),
+            lambda q, k, qw, kw: NormRotaryQK.apply(q, k, qw, kw, positions, freqs, EPS),
+            lambda q, k, v: attend(q, k, v, cu),
+            lambda z: distill(z, *loss_args))
+
+    def norms64(x, h, w1, w2):
+        out = fr.block_norm_forward_ref(x, h, w1, None, w2, 0.5, EPS)
+        return out[0], out[1]
+
+    true = (lambda w, i: fr.embedding_forward_ref(w, i, C ** 0.5),
+            norms64,
+            lambda q, k, qw, kw: (fr.norm_rotary_forward_ref(q, qw, positions, freqs, EPS),
+                                  fr.norm_rotary_forward_ref(k, kw, positions, freqs, EPS)),
+            lambda q, k, v: fr.packed_attention_forward_ref(q, k, v, cu),
+            lambda z: fr.topk_distillation_forward_ref(z, loss_args[0], loss_args[1].double(),
+                                                       *loss_args[2:]))
+
+    def step(ops, dt):
+        leaf = {n: t.detach().clone().to(dt).requires_grad_(True) for n, t in p.items()}
+        loss = model(ops, leaf, batch, H, KVH, D)
+        loss.backward()
+        return {"loss": loss.detach(), **{"d" + n: t.grad for n, t in leaf.items()}}
+
+    got, want = step(mine, dtype), step(true, torch.float64)
+    for name, value in want.items():
+        error = float((got[name].double() - value).norm() / value.norm())
+        assert error <= tol, (name, error)
+
+
+def test_a_tied_table_takes_both_gradients_in_place():
+    """The embedding's gradient added into the head's: the sum of the two, where the table's rows
+    of no token keep the head's bits."""
+    V, C, T = 300, 128, 90
+    g = torch.Generator().manual_seed(1)
+    head = torch.randn(V, C, generator=g).cuda()
+    ids = torch.randint(0, V, (T,), generator=g).cuda()
+    dout = torch.randn(T, C, generator=g).cuda()
+    _, saved = embedding.embedding_forward_with_saved(torch.empty(V, C, device="cuda"), ids, 3.0)
+    alone = embedding.embedding_backward_from_saved(dout, saved, 3.0)
+    both = embedding.embedding_backward_into(head.clone(), dout, saved, 3.0)
+    used = torch.zeros(V, dtype=torch.bool, device="cuda")
+    used[ids] = True
+    assert torch.equal(both[~used], head[~used])
+    # one rounding of the sum in place of the row's and the sum's
+    room = 2.0 ** -24 * (2 * alone.abs() + (head + alone).abs())
+    assert bool(((both - (head + alone)).abs() <= room + 2.0 ** -24 * both.abs()).all())

@@ -16,8 +16,15 @@
 // once for a workgroup's tokens, into LDS.
 //
 // Memory-bound: the forward reads x and writes y, the backward reads x and dy and writes dx.
-// The backward's workgroups walk the tokens, keep the sums for dw of their heads in registers
-// and leave one partial row each of q's and k's, which a second kernel adds in order.
+// Workgroups walk the tokens, a head a thread group, and load the next token's packs under the
+// present one's work; the backward's keep the sums for dw in registers over the walk and leave one
+// partial row each of q's and k's, which a second kernel adds in order.
+//
+// Kernel times, bf16 32768 tokens, 32 + 8 heads of 128: forward 125 us (5.4 TB/s), backward 171 to
+// 184 us (5.5 to 5.9 TB/s) and 5; fp16 5003 tokens, 16 + 16 heads of 96, 64 columns interleaved: 13
+// and 21 + 4; 32 tokens 4 us, a launch. With a workgroup per token and heads summed by LDS
+// permutes the first took 163 and 362 us; with branches around the walk's loads and stores,
+// where each step waited for the last one's stores, 127 and 236.
 #include "rotary_angles.hpp"
 
 #include <algorithm>
@@ -27,6 +34,19 @@ namespace eg {
 namespace {
 
 constexpr int kMostThreads = 512;
+// The backward's workgroups, which leave a partial row each, at most; or as many as one token's
+// heads take.
+constexpr int64_t kMostParts = 2048;
+// Waves per SIMD that the registers leave room for, and of them those that the backward's walk
+// starts (32768 tokens, 32 + 8 heads of 128, us: one or two 185, three 189, four 194, and 254 where
+// four have to fit the registers; the forward 122 to 124 with four to six, 239 with eight).
+constexpr int kFrontWaves = 6, kBackWaves = 3, kBackGrid = 2;
+// Past this size of q and k together a call streams: stores, and the backward's loads, with the
+// non-temporal hint. Plain and streamed, us, forward and backward: 32768 tokens, 32 + 8 heads of
+// 128 bf16 (336 MB) 132 / 126 and 191 / 172; 8192 of them (84 MB) 28 / 28 and 49 / 48; 5003 tokens,
+// 32 heads of 96 fp16 (31 MB) 12 / 13 and 23 / 26. The forward's loads gain nothing (126 / 124) and
+// lose in small calls.
+constexpr int64_t kStreamBytes = 64 << 20;
 
 struct HeadArgs {
   const void *q, *k, *dqo, *dko, *qw, *kw;
@@ -38,51 +58,66 @@ struct HeadArgs {
   int64_t tokens, q_token, q_head, k_token, k_head, dq_token, dq_head, dk_token, dk_head;
   int heads_q, heads_k, head_dim, pairs, pos64;
   int group, lanes, per_block;  // lanes of a head; heads along a token's threads; tokens
-  float amp, eps;
+  int ahead;                    // steps whose sines are formed at a time
+  float amp, eps, share;        // share: 1 / head_dim
 };
 
-template <typename T, int VEC>
-__device__ __forceinline__ void get(const T* p, bool in, Pack<T, VEC>& v) {
-  if (in) v = *reinterpret_cast<const Pack<T, VEC>*>(p);
+// Sum over the `group` lanes of a head, the same bits in each: neighbours, pairs of a quad, and
+// mirrored halves and rows of 16 lanes are register accesses of the addition itself (DPP).
+template <int CTRL>
+__device__ __forceinline__ float plus_lane(float v) {
+  const int other = __builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false);
+  return v + __int_as_float(other);
 }
-
-// Sum over the `group` lanes of a head, the same bits in each.
 __device__ __forceinline__ float group_sum(float v, int group) {
-  for (int off = 1; off < group; off <<= 1) v += __shfl_xor(v, off);
+  if (group > 1) v = plus_lane<0xB1>(v);   // quad_perm [1, 0, 3, 2]
+  if (group > 2) v = plus_lane<0x4E>(v);   // quad_perm [2, 3, 0, 1]
+  if (group > 4) v = plus_lane<0x141>(v);  // row_half_mirror
+  if (group > 8) v = plus_lane<0x140>(v);  // row_mirror
+  if (group > 16) v += __shfl_xor(v, 16);
+  if (group > 32) v += __shfl_xor(v, 32);
   return v;
 }
 
-// A thread's place: token of the workgroup, first head, columns.
+// A thread's place: token of the workgroup, head, columns. Every thread has valid ones: a lane
+// past its head's packs does the first lane's work again, a group past the workgroup's heads the
+// first group's, and a second pack past the head is the first one again. They store the same bits
+// to the same places and are left out of the sums, so that the walk's loads and stores need no
+// branches, which would keep a step's stores from staying in flight over the next one's loads.
 template <int VEC, bool INTER>
 struct Place {
   int tl, hl, c1, c2;
-  bool in, turn, one, two;  // of the workgroup's tokens; turned columns; has each of the packs
-  int pair;                 // first pair
+  bool in, one, two;  // of the workgroup's tokens; the lane and its second pack are a head's own
+  bool turn;          // turned columns
+  int pair;           // first pair
   __device__ __forceinline__ Place(const HeadArgs& a) {
     const unsigned per = a.lanes * a.group;  // threads of a token
     const unsigned e = blockIdx.y * blockDim.x + threadIdx.x;
     tl = e / per;
     const unsigned r = e - tl * per;
     hl = r / a.group;
-    const int ch = r - hl * a.group, turned = a.pairs / VEC;
+    int ch = r - hl * a.group;
     in = tl < a.per_block;
+    if (!in) tl = hl = 0;
+    const int turned = a.pairs / VEC;
+    one = ch < turned || 2 * a.pairs + (ch - turned) * 2 * VEC < a.head_dim;
+    if (!one) ch = 0;
     turn = ch < turned;
     pair = ch * VEC;
     c1 = !turn ? 2 * a.pairs + (ch - turned) * 2 * VEC : INTER ? 2 * ch * VEC : ch * VEC;
     c2 = turn && !INTER ? c1 + a.pairs : c1 + VEC;
-    one = in && c1 < a.head_dim;
-    two = in && c2 < a.head_dim;
+    two = one && c2 < a.head_dim;
+    if (c2 >= a.head_dim) c2 = c1;
   }
 };
 
 // The rows of head h (q's heads, then k's).
 struct Head {
-  bool isq, in;
+  bool isq;
   int at;
   __device__ __forceinline__ Head(const HeadArgs& a, int h) {
     isq = h < a.heads_q;
     at = isq ? h : h - a.heads_q;
-    in = isq || at < a.heads_k;
   }
   template <typename T>
   __device__ __forceinline__ const T* x(const HeadArgs& a, int64_t t) const {
@@ -105,10 +140,13 @@ struct Head {
   }
 };
 
-// (cos, sin) of per_block tokens from t0 on.
-__device__ __forceinline__ void form_table(const HeadArgs& a, int64_t t0, float sign, float2* table) {
-  for (int i = threadIdx.x; i < a.per_block * a.pairs; i += blockDim.x) {
-    const int64_t t = min(t0 + i / a.pairs, a.tokens - 1);
+// (cos, sin) of `steps` runs of per_block tokens, the first from t0 on, `stride` apart.
+__device__ __forceinline__ void form_table(const HeadArgs& a, int64_t t0, int steps, int64_t stride,
+                                           float sign, float2* table) {
+  const int each = a.per_block * a.pairs;
+  for (int i = threadIdx.x; i < steps * each; i += blockDim.x) {
+    const int step = i / each, tl = (i - step * each) / a.pairs;
+    const int64_t t = min(t0 + step * stride + tl, a.tokens - 1);
     table[i] = rotary_turn(rotary_position(a.pos, a.pos64, t), a.freq[i % a.pairs], a.amp, sign);
   }
 }
@@ -133,177 +171,156 @@ __device__ __forceinline__ void turn_packs(const float2* table, float (&n)[2 * V
   }
 }
 
-template <typename T, int VEC>
-__device__ __forceinline__ void widen(const Pack<T, VEC> (&raw)[2], bool one, bool two,
-                                      float (&f)[2 * VEC]) {
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    f[i] = one ? to_f32(raw[0].v[i]) : 0.f;
-    f[VEC + i] = two ? to_f32(raw[1].v[i]) : 0.f;
+// A thread's two packs of a row as they lie in memory.
+template <typename T, int VEC, bool NT>
+struct RawPacks {
+  Pack<T, VEC> v[2];
+  static __device__ __forceinline__ Pack<T, VEC> read(const T* p) {
+    if constexpr (NT && sizeof(T) * VEC == 16) return load_ragged_raw<T, VEC, true>(p);
+    else return *reinterpret_cast<const Pack<T, VEC>*>(p);
   }
-}
+  template <bool INTER>
+  __device__ __forceinline__ void load(const T* row, const Place<VEC, INTER>& at) {
+    v[0] = read(row + at.c1);
+    v[1] = read(row + at.c2);
+  }
+  __device__ __forceinline__ void get(float (&f)[2 * VEC]) const {
+#pragma unroll
+    for (int i = 0; i < 2 * VEC; ++i) f[i] = to_f32(v[i / VEC].v[i % VEC]);
+  }
+};
 
-template <typename T, int VEC, bool INTER>
+template <bool NT, typename T, int VEC, bool INTER>
 __device__ __forceinline__ void put(T* row, const Place<VEC, INTER>& at, const float (&f)[2 * VEC]) {
-  float v[VEC];
-  if (at.one) {
+  float u[VEC], v[VEC];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = f[i];
-    store_vec<T, VEC, true>(row + at.c1, v);
-  }
-  if (at.two) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = f[VEC + i];
-    store_vec<T, VEC, true>(row + at.c2, v);
-  }
+  for (int i = 0; i < VEC; ++i) u[i] = f[i], v[i] = f[VEC + i];
+  store_vec<T, VEC, NT>(row + at.c1, u);
+  store_vec<T, VEC, NT>(row + at.c2, v);
 }
 
-template <typename T, int VEC, int HPT, bool INTER>
-__global__ __launch_bounds__(kMostThreads) void norm_rotary_fwd_kernel(HeadArgs a) {
-  const Place<VEC, INTER> at(a);
-  const int64_t t0 = (int64_t)blockIdx.x * a.per_block, t = t0 + at.tl;
-  const bool live = at.in && t < a.tokens;
-  Pack<T, VEC> raw[HPT][2], w[HPT][2];
+// Sum of a head's products u v, over the packs that are its own.
+template <int GROUP, int VEC, bool INTER>
+__device__ __forceinline__ float head_dot(const Place<VEC, INTER>& at, const float (&u)[2 * VEC],
+                                          const float (&v)[2 * VEC], int group) {
+  float s = 0.f, s2 = 0.f;
 #pragma unroll
-  for (int j = 0; j < HPT; ++j) {
-    const Head h(a, at.hl + j * a.lanes);
-    if (!live || !h.in) continue;
-    const T* x = h.x<T>(a, t);
-    const T* g = h.weight<T>(a);
-    get<T, VEC>(x + at.c1, at.one, raw[j][0]);
-    get<T, VEC>(x + at.c2, at.two, raw[j][1]);
-    get<T, VEC>(g + at.c1, at.one, w[j][0]);
-    get<T, VEC>(g + at.c2, at.two, w[j][1]);
-  }
-  extern __shared__ float2 table[];
-  form_table(a, t0, 1.f, table);
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < HPT; ++j) {
-    const Head h(a, at.hl + j * a.lanes);
-    if (!live || !h.in) continue;
-    float x[2 * VEC], g[2 * VEC];
-    widen<T, VEC>(raw[j], at.one, at.two, x);
-    widen<T, VEC>(w[j], at.one, at.two, g);
-    float sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < 2 * VEC; ++i) sum += x[i] * x[i];
-    const float rstd = rsqrtf(group_sum(sum, a.group) / a.head_dim + a.eps);
-#pragma unroll
-    for (int i = 0; i < 2 * VEC; ++i) x[i] = x[i] * rstd * g[i];
-    if (at.turn) turn_packs<VEC, INTER>(table + at.tl * a.pairs + at.pair, x);
-    put<T, VEC, INTER>(h.out<T>(a, t), at, x);
-  }
+  for (int i = 0; i < VEC; ++i) s += u[i] * v[i], s2 += u[VEC + i] * v[VEC + i];
+  s += at.two ? s2 : 0.f;
+  return group_sum(at.one ? s : 0.f, GROUP ? GROUP : group);
 }
 
-template <typename T, int VEC, int HPT, bool INTER>
-__global__ __launch_bounds__(kMostThreads) void norm_rotary_bwd_kernel(HeadArgs a) {
-  extern __shared__ float2 table[];  // of this step's tokens and the next's; sums at the end
+// A workgroup walks the tokens in steps of the grid, one head a thread group, and loads the next
+// step's packs under the present one's work. The sines of a.ahead steps are formed at a time.
+template <typename T, int VEC, bool INTER, int GROUP, bool NT>
+__global__ __launch_bounds__(kMostThreads, kFrontWaves) void norm_rotary_fwd_kernel(HeadArgs a) {
+  extern __shared__ float2 table[];  // [ahead][per_block][pairs]
   const Place<VEC, INTER> at(a);
+  const Head h(a, at.hl);
   const int64_t stride = (int64_t)gridDim.x * a.per_block;
-  float acc[HPT][2 * VEC];
-#pragma unroll
-  for (int j = 0; j < HPT; ++j)
-#pragma unroll
-    for (int i = 0; i < 2 * VEC; ++i) acc[j][i] = 0.f;
-  Pack<T, VEC> rawx[HPT][2], rawd[HPT][2];
-  auto fetch = [&](int64_t t) {
-#pragma unroll
-    for (int j = 0; j < HPT; ++j) {
-      const Head h(a, at.hl + j * a.lanes);
-      if (t >= a.tokens || !h.in) continue;
-      const T *x = h.x<T>(a, t), *d = h.dy<T>(a, t);
-      get<T, VEC>(x + at.c1, at.one, rawx[j][0]);
-      get<T, VEC>(x + at.c2, at.two, rawx[j][1]);
-      get<T, VEC>(d + at.c1, at.one, rawd[j][0]);
-      get<T, VEC>(d + at.c2, at.two, rawd[j][1]);
+  int64_t t0 = (int64_t)blockIdx.x * a.per_block, t = min(t0 + at.tl, a.tokens - 1);
+  const T* x = h.x<T>(a, t);
+  RawPacks<T, VEC, false> raw, w;
+  raw.load(x, at);
+  w.load(h.weight<T>(a), at);
+  for (int ahead = 0; t0 < a.tokens; t0 += stride) {
+    if (ahead == 0) {
+      __syncthreads();
+      form_table(a, t0, a.ahead, stride, 1.f, table);
+      __syncthreads();
     }
-  };
-  int64_t t0 = (int64_t)blockIdx.x * a.per_block;
-  fetch(t0 + at.tl);
-  form_table(a, t0, -1.f, table);
-  __syncthreads();
-  for (int side = 0; t0 < a.tokens; t0 += stride, side ^= 1) {
-    const int64_t t = t0 + at.tl, next = t0 + stride;
-    const float2* turns = table + side * a.per_block * a.pairs + at.tl * a.pairs + at.pair;
-    float x[HPT][2 * VEC], d[HPT][2 * VEC];
+    const float2* turns = table + (ahead * a.per_block + at.tl) * a.pairs + at.pair;
+    if (++ahead == a.ahead) ahead = 0;
+    float n[2 * VEC], g[2 * VEC];
+    raw.get(n);
+    T* out = h.out<T>(a, t);
+    t = min(t0 + stride + at.tl, a.tokens - 1);
+    raw.load(h.x<T>(a, t), at);
+    w.get(g);
+    const float rstd = rsqrtf(head_dot<GROUP>(at, n, n, a.group) * a.share + a.eps);
 #pragma unroll
-    for (int j = 0; j < HPT; ++j) {
-      widen<T, VEC>(rawx[j], at.one, at.two, x[j]);
-      widen<T, VEC>(rawd[j], at.one, at.two, d[j]);
-    }
-    if (next < a.tokens) {
-      fetch(next + at.tl);
-      form_table(a, next, -1.f, table + (side ^ 1) * a.per_block * a.pairs);
-    }
-    if (at.in && t < a.tokens) {
-#pragma unroll
-      for (int j = 0; j < HPT; ++j) {
-        const Head h(a, at.hl + j * a.lanes);
-        if (!h.in) continue;
-        if (at.turn) turn_packs<VEC, INTER>(turns, d[j]);  // dn
-        Pack<T, VEC> w[2];
-        float g[2 * VEC], squares = 0.f, dot = 0.f;
-        get<T, VEC>(h.weight<T>(a) + at.c1, at.one, w[0]);
-        get<T, VEC>(h.weight<T>(a) + at.c2, at.two, w[1]);
-        widen<T, VEC>(w, at.one, at.two, g);
-#pragma unroll
-        for (int i = 0; i < 2 * VEC; ++i) {
-          squares += x[j][i] * x[j][i];
-          g[i] *= d[j][i];
-          dot += g[i] * x[j][i];
-        }
-        squares = group_sum(squares, a.group);
-        dot = group_sum(dot, a.group);
-        const float rstd = rsqrtf(squares / a.head_dim + a.eps), mean = dot * rstd / a.head_dim;
-#pragma unroll
-        for (int i = 0; i < 2 * VEC; ++i) {
-          const float xhat = x[j][i] * rstd;
-          acc[j][i] += d[j][i] * xhat;
-          g[i] = rstd * (g[i] - xhat * mean);
-        }
-        put<T, VEC, INTER>(h.out<T>(a, t), at, g);
-      }
-    }
-    __syncthreads();
+    for (int i = 0; i < 2 * VEC; ++i) n[i] = n[i] * rstd * g[i];
+    if (at.turn) turn_packs<VEC, INTER>(turns, n);
+    put<NT>(out, at, n);
   }
-  // this workgroup's sums: the heads' rows, one after the other
+}
+
+// The backward's walk is the forward's.
+template <typename T, int VEC, bool INTER, int GROUP, bool NT>
+__global__ __launch_bounds__(kMostThreads, kBackWaves) void norm_rotary_bwd_kernel(HeadArgs a) {
+  extern __shared__ float2 table[];  // [ahead][per_block][pairs]; sums at the end
+  const Place<VEC, INTER> at(a);
+  const Head h(a, at.hl);
+  const int64_t stride = (int64_t)gridDim.x * a.per_block;
+  float acc[2 * VEC];
+#pragma unroll
+  for (int i = 0; i < 2 * VEC; ++i) acc[i] = 0.f;
+  int64_t t0 = (int64_t)blockIdx.x * a.per_block, t = min(t0 + at.tl, a.tokens - 1);
+  RawPacks<T, VEC, NT> rawx, rawd;
+  RawPacks<T, VEC, false> w;
+  rawx.load(h.x<T>(a, t), at);
+  rawd.load(h.dy<T>(a, t), at);
+  w.load(h.weight<T>(a), at);
+  for (int ahead = 0; t0 < a.tokens; t0 += stride) {
+    if (ahead == 0) {
+      __syncthreads();
+      form_table(a, t0, a.ahead, stride, -1.f, table);
+      __syncthreads();
+    }
+    const float2* turns = table + (ahead * a.per_block + at.tl) * a.pairs + at.pair;
+    if (++ahead == a.ahead) ahead = 0;
+    float x[2 * VEC], d[2 * VEC], g[2 * VEC];
+    rawx.get(x);
+    rawd.get(d);
+    T* out = h.out<T>(a, t);
+    t = min(t0 + stride + at.tl, a.tokens - 1);
+    rawx.load(h.x<T>(a, t), at);
+    rawd.load(h.dy<T>(a, t), at);
+    w.get(g);
+    if (at.turn) turn_packs<VEC, INTER>(turns, d);  // dn
+#pragma unroll
+    for (int i = 0; i < 2 * VEC; ++i) g[i] *= d[i];
+    const float squares = head_dot<GROUP>(at, x, x, a.group), dot = head_dot<GROUP>(at, g, x, a.group);
+    const float rstd = rsqrtf(squares * a.share + a.eps), mean = dot * rstd * a.share;
+#pragma unroll
+    for (int i = 0; i < 2 * VEC; ++i) {
+      x[i] *= rstd;
+      g[i] = rstd * (g[i] - x[i] * mean);
+    }
+    put<NT>(out, at, g);
+    if (t0 + at.tl < a.tokens)
+#pragma unroll
+      for (int i = 0; i < 2 * VEC; ++i) acc[i] += d[i] * x[i];
+  }
+  // this workgroup's sums, column by column over its heads' rows
   float* rows = (float*)table;
   const int heads = blockDim.x / a.group, me = threadIdx.x / a.group;
   float* part = a.part + ((int64_t)blockIdx.x * gridDim.y + blockIdx.y) * 2 * a.head_dim;
-  const int per = a.lanes * a.group;
-  float sum[2] = {0.f, 0.f};
-  // column by column of the partial rows; head_dim may pass the workgroup's threads
-  for (int c0 = 0; c0 < a.head_dim; c0 += blockDim.x) {
-    sum[0] = sum[1] = 0.f;
-    const int c = c0 + threadIdx.x;
+  __syncthreads();
 #pragma unroll
-    for (int j = 0; j < HPT; ++j) {
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        if (at.one) rows[me * a.head_dim + at.c1 + i] = acc[j][i];
-        if (at.two) rows[me * a.head_dim + at.c2 + i] = acc[j][VEC + i];
-      }
-      __syncthreads();
-      if (c < a.head_dim)
-        for (int m = 0; m < heads; ++m) {
-          const int e = blockIdx.y * blockDim.x + m * a.group;
-          const Head h(a, e % per / a.group + j * a.lanes);
-          if (e / per < a.per_block && h.in) sum[!h.isq] += rows[m * a.head_dim + c];
-        }
+  for (int i = 0; i < VEC; ++i) {
+    if (at.one) rows[me * a.head_dim + at.c1 + i] = acc[i];
+    if (at.two) rows[me * a.head_dim + at.c2 + i] = acc[VEC + i];
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < a.head_dim; c += blockDim.x) {
+    float sum[2] = {0.f, 0.f};
+    const int first = blockIdx.y * heads, left = a.per_block * a.lanes - first;
+    int head = first % a.lanes;
+    for (int m = 0; m < min(heads, left); ++m) {
+      const float v = rows[m * a.head_dim + c];
+      if (head < a.heads_q) sum[0] += v;
+      else sum[1] += v;
+      if (++head == a.lanes) head = 0;
     }
-    if (c < a.head_dim) {
-      part[c] = sum[0];
-      part[a.head_dim + c] = sum[1];
-    }
+    part[c] = sum[0];
+    part[a.head_dim + c] = sum[1];
   }
 }
 
 // Heads of more than 64 lanes' packs (single columns of wide heads): a wave per head, which reads
 // its columns again for every step and forms its own sines. Column sums lie in LDS, each
 // column with the lane that works on it.
-constexpr int kWideWaves = 2048;
 
 template <typename T, bool INTER, bool BACK>
 __global__ __launch_bounds__(kWave) void norm_rotary_wide_kernel(HeadArgs a) {
@@ -400,23 +417,19 @@ __global__ __launch_bounds__(kSumCols* kSumRows) void norm_rotary_sum_kernel(Hea
   else if (a.dkw) ((T*)a.dkw)[c - a.head_dim] = from_f32<T>(s);
 }
 
-// The backward's workgroups, a partial row each: as many as a card holds at once, or as many as
-// one token's heads take.
-constexpr int64_t kBackBlocks = 1024;
-
 // How a call's heads lie on threads: 0 lanes if a head does not fit a wave.
 struct Shape {
   int group, lanes, per_block, threads;
   int64_t gx, gy;
 };
-Shape shape_of(const HeadArgs& a, int vec, int hpt) {
+Shape shape_of(const HeadArgs& a, int vec) {
   Shape s = {};
   const int64_t heads = a.heads_q + a.heads_k;
   const int chunks = a.pairs / vec + (a.head_dim - 2 * a.pairs + 2 * vec - 1) / (2 * vec);
   s.group = 1;
   while (s.group < chunks) s.group *= 2;
   if (s.group > kWave) return s;
-  s.lanes = (int)((heads + hpt - 1) / hpt);
+  s.lanes = (int)heads;
   // As many whole tokens as fill the waves of a workgroup best, from 256 threads on; a token of
   // more than 512 threads lies over several workgroups.
   const int64_t per = (int64_t)s.group * s.lanes;
@@ -433,6 +446,17 @@ Shape shape_of(const HeadArgs& a, int vec, int hpt) {
   return s;
 }
 
+// A walk of `waves` waves per SIMD: a grid of the workgroups that are resident, and sines of as
+// many steps at a time as give each thread two, within 16 KB.
+void place(HeadArgs& a, Shape& s, int waves) {
+  a.group = s.group, a.lanes = s.lanes, a.per_block = s.per_block;
+  const int64_t resident = 256 * std::max(1, 4 * waves / (s.threads / 64));
+  s.gx = std::min(s.gx, std::max<int64_t>(1, std::min(resident, kMostParts) / s.gy));
+  const int64_t steps = (a.tokens + s.gx * s.per_block - 1) / (s.gx * s.per_block);
+  const int each = std::max(1, a.per_block * a.pairs);
+  a.ahead = (int)std::max<int64_t>(1, std::min<int64_t>(steps, std::min(2 * s.threads, 2048) / each));
+}
+
 // go(VEC) with the widest pack (at most 16 bytes) that divides the halves, the head and every
 // stride, and to which the tensors are aligned.
 template <typename T, int VEC, typename F>
@@ -447,6 +471,25 @@ int by_width(const HeadArgs& a, F&& go) {
     if (!fits) return by_width<T, VEC / 2>(a, go);
   }
   return go(std::integral_constant<int, VEC>{});
+}
+
+// f(GROUP, NT): the lanes of a head where 16-byte packs make it a usual count, else 0; whether the
+// call streams.
+template <int VEC, typename T, typename F>
+int by_group(const HeadArgs& a, F&& f) {
+  if constexpr (VEC * sizeof(T) == 16) {
+    const int64_t heads = a.heads_q + a.heads_k;
+    const bool stream = a.tokens * heads * a.head_dim * (int64_t)sizeof(T) > kStreamBytes;
+    auto with = [&](auto group) {
+      return stream ? f(group, std::true_type{}) : f(group, std::false_type{});
+    };
+    if (a.group == 4) return with(std::integral_constant<int, 4>{});
+    if (a.group == 8) return with(std::integral_constant<int, 8>{});
+    if (a.group == 16) return with(std::integral_constant<int, 16>{});
+    return with(std::integral_constant<int, 0>{});
+  } else {
+    return f(std::integral_constant<int, 0>{}, std::false_type{});
+  }
 }
 
 template <typename F>
@@ -484,9 +527,7 @@ int check(const char* name, int64_t tokens, int64_t heads_q, int64_t heads_k, in
 
 int64_t part_rows(int64_t tokens, int64_t heads) {
   // a token of more than 512 threads (64 lanes a head at most) takes several workgroups
-  return tokens ? std::max<int64_t>({kBackBlocks, (heads * kWave + kMostThreads - 1) / kMostThreads,
-                                     kWideWaves})
-                : 0;
+  return tokens ? std::max(kMostParts, (heads * kWave + kMostThreads - 1) / kMostThreads) : 0;
 }
 
 }  // namespace
@@ -516,32 +557,28 @@ extern "C" int eg_norm_rotary_fwd(const void* q, const void* k, const void* q_we
   a.tokens = tokens;
   a.q_token = strides[0], a.q_head = strides[1], a.k_token = strides[2], a.k_head = strides[3];
   a.heads_q = (int)heads_q, a.heads_k = (int)heads_k, a.head_dim = (int)head_dim;
-  a.pairs = (int)pairs, a.pos64 = positions_64, a.amp = amplitude, a.eps = eps;
+  a.pairs = (int)pairs, a.pos64 = positions_64, a.amp = amplitude, a.eps = eps, a.share = 1.f / head_dim;
   return EG_DISPATCH_FLOAT(dtype, name, [&]() -> int {
     using T = scalar_t;
     return by_layout(interleaved, [&](auto inter) -> int {
       constexpr bool I = decltype(inter)::value;
       return by_width<T, 16 / (int)sizeof(T)>(a, [&](auto vec) -> int {
         constexpr int V = decltype(vec)::value;
-        auto go = [&](auto hpt) -> int {
-          constexpr int N = decltype(hpt)::value;
-          const Shape s = shape_of(a, V, N);
-          a.group = s.group, a.lanes = s.lanes, a.per_block = s.per_block;
-          if (s.gx > 0x7fffffffLL || s.gy > 65535 || check_grid(name, s.gx, s.threads)) {
-            set_error("%s: grid too large", name);
-            return 1;
-          }
-          EG_LAUNCH((norm_rotary_fwd_kernel<T, V, N, I>), dim3((unsigned)s.gx, (unsigned)s.gy),
-                    dim3(s.threads), a.per_block * a.pairs * sizeof(float2), as_stream(stream), a);
-          return check_launch(name);
-        };
-        if (shape_of(a, V, 1).lanes == 0) {
-          const int64_t waves = std::min<int64_t>(tokens * (heads_q + heads_k), kWideWaves);
+        Shape s = shape_of(a, V);
+        if (s.lanes == 0) {
+          const int64_t waves = std::min<int64_t>(tokens * (heads_q + heads_k), kMostParts);
           EG_LAUNCH((norm_rotary_wide_kernel<T, I, false>), dim3((unsigned)waves), dim3(kWave), 0,
                     as_stream(stream), a);
           return check_launch(name);
         }
-        return go(std::integral_constant<int, 1>{});
+        place(a, s, kFrontWaves);
+        if (s.gy > 65535) { set_error("%s: grid too large", name); return 1; }
+        return by_group<V, T>(a, [&](auto group, auto nt) -> int {
+          EG_LAUNCH((norm_rotary_fwd_kernel<T, V, I, decltype(group)::value, decltype(nt)::value>),
+                    dim3((unsigned)s.gx, (unsigned)s.gy), dim3(s.threads),
+                    (size_t)a.ahead * a.per_block * a.pairs * sizeof(float2), as_stream(stream), a);
+          return check_launch(name);
+        });
       });
     });
   });
@@ -581,7 +618,7 @@ extern "C" int eg_norm_rotary_bwd(const void* dq_out, const void* dk_out, const 
   a.q_token = strides[0], a.q_head = strides[1], a.k_token = strides[2], a.k_head = strides[3];
   a.dq_token = strides[4], a.dq_head = strides[5], a.dk_token = strides[6], a.dk_head = strides[7];
   a.heads_q = (int)heads_q, a.heads_k = (int)heads_k, a.head_dim = (int)head_dim;
-  a.pairs = (int)pairs, a.pos64 = positions_64, a.amp = amplitude, a.eps = eps;
+  a.pairs = (int)pairs, a.pos64 = positions_64, a.amp = amplitude, a.eps = eps, a.share = 1.f / head_dim;
   return EG_DISPATCH_FLOAT(dtype, name, [&]() -> int {
     using T = scalar_t;
     int parts = 0;
@@ -590,22 +627,23 @@ extern "C" int eg_norm_rotary_bwd(const void* dq_out, const void* dk_out, const 
         constexpr bool I = decltype(inter)::value;
         return by_width<T, 16 / (int)sizeof(T)>(a, [&](auto vec) -> int {
           constexpr int V = decltype(vec)::value;
-          Shape s = shape_of(a, V, 1);
+          Shape s = shape_of(a, V);
           if (s.lanes == 0) {
-            parts = (int)std::min<int64_t>(tokens * (heads_q + heads_k), kWideWaves);
+            parts = (int)std::min<int64_t>(tokens * (heads_q + heads_k), kMostParts);
             EG_LAUNCH((norm_rotary_wide_kernel<T, I, true>), dim3((unsigned)parts), dim3(kWave),
                       2 * head_dim * sizeof(float), as_stream(stream), a);
             return check_launch(name);
           }
-          a.group = s.group, a.lanes = s.lanes, a.per_block = s.per_block;
-          s.gx = std::min(s.gx, std::max<int64_t>(1, kBackBlocks / s.gy));
+          place(a, s, kBackGrid);
           if (s.gy > 65535) { set_error("%s: grid too large", name); return 1; }
           parts = (int)(s.gx * s.gy);
-          const size_t lds = std::max<size_t>(2 * a.per_block * a.pairs * sizeof(float2),
+          const size_t lds = std::max<size_t>((size_t)a.ahead * a.per_block * a.pairs * sizeof(float2),
                                               (size_t)s.threads / s.group * head_dim * sizeof(float));
-          EG_LAUNCH((norm_rotary_bwd_kernel<T, V, 1, I>), dim3((unsigned)s.gx, (unsigned)s.gy),
-                    dim3(s.threads), lds, as_stream(stream), a);
-          return check_launch(name);
+          return by_group<V, T>(a, [&](auto group, auto nt) -> int {
+            EG_LAUNCH((norm_rotary_bwd_kernel<T, V, I, decltype(group)::value, decltype(nt)::value>),
+                      dim3((unsigned)s.gx, (unsigned)s.gy), dim3(s.threads), lds, as_stream(stream), a);
+            return check_launch(name);
+          });
         });
       });
       if (rc) return rc;

@@ -16,6 +16,14 @@
 // the backward's exponents are small differences, and p with the entries of one column added
 // up in the first of them: every column of the backward has one term at most, which it finds in
 // LDS.
+//
+// Kernels: distill_row_kernel streams the rows (a workgroup a row, or a part of one where rows
+// are few) and leaves their sums; distill_finish_kernel does the rest of a row, whose work is a
+// chain of short steps, in one wave; distill_mean_kernel adds the rows; distill_bwd_kernel. With
+// the finish at the end of the row's own workgroup, bf16 [8192, 128256] with 64 entries, a tenth
+// of the rows ignored, took 597 us forward instead of 309 + 19 + 5: the streams of a CU's other
+// workgroup do not fill it. Backward 692 us, 5.8 TB/s; with the entries loaded after the
+// first barrier 939.
 #include "rowwise.hpp"
 
 #include <algorithm>
@@ -29,9 +37,14 @@ using rowwise::kUnroll;
 using rowwise::lse_ref;
 
 constexpr int kMaxEntries = 1024;
-constexpr int kFinishBlock = 256, kMeanBlock = 1024;
+constexpr int kMeanBlock = 1024;
+constexpr int64_t kFewRows = 32;  // that one workgroup finishes, two a wave
 constexpr int kFlatBlock = rowwise::kFlatBlock, kFlatUnroll = rowwise::kFlatUnroll,
               kFlatPer = rowwise::kFlatPer;
+
+// The exponentials of a column: one of them (no hard label, no soft part or a temperature of 1),
+// both, or, at a temperature of 2, the hard label's as the soft one's square.
+enum Exps { kOne, kTwo, kSquare };
 
 struct DistillArgs {
   const void *logits, *teacher, *ids;
@@ -43,6 +56,7 @@ struct DistillArgs {
   int64_t rows, ignore_index;
   int cols, k, slots, splits, ids_64, teacher_type;
   float tau, soft, hard;
+  float c1, ct;  // log2(e), log2(e) / tau
 };
 
 __device__ __forceinline__ int64_t entry_id(const DistillArgs& a, int64_t i) {
@@ -54,34 +68,44 @@ __device__ __forceinline__ float entry_value(const DistillArgs& a, int64_t i) {
                                     : to_f32(((const bf16_t*)a.teacher)[i]);
 }
 
-// A running (max, sum of exp(z - max), sum of exp((z - max) / tau)) of a row's part.
-struct RowSums {
-  float m, s1, st;
-};
+// exp(d) and exp(d / tau) of a difference to the row's maximum; kOne: both the one that is used.
+template <int E>
+__device__ __forceinline__ void exps(const DistillArgs& a, float d, float& e1, float& et) {
+  et = __builtin_amdgcn_exp2f(d * a.ct);
+  e1 = E == kTwo ? __builtin_amdgcn_exp2f(d * a.c1) : E == kSquare ? et * et : et;
+}
+
 // Brings `s`, a sum relative to `from`, to the reference `to` (both as lse_ref gives them).
 __device__ __forceinline__ float rescale(float s, float from, float to, float c) {
   return s == 0.f ? 0.f : s * __builtin_amdgcn_exp2f((from - to) * c);
 }
 
-// One workgroup's columns [c0, c1) of a row, the same result in every thread.
-template <typename T, int VEC, int BLOCK, bool RAG>
-__device__ __forceinline__ RowSums row_sums(const T* __restrict__ xr, int c0, int c1, int cols,
-                                            float ct, float* red) {
+// (max, sum of exp(z - max), sum of exp((z - max) / tau)) of a row's part, by a workgroup.
+template <typename T, int VEC, int BLOCK, bool RAG, int E>
+__global__ __launch_bounds__(BLOCK) void distill_row_kernel(DistillArgs a) {
+  __shared__ float red[BLOCK / kWave], red2[BLOCK / kWave];
   constexpr int STEP = BLOCK * VEC;
-  RowSums r = {-INFINITY, 0.f, 0.f};
+  const int64_t row = blockIdx.x;
+  if (a.target[row] == a.ignore_index) return;
+  const T* __restrict__ xr = (const T*)a.logits + row * a.cols;
+  const int64_t packs = (a.cols + VEC - 1) / VEC;
+  const int64_t each = (packs + a.splits - 1) / a.splits * VEC;
+  const int c0 = (int)min((int64_t)blockIdx.y * each, (int64_t)a.cols);
+  const int c1 = (int)min(c0 + each, (int64_t)a.cols);
+  float m = -INFINITY, s1 = 0.f, st = 0.f;
   for (int64_t base = c0 + (int64_t)threadIdx.x * VEC; base < c1; base += STEP * kUnroll) {
     float v[kUnroll][VEC];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const int64_t c = base + u * STEP;
       if (c < c1) {
-        rowwise::load_pack<T, VEC, VEC * sizeof(T) == 16, RAG>(xr, (int)c, cols, -INFINITY, v[u]);
+        rowwise::load_pack<T, VEC, VEC * sizeof(T) == 16, RAG>(xr, (int)c, a.cols, -INFINITY, v[u]);
       } else {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) v[u][i] = -INFINITY;
       }
     }
-    float bm = r.m;
+    float bm = m;
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
 #pragma unroll
@@ -92,164 +116,139 @@ __device__ __forceinline__ RowSums row_sums(const T* __restrict__ xr, int c0, in
     for (int u = 0; u < kUnroll; ++u)
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        const float d = v[u][i] - ref;
-        a1 += __builtin_amdgcn_exp2f(d * kLog2e);
-        at += __builtin_amdgcn_exp2f(d * ct);
+        float e1, et;
+        exps<E>(a, v[u][i] - ref, e1, et);
+        a1 += e1;
+        if (E != kOne) at += et;
       }
-    r.s1 = rescale(r.s1, lse_ref(r.m), ref, kLog2e) + a1;
-    r.st = rescale(r.st, lse_ref(r.m), ref, ct) + at;
-    r.m = bm;
+    s1 = rescale(s1, lse_ref(m), ref, E == kOne ? a.ct : a.c1) + a1;
+    if (E != kOne) st = rescale(st, lse_ref(m), ref, a.ct) + at;
+    m = bm;
   }
-  const float gm = block_reduce<BLOCK>(r.m, MaxOp(), red), ref = lse_ref(gm);
-  r.s1 = block_reduce<BLOCK>(rescale(r.s1, lse_ref(r.m), ref, kLog2e), SumOp(), red);
-  r.st = block_reduce<BLOCK>(rescale(r.st, lse_ref(r.m), ref, ct), SumOp(), red);
-  r.m = gm;
-  return r;
+  const float gm = block_reduce<BLOCK>(m, MaxOp(), red), ref = lse_ref(gm);
+  s1 = block_reduce<BLOCK>(rescale(s1, lse_ref(m), ref, E == kOne ? a.ct : a.c1), SumOp(), red2);
+  if (E == kOne) st = s1;
+  else st = block_reduce<BLOCK>(rescale(st, lse_ref(m), ref, a.ct), SumOp(), red);
+  if (threadIdx.x == 0) {
+    float* p = a.part + (row * a.splits + blockIdx.y) * 3;
+    p[0] = gm, p[1] = s1, p[2] = st;
+  }
 }
 
-// The rest of a counted row by one workgroup: its loss, saved statistics and probabilities.
-// `lds` holds slots x 2 ints and K floats.
-template <typename T, int BLOCK>
-__device__ __forceinline__ void finish_row(const DistillArgs& a, int64_t row, RowSums r, int* lds,
-                                           float* red) {
-  int *table = lds, *holder = lds + a.slots;
-  float* p = (float*)(lds + 2 * a.slots);
+// A wave's stores to LDS before its later loads of them by other lanes.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// The rest of a row by one wave: its parts joined, the teacher's distribution, the loss, what the
+// backward needs. `lds` holds 2 slots + 3 K words. Returns the row's loss.
+template <typename T>
+__device__ __forceinline__ float finish_row(const DistillArgs& a, int64_t row, int* lds) {
+  const int lane = threadIdx.x & 63;
+  const int64_t e0 = row * a.k, t = a.target[row];
+  float* s = a.stats + row * 4;
+  if (t == a.ignore_index) {
+    for (int k = lane; k < a.k; k += kWave) a.probs[e0 + k] = 0.f;
+    if (lane < 4) s[lane] = 0.f;
+    return 0.f;
+  }
+  int *table = lds, *holder = lds + a.slots, *ids = lds + 2 * a.slots;
+  float *p = (float*)(ids + a.k), *zs = p + a.k;
   const T* xr = (const T*)a.logits + row * a.cols;
-  const int64_t e0 = row * a.k;
-  const float ref = lse_ref(r.m), rtau = 1.f / a.tau;
-  for (int i = threadIdx.x; i < a.slots; i += BLOCK) table[i] = -1, holder[i] = kMaxEntries;
-  float tm = -INFINITY, bad = 0.f;
-  for (int k = threadIdx.x; k < a.k; k += BLOCK) {
+  // every load first: parts, the target's logit, entries, their logits
+  const bool part = lane < a.splits;
+  const float* q = a.part + (row * a.splits + (part ? lane : 0)) * 3;
+  const float pm = part ? q[0] : -INFINITY, p1 = part ? q[1] : 0.f, pt = part ? q[2] : 0.f;
+  const bool label = t >= 0 && t < a.cols;
+  const float zt = label ? to_f32(xr[t]) : NAN;
+  float tm = -INFINITY, bad = a.hard != 0.f && !label ? 1.f : 0.f;
+  for (int i = lane; i < a.slots; i += kWave) table[i] = -1, holder[i] = kMaxEntries;
+  for (int k = lane; k < a.k; k += kWave) {
     const int64_t id = entry_id(a, e0 + k);
+    const float v = entry_value(a, e0 + k);
     if (id >= a.cols) bad = 1.f;
-    if (id >= 0 && id < a.cols) tm = fmaxf(tm, entry_value(a, e0 + k));
-  }
-  __syncthreads();
-  tm = lse_ref(block_reduce<BLOCK>(tm, MaxOp(), red));
-  bad = block_reduce<BLOCK>(bad, SumOp(), red);
-  float total = 0.f;
-  for (int k = threadIdx.x; k < a.k; k += BLOCK) {
-    const int64_t id = entry_id(a, e0 + k);
     const bool in = id >= 0 && id < a.cols;
-    total += p[k] = in ? expf((entry_value(a, e0 + k) - tm) * rtau) : 0.f;
+    ids[k] = in ? (int)id : -1;
+    p[k] = v;
+    zs[k] = in ? to_f32(xr[id]) : 0.f;
+    if (in) tm = fmaxf(tm, v);
   }
-  total = block_reduce<BLOCK>(total, SumOp(), red);
+  const float m = wave_reduce(pm, MaxOp()), ref = lse_ref(m);
+  const bool one = a.soft == 0.f || a.hard == 0.f || a.tau == 1.f;
+  const float s1 = wave_reduce(rescale(p1, lse_ref(pm), ref, one ? a.ct : a.c1), SumOp());
+  const float st = wave_reduce(rescale(pt, lse_ref(pm), ref, a.ct), SumOp());
+  tm = lse_ref(wave_reduce(tm, MaxOp()));
+  bad = wave_reduce(bad, SumOp());
+  const float rtau = 1.f / a.tau;
+  float total = 0.f;
+  for (int k = lane; k < a.k; k += kWave)
+    if (ids[k] >= 0) total += expf((p[k] - tm) * rtau);
+  total = wave_reduce(total, SumOp());
   const bool some = total != 0.f;  // a NaN is one
-  const float lt = logf(total), lq = logf(r.st);
+  const float lt = logf(total), lq = logf(st);
   float kl = 0.f;
-  for (int k = threadIdx.x; k < a.k; k += BLOCK) {
-    const int64_t id = entry_id(a, e0 + k);
-    const float pk = some && id >= 0 && id < a.cols ? p[k] / total : 0.f;
+  bool again = false;  // an entry of another one's column
+  wave_sync();
+  for (int k = lane; k < a.k; k += kWave) {
+    const int id = ids[k];
+    const float logit = (p[k] - tm) * rtau, pk = some && id >= 0 ? expf(logit) / total : 0.f;
     p[k] = pk;
     if (pk == 0.f) continue;
-    const float logq = (to_f32(xr[id]) - ref) * rtau - lq;
-    kl += pk * ((entry_value(a, e0 + k) - tm) * rtau - lt - logq);
+    kl += pk * (logit - lt - ((zs[k] - ref) * rtau - lq));
     // the first entry of each column, in a hash table of at least twice the entries
-    unsigned s = (unsigned)id * 2654435761u >> 16;
-    for (;; ++s) {
-      s &= a.slots - 1;
-      const int was = atomicCAS(&table[s], -1, (int)id);
-      if (was == -1 || was == (int)id) break;
+    unsigned at = (unsigned)id * 2654435761u >> 16;
+    for (;; ++at) {
+      at &= a.slots - 1;
+      const int was = atomicCAS(&table[at], -1, id);
+      again = again || was == id;
+      if (was == -1 || was == id) break;
     }
-    atomicMin(&holder[s], k);
+    atomicMin(&holder[at], k);
   }
-  kl = block_reduce<BLOCK>(kl, SumOp(), red);
-  __syncthreads();
-  for (int k = threadIdx.x; k < a.k; k += BLOCK) {
-    const int64_t id = entry_id(a, e0 + k);
+  kl = wave_reduce(kl, SumOp());
+  again = __any(again);
+  wave_sync();
+  for (int k = lane; k < a.k; k += kWave) {
     float sum = p[k];
-    if (sum != 0.f) {
-      unsigned s = (unsigned)id * 2654435761u >> 16;
-      for (;; ++s) {
-        s &= a.slots - 1;
-        if (table[s] == (int)id) break;
+    if (again && sum != 0.f) {
+      const int id = ids[k];
+      unsigned at = (unsigned)id * 2654435761u >> 16;
+      for (;; ++at) {
+        at &= a.slots - 1;
+        if (table[at] == id) break;
       }
-      if (holder[s] != k) {
+      if (holder[at] != k) {
         sum = 0.f;
       } else {
         for (int j = k + 1; j < a.k; ++j)
-          if (entry_id(a, e0 + j) == id) sum += p[j];
+          if (ids[j] == id) sum += p[j];
       }
     }
     a.probs[e0 + k] = sum;
   }
-  if (threadIdx.x == 0) {
-    float loss = 0.f;
-    const int64_t t = a.target[row];
-    if (a.soft != 0.f && some) loss += a.soft * a.tau * a.tau * kl;
-    if (a.hard != 0.f) {
-      if (t < 0 || t >= a.cols) bad = 1.f;
-      else loss += a.hard * (logf(r.s1) - (to_f32(xr[t]) - ref));
-    }
-    const float fail = bad != 0.f ? NAN : 0.f;
-    a.rowloss[row] = loss + fail;
-    float* s = a.stats + row * 4;
+  float loss = 0.f;
+  if (a.soft != 0.f && some) loss += a.soft * a.tau * a.tau * kl;
+  if (a.hard != 0.f && label) loss += a.hard * (logf(s1) - (zt - ref));
+  const float fail = bad != 0.f ? NAN : 0.f;
+  if (lane == 0) {
     s[0] = ref;
-    s[1] = 1.f / r.s1 + fail;
-    s[2] = some ? 1.f / r.st + fail : fail;
+    s[1] = 1.f / s1 + fail;
+    s[2] = some ? 1.f / st + fail : fail;
     s[3] = 0.f;
   }
+  return loss + fail;
 }
 
-template <int BLOCK>
-__device__ __forceinline__ void skip_row(const DistillArgs& a, int64_t row) {
-  for (int k = threadIdx.x; k < a.k; k += BLOCK) a.probs[row * a.k + k] = 0.f;
-  if (threadIdx.x < 4) a.stats[row * 4 + threadIdx.x] = 0.f;
-  if (threadIdx.x == 0) a.rowloss[row] = 0.f;
-}
-
-// A workgroup a row, or (splits > 1) a part of one.
-template <typename T, int VEC, int BLOCK, bool RAG>
-__global__ __launch_bounds__(BLOCK) void distill_row_kernel(DistillArgs a) {
-  extern __shared__ int lds[];
-  __shared__ float red[BLOCK / kWave];
-  const int64_t row = blockIdx.x;
-  if (a.target[row] == a.ignore_index) {
-    if (a.splits == 1) skip_row<BLOCK>(a, row);
-    return;
-  }
-  const T* xr = (const T*)a.logits + row * a.cols;
-  const int64_t packs = (a.cols + VEC - 1) / VEC;
-  const int64_t each = (packs + a.splits - 1) / a.splits * VEC;
-  const int c0 = (int)min((int64_t)blockIdx.y * each, (int64_t)a.cols);
-  const int c1 = (int)min(c0 + each, (int64_t)a.cols);
-  const RowSums r = row_sums<T, VEC, BLOCK, RAG>(xr, c0, c1, a.cols, kLog2e / a.tau, red);
-  if (a.splits == 1) {
-    finish_row<T, BLOCK>(a, row, r, lds, red);
-  } else if (threadIdx.x == 0) {
-    float* p = a.part + (row * a.splits + blockIdx.y) * 3;
-    p[0] = r.m, p[1] = r.s1, p[2] = r.st;
-  }
-}
-
+// A wave a row.
 template <typename T>
-__global__ __launch_bounds__(kFinishBlock) void distill_finish_kernel(DistillArgs a) {
+__global__ __launch_bounds__(kWave) void distill_finish_kernel(DistillArgs a) {
   extern __shared__ int lds[];
-  __shared__ float red[kFinishBlock / kWave];
-  const int64_t row = blockIdx.x;
-  if (a.target[row] == a.ignore_index) {
-    skip_row<kFinishBlock>(a, row);
-    return;
-  }
-  const float ct = kLog2e / a.tau;
-  RowSums r = {-INFINITY, 0.f, 0.f};
-  for (int i = 0; i < a.splits; ++i) r.m = fmaxf(r.m, a.part[(row * a.splits + i) * 3]);
-  const float ref = lse_ref(r.m);
-  for (int i = 0; i < a.splits; ++i) {
-    const float* p = a.part + (row * a.splits + i) * 3;
-    r.s1 += rescale(p[1], lse_ref(p[0]), ref, kLog2e);
-    r.st += rescale(p[2], lse_ref(p[0]), ref, ct);
-  }
-  finish_row<T, kFinishBlock>(a, row, r, lds, red);
+  const float loss = finish_row<T>(a, blockIdx.x, lds);
+  if (threadIdx.x == 0) a.rowloss[blockIdx.x] = loss;
 }
 
-__global__ __launch_bounds__(kMeanBlock) void distill_mean_kernel(DistillArgs a) {
-  __shared__ float red[kMeanBlock / kWave];
-  float sum = 0.f, count = 0.f;
-  for (int64_t r = threadIdx.x; r < a.rows; r += kMeanBlock) {
-    sum += a.rowloss[r];
-    count += a.target[r] != a.ignore_index ? 1.f : 0.f;
-  }
+__device__ __forceinline__ void write_mean(const DistillArgs& a, float sum, float count, float* red) {
   sum = block_reduce<kMeanBlock>(sum, SumOp(), red);
   count = block_reduce<kMeanBlock>(count, SumOp(), red);
   if (threadIdx.x == 0) {
@@ -258,95 +257,161 @@ __global__ __launch_bounds__(kMeanBlock) void distill_mean_kernel(DistillArgs a)
   }
 }
 
-// What a row's gradient takes: dz = g1 exp(z - m) + gt exp((z - m) / tau) - gp p - [target] gh.
+constexpr int kMeanRows = 8;  // in flight per thread
+__global__ __launch_bounds__(kMeanBlock) void distill_mean_kernel(DistillArgs a) {
+  __shared__ float red[kMeanBlock / kWave];
+  float sum = 0.f, count = 0.f;
+  for (int64_t r0 = threadIdx.x; r0 < a.rows; r0 += kMeanBlock * kMeanRows) {
+    float l[kMeanRows], ok[kMeanRows];
+#pragma unroll
+    for (int j = 0; j < kMeanRows; ++j) {
+      const int64_t r = r0 + (int64_t)j * kMeanBlock;
+      const bool in = r < a.rows;
+      ok[j] = in && a.target[r] != a.ignore_index ? 1.f : 0.f;
+      l[j] = in ? a.rowloss[r] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < kMeanRows; ++j) sum += l[j], count += ok[j];
+  }
+  write_mean(a, sum, count, red);
+}
+
+// Both, by one workgroup, where rows are few: a launch less.
+template <typename T>
+__global__ __launch_bounds__(kMeanBlock) void distill_finish_all_kernel(DistillArgs a) {
+  extern __shared__ int lds[];
+  __shared__ float red[kMeanBlock / kWave];
+  const int wave = threadIdx.x >> 6;
+  float sum = 0.f, count = 0.f;
+  for (int64_t row = wave; row < a.rows; row += kMeanBlock / kWave) {
+    const float loss = finish_row<T>(a, row, lds + wave * (2 * a.slots + 3 * a.k));
+    if ((threadIdx.x & 63) == 0) {
+      sum += loss;
+      count += a.target[row] != a.ignore_index ? 1.f : 0.f;
+    }
+  }
+  write_mean(a, sum, count, red);
+}
+
+// What a row's gradient takes: dz = g1 exp(z - m) + gt exp((z - m) / tau), less what its entries
+// and target have.
 struct RowGrad {
   float m, g1, gt;
-  int target;
   bool live;
 };
+__device__ __forceinline__ RowGrad row_grad(const DistillArgs& a, int64_t row, float gh, float gp) {
+  RowGrad g;
+  g.live = a.target[row] != a.ignore_index;
+  const float* s = a.stats + row * 4;
+  g.m = s[0], g.g1 = gh * s[1], g.gt = gp * s[2];
+  return g;
+}
 
-// The matrix as one run of packs, kFlatPer a workgroup (rowwise.hpp). The entries' terms of its
-// packs are laid out in LDS first. TWO: both exponentials, else the one of factor c.
-template <typename T, int VEC, bool RAG, bool TWO>
+// The matrix as one run of packs, kFlatPer a workgroup (rowwise.hpp). What entries and targets
+// take from its columns is laid out in LDS, while the packs are on their way: entries of a column
+// are one (finish_row), so that a place has two addends at most and their order does not matter.
+// MANY: rows of fewer than kFlatPer packs.
+template <typename T, int VEC, bool RAG, int E, bool MANY>
 __global__ __launch_bounds__(kFlatBlock) void distill_bwd_kernel(DistillArgs a) {
   __shared__ __attribute__((aligned(16))) float terms[kFlatPer * VEC];
   constexpr bool NT = VEC * sizeof(T) == 16;
   const unsigned ppr = (a.cols + VEC - 1) / VEC;  // packs per row
   const int64_t npack = a.rows * ppr, first = (int64_t)blockIdx.x * kFlatPer;
-  const int64_t row0 = first / ppr;
+  const int64_t row0 = npack >> 32 ? first / ppr : (unsigned)first / ppr;
   const unsigned in0 = (unsigned)(first - row0 * ppr);  // the workgroup's first pack in its row
+  const int64_t last = min(first + kFlatPer, npack) - 1;
+  const int rows = 1 + (MANY ? (int)((in0 + (unsigned)(last - first)) / ppr)
+                             : in0 + (unsigned)(last - first) >= ppr ? 1 : 0);
   const float scale = a.dloss[0] / a.n_valid[0];
   const float gh = scale * a.hard, gp = scale * a.soft * a.tau;
-  const float ct = kLog2e / a.tau;
+  // this thread's first entry
+  const int64_t e0 = row0 * a.k;
+  const int n = a.soft != 0.f ? rows * a.k : 0;
+  float p0 = 0.f;
+  int64_t id0 = -1;
+  if ((int)threadIdx.x < n) p0 = a.probs[e0 + threadIdx.x], id0 = entry_id(a, e0 + threadIdx.x);
+  RowGrad g[MANY ? kFlatUnroll : 2];
+  if constexpr (!MANY) {
+    g[0] = row_grad(a, row0, gh, gp);
+    g[1] = rows > 1 ? row_grad(a, row0 + 1, gh, gp) : g[0];
+  }
   float v[kFlatUnroll][VEC];
-  RowGrad g[kFlatUnroll];
-  unsigned rows[kFlatUnroll], packs[kFlatUnroll];
+  unsigned at[kFlatUnroll], pack[kFlatUnroll];  // row, counted from row0, and pack in it
 #pragma unroll
   for (int u = 0; u < kFlatUnroll; ++u) {
     const unsigned q = in0 + u * kFlatBlock + threadIdx.x;
-    rows[u] = q / ppr, packs[u] = q - rows[u] * ppr;
-    g[u].live = false;
-    if (first + u * kFlatBlock + threadIdx.x >= npack) continue;
-    const int64_t row = row0 + rows[u];
-    const int64_t t = a.target[row];
-    g[u].live = t != a.ignore_index;
-    if (!g[u].live) continue;
-    rowwise::load_pack<T, VEC, NT, RAG>((const T*)a.logits + row * a.cols, packs[u] * VEC, a.cols, 0.f,
-                                        v[u]);
-    const float* s = a.stats + row * 4;
-    g[u].m = s[0], g[u].g1 = gh * s[1], g[u].gt = gp * s[2];
-    g[u].target = a.hard != 0.f && t >= 0 && t < a.cols ? (int)t : -1;
+    at[u] = MANY ? q / ppr : q >= ppr ? 1 : 0;
+    pack[u] = q - at[u] * ppr;
+    if (first + u * kFlatBlock + threadIdx.x > last) continue;
+    if constexpr (MANY) g[u] = row_grad(a, row0 + at[u], gh, gp);
+    if (MANY ? g[u].live : at[u] ? g[1].live : g[0].live)
+      rowwise::load_pack<T, VEC, NT, RAG>((const T*)a.logits + (row0 + at[u]) * a.cols, pack[u] * VEC,
+                                          a.cols, 0.f, v[u]);
   }
-  const bool entries = a.k > 0 && a.soft != 0.f;
-  if (entries) {
-#pragma unroll
-    for (int u = 0; u < kFlatUnroll; ++u)
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) terms[(u * kFlatBlock + threadIdx.x) * VEC + i] = 0.f;
-    __syncthreads();
-    const int64_t last = min(first + kFlatPer, npack) - 1;
-    const int64_t e0 = row0 * a.k, n = (last / ppr + 1) * a.k - e0;
-    for (int64_t i = threadIdx.x; i < n; i += kFlatBlock) {
-      const float p = a.probs[e0 + i];
-      if (p == 0.f) continue;
-      const int64_t id64 = entry_id(a, e0 + i);
-      if (id64 < 0 || id64 >= a.cols) continue;  // written over since the forward
-      const int id = (int)id64;
-      const int64_t at = i / a.k * ppr - in0;  // the row's first pack, from the workgroup's first
-      const int64_t k = at + id / VEC;
-      const int lo = RAG ? a.cols - VEC : 0;
-      if (RAG && id >= lo) {  // the last pack, which overlaps the one before it
-        const int64_t l = at + ppr - 1;
-        if (l >= 0 && l < kFlatPer) terms[l * VEC + id - lo] = p;
-        if (id / VEC == (int)ppr - 1) continue;
-      }
-      if (k >= 0 && k < kFlatPer) terms[k * VEC + id % VEC] = p;
-    }
-    __syncthreads();
-  }
+  float* own[kFlatUnroll];
 #pragma unroll
   for (int u = 0; u < kFlatUnroll; ++u) {
-    if (first + u * kFlatBlock + threadIdx.x >= npack) continue;
+    own[u] = terms + (u * kFlatBlock + threadIdx.x) * VEC;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) own[u][i] = 0.f;
+  }
+  __syncthreads();
+  // takes `value` from a column of row r (from row0)
+  auto take = [&](int r, int64_t id64, float value) {
+    if (id64 < 0 || id64 >= a.cols) return;
+    const int id = (int)id64;
+    const int64_t row = (int64_t)r * ppr - in0;  // its first pack, from the workgroup's first
+    const int64_t k = row + id / VEC;
+    if (RAG && id >= a.cols - VEC) {  // the last pack, which overlaps the one before it
+      const int64_t l = row + ppr - 1;
+      if (l >= 0 && l < kFlatPer) atomicAdd(&terms[l * VEC + id - (a.cols - VEC)], value);
+      if (id / VEC == (int)ppr - 1) return;
+    }
+    if (k >= 0 && k < kFlatPer) atomicAdd(&terms[k * VEC + id % VEC], value);
+  };
+  if (p0 != 0.f) take((int)threadIdx.x / a.k, id0, gp * p0);
+  for (int i = threadIdx.x + kFlatBlock; i < n; i += kFlatBlock) {
+    const float p = a.probs[e0 + i];
+    if (p != 0.f) take(i / a.k, entry_id(a, e0 + i), gp * p);
+  }
+  if (a.hard != 0.f)
+    for (int r = threadIdx.x; r < rows; r += kFlatBlock) take(r, a.target[row0 + r], gh);
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kFlatUnroll; ++u) {
+    if (first + u * kFlatBlock + threadIdx.x > last) continue;
+    const RowGrad& r = g[MANY ? u : at[u] ? 1 : 0];
     float o[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) o[i] = 0.f;
-    if (g[u].live) {
-      const int c = packs[u] * VEC, c0 = RAG ? min(c, a.cols - VEC) : c;
+    if (r.live) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        const float d = v[u][i] - g[u].m;
-        if constexpr (TWO)
-          o[i] = g[u].g1 * __builtin_amdgcn_exp2f(d * kLog2e) +
-                 g[u].gt * __builtin_amdgcn_exp2f(d * ct);
-        else
-          o[i] = a.soft != 0.f ? (g[u].g1 + g[u].gt) * __builtin_amdgcn_exp2f(d * ct)
-                               : g[u].g1 * __builtin_amdgcn_exp2f(d * kLog2e);
-        if (entries) o[i] -= gp * terms[(u * kFlatBlock + threadIdx.x) * VEC + i];
-        if (c0 + i == g[u].target) o[i] -= gh;
+        float e1, et;
+        exps<E>(a, v[u][i] - r.m, e1, et);
+        if constexpr (E == kOne) o[i] = __builtin_fmaf(r.g1 + r.gt, et, -own[u][i]);
+        else if constexpr (E == kTwo) o[i] = __builtin_fmaf(r.g1, e1, __builtin_fmaf(r.gt, et, -own[u][i]));
+        else o[i] = __builtin_fmaf(__builtin_fmaf(r.g1, et, r.gt), et, -own[u][i]);
       }
     }
-    rowwise::store_pack<T, VEC, NT, RAG>((T*)a.dlogits + (row0 + rows[u]) * a.cols, packs[u] * VEC,
-                                         a.cols, o);
+    rowwise::store_pack<T, VEC, NT, RAG>((T*)a.dlogits + (row0 + at[u]) * a.cols, pack[u] * VEC, a.cols,
+                                         o);
+  }
+}
+
+// How the exponentials are formed; for kOne the factor of the one that is used becomes ct.
+int exps_of(DistillArgs& a) {
+  a.c1 = kLog2e, a.ct = kLog2e / a.tau;
+  if (a.soft == 0.f) a.ct = kLog2e;
+  if (a.soft == 0.f || a.hard == 0.f || a.tau == 1.f) return kOne;
+  return a.tau == 2.f ? kSquare : kTwo;
+}
+template <typename F>
+int by_exps(int e, F&& f) {
+  switch (e) {
+    case kOne: return f(std::integral_constant<int, kOne>{});
+    case kTwo: return f(std::integral_constant<int, kTwo>{});
+    default: return f(std::integral_constant<int, kSquare>{});
   }
 }
 
@@ -355,23 +420,23 @@ int slots_for(int k) {
   while (s < 2 * k) s *= 2;
   return s;
 }
-size_t finish_lds(const DistillArgs& a) { return (2 * a.slots + a.k) * sizeof(int); }
+size_t finish_lds(const DistillArgs& a) { return (2 * a.slots + 3 * a.k) * sizeof(int); }
 
-// Parts of a row, where rows are few.
+// Parts of a row, where rows are few; a lane each in the finish.
 constexpr int kMostSplits = 64;
 int splits_for(int64_t rows, int64_t cols) {
   const int64_t want = 512 / std::max<int64_t>(rows, 1), most = cols / 8192;
   return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, kMostSplits}));
 }
 
-template <typename T, int VEC, bool RAG>
+template <typename T, int VEC, bool RAG, int E>
 struct RowLaunch {
   const DistillArgs& a;
   hipStream_t st;
   template <int BLOCK>
   void go() {
-    EG_LAUNCH((distill_row_kernel<T, VEC, BLOCK, RAG>), dim3((unsigned)a.rows, a.splits), dim3(BLOCK),
-              a.splits == 1 ? finish_lds(a) : 0, st, a);
+    EG_LAUNCH((distill_row_kernel<T, VEC, BLOCK, RAG, E>), dim3((unsigned)a.rows, a.splits),
+              dim3(BLOCK), 0, st, a);
   }
 };
 
@@ -408,8 +473,7 @@ using namespace eg;
 
 extern "C" size_t eg_topk_distill_workspace_bytes(int64_t rows, int64_t cols) {
   if (rows <= 0 || cols <= 0) return 0;
-  const int splits = splits_for(rows, cols);
-  return (size_t)rows * (1 + (splits > 1 ? 3 * splits : 0)) * sizeof(float);
+  return (size_t)rows * (1 + 3 * splits_for(rows, cols)) * sizeof(float);
 }
 
 extern "C" int eg_topk_distill_fwd(const void* logits, const int64_t* target, const void* teacher,
@@ -443,15 +507,22 @@ extern "C" int eg_topk_distill_fwd(const void* logits, const int64_t* target, co
     using T = scalar_t;
     if (rows) {
       if (check_grid(name, rows, 1024)) return 1;
-      by_width<T>(cols, {logits}, [&](auto vec, auto rag) {
-        constexpr int V = decltype(vec)::value;
-        const int64_t packs = ((cols + V - 1) / V + a.splits - 1) / a.splits;
-        rowwise::pick_row_block(packs, RowLaunch<T, V, decltype(rag)::value>{a, st});
-        return 0;
+      by_exps(exps_of(a), [&](auto e) {
+        return by_width<T>(cols, {logits}, [&](auto vec, auto rag) {
+          constexpr int V = decltype(vec)::value;
+          const int64_t packs = ((cols + V - 1) / V + a.splits - 1) / a.splits;
+          rowwise::pick_row_block(packs,
+                                  RowLaunch<T, V, decltype(rag)::value, decltype(e)::value>{a, st});
+          return 0;
+        });
       });
-      if (a.splits > 1)
-        EG_LAUNCH((distill_finish_kernel<T>), dim3((unsigned)rows), dim3(kFinishBlock), finish_lds(a),
-                  st, a);
+      const size_t lds = finish_lds(a);
+      if (rows <= kFewRows && kMeanBlock / kWave * lds <= 65536) {
+        EG_LAUNCH((distill_finish_all_kernel<T>), dim3(1), dim3(kMeanBlock), kMeanBlock / kWave * lds, st,
+                  a);
+        return check_launch(name);
+      }
+      EG_LAUNCH((distill_finish_kernel<T>), dim3((unsigned)rows), dim3(kWave), lds, st, a);
     }
     EG_LAUNCH(distill_mean_kernel, dim3(1), dim3(kMeanBlock), 0, st, a);
     return check_launch(name);
@@ -479,20 +550,24 @@ extern "C" int eg_topk_distill_bwd(const float* dloss, const void* logits, const
   a.n_valid = const_cast<float*>(n_valid), a.dlogits = dlogits;
   a.rows = rows, a.cols = (int)cols, a.k = (int)entries, a.ignore_index = ignore_index;
   a.ids_64 = ids_64, a.tau = temperature, a.soft = soft_weight, a.hard = hard_weight;
-  const bool two = soft_weight != 0.f && hard_weight != 0.f && temperature != 1.f;
+  const int exponentials = exps_of(a);
   return EG_DISPATCH_FLOAT(dtype, name, [&]() -> int {
     using T = scalar_t;
     return by_width<T>(cols, {logits, (const void*)dlogits}, [&](auto vec, auto rag) -> int {
       constexpr int V = decltype(vec)::value;
       constexpr bool R = decltype(rag)::value;
-      const int64_t blocks = (rows * ((cols + V - 1) / V) + kFlatPer - 1) / kFlatPer;
+      const int64_t ppr = (cols + V - 1) / V, blocks = (rows * ppr + kFlatPer - 1) / kFlatPer;
       if (check_grid(name, blocks, kFlatBlock)) return 1;
-      const dim3 grid((unsigned)blocks), block(kFlatBlock);
-      if (two)
-        EG_LAUNCH((distill_bwd_kernel<T, V, R, true>), grid, block, 0, as_stream(stream), a);
-      else
-        EG_LAUNCH((distill_bwd_kernel<T, V, R, false>), grid, block, 0, as_stream(stream), a);
-      return check_launch(name);
+      return by_exps(exponentials, [&](auto e) -> int {
+        const dim3 grid((unsigned)blocks), block(kFlatBlock);
+        if (ppr >= kFlatPer)
+          EG_LAUNCH((distill_bwd_kernel<T, V, R, decltype(e)::value, false>), grid, block, 0,
+                    as_stream(stream), a);
+        else
+          EG_LAUNCH((distill_bwd_kernel<T, V, R, decltype(e)::value, true>), grid, block, 0,
+                    as_stream(stream), a);
+        return check_launch(name);
+      });
     });
   });
 }

@@ -212,7 +212,7 @@ def test_workspaces():
     assert q("eg_norm_rotary_workspace_bytes", 0, 8, 2, 64) == 0
     assert q("eg_norm_rotary_workspace_bytes", 5, 8, 2, 64) == 2048 * 2 * 64 * 4
     assert q("eg_topk_distill_workspace_bytes", 0, 100) == 0
-    assert q("eg_topk_distill_workspace_bytes", 8192, 128256) == 8192 * 4
+    assert q("eg_topk_distill_workspace_bytes", 8192, 128256) == 8192 * 4 * 4
     assert q("eg_topk_distill_workspace_bytes", 4, 128256) == 4 * (1 + 3 * 15) * 4
 
 

@@ -12,11 +12,20 @@
 //                       workgroup reads all tokens twice: first it counts its own ids per wave
 //                       (a wave holds a range of positions) and those of the buckets before it,
 //                       which is where its part of the order begins, then it places its tokens.
-//   embed_sum_kernel    cuts the order into pieces of kPiece tokens and adds the rows of each; a
-//                       run of one id that lies within a piece is a finished row, the others
-//                       leave an fp32 partial row per piece. The same launch writes the rows of
-//                       ids without a token.
-//   embed_join_kernel   adds the partial rows of the runs that cross pieces, in order.
+//                       Workgroups behind those zero the beginning of the table: most of it is
+//                       rows without a token, and nothing else moves meanwhile.
+//   embed_sum_kernel    cuts the order into pieces and adds the rows of each; a run of one id that
+//                       lies within a piece is a finished row, the others leave an fp32 partial
+//                       row per piece.
+//   embed_join_kernel   adds the partial rows of the runs that cross pieces, in order; the same
+//                       launch writes the rows of ids without a token behind the beginning.
+//
+// Memory-bound: the backward reads T rows and writes the table. bf16, 16384 tokens of [128256,
+// 4096] whose frequencies fall as one over their rank: forward 32 us, backward 197 (6.0 TB/s);
+// fp16 8191 tokens of [50257, 1538], a third of them the same: 9 and 44; 32 tokens forward 3 us, a
+// launch. Steps of the first backward (259 us): ids loaded eight at a time and matched one by one
+// where they are few, the zeros beside the join and not the sums, two packs of zeros a thread (4: 234,
+// 8: 250, one: 242 where two took 213), zeros under the ordering.
 #include "eg_common.hpp"
 
 #include <algorithm>
@@ -28,10 +37,14 @@ namespace {
 constexpr int kGatherThreads = 256;
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / kWave;
 constexpr int kBucketIds = 1024;  // at most, an id per thread in the scan
-constexpr int kPiece = 32;
+constexpr int kMostPiece = 32;
 constexpr int kSumThreads = 256, kFewestLanes = 16, kMostGroups = kSumThreads / kFewestLanes;
-constexpr int kZeroPacks = 8;  // per thread
-constexpr int kJoinLanes = 64, kJoinAdders = 8;
+constexpr int kSingly = 4;
+constexpr int kEarlyPacks = 2;  // of 16 bytes, per thread
+constexpr int kAhead = 8;  // loads of a thread on their way at once
+constexpr int kJoinLanes = 64, kJoinAdders = 8, kJoinThreads = kJoinLanes * kJoinAdders;
+constexpr int kJoinParts = 4;  // workgroups that share a piece's columns, at most
+constexpr int kZeroPacks = 2;  // per thread
 
 struct EmbedArgs {
   const void *weight, *dout;
@@ -44,8 +57,10 @@ struct EmbedArgs {
   int *order, *key;
   unsigned* first;
   float* part;  // [pieces][2][hidden]: of the run a piece begins in, of the one it ends in
-  int shift;    // 2^shift buckets
-  int per;      // ids of a bucket
+  int64_t early;  // bytes from the table's beginning that are zeroed while the order is found
+  int piece;      // tokens of a piece
+  int shift;      // 2^shift buckets
+  int per;        // ids of a bucket
 };
 
 // The token's id, or -1 for one that has no row of the table.
@@ -117,27 +132,57 @@ __device__ __forceinline__ uint64_t same_value(unsigned v, uint64_t in, int bits
   return in;
 }
 
+template <typename ID>
 __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(EmbedArgs a) {
   extern __shared__ unsigned counts[];  // [waves][per]
   __shared__ unsigned sums[kSortWaves], base;
+  __shared__ unsigned staged[kSortWaves][kAhead * kWave];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const unsigned bucket = blockIdx.x, mask = (1u << a.shift) - 1;
+  if (bucket > mask) {  // the table's beginning
+    typedef unsigned int words __attribute__((ext_vector_type(4)));
+    words* p = (words*)a.dweight + (int64_t)(bucket - mask - 1) * (kSortThreads * kEarlyPacks);
+#pragma unroll
+    for (int u = 0; u < kEarlyPacks; ++u)
+      __builtin_nontemporal_store((words){0, 0, 0, 0}, p + u * kSortThreads + threadIdx.x);
+    return;
+  }
   unsigned* mine = counts + wave * a.per;
   for (int i = threadIdx.x; i < kSortWaves * a.per; i += kSortThreads) counts[i] = 0;
   __syncthreads();
   // this wave's positions
-  const int64_t share = (a.tokens + kSortThreads - 1) / kSortThreads * kWave;
-  const int64_t from = min((int64_t)wave * share, a.tokens), to = min(from + share, a.tokens);
-  unsigned before = 0;
-  for (int64_t t = from + lane; t < to; t += kWave) {
-    const int64_t id = token_id(a, t);
-    if (id < 0) continue;
-    const unsigned b = (unsigned)id & mask;
-    before += b < bucket;
-    if (b == bucket) atomicAdd(&mine[id >> a.shift], 1u);
-  }
+  const int tokens = (int)a.tokens, share = (tokens + kSortThreads - 1) / kSortThreads * kWave;
+  const int from = (int)min((int64_t)wave * share, a.tokens), to = min(from + share, tokens);
+  // The ids of kAhead runs of 64 positions, all on their way at once, as (bucket, place in it) in
+  // one word; all bits set for a token of no row.
+  unsigned code[kAhead];
+  const unsigned first = bucket * kBucketIds;
+  auto fetch = [&](int t0) {
+    ID id[kAhead];
+    const ID* at = (const ID*)a.ids + t0 + lane;
+    if (t0 + kAhead * kWave <= to) {
 #pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) before += __shfl_xor(before, off);
+      for (int u = 0; u < kAhead; ++u) id[u] = at[u * kWave];
+    } else {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) id[u] = t0 + u * kWave + lane < to ? at[u * kWave] : (ID)-1;
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const bool row = id[u] >= 0 && (int64_t)id[u] < a.vocab && id[u] != a.ignore_index;
+      const unsigned v = (unsigned)id[u];
+      code[u] = row ? (v & mask) * kBucketIds | v >> a.shift : ~0u;
+    }
+  };
+  unsigned before = 0;  // the wave's tokens of earlier buckets
+  for (int t0 = from; t0 < to; t0 += kAhead * kWave) {
+    fetch(t0);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      before += __popcll(__ballot(code[u] < first));
+      if (code[u] - first < kBucketIds) atomicAdd(&mine[code[u] - first], 1u);
+    }
+  }
   if (lane == 0) sums[wave] = before;
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -172,27 +217,46 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(EmbedArgs a) {
     }
   }
   __syncthreads();
-  const int bits = 32 - __clz(a.per);  // of a bucket's id
-  for (int64_t t0 = from; t0 < to; t0 += kWave) {
-    const int64_t t = t0 + lane;
-    const int64_t id = t < to ? token_id(a, t) : -1;
-    const bool in = id >= 0 && ((unsigned)id & mask) == bucket;
-    const uint64_t any = __ballot(in);
-    if (!any) continue;
-    const unsigned local = in ? (unsigned)(id >> a.shift) : 0;
-    const uint64_t same = same_value(local, any, bits);
-    const uint64_t below = same & ((1ull << lane) - 1);
-    const unsigned place = mine[local] + __popcll(below);
-    if (in) {
-      a.order[place] = (int)t;
-      a.key[place] = (int)id;
+  const int bits = 32 - __clz(a.per);  // of a place in the bucket
+  for (int t0 = from; t0 < to; t0 += kAhead * kWave) {
+    if (share > kAhead * kWave) fetch(t0);  // else they are still there
+    unsigned runs = 0;                      // that hold ids of the bucket
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (__ballot(code[u] - first < kBucketIds)) {
+        staged[wave][u * kWave + lane] = code[u];
+        runs |= 1u << u;
+      }
+    while (runs) {
+      const int u = __ffs(runs) - 1;
+      runs &= runs - 1;
+      const unsigned local = staged[wave][u * kWave + lane] - first;  // the lane's own
+      const bool in = local < kBucketIds;
+      uint64_t left = __ballot(in);
+      // `same`: the lanes of this lane's id, which stand behind the id's earlier ones in their order;
+      // the last of them moves the id's place on, after all have read it and before any reads again
+      auto put = [&](bool now, uint64_t same) {
+        const uint64_t below = same & ((1ull << lane) - 1);
+        const unsigned place = mine[now ? local : 0] + __popcll(below);
+        if (now) {
+          a.order[place] = t0 + u * kWave + lane;
+          a.key[place] = (int)(local << a.shift | bucket);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (now && below == (same & ~(1ull << lane))) mine[local] = place + 1;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+      };
+      // a few ids one by one, more of them by their bits
+      for (int n = 0; n < kSingly && left; ++n) {
+        const unsigned v = __builtin_amdgcn_readlane(local, __ffsll((unsigned long long)left) - 1);
+        const uint64_t same = __ballot(local == v);
+        put(local == v, same);
+        left &= ~same;
+      }
+      if (left) put(left >> lane & 1, same_value(local, left, bits));
     }
-    // the last of them moves the id's place on, after all have read it and before any reads again
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    if (in && below == (same & ~(1ull << lane))) mine[local] = place + 1;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
   }
 }
 
@@ -214,62 +278,59 @@ __device__ void write_row(const EmbedArgs& a, const RowAt<T, VEC, RAG>& at, int 
 // Rows of ids without a token, over the table as one run of packs.
 template <typename T, int VEC>
 __device__ void zero_rows(const EmbedArgs& a, int64_t block) {
-  const int64_t first = block * (kSumThreads * kZeroPacks * VEC);
-  const int64_t row0 = first / a.hidden, total = a.vocab * a.hidden;
-  const int rest = (int)(first - row0 * a.hidden);
-  auto empty = [&](int64_t row) {
-    const int64_t s = slot_of(a, (unsigned)row);
-    return a.first[s] == a.first[s + 1];
-  };
-  T* p = (T*)a.dweight + first;
-  bool clear[kZeroPacks];
-#pragma unroll
-  for (int u = 0; u < kZeroPacks; ++u) {
-    const unsigned e = (u * kSumThreads + threadIdx.x) * VEC, in = rest + e;
-    clear[u] = first + e < total && empty(row0 + in / (unsigned)a.hidden);
+  constexpr int kChunk = kJoinThreads * kZeroPacks * VEC;
+  __shared__ uint64_t bits[kChunk / kWave + 1];  // of the rows that the chunk touches
+  const int64_t first = a.early / (int64_t)sizeof(T) + block * kChunk, total = a.vocab * a.hidden;
+  const int64_t row0 = first / a.hidden;
+  const unsigned rest = (unsigned)(first - row0 * a.hidden), hidden = a.hidden;
+  const int rows = (int)min((int64_t)((rest + kChunk - 1) / hidden + 1), a.vocab - row0);
+  for (int r = threadIdx.x; r < (rows + kWave - 1) / kWave * kWave; r += kJoinThreads) {
+    const int64_t s = slot_of(a, (unsigned)(row0 + min(r, rows - 1)));
+    const uint64_t b = __ballot(a.first[s] == a.first[s + 1]);
+    if ((threadIdx.x & 63) == 0) bits[r / kWave] = b;
   }
+  __syncthreads();
+  auto empty = [&](unsigned r) { return (bool)(bits[r / kWave] >> (r % kWave) & 1); };
+  T* p = (T*)a.dweight + first;
 #pragma unroll
   for (int u = 0; u < kZeroPacks; ++u) {
-    const unsigned e = (u * kSumThreads + threadIdx.x) * VEC, in = rest + e;
-    if (first + e >= total) continue;
-    const int64_t r = in / (unsigned)a.hidden, last = (in + VEC - 1) / (unsigned)a.hidden;
-    if (r == last && first + e + VEC <= total) {
-      float z[VEC] = {};
-      if (clear[u]) store_vec<T, VEC, true>(p + e, z);
-    } else {  // a pack of several rows, or the table's end
+    const unsigned e = (u * kJoinThreads + threadIdx.x) * VEC, in = rest + e;
+    if (first + e >= total) break;
+    // the pack's first row and the last one; between them lie others only in rows below a pack
+    const unsigned r = in / hidden, end = min((unsigned)rows - 1, (in + VEC - 1) / hidden);
+    const bool whole = first + e + VEC <= total && (hidden >= VEC || r == end);
+    if (whole && empty(r) && empty(end)) {
+      const float z[VEC] = {};
+      store_vec<T, VEC, true>(p + e, z);
+    } else if (!whole || empty(r) || empty(end)) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i)
-        if (first + e + i < total && empty(row0 + (in + i) / (unsigned)a.hidden))
-          p[e + i] = from_f32<T>(0.f);
+        if (first + e + i < total && empty((in + i) / hidden)) p[e + i] = from_f32<T>(0.f);
     }
   }
 }
 
 // kSumThreads / lanes pieces a workgroup, `lanes` threads (a power of two) over the columns of one.
-template <typename T, int VEC, bool RAG, int ZVEC>
-__global__ __launch_bounds__(kSumThreads) void embed_sum_kernel(EmbedArgs a, int lanes, int column_blocks,
-                                                                int64_t sum_blocks) {
-  if ((int64_t)blockIdx.x >= sum_blocks) {
-    zero_rows<T, ZVEC>(a, (int64_t)blockIdx.x - sum_blocks);
-    return;
-  }
+template <typename T, int VEC, bool RAG>
+__global__ __launch_bounds__(kSumThreads) void embed_sum_kernel(EmbedArgs a, int lanes,
+                                                                int column_blocks) {
   // a piece's tokens and ids, and the ids before and behind it
-  __shared__ int where[kMostGroups][kPiece], ids[kMostGroups][kPiece + 2];
+  __shared__ int where[kMostGroups][kMostPiece], ids[kMostGroups][kMostPiece + 2];
   const int64_t n = a.first[(int64_t)a.per << a.shift];
   const int groups = kSumThreads / lanes, group = threadIdx.x / lanes;
   const int64_t piece0 = (int64_t)(blockIdx.x / column_blocks) * groups;
-  for (int i = threadIdx.x; i < groups * (kPiece + 2); i += kSumThreads) {
-    const int g = i / (kPiece + 2), j = i - g * (kPiece + 2);
-    const int64_t at = (piece0 + g) * kPiece + j - 1;
+  for (int i = threadIdx.x; i < groups * (a.piece + 2); i += kSumThreads) {
+    const int g = i / (a.piece + 2), j = i - g * (a.piece + 2);
+    const int64_t at = (piece0 + g) * a.piece + j - 1;
     const bool in = at >= 0 && at < n;
     ids[g][j] = in ? a.key[at] : -1;
-    if (in && j >= 1 && j <= kPiece) where[g][j - 1] = a.order[at];
+    if (in && j >= 1 && j <= a.piece) where[g][j - 1] = a.order[at];
   }
   __syncthreads();
   const int64_t piece = piece0 + group;
   const int pack = blockIdx.x % column_blocks * lanes + (threadIdx.x & (lanes - 1));
-  if (piece * kPiece >= n || pack * VEC >= a.hidden) return;
-  const int len = (int)min((int64_t)kPiece, n - piece * kPiece);
+  if (piece * a.piece >= n || pack * VEC >= a.hidden) return;
+  const int len = (int)min((int64_t)a.piece, n - piece * a.piece);
   const RowAt<T, VEC, RAG> at(pack, a.hidden);
   float acc[VEC] = {};
   bool crosses = ids[group][0] == ids[group][1];  // the run began before the piece
@@ -287,7 +348,6 @@ __global__ __launch_bounds__(kSumThreads) void embed_sum_kernel(EmbedArgs a, int
 #pragma unroll
     for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
   };
-  constexpr int kAhead = 8;
   for (int j0 = 0; j0 < len; j0 += kAhead) {
     Pack<T, VEC> x[kAhead];
 #pragma unroll
@@ -306,37 +366,63 @@ __global__ __launch_bounds__(kSumThreads) void embed_sum_kernel(EmbedArgs a, int
 
 // The run that begins in a piece and goes on behind it: the piece's second partial row and the
 // first ones of the pieces behind, dealt to kJoinAdders adders whose sums are added in order.
-template <typename T>
-__global__ __launch_bounds__(kJoinLanes* kJoinAdders) void embed_join_kernel(EmbedArgs a) {
-  __shared__ float sums[kJoinAdders][kJoinLanes];
+// `parts` workgroups share the columns of a piece. Those past `joins` write the rows without tokens.
+template <typename T, int VEC, int ZVEC>
+__global__ __launch_bounds__(kJoinThreads) void embed_join_kernel(EmbedArgs a, int64_t joins, int parts) {
+  if ((int64_t)blockIdx.x >= joins) {
+    zero_rows<T, ZVEC>(a, (int64_t)blockIdx.x - joins);
+    return;
+  }
+  __shared__ Pack<float, VEC> sums[kJoinAdders][kJoinLanes];
   const int64_t n = a.first[(int64_t)a.per << a.shift];
-  const int64_t piece = blockIdx.x, end = (piece + 1) * kPiece;
+  const int64_t piece = blockIdx.x / parts, end = (piece + 1) * a.piece;
   if (end >= n) return;
   const int id = a.key[end];
   if (id != a.key[end - 1]) return;  // no run crosses the piece's end
   const int64_t slot = slot_of(a, (unsigned)id);
-  if (a.first[slot] < piece * kPiece) return;  // it began in an earlier piece
-  const int64_t last = (a.first[slot + 1] - 1) / kPiece;
+  if (a.first[slot] < piece * a.piece) return;  // it began in an earlier piece
+  const int64_t last = (a.first[slot + 1] - 1) / a.piece;
   const int lane = threadIdx.x % kJoinLanes, adder = threadIdx.x / kJoinLanes;
-  const int c = blockIdx.y * kJoinLanes + lane;
-  float s = 0.f;
-  if (c < a.hidden) {
-    if (adder == 0) s = a.part[(piece * 2 + 1) * a.hidden + c];
+  const int step = parts * kJoinLanes * VEC;
+  for (int c0 = (int)(blockIdx.x % parts) * kJoinLanes * VEC; c0 < a.hidden; c0 += step) {
+    const int c = c0 + lane * VEC;
+    float s[VEC] = {}, v[VEC];
+    if (c < a.hidden) {
+      if (adder == 0) load_f32<float, VEC>(a.part + (piece * 2 + 1) * a.hidden + c, s);
 #pragma unroll 8
-    for (int64_t p = piece + 1 + adder; p <= last; p += kJoinAdders) s += a.part[p * 2 * a.hidden + c];
+      for (int64_t p = piece + 1 + adder; p <= last; p += kJoinAdders) {
+        load_f32<float, VEC>(a.part + p * 2 * a.hidden + c, v);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) s[i] += v[i];
+      }
+    }
+    __syncthreads();  // the last columns' sums have been read
+    store_f32<float, VEC>(sums[adder][lane].v, s);
+    __syncthreads();
+    if (adder || c >= a.hidden) continue;
+    for (int k = 1; k < kJoinAdders; ++k)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) s[i] += sums[k][lane].v[i];
+    RowAt<T, VEC, false> at(c / VEC, a.hidden);
+    write_row(a, at, id, s);
   }
-  sums[adder][lane] = s;
-  __syncthreads();
-  if (adder || c >= a.hidden) return;
-  for (int i = 1; i < kJoinAdders; ++i) s += sums[i][lane];
-  const float sum[1] = {s};
-  RowAt<T, 1, false> at(c, a.hidden);
-  write_row(a, at, id, sum);
 }
+
+// Tokens of a piece: a piece's rows are added one after the other, its partial rows are read again.
+// Backward, us, with 8 / 16 / 32: 700 tokens of [5003, 768] fp32 15.2 / 16.8 / 19.9; 4096 of [32000,
+// 1024] bf16 28.0 / 29.0 / 33.5; 8191 of [50257, 1538] fp16 59.7 / 55.9 / 57.7; 16384 of [128256,
+// 4096] bf16 255 / 244 / 241; 65536 of [50257, 768] 137 / 122 / 111.
+int piece_for(int64_t tokens) { return tokens < 4096 ? 8 : tokens < 16384 ? 16 : 32; }
+
+// Bytes of the table that the ordering's launch zeroes under way, as many as its time has room
+// for. Backward, us, none / 32 MB / this: 16384 tokens of [128256, 4096] bf16 211 / 206 / 197, 2048
+// of [128256, 2048] 97 / 91 / 90, 65536 of [50257, 768] 83 / 79 / 75, 700 of [5003, 768] fp32 15 /
+// 14 / 14.
+int64_t early_bytes(int64_t tokens) { return ((int64_t)32 << 20) + tokens * 3500; }
 
 // A table [vocab, hidden] with `tokens` of it: how the ids are dealt and where the order lies.
 struct Layout {
-  int shift, per;
+  int shift, per, piece;
   int64_t pieces;
   size_t order, key, first, part, bytes;  // offsets into the workspace
 };
@@ -346,7 +432,8 @@ Layout layout(int64_t tokens, int64_t vocab, int64_t hidden) {
   l.shift = 8;
   while (vocab > ((int64_t)kBucketIds << l.shift)) ++l.shift;
   l.per = (int)((vocab + ((int64_t)1 << l.shift) - 1) >> l.shift);
-  l.pieces = (tokens + kPiece - 1) / kPiece;
+  l.piece = piece_for(tokens);
+  l.pieces = (tokens + l.piece - 1) / l.piece;
   l.key = up(tokens * sizeof(int));
   l.first = l.key + up(tokens * sizeof(int));
   l.part = l.first + up((((size_t)l.per << l.shift) + 1) * sizeof(unsigned));
@@ -436,7 +523,7 @@ extern "C" int eg_embedding_bwd(const void* dout, const void* ids, int ids_64, v
   char* ws = (char*)workspace;
   a.order = (int*)ws, a.key = (int*)(ws + l.key), a.first = (unsigned*)(ws + l.first);
   a.part = (float*)(ws + l.part);
-  a.shift = l.shift, a.per = l.per;
+  a.shift = l.shift, a.per = l.per, a.piece = l.piece;
   hipStream_t st = as_stream(stream);
   return EG_DISPATCH_FLOAT(dtype, name, [&]() -> int {
     return by_width<scalar_t>(a.hidden, {dout, (const void*)dweight}, [&](auto vec, auto rag) -> int {
@@ -446,30 +533,39 @@ extern "C" int eg_embedding_bwd(const void* dout, const void* ids, int ids_64, v
       const int lanes = lanes_for(packs, kSumThreads), groups = kSumThreads / lanes;
       const int64_t columns = (packs + lanes - 1) / lanes;
       const int64_t sums = (l.pieces + groups - 1) / groups * columns;
-      const bool flat = aligned16(dweight);
-      const int64_t zpacks = (vocab * hidden + (flat ? W : 1) - 1) / (flat ? W : 1);
-      const int64_t zeros = accumulate ? 0 : (zpacks + kSumThreads * kZeroPacks - 1) /
-                                                 (kSumThreads * kZeroPacks);
-      if (check_grid(name, (int64_t)1 << l.shift, kSortThreads) ||
-          check_grid(name, sums + zeros, kSumThreads) ||
-          check_grid(name, l.pieces, kJoinLanes * kJoinAdders))
+      // the join in fours of columns where a row's fours are aligned, zeros in whole packs
+      const bool flat = aligned16(dweight), fours = flat && hidden % 4 == 0;
+      const int64_t span = kJoinLanes * (fours ? 4 : 1);
+      const int parts = (int)std::min<int64_t>((hidden + span - 1) / span, kJoinParts);
+      const int64_t joins = l.pieces > 1 ? (l.pieces - 1) * parts : 0;
+      const int64_t chunk = (int64_t)kJoinThreads * kZeroPacks * (flat ? W : 1);
+      const int64_t bytes = vocab * hidden * (int64_t)sizeof(T), at_once = kSortThreads * kEarlyPacks * 16;
+      const int64_t early = accumulate || !flat ? 0 : std::min(early_bytes(tokens), bytes) / at_once;
+      a.early = early * at_once;
+      const int64_t zeros =
+          accumulate ? 0 : ((bytes - a.early) / (int64_t)sizeof(T) + chunk - 1) / chunk;
+      const int64_t sorts = ((int64_t)1 << l.shift) + early;
+      if (check_grid(name, sorts, kSortThreads) ||
+          check_grid(name, sums, kSumThreads) || check_grid(name, joins + zeros, kJoinThreads))
         return 1;
-      const int64_t joins = (hidden + kJoinLanes - 1) / kJoinLanes;
-      EG_LAUNCH((embed_sort_kernel), dim3(1u << l.shift), dim3(kSortThreads),
-                (size_t)kSortWaves * l.per * sizeof(unsigned), st, a);
-      if (sums + zeros) {
-        if (flat)
-          EG_LAUNCH((embed_sum_kernel<T, V, decltype(rag)::value, W>),
-                    dim3((unsigned)(sums + zeros)), dim3(kSumThreads), 0, st, a, lanes,
-                    (int)columns, sums);
-        else
-          EG_LAUNCH((embed_sum_kernel<T, V, decltype(rag)::value, 1>),
-                    dim3((unsigned)(sums + zeros)), dim3(kSumThreads), 0, st, a, lanes,
-                    (int)columns, sums);
+      const size_t lds = (size_t)kSortWaves * l.per * sizeof(unsigned);
+      if (ids_64)
+        EG_LAUNCH((embed_sort_kernel<int64_t>), dim3((unsigned)sorts), dim3(kSortThreads), lds, st, a);
+      else
+        EG_LAUNCH((embed_sort_kernel<int>), dim3((unsigned)sorts), dim3(kSortThreads), lds, st, a);
+      if (sums)
+        EG_LAUNCH((embed_sum_kernel<T, V, decltype(rag)::value>), dim3((unsigned)sums),
+                  dim3(kSumThreads), 0, st, a, lanes, (int)columns);
+      auto join = [&](auto c, auto z) {
+        EG_LAUNCH((embed_join_kernel<T, decltype(c)::value, decltype(z)::value>),
+                  dim3((unsigned)(joins + zeros)), dim3(kJoinThreads), 0, st, a, joins, parts);
+      };
+      if (joins + zeros) {
+        using std::integral_constant;
+        if (fours) join(integral_constant<int, 4>{}, integral_constant<int, W>{});
+        else if (flat) join(integral_constant<int, 1>{}, integral_constant<int, W>{});
+        else join(integral_constant<int, 1>{}, integral_constant<int, 1>{});
       }
-      if (l.pieces > 1)
-        EG_LAUNCH((embed_join_kernel<T>), dim3((unsigned)(l.pieces - 1), (unsigned)joins),
-                  dim3(kJoinLanes * kJoinAdders), 0, st, a);
       return check_launch(name);
     });
   });

@@ -28,13 +28,17 @@ if not __package__:
     if _ROOT not in _sys.path:
         _sys.path.insert(0, _ROOT)
 
+import struct
+
 import torch
 from torch.autograd.function import once_differentiable
 
 from evograd_amd import _lib
-from evograd_amd.pairs._util import (as_contiguous, check_same, contiguous_like, head_rows,
-                                     strides_arg, tag, workspace)
+from evograd_amd.pairs._util import (MAX_HEAD_STRIDE, MAX_TOKEN_STRIDE, as_contiguous, check_same,
+                                     head_rows, tag, workspace)
 from evograd_amd.pairs.rotary import _check as _check_positions
+
+_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 
 
 def _check(name, x, weight, positions, freqs):
@@ -45,61 +49,91 @@ def _check(name, x, weight, positions, freqs):
     check_same(name, x, weight)
 
 
-def _check_qk(name, q, k, q_weight, k_weight, positions, freqs):
-    """k and k_weight may be None."""
-    given = (q, q_weight) if k is None else (q, k, q_weight, k_weight)
-    _lib.require_gpu(name, *given, positions, freqs)
-    _check(name, q, q_weight, positions, freqs)
-    if k is not None:
-        _check(name, k, k_weight, positions, freqs)
-        if k.shape[2] != q.shape[2] or k.dtype != q.dtype:
-            raise ValueError(f"{name}: q and k must share head_dim and dtype")
+def _fits(x, weight, positions, freqs):
+    """Whether _check has nothing to say, in a few lookups (small calls are bound by the host)."""
+    shape, dtype = x.shape, x.dtype
+    return (len(shape) == 3 and dtype in _FLOATS and weight.dtype is dtype
+            and weight.shape == shape[2:] and positions.shape == shape[:1]
+            and positions.dtype in (torch.int32, torch.int64) and freqs.dtype is torch.float64
+            and freqs.dim() == 1 and 2 * freqs.shape[0] <= shape[2])
+
+
+_PACKERS = {n: struct.Struct(f"{n}q").pack for n in (2, 4, 8)}
+
+
+def _steps(*tensors):
+    """[tokens, heads, head_dim] tensors as the kernels take them (head_rows), and their token and
+    head steps as a C array of int64."""
+    out, steps = [], []
+    for t in tensors:
+        tokens, heads, dim = t.shape
+        token, head, column = t.stride()
+        # an axis of one element has the step of a contiguous tensor, whatever torch notes for it
+        if tokens <= 1:
+            token = heads * dim
+        if heads <= 1:
+            head = dim
+        if not (column == 1 and dim <= token <= MAX_TOKEN_STRIDE and head <= MAX_HEAD_STRIDE):
+            t = head_rows(t)
+            if t.is_contiguous():
+                token, head = heads * dim, dim
+        out.append(t)
+        steps.append(token)
+        steps.append(head)
+    return out, _PACKERS[len(steps)](*steps)
 
 
 def _forward(name, q, k, q_weight, k_weight, positions, freqs, eps, amplitude, interleaved):
     """y of q, and of k unless it is None, and the tensors as the kernels take them."""
-    _check_qk(name, q, k, q_weight, k_weight, positions, freqs)
-    q, q_weight = head_rows(q), as_contiguous("q_weight", q_weight)
-    qo, ko = contiguous_like(q), None
-    if k is not None:
-        k, k_weight = head_rows(k), as_contiguous("k_weight", k_weight)
-        ko = contiguous_like(k)
-    positions, freqs = as_contiguous("positions", positions), as_contiguous("freqs", freqs)
+    if k is None:
+        _lib.require_gpu(name, q, q_weight, positions, freqs)
+    else:
+        _lib.require_gpu(name, q, k, q_weight, k_weight, positions, freqs)
+        if not _fits(k, k_weight, positions, freqs):
+            _check(name, k, k_weight, positions, freqs)
+    if not _fits(q, q_weight, positions, freqs):
+        _check(name, q, q_weight, positions, freqs)
     T, H, D = q.shape
+    positions, freqs = as_contiguous("positions", positions), as_contiguous("freqs", freqs)
+    q_weight, qo = as_contiguous("q_weight", q_weight), q.new_empty((T, H, D))
+    if k is None:
+        (q,), steps = _steps(q)
+        steps, ko, heads_k = steps + steps, None, 0
+    else:
+        heads_k = k.shape[1]
+        if k.shape[2] != D or k.dtype is not q.dtype:
+            raise ValueError(f"{name}: q and k must share head_dim and dtype")
+        (q, k), steps = _steps(q, k)
+        k_weight, ko = as_contiguous("k_weight", k_weight), k.new_empty((T, heads_k, D))
     _lib.call_on(q, "eg_norm_rotary_fwd", q.data_ptr(), _lib.ptr(k), q_weight.data_ptr(),
                  _lib.ptr(k_weight), qo.data_ptr(), _lib.ptr(ko), positions.data_ptr(),
-                 positions.dtype == torch.int64, freqs.data_ptr(), T, H,
-                 0 if k is None else k.shape[1], D, freqs.shape[0],
-                 strides_arg(q, q if k is None else k), eps, amplitude, bool(interleaved),
-                 tag(q.dtype), _lib.stream_of(q))
+                 positions.dtype is torch.int64, freqs.data_ptr(), T, H, heads_k, D, freqs.shape[0],
+                 steps, eps, amplitude, interleaved != 0, tag(q.dtype), _lib.stream_of(q))
     return qo, ko, (q, k, q_weight, k_weight, positions, freqs)
 
 
-def _backward(name, dq_out, dk_out, q, k, q_weight, k_weight, positions, freqs, eps, amplitude,
-              interleaved):
-    _lib.require_gpu(name, *(t for t in (dq_out, dk_out) if t is not None))
-    _check_qk(name, q, k, q_weight, k_weight, positions, freqs)
+def _backward(name, dq_out, dk_out, saved, eps, amplitude, interleaved):
+    """Gradients of the saved tensors, which are as _forward leaves them."""
+    q, k, q_weight, k_weight, positions, freqs = saved
+    _lib.require_gpu(name, *(t for t in (dq_out, dk_out, *saved) if t is not None))
     for d, x in ((dq_out, q), (dk_out, k)):
-        if x is not None and (d.shape != x.shape or d.dtype != x.dtype):
+        if x is not None and (d.shape != x.shape or d.dtype is not x.dtype):
             raise ValueError(f"{name}: the upstream gradients must match q and k in shape and dtype")
-    q, dq_out = head_rows(q), head_rows(dq_out)
-    q_weight = as_contiguous("q_weight", q_weight)
-    dq, dqw, dk, dkw = contiguous_like(q), torch.empty_like(q_weight), None, None
-    if k is not None:
-        k, dk_out = head_rows(k), head_rows(dk_out)
-        k_weight = as_contiguous("k_weight", k_weight)
-        dk, dkw = contiguous_like(k), torch.empty_like(k_weight)
-    positions, freqs = as_contiguous("positions", positions), as_contiguous("freqs", freqs)
     T, H, D = q.shape
-    heads_k = 0 if k is None else k.shape[1]
+    dq, dqw, dk, dkw, heads_k = q.new_empty((T, H, D)), torch.empty_like(q_weight), None, None, 0
+    if k is None:
+        (q, dq_out), steps = _steps(q, dq_out)
+        steps = steps[:16] * 2 + steps[16:] * 2
+    else:
+        heads_k = k.shape[1]
+        dk, dkw = k.new_empty((T, heads_k, D)), torch.empty_like(k_weight)
+        (q, k, dq_out, dk_out), steps = _steps(q, k, dq_out, dk_out)
     ws = workspace(_lib.query("eg_norm_rotary_workspace_bytes", T, H, heads_k, D), q.device)
-    steps = (q, q, dq_out, dq_out) if k is None else (q, k, dq_out, dk_out)
     _lib.call_on(q, "eg_norm_rotary_bwd", dq_out.data_ptr(), _lib.ptr(dk_out), q.data_ptr(),
                  _lib.ptr(k), q_weight.data_ptr(), _lib.ptr(k_weight), positions.data_ptr(),
-                 positions.dtype == torch.int64, freqs.data_ptr(), dq.data_ptr(), _lib.ptr(dk),
+                 positions.dtype is torch.int64, freqs.data_ptr(), dq.data_ptr(), _lib.ptr(dk),
                  dqw.data_ptr(), _lib.ptr(dkw), ws.data_ptr(), T, H, heads_k, D, freqs.shape[0],
-                 strides_arg(*steps), eps, amplitude, bool(interleaved), tag(q.dtype),
-                 _lib.stream_of(q))
+                 steps, eps, amplitude, interleaved != 0, tag(q.dtype), _lib.stream_of(q))
     return dq, dk, dqw, dkw
 
 
@@ -114,8 +148,9 @@ def norm_rotary_forward_with_saved(x: torch.Tensor, weight: torch.Tensor, positi
 def norm_rotary_backward_from_saved(dy: torch.Tensor, saved, eps: float = 1e-6,
                                     amplitude: float = 1.0, interleaved: int = 0):
     x, weight, positions, freqs = saved
-    dx, _, dweight, _ = _backward("norm_rotary_backward_from_saved", dy, None, x, None, weight,
-                                  None, positions, freqs, eps, amplitude, interleaved)
+    dx, _, dweight, _ = _backward("norm_rotary_backward_from_saved", dy, None,
+                                  (x, None, weight, None, positions, freqs), eps, amplitude,
+                                  interleaved)
     return dx, dweight
 
 
@@ -132,7 +167,7 @@ def norm_rotary_qk_backward_from_saved(grads, saved, eps: float = 1e-6, amplitud
                                        interleaved: int = 0):
     """``(dq, dk, dq_weight, dk_weight)`` from the pair of upstream gradients."""
     dq_out, dk_out = grads
-    return _backward("norm_rotary_qk_backward_from_saved", dq_out, dk_out, *saved, eps, amplitude,
+    return _backward("norm_rotary_qk_backward_from_saved", dq_out, dk_out, saved, eps, amplitude,
                      interleaved)
 
 

@@ -21,8 +21,8 @@ the logits have a gradient:
     dlogits = dloss / n * (hard_weight * (softmax(logits) - onehot(target))
                            + soft_weight * temperature * (q - sum of p at their tokens))
 
-Saved state: ``(logits, target, teacher_ids, stats, probs, n_valid)``: the inputs, fp32 [rows, 4]
-row statistics, fp32 [rows, entries] probabilities and the count of rows.
+Saved state: ``(logits, target, teacher_ids, state)``: the inputs and one fp32 tensor that holds
+[rows, 4] row statistics, [rows, entries] probabilities and the count of rows.
 """
 
 from __future__ import annotations
@@ -58,6 +58,12 @@ def _check(name, logits, target, teacher_ids):
         raise TypeError(f"{name}: teacher_ids must be int32 or int64, got {teacher_ids.dtype}")
 
 
+def _parts(state: torch.Tensor, rows: int, entries: int):
+    """Addresses of the state's statistics, probabilities and count."""
+    at = state.data_ptr()
+    return at, at + 16 * rows, at + 4 * rows * (4 + entries)
+
+
 def topk_distillation_forward_with_saved(logits: torch.Tensor, target: torch.Tensor,
                                          teacher_logits: torch.Tensor, teacher_ids: torch.Tensor,
                                          temperature: float = 1.0, soft_weight: float = 1.0,
@@ -75,35 +81,33 @@ def topk_distillation_forward_with_saved(logits: torch.Tensor, target: torch.Ten
     logits, target = as_contiguous("logits", logits), as_contiguous("target", target)
     teacher_logits = as_contiguous("teacher_logits", teacher_logits)
     teacher_ids = as_contiguous("teacher_ids", teacher_ids)
-    loss = logits.new_empty((), dtype=torch.float32)
-    n_valid = logits.new_empty(1, dtype=torch.float32)
-    stats = logits.new_empty((rows, 4), dtype=torch.float32)
-    probs = logits.new_empty((rows, entries), dtype=torch.float32)
+    loss = torch.empty((), dtype=torch.float32, device=logits.device)
+    state = torch.empty(rows * (4 + entries) + 1, dtype=torch.float32, device=logits.device)
     ws = workspace(_lib.query("eg_topk_distill_workspace_bytes", rows, cols), logits.device)
     _lib.call_on(logits, "eg_topk_distill_fwd", logits.data_ptr(), target.data_ptr(),
                  teacher_logits.data_ptr(), teacher_dtype, teacher_ids.data_ptr(),
-                 teacher_ids.dtype == torch.int64, loss.data_ptr(), stats.data_ptr(),
-                 probs.data_ptr(), n_valid.data_ptr(), ws.data_ptr(), rows, cols, entries,
-                 temperature, soft_weight, hard_weight, ignore_index, dtype,
-                 _lib.stream_of(logits))
-    return loss, (logits, target, teacher_ids, stats, probs, n_valid)
+                 teacher_ids.dtype is torch.int64, loss.data_ptr(), *_parts(state, rows, entries),
+                 ws.data_ptr(), rows, cols, entries, temperature, soft_weight, hard_weight,
+                 ignore_index, dtype, _lib.stream_of(logits))
+    return loss, (logits, target, teacher_ids, state)
 
 
 def topk_distillation_backward_from_saved(dloss: torch.Tensor, saved, temperature: float = 1.0,
                                           soft_weight: float = 1.0, hard_weight: float = 0.0,
                                           ignore_index: int = -100):
     name = "topk_distillation_backward_from_saved"
-    logits, target, teacher_ids, stats, probs, n_valid = saved
-    _lib.require_gpu(name, dloss, logits, target, teacher_ids, stats, probs, n_valid)
-    if dloss.numel() != 1 or dloss.dtype != torch.float32:
+    logits, target, teacher_ids, state = saved
+    _lib.require_gpu(name, dloss, logits, target, teacher_ids, state)
+    if dloss.numel() != 1 or dloss.dtype is not torch.float32:
         raise ValueError(f"{name}: dloss must be one float32 element, got {tuple(dloss.shape)} of "
                          f"{dloss.dtype}")
-    _check(name, logits, target, teacher_ids)
     rows, cols = logits.shape
+    entries = teacher_ids.shape[1]
+    if state.shape != (rows * (4 + entries) + 1,):
+        raise ValueError(f"{name}: the saved state is not of [{rows}, {entries}] entries")
     dlogits = torch.empty_like(logits)
     _lib.call_on(logits, "eg_topk_distill_bwd", dloss.data_ptr(), logits.data_ptr(),
-                 target.data_ptr(), teacher_ids.data_ptr(), teacher_ids.dtype == torch.int64,
-                 stats.data_ptr(), probs.data_ptr(), n_valid.data_ptr(), dlogits.data_ptr(), rows,
-                 cols, teacher_ids.shape[1], temperature, soft_weight, hard_weight, ignore_index,
-                 tag(logits.dtype), _lib.stream_of(logits))
+                 target.data_ptr(), teacher_ids.data_ptr(), teacher_ids.dtype is torch.int64,
+                 *_parts(state, rows, entries), dlogits.data_ptr(), rows, cols, entries, temperature,
+                 soft_weight, hard_weight, ignore_index, tag(logits.dtype), _lib.stream_of(logits))
     return dlogits

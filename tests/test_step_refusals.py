@@ -120,10 +120,13 @@ def test_distillation_arguments(no_device_check, z, target, t, ids, error, words
 
 
 def test_distillation_gradient_arguments(no_device_check):
-    saved = (Z, TARGET, TI, torch.zeros(4, 4), torch.zeros(4, 3), torch.ones(1))
+    back = topk_distillation.topk_distillation_backward_from_saved
+    saved = (Z, TARGET, TI, torch.zeros(4 * 7 + 1))
+    with pytest.raises(ValueError, match="saved state"):
+        back(torch.ones(()), (Z, TARGET, TI, torch.zeros(4 * 7)))
     for bad in (torch.ones(2), torch.ones((), dtype=torch.float64), torch.ones(()).half()):
         with pytest.raises(ValueError, match="one float32"):
-            topk_distillation.topk_distillation_backward_from_saved(bad, saved)
+            back(bad, saved)
 
 
 @built
@@ -206,8 +209,10 @@ def test_workspaces():
     al = lambda n: (n + 255) // 256 * 256  # noqa: E731
     q = _lib.query
     assert q("eg_embedding_workspace_bytes", 100, 0, 8) == 0
-    # one piece of 32 tokens: the order, its ids and 256 buckets of 4 ids' bounds
-    assert q("eg_embedding_workspace_bytes", 32, 1000, 8) == 2 * al(32 * 4) + al((256 * 4 + 1) * 4)
+    # one piece of 8 tokens: the order, its ids and 256 buckets of 4 ids' bounds
+    assert q("eg_embedding_workspace_bytes", 8, 1000, 8) == 2 * al(8 * 4) + al((256 * 4 + 1) * 4)
+    assert (q("eg_embedding_workspace_bytes", 9, 1000, 8)
+            == 2 * al(9 * 4) + al((256 * 4 + 1) * 4) + 2 * 2 * 8 * 4)
     assert (q("eg_embedding_workspace_bytes", 16384, 128256, 4096)
             == 2 * 16384 * 4 + al((256 * 501 + 1) * 4) + 512 * 2 * 4096 * 4)
     assert q("eg_norm_rotary_workspace_bytes", 0, 8, 2, 64) == 0

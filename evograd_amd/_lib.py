@@ -105,7 +105,7 @@ SIGNATURES: dict[str, tuple] = {
     "eg_norm_rotary_workspace_bytes": (_size, [_i64, _i64, _i64, _i64]),
     "eg_norm_rotary_bwd": (_i32, [_p, _p, _p, _p, _p, _p, _p, _i32, _p, _p, _p, _p, _p, _p, _i64,
                                   _i64, _i64, _i64, _i64, _p, _f32, _f32, _i32, _i32, _p]),
-    "eg_topk_distill_workspace_bytes": (_size, [_i64, _i64]),
+    "eg_topk_distill_workspace_bytes": (_size, [_i64, _i64, _i64]),
     "eg_topk_distill_fwd": (_i32, [_p, _p, _p, _i32, _p, _i32, _p, _p, _p, _p, _p, _i64, _i64, _i64,
                                    _f32, _f32, _f32, _i64, _i32, _p]),
     "eg_topk_distill_bwd": (_i32, [_p, _p, _p, _p, _i32, _p, _p, _p, _p, _i64, _i64, _i64, _f32,

@@ -33,14 +33,19 @@ namespace eg {
 namespace {
 
 using rowwise::kLog2e;
-using rowwise::kUnroll;
 using rowwise::lse_ref;
 
 constexpr int kMaxEntries = 1024;
 constexpr int kMeanBlock = 1024;
 constexpr int64_t kFewRows = 32;  // that one workgroup finishes, two a wave
-constexpr int kFlatBlock = rowwise::kFlatBlock, kFlatUnroll = rowwise::kFlatUnroll,
-              kFlatPer = rowwise::kFlatPer;
+// Threads of a row's workgroup at most and packs in flight per thread. Forward, us, at 1024 / 512
+// / 256 threads: bf16 [8192, 128256] with one exponential 308 / 309 / 308, a squared one 330 / 309 /
+// 314, two 366 / 338 / 336, 16 rows 11.4 / 11.8 / 11.6; with 512 threads at 8 / 4 / 2 packs: 316 / 313
+// / 305, 328 / 315 / 308, 362 / 344 / 338.
+constexpr int kMostRow = 512, kUnroll = 2;
+// The backward's workgroup (bf16 [8192, 128256], us: 512 threads 671, 256 655, 128 652 but 814 with 256
+// entries a row for 690, 256 of four packs 788).
+constexpr int kFlatBlock = 256, kFlatUnroll = 2, kFlatPer = kFlatBlock * kFlatUnroll;
 
 // The exponentials of a column: one of them (no hard label, no soft part or a temperature of 1),
 // both, or, at a temperature of 2, the hard label's as the soft one's square.
@@ -52,7 +57,7 @@ struct DistillArgs {
   const float* dloss;
   float *loss, *stats, *probs, *n_valid;
   void* dlogits;
-  float *rowloss, *part;  // part: [rows][splits][3] (max, sum, sum at tau)
+  float *rowloss, *part, *zs;  // part: [rows][splits][3] (max, sum, sum at tau); zs: [rows][k]
   int64_t rows, ignore_index;
   int cols, k, slots, splits, ids_64, teacher_type;
   float tau, soft, hard;
@@ -92,6 +97,9 @@ __global__ __launch_bounds__(BLOCK) void distill_row_kernel(DistillArgs a) {
   const int64_t each = (packs + a.splits - 1) / a.splits * VEC;
   const int c0 = (int)min((int64_t)blockIdx.y * each, (int64_t)a.cols);
   const int c1 = (int)min(c0 + each, (int64_t)a.cols);
+  // the entries' logits: read while the row is still near, for the finish
+  int64_t id = -1;
+  if (blockIdx.y == 0 && (int)threadIdx.x < a.k) id = entry_id(a, row * a.k + threadIdx.x);
   float m = -INFINITY, s1 = 0.f, st = 0.f;
   for (int64_t base = c0 + (int64_t)threadIdx.x * VEC; base < c1; base += STEP * kUnroll) {
     float v[kUnroll][VEC];
@@ -99,7 +107,8 @@ __global__ __launch_bounds__(BLOCK) void distill_row_kernel(DistillArgs a) {
     for (int u = 0; u < kUnroll; ++u) {
       const int64_t c = base + u * STEP;
       if (c < c1) {
-        rowwise::load_pack<T, VEC, VEC * sizeof(T) == 16, RAG>(xr, (int)c, a.cols, -INFINITY, v[u]);
+        // unaligned packs share cache lines: without the non-temporal hint
+        rowwise::load_pack<T, VEC, VEC * sizeof(T) == 16 && !RAG, RAG>(xr, (int)c, a.cols, -INFINITY, v[u]);
       } else {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) v[u][i] = -INFINITY;
@@ -125,6 +134,8 @@ __global__ __launch_bounds__(BLOCK) void distill_row_kernel(DistillArgs a) {
     if (E != kOne) st = rescale(st, lse_ref(m), ref, a.ct) + at;
     m = bm;
   }
+  float z = 0.f;
+  if (id >= 0 && id < a.cols) z = to_f32(xr[id]);
   const float gm = block_reduce<BLOCK>(m, MaxOp(), red), ref = lse_ref(gm);
   s1 = block_reduce<BLOCK>(rescale(s1, lse_ref(m), ref, E == kOne ? a.ct : a.c1), SumOp(), red2);
   if (E == kOne) st = s1;
@@ -132,6 +143,13 @@ __global__ __launch_bounds__(BLOCK) void distill_row_kernel(DistillArgs a) {
   if (threadIdx.x == 0) {
     float* p = a.part + (row * a.splits + blockIdx.y) * 3;
     p[0] = gm, p[1] = s1, p[2] = st;
+  }
+  if (blockIdx.y) return;
+  float* zr = a.zs + row * a.k;
+  if ((int)threadIdx.x < a.k) zr[threadIdx.x] = z;
+  for (int k = threadIdx.x + BLOCK; k < a.k; k += BLOCK) {
+    id = entry_id(a, row * a.k + k);
+    zr[k] = id >= 0 && id < a.cols ? to_f32(xr[id]) : 0.f;
   }
 }
 
@@ -156,7 +174,7 @@ __device__ __forceinline__ float finish_row(const DistillArgs& a, int64_t row, i
   int *table = lds, *holder = lds + a.slots, *ids = lds + 2 * a.slots;
   float *p = (float*)(ids + a.k), *zs = p + a.k;
   const T* xr = (const T*)a.logits + row * a.cols;
-  // every load first: parts, the target's logit, entries, their logits
+  // every load first: parts, the target's logit, entries
   const bool part = lane < a.splits;
   const float* q = a.part + (row * a.splits + (part ? lane : 0)) * 3;
   const float pm = part ? q[0] : -INFINITY, p1 = part ? q[1] : 0.f, pt = part ? q[2] : 0.f;
@@ -171,7 +189,7 @@ __device__ __forceinline__ float finish_row(const DistillArgs& a, int64_t row, i
     const bool in = id >= 0 && id < a.cols;
     ids[k] = in ? (int)id : -1;
     p[k] = v;
-    zs[k] = in ? to_f32(xr[id]) : 0.f;
+    zs[k] = a.zs[e0 + k];
     if (in) tm = fmaxf(tm, v);
   }
   const float m = wave_reduce(pm, MaxOp()), ref = lse_ref(m);
@@ -345,7 +363,7 @@ __global__ __launch_bounds__(kFlatBlock) void distill_bwd_kernel(DistillArgs a) 
     if (first + u * kFlatBlock + threadIdx.x > last) continue;
     if constexpr (MANY) g[u] = row_grad(a, row0 + at[u], gh, gp);
     if (MANY ? g[u].live : at[u] ? g[1].live : g[0].live)
-      rowwise::load_pack<T, VEC, NT, RAG>((const T*)a.logits + (row0 + at[u]) * a.cols, pack[u] * VEC,
+      rowwise::load_pack<T, VEC, NT && !RAG, RAG>((const T*)a.logits + (row0 + at[u]) * a.cols, pack[u] * VEC,
                                           a.cols, 0.f, v[u]);
   }
   float* own[kFlatUnroll];
@@ -471,9 +489,9 @@ int check(const char* name, int64_t rows, int64_t cols, int64_t k, float tempera
 
 using namespace eg;
 
-extern "C" size_t eg_topk_distill_workspace_bytes(int64_t rows, int64_t cols) {
-  if (rows <= 0 || cols <= 0) return 0;
-  return (size_t)rows * (1 + 3 * splits_for(rows, cols)) * sizeof(float);
+extern "C" size_t eg_topk_distill_workspace_bytes(int64_t rows, int64_t cols, int64_t entries) {
+  if (rows <= 0 || cols <= 0 || entries < 0) return 0;
+  return (size_t)rows * (1 + 3 * splits_for(rows, cols) + entries) * sizeof(float);
 }
 
 extern "C" int eg_topk_distill_fwd(const void* logits, const int64_t* target, const void* teacher,
@@ -498,6 +516,7 @@ extern "C" int eg_topk_distill_fwd(const void* logits, const int64_t* target, co
   a.logits = logits, a.teacher = teacher, a.ids = teacher_ids, a.target = target;
   a.loss = loss, a.stats = stats, a.probs = probs, a.n_valid = n_valid;
   a.rowloss = (float*)workspace, a.part = a.rowloss + rows;
+  a.zs = a.part + rows * 3 * splits_for(rows, cols);
   a.rows = rows, a.cols = (int)cols, a.k = (int)entries, a.ignore_index = ignore_index;
   a.slots = slots_for(a.k), a.splits = splits_for(rows, cols), a.ids_64 = ids_64;
   a.teacher_type = teacher_dtype;
@@ -511,8 +530,9 @@ extern "C" int eg_topk_distill_fwd(const void* logits, const int64_t* target, co
         return by_width<T>(cols, {logits}, [&](auto vec, auto rag) {
           constexpr int V = decltype(vec)::value;
           const int64_t packs = ((cols + V - 1) / V + a.splits - 1) / a.splits;
-          rowwise::pick_row_block(packs,
-                                  RowLaunch<T, V, decltype(rag)::value, decltype(e)::value>{a, st});
+          RowLaunch<T, V, decltype(rag)::value, decltype(e)::value> row{a, st};
+          if (packs > kMostRow * rowwise::kUnroll) row.template go<kMostRow>();
+          else rowwise::pick_row_block(packs, row);
           return 0;
         });
       });

@@ -83,7 +83,7 @@ def topk_distillation_forward_with_saved(logits: torch.Tensor, target: torch.Ten
     teacher_ids = as_contiguous("teacher_ids", teacher_ids)
     loss = torch.empty((), dtype=torch.float32, device=logits.device)
     state = torch.empty(rows * (4 + entries) + 1, dtype=torch.float32, device=logits.device)
-    ws = workspace(_lib.query("eg_topk_distill_workspace_bytes", rows, cols), logits.device)
+    ws = workspace(_lib.query("eg_topk_distill_workspace_bytes", rows, cols, entries), logits.device)
     _lib.call_on(logits, "eg_topk_distill_fwd", logits.data_ptr(), target.data_ptr(),
                  teacher_logits.data_ptr(), teacher_dtype, teacher_ids.data_ptr(),
                  teacher_ids.dtype is torch.int64, loss.data_ptr(), *_parts(state, rows, entries),

@@ -574,7 +574,7 @@ int eg_norm_rotary_bwd(const void* dq_out, const void* dk_out, const void* q, co
                        float eps, float amplitude, int interleaved, int dtype, void* stream);
 
 /* Bytes of workspace eg_topk_distill_fwd needs. */
-size_t eg_topk_distill_workspace_bytes(int64_t rows, int64_t cols);
+size_t eg_topk_distill_workspace_bytes(int64_t rows, int64_t cols, int64_t entries);
 
 /* Distillation from a teacher's top logits with a share of hard-label cross entropy: over the
  * rows whose target is not ignore_index, n_valid of them,

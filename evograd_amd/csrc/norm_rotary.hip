@@ -307,10 +307,11 @@ __global__ __launch_bounds__(kMostThreads, kBackWaves) void norm_rotary_bwd_kern
     float sum[2] = {0.f, 0.f};
     const int first = blockIdx.y * heads, left = a.per_block * a.lanes - first;
     int head = first % a.lanes;
+#pragma unroll 8
     for (int m = 0; m < min(heads, left); ++m) {
       const float v = rows[m * a.head_dim + c];
-      if (head < a.heads_q) sum[0] += v;
-      else sum[1] += v;
+      sum[0] += head < a.heads_q ? v : 0.f;
+      sum[1] += head < a.heads_q ? 0.f : v;
       if (++head == a.lanes) head = 0;
     }
     part[c] = sum[0];

@@ -248,7 +248,8 @@ __device__ __forceinline__ float finish_row(const DistillArgs& a, int64_t row, i
   float loss = 0.f;
   if (a.soft != 0.f && some) loss += a.soft * a.tau * a.tau * kl;
   if (a.hard != 0.f && label) loss += a.hard * (logf(s1) - (zt - ref));
-  const float fail = bad != 0.f ? NAN : 0.f;
+  // a NaN or +inf among the entries is one in p's sum, which every column's gradient has
+  const float fail = bad != 0.f || !(total < INFINITY) ? NAN : 0.f;
   if (lane == 0) {
     s[0] = ref;
     s[1] = 1.f / s1 + fail;
@@ -344,7 +345,7 @@ __global__ __launch_bounds__(kFlatBlock) void distill_bwd_kernel(DistillArgs a) 
   const float gh = scale * a.hard, gp = scale * a.soft * a.tau;
   // this thread's first entry
   const int64_t e0 = row0 * a.k;
-  const int n = a.soft != 0.f ? rows * a.k : 0;
+  const int n = rows * a.k;
   float p0 = 0.f;
   int64_t id0 = -1;
   if ((int)threadIdx.x < n) p0 = a.probs[e0 + threadIdx.x], id0 = entry_id(a, e0 + threadIdx.x);
@@ -517,7 +518,8 @@ extern "C" int eg_topk_distill_fwd(const void* logits, const int64_t* target, co
   a.loss = loss, a.stats = stats, a.probs = probs, a.n_valid = n_valid;
   a.rowloss = (float*)workspace, a.part = a.rowloss + rows;
   a.zs = a.part + rows * 3 * splits_for(rows, cols);
-  a.rows = rows, a.cols = (int)cols, a.k = (int)entries, a.ignore_index = ignore_index;
+  a.rows = rows, a.cols = (int)cols, a.ignore_index = ignore_index;
+  a.k = soft_weight != 0.f ? (int)entries : 0;  // else they have no part
   a.slots = slots_for(a.k), a.splits = splits_for(rows, cols), a.ids_64 = ids_64;
   a.teacher_type = teacher_dtype;
   a.tau = temperature, a.soft = soft_weight, a.hard = hard_weight;
@@ -568,7 +570,8 @@ extern "C" int eg_topk_distill_bwd(const float* dloss, const void* logits, const
   a.logits = logits, a.ids = teacher_ids, a.target = target, a.dloss = dloss;
   a.stats = const_cast<float*>(stats), a.probs = const_cast<float*>(probs);
   a.n_valid = const_cast<float*>(n_valid), a.dlogits = dlogits;
-  a.rows = rows, a.cols = (int)cols, a.k = (int)entries, a.ignore_index = ignore_index;
+  a.rows = rows, a.cols = (int)cols, a.ignore_index = ignore_index;
+  a.k = soft_weight != 0.f ? (int)entries : 0;  // else they have no part
   a.ids_64 = ids_64, a.tau = temperature, a.soft = soft_weight, a.hard = hard_weight;
   const int exponentials = exps_of(a);
   return EG_DISPATCH_FLOAT(dtype, name, [&]() -> int {

@@ -6,7 +6,7 @@
 ``weight`` is [vocab, hidden], ``ids`` int32 or int64 of any shape, ``out`` [*ids.shape, hidden].
 Sums are fp32 in the tokens' order (the same bits every run), each result rounded once. A token
 equal to ``ignore_index`` gives a row of zeros; any other one outside [0, vocab) gives a row of
-NaN. Neither has a gradient. Saved state: ``(ids, vocab)``; the table itself is not kept.
+NaN. Neither has a gradient. Saved state: ``(ids, vocab, hidden, dtype)``, and not the table.
 
 ``embedding_backward_into(dweight, dout, saved, ...)`` adds the gradient to one that is there
 (a table shared with the output projection): only the rows of the batch's own tokens are read and
@@ -49,24 +49,23 @@ def embedding_forward_with_saved(weight: torch.Tensor, ids: torch.Tensor, scale:
     _lib.call_on(weight, "eg_embedding_fwd", weight.data_ptr(), ids.data_ptr(),
                  ids.dtype == torch.int64, out.data_ptr(), ids.numel(), vocab, hidden, scale,
                  ignore_index, dtype, _lib.stream_of(weight))
-    return out, (ids, vocab)
+    return out, (ids, vocab, hidden, weight.dtype)
 
 
 def _backward(name, dweight, dout, saved, scale, ignore_index):
     """Writes dweight, or adds to it if there is one."""
-    ids, vocab = saved
+    ids, vocab, hidden, kind = saved
     _lib.require_gpu(name, dout, ids)
     _check_ids(name, ids)
-    if dout.dim() != ids.dim() + 1 or dout.shape[:-1] != ids.shape:
-        raise ValueError(f"{name}: dout must be [*{tuple(ids.shape)}, hidden], got "
-                         f"{tuple(dout.shape)}")
-    dtype = tag(dout.dtype)
-    hidden = dout.shape[-1]
+    if dout.shape != (*ids.shape, hidden) or dout.dtype is not kind:
+        raise ValueError(f"{name}: dout must be {[*ids.shape, hidden]} of {kind}, got "
+                         f"{tuple(dout.shape)} of {dout.dtype}")
+    dtype = tag(kind)
     add = dweight is not None
     if add:
         _lib.require_gpu(name, dout, dweight)
-        if tuple(dweight.shape) != (vocab, hidden) or dweight.dtype != dout.dtype:
-            raise ValueError(f"{name}: dweight must be [{vocab}, {hidden}] of {dout.dtype}, got "
+        if dweight.shape != (vocab, hidden) or dweight.dtype is not kind:
+            raise ValueError(f"{name}: dweight must be [{vocab}, {hidden}] of {kind}, got "
                              f"{tuple(dweight.shape)} of {dweight.dtype}")
         if not dweight.is_contiguous():
             raise ValueError(f"{name}: dweight must be contiguous")

@@ -551,8 +551,9 @@ int eg_embedding_bwd(const void* dout, const void* ids, int ids_64, void* dweigh
 /* RMSNorm of every head with the rotation of eg_rotary behind it: n = x * rsqrt(mean(x^2) + eps)
  * * weight over a head's columns, then pairs of n rotated and scaled by amplitude as there, the
  * columns from 2 * pairs on left as n. q [tokens, heads_q, head_dim] with q_weight [head_dim], k
- * [tokens, heads_k, head_dim] with k_weight (heads_k = 0: q alone), one launch; strides, positions,
- * freqs and sizes as for eg_rotary. fp32 arithmetic, one rounding. */
+ * [tokens, heads_k, head_dim] with k_weight (heads_k = 0: q alone), one launch; strides, positions
+ * and freqs as for eg_rotary. fp32 arithmetic, one rounding. Outputs overlap no input, here and in
+ * the backward. Sizes: tokens <= 2^32, heads_q and heads_k <= 2^16 each, head_dim <= 2^13. */
 int eg_norm_rotary_fwd(const void* q, const void* k, const void* q_weight, const void* k_weight,
                        void* q_out, void* k_out, const void* positions, int positions_64,
                        const double* freqs, int64_t tokens, int64_t heads_q, int64_t heads_k,
@@ -583,10 +584,11 @@ size_t eg_topk_distill_workspace_bytes(int64_t rows, int64_t cols, int64_t entri
  * p = softmax(teacher / tau) over the row's entries, q = softmax(logits / tau) over cols.
  * logits [rows, cols] (dtype); teacher [rows, entries] (teacher_dtype) at the columns teacher_ids
  * [rows, entries] int32, or int64 with ids_64; a negative id is no entry, several entries of one
- * column all count, a row without entries has no soft part. An id >= cols, and with hard_weight
- * != 0 a target outside [0, cols), makes the row's loss and gradient NaN. loss and n_valid: one
- * fp32 each. Saved: stats fp32 [rows, 4], probs fp32 [rows, entries]. tau > 0; entries <= 1024,
- * rows < 2^22, cols <= 2^30. */
+ * column all count, a row without entries has no soft part. With soft_weight != 0 an id >= cols or
+ * a value of NaN or +inf, and with hard_weight != 0 a target outside [0, cols), makes the row's
+ * loss and gradient NaN; with a weight of 0 entries or targets are not looked at. loss and
+ * n_valid: one fp32 each. Saved: stats fp32 [rows, 4], probs fp32 [rows, entries]. tau > 0;
+ * entries <= 1024, rows < 2^22, cols <= 2^30. */
 int eg_topk_distill_fwd(const void* logits, const int64_t* target, const void* teacher,
                         int teacher_dtype, const void* teacher_ids, int ids_64, float* loss,
                         float* stats, float* probs, float* n_valid, void* workspace, int64_t rows,

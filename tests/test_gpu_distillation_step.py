@@ -6,17 +6,30 @@ own table) and the loss against the teacher's top logits; and back to every weig
 import pytest
 import torch
 
+from evograd_amd import decls, pair_module
 from evograd_amd.bind import bind
 from evograd_amd.decls import EMBEDDING, PACKED_ATTENTION, TOPK_DISTILLATION
 from evograd_amd.pairs import embedding, packed_attention, rotary, topk_distillation
 from evograd_amd.pairs.block_norm import BlockNorm
 from evograd_amd.pairs.norm_rotary import NormRotaryQK
 from oracle import forward_refs as fr
+from oracle.verify import verify
 
 pytestmark = pytest.mark.gpu
 
 EPS = 1e-6
 TAU, SOFT, HARD = 2.0, 0.7, 0.3
+
+
+@pytest.mark.parametrize("name,w", [
+    pytest.param(name, w, id=f"{name}-{w.key()}")
+    for name in ("embedding", "norm_rotary", "topk_distillation")
+    for w in (*decls.get_op(name).correctness, *decls.get_op(name).benchmark)
+    if w.dims.get("rows", 0) <= 64])  # the oracle of the loss goes row by row
+def test_declared_workloads(name, w):
+    print(f"\n[gpu-step] {name} {w.dims} {w.dtype} {w.extra}", flush=True)
+    rep = verify(decls.get_op(name), pair_module(name), device="cuda", workloads=(w,))
+    assert rep.ok, "\n".join(rep.failures())
 
 
 def model(ops, p, batch, H, KVH, D):

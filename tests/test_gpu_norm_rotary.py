@@ -228,3 +228,52 @@ def test_two_streams_and_a_captured_graph():
         got = [x.clone() for x in out]
         for x, y in zip(got, step()):
             assert torch.equal(x, y)
+
+
+def test_tensors_past_32_bit_offsets():
+    """The last tokens of q and k of 2.5e9 elements, against a call on those tokens alone."""
+    T, H, KVH, D = 480000, 32, 8, 128
+    q, k = (torch.zeros(T, h, D, dtype=BF16, device="cuda") for h in (H, KVH))
+    n = 7
+    tail = [make(n, h, D, dtype=BF16, seed=i) for i, h in enumerate((H, KVH, H, KVH))]
+    q[-n:], k[-n:] = tail[0], tail[1]
+    qw, kw, freqs = gain(D, BF16, 3), gain(D, BF16, 4), turns(64)
+    pos = torch.arange(T, device="cuda", dtype=torch.int32)
+    outs, saved = pair.norm_rotary_qk_forward_with_saved(q, k, qw, kw, pos, freqs)
+    want, s = pair.norm_rotary_qk_forward_with_saved(*tail[:2], qw, kw, pos[-n:], freqs)
+    assert torch.equal(outs[0][-n:], want[0]) and torch.equal(outs[1][-n:], want[1])
+    assert not bool(outs[0][:-n].any()) and not bool(outs[1][:-n].any())
+    del outs
+    dq, dk = torch.zeros_like(q), torch.zeros_like(k)
+    dq[-n:], dk[-n:] = tail[2], tail[3]
+    grads = pair.norm_rotary_qk_backward_from_saved((dq, dk), saved)
+    wants = pair.norm_rotary_qk_backward_from_saved(tail[2:], s)
+    for got, w in zip(grads[:2], wants[:2]):
+        assert torch.equal(got[-n:], w) and not bool(got[:-n].any())
+    for i, (x, w, d) in enumerate(((tail[0], qw, tail[2]), (tail[1], kw, tail[3]))):
+        assert_within("dweight", grads[2 + i],
+                      *norm_rotary64(x, w, pos[-n:], freqs, EPS, 1.0, 0, d)["dweight"])
+
+
+def test_two_graphs_with_a_workspace_each():
+    """Two captured backward passes, replayed one over the other."""
+    q, w, pos, freqs = make(700, 5, 64, dtype=BF16), gain(64, BF16, 1), spots(700, 1000), turns(32)
+    grads = [make(700, 5, 64, dtype=BF16, seed=s) for s in (2, 3)]
+    _, saved = pair.norm_rotary_forward_with_saved(q, w, pos, freqs)
+    want = [pair.norm_rotary_backward_from_saved(d, saved) for d in grads]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for d in grads:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(pair.norm_rotary_backward_from_saved(d, saved))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(3):
+        for s, graph in zip(streams, graphs):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for got, ref in zip(outs, want):
+            assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])

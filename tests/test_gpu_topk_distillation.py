@@ -186,10 +186,22 @@ def test_a_non_finite_row_stays_in_its_row():
         clean = step(logits, target, teacher, ids, 2.0, 0.5, 0.5)[1]
         logits[4, 33] = what
         teacher[9, 2] = what
-        _, grad = step(logits, target, teacher, ids, 2.0, 0.5, 0.5)
-        assert not bool(grad[4].isfinite().all()) and not bool(grad[9].isfinite().all())
+        loss, grad = step(logits, target, teacher, ids, 2.0, 0.5, 0.5)
+        assert not bool(loss.isfinite()) and not bool(grad[4].isfinite().all())
+        assert bool(grad[9].isnan().all())
         grad[4], grad[9] = clean[4], clean[9]
         assert torch.equal(grad, clean)
+
+
+def test_parts_with_no_weight_are_not_looked_at():
+    logits, target, teacher, ids = make(10, 300, 5, BF16, ignore=0.0)
+    want = step(logits, target, teacher, ids, 2.0, 0.0, 1.0)
+    got = step(logits, target, torch.full_like(teacher, float("nan")), torch.full_like(ids, 300), 2.0,
+               0.0, 1.0)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert bool(want[0].isfinite())
+    nothing = step(logits, target, teacher, ids, 2.0, 0.0, 0.0)
+    assert float(nothing[0]) == 0.0 and int(torch.count_nonzero(nothing[1])) == 0
 
 
 def test_no_rows():

@@ -39,7 +39,7 @@ def test_cpu_tensors_are_refused():
     with pytest.raises(RuntimeError, match="GPU"):
         embedding.embedding_forward_with_saved(W, IDS)
     with pytest.raises(RuntimeError, match="GPU"):
-        embedding.embedding_backward_into(W, torch.zeros(4, 8), (IDS, 6))
+        embedding.embedding_backward_into(W, torch.zeros(4, 8), (IDS, 6, 8, torch.float32))
     with pytest.raises(RuntimeError, match="GPU"):
         norm_rotary.norm_rotary_forward_with_saved(x, torch.ones(8), POS, FREQ)
     with pytest.raises(RuntimeError, match="GPU"):
@@ -57,16 +57,16 @@ def test_embedding_arguments(no_device_check):
     with pytest.raises(TypeError, match="unsupported dtype"):
         call(W.double(), IDS)
     back, into = embedding.embedding_backward_from_saved, embedding.embedding_backward_into
-    for bad in (torch.zeros(8), torch.zeros(3, 8), torch.zeros(2, 2, 8)):
+    saved = (IDS, 6, 8, torch.float32)
+    for bad in (torch.zeros(8), torch.zeros(3, 8), torch.zeros(4, 7), torch.zeros(2, 2, 8),
+                torch.zeros(4, 8).half(), torch.zeros(4, 8).double()):
         with pytest.raises(ValueError, match="dout must be"):
-            back(bad, (IDS, 6))
-    with pytest.raises(TypeError, match="unsupported dtype"):
-        back(torch.zeros(4, 8).double(), (IDS, 6))
+            back(bad, saved)
     for bad in (torch.zeros(5, 8), torch.zeros(6, 7), torch.zeros(6, 8).half()):
         with pytest.raises(ValueError, match="dweight must be"):
-            into(bad, torch.zeros(4, 8), (IDS, 6))
+            into(bad, torch.zeros(4, 8), saved)
     with pytest.raises(ValueError, match="contiguous"):
-        into(torch.zeros(8, 6).t(), torch.zeros(4, 8), (IDS, 6))
+        into(torch.zeros(8, 6).t(), torch.zeros(4, 8), saved)
 
 
 @pytest.mark.parametrize("x,w,pos,freqs,error,words", (
@@ -234,4 +234,4 @@ def test_gradients_of_gradients_are_refused(no_kernels):
 
 def test_the_embedding_keeps_no_table(no_kernels):
     _, saved = embedding.embedding_forward_with_saved(W, IDS)
-    assert saved[1] == 6 and saved[0] is IDS and len(saved) == 2
+    assert saved[0] is IDS and saved[1:] == (6, 8, torch.float32)

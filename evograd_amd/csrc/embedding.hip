@@ -39,9 +39,9 @@ constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / kWave;
 constexpr int kBucketIds = 1024;  // at most, an id per thread in the scan
 constexpr int kMostPiece = 32;
 constexpr int kSumThreads = 256, kFewestLanes = 16, kMostGroups = kSumThreads / kFewestLanes;
-constexpr int kSingly = 4;
+constexpr int kSingly = 4;      // ids of 64 positions that are placed one by one
 constexpr int kEarlyPacks = 2;  // of 16 bytes, per thread
-constexpr int kAhead = 8;  // loads of a thread on their way at once
+constexpr int kAhead = 8;       // loads of a thread on their way at once
 constexpr int kJoinLanes = 64, kJoinAdders = 8, kJoinThreads = kJoinLanes * kJoinAdders;
 constexpr int kJoinParts = 4;  // workgroups that share a piece's columns, at most
 constexpr int kZeroPacks = 2;  // per thread

@@ -537,7 +537,7 @@ int eg_embedding_fwd(const void* weight, const void* ids, int ids_64, void* out,
                      void* stream);
 
 /* Bytes of workspace eg_embedding_bwd needs: the tokens' order, a bound for every id, and two
- * fp32 partial rows per 32 tokens. */
+ * fp32 partial rows per piece of 8 to 32 tokens. */
 size_t eg_embedding_workspace_bytes(int64_t tokens, int64_t vocab, int64_t hidden);
 
 /* Its gradient: dweight[v] = scale * sum of dout[t] over the tokens with ids[t] == v, fp32 sums in

@@ -50,7 +50,8 @@ def both_ways(weight, ids, dout, scale=1.0, ignore_index=-100):
     (33, 50, 136, "flat"), (64, 2, 24, "flat"), (65, 1, 40, "flat"), (257, 1000, 127, "mixed"),
     (1000, 255, 512, "low"), (1000, 256, 520, "same"), (1024, 257, 64, "mixed"),
     (1025, 4096, 65, "low"), (3000, 70000, 100, "low"), (5000, 300, 2056, "mixed"),
-    (2100, 3, 4100, "flat")))
+    (2100, 3, 4100, "flat"), (900, 262144, 8, "low"), (9000, 262145, 9, "mixed"),
+    (70, 2500000, 16, "flat"), (17000, 5000, 33, "low"), (40000, 600, 20, "mixed")))
 def test_against_64_bits(T, V, H, how, dtype):
     print(f"\n[gpu-embedding] {T} {V}x{H} {how} {dtype}", flush=True)
     weight, dout, ids = normal(V, H, dtype=dtype), normal(T, H, dtype=dtype, seed=1), tokens(T, V, how)
@@ -86,6 +87,19 @@ def test_a_scale_of_one_copies_bits():
         weight, ids = normal(99, 130, dtype=dtype), tokens(50, 99)
         out, _ = pair.embedding_forward_with_saved(weight, ids)
         assert torch.equal(out, weight[ids.long()])
+
+
+def test_ids_of_one_bucket_and_a_run_over_many_pieces():
+    """Ids a power of two apart share a bucket; then one id takes every token but a few."""
+    V, H = 70000, 24
+    weight, dout = normal(V, H, dtype=F32), normal(20000, H, dtype=F32, seed=1)
+    strided = (tokens(20000, 270).long() * 256 + 5).to(torch.int32)
+    alone = torch.full((20000,), 4100, dtype=torch.int32, device="cuda")
+    alone[[0, 7, 31, 32, 9999, 19999]] = torch.tensor([1, 4099, 4101, 69999, 0, 2], dtype=torch.int32,
+                                                      device="cuda")
+    for ids in (strided, alone):
+        _, grad = both_ways(weight, ids, dout)
+        assert_within("dweight", grad, *embedding64(weight, ids, 1.0, -100, dout)[1])
 
 
 def test_no_tokens_and_empty_tables():

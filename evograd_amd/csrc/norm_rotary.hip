@@ -212,7 +212,7 @@ __device__ __forceinline__ float head_dot(const Place<VEC, INTER>& at, const flo
 
 // A workgroup walks the tokens in steps of the grid, one head a thread group, and loads the next
 // step's packs under the present one's work. The sines of a.ahead steps are formed at a time.
-template <typename T, int VEC, bool INTER, int GROUP, bool NT>
+template <typename T, int VEC, bool INTER, bool NT>
 __global__ __launch_bounds__(kMostThreads, kFrontWaves) void norm_rotary_fwd_kernel(HeadArgs a) {
   extern __shared__ float2 table[];  // [ahead][per_block][pairs]
   const Place<VEC, INTER> at(a);
@@ -237,7 +237,7 @@ __global__ __launch_bounds__(kMostThreads, kFrontWaves) void norm_rotary_fwd_ker
     t = min(t0 + stride + at.tl, a.tokens - 1);
     raw.load(h.x<T>(a, t), at);
     w.get(g);
-    const float rstd = rsqrtf(head_dot<GROUP>(at, n, n, a.group) * a.share + a.eps);
+    const float rstd = rsqrtf(head_dot<0>(at, n, n, a.group) * a.share + a.eps);
 #pragma unroll
     for (int i = 0; i < 2 * VEC; ++i) n[i] = n[i] * rstd * g[i];
     if (at.turn) turn_packs<VEC, INTER>(turns, n);
@@ -474,23 +474,27 @@ int by_width(const HeadArgs& a, F&& go) {
   return go(std::integral_constant<int, VEC>{});
 }
 
-// f(GROUP, NT): the lanes of a head where 16-byte packs make it a usual count, else 0; whether the
-// call streams.
+// f(NT): whether the call streams.
+template <int VEC, typename T, typename F>
+int by_size(const HeadArgs& a, F&& f) {
+  if constexpr (VEC * sizeof(T) == 16) {
+    const int64_t heads = a.heads_q + a.heads_k;
+    if (a.tokens * heads * a.head_dim * (int64_t)sizeof(T) > kStreamBytes) return f(std::true_type{});
+  }
+  return f(std::false_type{});
+}
+
+// f(GROUP): the backward's lanes of a head where 16-byte packs make it a usual count, else 0, the
+// count at run time. 32768 tokens, 32 + 8 heads of 128 bf16 173 us / 181 at run time, 16384 tokens,
+// 18 heads of 256 93 / 103; the forward is the same either way.
 template <int VEC, typename T, typename F>
 int by_group(const HeadArgs& a, F&& f) {
   if constexpr (VEC * sizeof(T) == 16) {
-    const int64_t heads = a.heads_q + a.heads_k;
-    const bool stream = a.tokens * heads * a.head_dim * (int64_t)sizeof(T) > kStreamBytes;
-    auto with = [&](auto group) {
-      return stream ? f(group, std::true_type{}) : f(group, std::false_type{});
-    };
-    if (a.group == 4) return with(std::integral_constant<int, 4>{});
-    if (a.group == 8) return with(std::integral_constant<int, 8>{});
-    if (a.group == 16) return with(std::integral_constant<int, 16>{});
-    return with(std::integral_constant<int, 0>{});
-  } else {
-    return f(std::integral_constant<int, 0>{}, std::false_type{});
+    if (a.group == 4) return f(std::integral_constant<int, 4>{});
+    if (a.group == 8) return f(std::integral_constant<int, 8>{});
+    if (a.group == 16) return f(std::integral_constant<int, 16>{});
   }
+  return f(std::integral_constant<int, 0>{});
 }
 
 template <typename F>
@@ -574,8 +578,8 @@ extern "C" int eg_norm_rotary_fwd(const void* q, const void* k, const void* q_we
         }
         place(a, s, kFrontWaves);
         if (s.gy > 65535) { set_error("%s: grid too large", name); return 1; }
-        return by_group<V, T>(a, [&](auto group, auto nt) -> int {
-          EG_LAUNCH((norm_rotary_fwd_kernel<T, V, I, decltype(group)::value, decltype(nt)::value>),
+        return by_size<V, T>(a, [&](auto nt) -> int {
+          EG_LAUNCH((norm_rotary_fwd_kernel<T, V, I, decltype(nt)::value>),
                     dim3((unsigned)s.gx, (unsigned)s.gy), dim3(s.threads),
                     (size_t)a.ahead * a.per_block * a.pairs * sizeof(float2), as_stream(stream), a);
           return check_launch(name);
@@ -640,10 +644,13 @@ extern "C" int eg_norm_rotary_bwd(const void* dq_out, const void* dk_out, const 
           parts = (int)(s.gx * s.gy);
           const size_t lds = std::max<size_t>((size_t)a.ahead * a.per_block * a.pairs * sizeof(float2),
                                               (size_t)s.threads / s.group * head_dim * sizeof(float));
-          return by_group<V, T>(a, [&](auto group, auto nt) -> int {
-            EG_LAUNCH((norm_rotary_bwd_kernel<T, V, I, decltype(group)::value, decltype(nt)::value>),
-                      dim3((unsigned)s.gx, (unsigned)s.gy), dim3(s.threads), lds, as_stream(stream), a);
-            return check_launch(name);
+          return by_group<V, T>(a, [&](auto group) -> int {
+            return by_size<V, T>(a, [&](auto nt) -> int {
+              EG_LAUNCH((norm_rotary_bwd_kernel<T, V, I, decltype(group)::value, decltype(nt)::value>),
+                        dim3((unsigned)s.gx, (unsigned)s.gy), dim3(s.threads), lds, as_stream(stream),
+                        a);
+              return check_launch(name);
+            });
           });
         });
       });

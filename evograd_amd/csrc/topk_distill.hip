@@ -18,12 +18,15 @@
 // LDS.
 //
 // Kernels: distill_row_kernel streams the rows (a workgroup a row, or a part of one where rows
-// are few) and leaves their sums; distill_finish_kernel does the rest of a row, whose work is a
-// chain of short steps, in one wave; distill_mean_kernel adds the rows; distill_bwd_kernel. With
-// the finish at the end of the row's own workgroup, bf16 [8192, 128256] with 64 entries, a tenth
-// of the rows ignored, took 597 us forward instead of 309 + 19 + 5: the streams of a CU's other
-// workgroup do not fill it. Backward 692 us, 5.8 TB/s; with the entries loaded after the
-// first barrier 939.
+// are few), leaves their sums and reads the entries' logits while the row is near;
+// distill_finish_kernel does the rest of a row, whose work is a chain of short steps, in one wave;
+// distill_mean_kernel adds the rows; distill_bwd_kernel. bf16 [8192, 128256] with 64 entries at a
+// temperature of 2 with hard labels, a tenth of the rows ignored: 306 + 12 + 5 us forward (6.2
+// TB/s) and 684 backward (5.8 TB/s). With the finish at the end of the row's own workgroup the
+// forward took 597, as the streams of a CU's other workgroup do not fill it, and with the entries
+// loaded after the first barrier the backward 939. Rows that are no multiple of a pack: fp16 [2047,
+// 50257] 36 + 6 + 5 and 58; with the non-temporal hint on their loads 52 and 68, for unaligned packs
+// share cache lines.
 #include "rowwise.hpp"
 
 #include <algorithm>
@@ -37,7 +40,10 @@ using rowwise::lse_ref;
 
 constexpr int kMaxEntries = 1024;
 constexpr int kMeanBlock = 1024;
-constexpr int64_t kFewRows = 32;  // that one workgroup finishes, two a wave
+// Rows that one workgroup finishes, a wave each, with their mean. Forward of 128256 columns, us, so
+// and with a launch for each: 1 row 10.0 / 10.9, 4 rows 10.6 / 11.5, 16 rows 11.3 / 11.5, 32 rows (two
+// a wave) 17.3 / 12.6.
+constexpr int64_t kFewRows = 16;
 // Threads of a row's workgroup at most and packs in flight per thread. Forward, us, at 1024 / 512
 // / 256 threads: bf16 [8192, 128256] with one exponential 308 / 309 / 308, a squared one 330 / 309 /
 // 314, two 366 / 338 / 336, 16 rows 11.4 / 11.8 / 11.6; with 512 threads at 8 / 4 / 2 packs: 316 / 313
@@ -48,7 +54,8 @@ constexpr int kMostRow = 512, kUnroll = 2;
 constexpr int kFlatBlock = 256, kFlatUnroll = 2, kFlatPer = kFlatBlock * kFlatUnroll;
 
 // The exponentials of a column: one of them (no hard label, no soft part or a temperature of 1),
-// both, or, at a temperature of 2, the hard label's as the soft one's square.
+// both, or, at a temperature of 2, the hard label's as the soft one's square (bf16 [8192, 128256],
+// forward and backward, us: one 308 and 635, both 350 and 675, the square 306 and 655).
 enum Exps { kOne, kTwo, kSquare };
 
 struct DistillArgs {
@@ -107,7 +114,6 @@ __global__ __launch_bounds__(BLOCK) void distill_row_kernel(DistillArgs a) {
     for (int u = 0; u < kUnroll; ++u) {
       const int64_t c = base + u * STEP;
       if (c < c1) {
-        // unaligned packs share cache lines: without the non-temporal hint
         rowwise::load_pack<T, VEC, VEC * sizeof(T) == 16 && !RAG, RAG>(xr, (int)c, a.cols, -INFINITY, v[u]);
       } else {
 #pragma unroll
@@ -441,10 +447,13 @@ int slots_for(int k) {
 }
 size_t finish_lds(const DistillArgs& a) { return (2 * a.slots + 3 * a.k) * sizeof(int); }
 
-// Parts of a row, where rows are few; a lane each in the finish.
+// Parts of a row, where rows are few: up to the card's 1024 workgroups, of 4096 columns or more; a
+// lane each in the finish. Forward of bf16 rows of 128256, us, whole / so: 1 row 17.5 / 9.7, 16 rows
+// 21.2 / 11.6, 64 rows 24.5 / 14.3, 300 rows 31.2 / 24.6 (with up to 512 workgroups 32.8); 100 rows of
+// 32000 14.4 / 12.6 (in parts of 8192 13.5), 500 of them 17.2 / 17.4.
 constexpr int kMostSplits = 64;
 int splits_for(int64_t rows, int64_t cols) {
-  const int64_t want = 512 / std::max<int64_t>(rows, 1), most = cols / 8192;
+  const int64_t want = 1024 / std::max<int64_t>(rows, 1), most = cols / 4096;
   return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, kMostSplits}));
 }
 

@@ -219,7 +219,8 @@ def test_workspaces():
     assert q("eg_norm_rotary_workspace_bytes", 5, 8, 2, 64) == 2048 * 2 * 64 * 4
     assert q("eg_topk_distill_workspace_bytes", 0, 100, 3) == 0
     assert q("eg_topk_distill_workspace_bytes", 8192, 128256, 64) == 8192 * (4 + 64) * 4
-    assert q("eg_topk_distill_workspace_bytes", 4, 128256, 0) == 4 * (1 + 3 * 15) * 4
+    assert q("eg_topk_distill_workspace_bytes", 4, 128256, 0) == 4 * (1 + 3 * 31) * 4
+    assert q("eg_topk_distill_workspace_bytes", 300, 128256, 9) == 300 * (1 + 3 * 3 + 9) * 4
 
 
 def test_gradients_of_gradients_are_refused(no_kernels):

@@ -22,7 +22,7 @@
 //
 // Memory-bound: the backward reads T rows and writes the table. bf16, 16384 tokens of [128256,
 // 4096] whose frequencies fall as one over their rank: forward 32 us, backward 197 (6.0 TB/s);
-// fp16 8191 tokens of [50257, 1538], a third of them the same: 9 and 44; 32 tokens forward 3 us, a
+// fp16 8191 tokens of [50257, 1538], a third of them the same: 9 and 40; 32 tokens forward 3 us, a
 // launch. Steps of the first backward (259 us): ids loaded eight at a time and matched one by one
 // where they are few, the zeros beside the join and not the sums, two packs of zeros a thread (4: 234,
 // 8: 250, one: 242 where two took 213), zeros under the ordering.
@@ -322,9 +322,10 @@ __global__ __launch_bounds__(kSumThreads) void embed_sum_kernel(EmbedArgs a, int
   for (int i = threadIdx.x; i < groups * (a.piece + 2); i += kSumThreads) {
     const int g = i / (a.piece + 2), j = i - g * (a.piece + 2);
     const int64_t at = (piece0 + g) * a.piece + j - 1;
-    const bool in = at >= 0 && at < n;
-    ids[g][j] = in ? a.key[at] : -1;
-    if (in && j >= 1 && j <= a.piece) where[g][j - 1] = a.order[at];
+    const int64_t safe = max((int64_t)0, min(at, a.tokens - 1));  // read before n has come
+    const int id = a.key[safe], pos = a.order[safe];
+    ids[g][j] = at >= 0 && at < n ? id : -1;
+    if (j >= 1 && j <= a.piece) where[g][j - 1] = pos;
   }
   __syncthreads();
   const int64_t piece = piece0 + group;
@@ -533,9 +534,11 @@ extern "C" int eg_embedding_bwd(const void* dout, const void* ids, int ids_64, v
       const int lanes = lanes_for(packs, kSumThreads), groups = kSumThreads / lanes;
       const int64_t columns = (packs + lanes - 1) / lanes;
       const int64_t sums = (l.pieces + groups - 1) / groups * columns;
-      // the join in fours of columns where a row's fours are aligned, zeros in whole packs
-      const bool flat = aligned16(dweight), fours = flat && hidden % 4 == 0;
-      const int64_t span = kJoinLanes * (fours ? 4 : 1);
+      // the join in fours or twos of columns where a row's are aligned, zeros in whole packs (8191
+      // tokens of [50257, 1538] fp16, a third of them one: 44 us in single columns, 40 in twos)
+      const bool flat = aligned16(dweight);
+      const bool fours = flat && hidden % 4 == 0, twos = flat && hidden % 2 == 0;
+      const int64_t span = kJoinLanes * (fours ? 4 : twos ? 2 : 1);
       const int parts = (int)std::min<int64_t>((hidden + span - 1) / span, kJoinParts);
       const int64_t joins = l.pieces > 1 ? (l.pieces - 1) * parts : 0;
       const int64_t chunk = (int64_t)kJoinThreads * kZeroPacks * (flat ? W : 1);
@@ -563,6 +566,7 @@ extern "C" int eg_embedding_bwd(const void* dout, const void* ids, int ids_64, v
       if (joins + zeros) {
         using std::integral_constant;
         if (fours) join(integral_constant<int, 4>{}, integral_constant<int, W>{});
+        else if (twos) join(integral_constant<int, 2>{}, integral_constant<int, W>{});
         else if (flat) join(integral_constant<int, 1>{}, integral_constant<int, W>{});
         else join(integral_constant<int, 1>{}, integral_constant<int, 1>{});
       }

@@ -403,7 +403,7 @@ __global__ __launch_bounds__(kSumCols* kSumRows) void norm_rotary_sum_kernel(Hea
   const int c = blockIdx.x * kSumCols + lane, cols = 2 * a.head_dim;
   float s = 0.f;
   if (c < cols) {
-#pragma unroll 4
+#pragma unroll 8
     for (int r = adder; r < parts; r += kSumRows) s += a.part[(int64_t)r * cols + c];
   }
   sums[adder][lane] = s;

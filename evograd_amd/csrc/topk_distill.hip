@@ -177,6 +177,7 @@ __device__ __forceinline__ float finish_row(const DistillArgs& a, int64_t row, i
     if (lane < 4) s[lane] = 0.f;
     return 0.f;
   }
+  wave_sync();  // an earlier row's words have been read
   int *table = lds, *holder = lds + a.slots, *ids = lds + 2 * a.slots;
   float *p = (float*)(ids + a.k), *zs = p + a.k;
   const T* xr = (const T*)a.logits + row * a.cols;

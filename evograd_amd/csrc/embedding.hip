@@ -5,7 +5,8 @@
 // in fp32, each output rounded once. A token equal to ignore_index gives a row of zeros, any
 // other one outside [0, vocab) a row of NaN; neither is used as an index or has a gradient.
 //
-// The gradient runs in three launches and without atomics on its sums:
+// The gradient of few tokens is one launch (embed_few_kernel), that of more runs in three, both
+// without atomics on their sums:
 //   embed_sort_kernel   orders the tokens by id, equal ones by position. The ids are dealt to
 //                       buckets, id modulo their number (a power of two): frequent tokens tend
 //                       to have low ids, which ranges of ids would put into one bucket. Each bucket's
@@ -29,6 +30,7 @@
 #include "eg_common.hpp"
 
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 namespace eg {
@@ -42,6 +44,7 @@ constexpr int kSumThreads = 256, kFewestLanes = 16, kMostGroups = kSumThreads / 
 constexpr int kSingly = 4;      // ids of 64 positions that are placed one by one
 constexpr int kEarlyPacks = 2;  // of 16 bytes, per thread
 constexpr int kAhead = 8;       // loads of a thread on their way at once
+constexpr int kFewTokens = 256, kFewThreads = 512, kFewLanes = 128;
 constexpr int kJoinLanes = 64, kJoinAdders = 8, kJoinThreads = kJoinLanes * kJoinAdders;
 constexpr int kJoinParts = 4;  // workgroups that share a piece's columns, at most
 constexpr int kZeroPacks = 2;  // per thread
@@ -409,6 +412,101 @@ __global__ __launch_bounds__(kJoinThreads) void embed_join_kernel(EmbedArgs a, i
   }
 }
 
+// All of it for few tokens: a workgroup of a bucket and a block of columns finds the bucket's tokens
+// (one a thread), orders them by counting those before each, adds their rows and writes the rows
+// without tokens. `lanes` threads (a power of two) hold the columns; each group of them adds a piece
+// of the order, and the runs that cross pieces are joined through LDS.
+template <typename T, int VEC, bool RAG, typename ID>
+__global__ __launch_bounds__(kFewThreads) void embed_few_kernel(EmbedArgs a, int lanes, int column_blocks) {
+  __shared__ int ids[kFewTokens], order[kFewTokens];
+  __shared__ __align__(16) int found[kFewTokens + 4];  // (place in the bucket, which of its tokens)
+  __shared__ unsigned used[kBucketIds / 32], waves[kFewThreads / kWave];
+  __shared__ Pack<float, VEC> part[2][kFewThreads];  // as embed_sum_kernel's partial rows
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const unsigned bucket = blockIdx.x / column_blocks, mask = (1u << a.shift) - 1;
+  const int64_t id = t < a.tokens ? (int64_t)((const ID*)a.ids)[t] : -1;
+  const bool in = id >= 0 && id < a.vocab && id != a.ignore_index && ((unsigned)id & mask) == bucket;
+  const int local = (int)((unsigned)id >> a.shift);  // its place in the bucket
+  const uint64_t here = __ballot(in);
+  if (lane == 0) waves[wave] = __popcll(here);
+  if (t < kBucketIds / 32) used[t] = 0;
+  __syncthreads();
+  int n = 0, mine = 0;  // the bucket's tokens; those before this one
+  for (int w = 0; w < kFewThreads / kWave; ++w) {
+    if (w == wave) mine = n;
+    n += waves[w];
+  }
+  mine += __popcll(here & ((1ull << lane) - 1));
+  if (in) {
+    found[mine] = local * kFewTokens + mine;
+    atomicOr(&used[local / 32], 1u << local % 32);
+  }
+  if (t < 4) found[n + t] = INT_MAX;
+  __syncthreads();
+  const int groups = kFewThreads / lanes, group = t / lanes;
+  const int pack = blockIdx.x % column_blocks * lanes + (t & (lanes - 1));
+  const bool live = pack * VEC < a.hidden;
+  const RowAt<T, VEC, RAG> at(live ? pack : 0, a.hidden);
+  if (live && !a.accumulate) {
+    const float zero[VEC] = {};
+    const int rows = (int)((a.vocab - bucket + mask) >> a.shift);  // of the bucket
+    for (int r = group; r < rows; r += groups)
+      if (!(used[r / 32] >> r % 32 & 1))
+        at.store((T*)a.dweight + ((int64_t)r << a.shift | bucket) * a.hidden, zero);
+  }
+  if (n == 0) return;
+  if (in) {
+    int before = 0;
+    const int own = local * kFewTokens + mine;
+    for (int j = 0; j < n; j += 4) {
+      int other[4];
+      *(Pack<int, 4>*)other = *(const Pack<int, 4>*)(found + j);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) before += other[i] < own;
+    }
+    order[before] = t, ids[before] = (int)id;
+  }
+  __syncthreads();
+  const int piece = (n + groups - 1) / groups, from = min(group * piece, n), to = min(from + piece, n);
+  if (live && from < to) {
+    bool crosses = from > 0 && ids[from - 1] == ids[from];
+    float acc[VEC] = {};
+    for (int e0 = from; e0 < to; e0 += kAhead) {
+      Pack<T, VEC> x[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (e0 + u < to) x[u] = at.load((const T*)a.dout + (int64_t)order[e0 + u] * a.hidden);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int e = e0 + u;
+        if (e >= to) break;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] += to_f32(x[u].v[i]);
+        const bool last = e + 1 == n || ids[e + 1] != ids[e];
+        if (!last && e + 1 < to) continue;
+        if (last && !crosses) write_row(a, at, ids[e], acc);
+        else store_f32<float, VEC>(part[!crosses][t].v, acc);
+        crosses = false;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
+      }
+    }
+  }
+  __syncthreads();
+  // the run that begins in this piece and goes on behind it
+  if (!live || from >= to || to == n || ids[to] != ids[to - 1]) return;
+  const int id_out = ids[to - 1];
+  if (from > 0 && ids[from - 1] == id_out) return;  // it began in an earlier piece
+  float s[VEC];
+  load_f32<float, VEC>(part[1][t].v, s);
+  for (int g = group + 1; g * piece < n && ids[g * piece] == id_out; ++g) {
+    const Pack<float, VEC>& other = part[0][g * lanes + (t & (lanes - 1))];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) s[i] += other.v[i];
+  }
+  write_row(a, at, id_out, s);
+}
+
 // Tokens of a piece: a piece's rows are added one after the other, its partial rows are read again.
 // Backward, us, with 8 / 16 / 32: 700 tokens of [5003, 768] fp32 15.2 / 16.8 / 19.9; 4096 of [32000,
 // 1024] bf16 28.0 / 29.0 / 33.5; 8191 of [50257, 1538] fp16 59.7 / 55.9 / 57.7; 16384 of [128256,
@@ -420,6 +518,18 @@ int piece_for(int64_t tokens) { return tokens < 4096 ? 8 : tokens < 16384 ? 16 :
 // of [128256, 2048] 97 / 91 / 90, 65536 of [50257, 768] 83 / 79 / 75, 700 of [5003, 768] fp32 15 /
 // 14 / 14.
 int64_t early_bytes(int64_t tokens) { return ((int64_t)32 << 20) + tokens * 3500; }
+
+// One launch for few tokens. It leaves HBM idle under its ordering, and its zeros of rows that are
+// not whole packs are slower, which a large table outweighs. Backward, us, three launches / one: 1
+// token of [5003, 768] fp32 10.8 / 5.2; 32 of [32000, 1024] bf16 18.4 / 11.8; 256 of [1000, 4096],
+// a third of them one id, 16.0 / 11.9 and 512 of those 17.3 / 19.0; 256 equal ones of [1, 4096] 16.9
+// / 21; 128 of [48000, 1024] bf16 23.4 / 17.8, of [30000, 4096] 43 / 46; rows in ragged packs, 128 of
+// [20000, 1538] fp16 (62 MB) 19.8 / 18.6, of [50257, 770] (77 MB) 22.4 / 25.5; more than kBucketIds
+// 2^8 ids, 4000000 of 8: 87 / 157. Added into a table, 128 of [30000, 4096] 12.1 / 4.9.
+bool few_tokens(int64_t tokens, int64_t vocab, int64_t bytes, bool accumulate, bool ragged) {
+  if (tokens > kFewTokens) return false;
+  return accumulate || (vocab <= kBucketIds << 8 && bytes <= (int64_t)(ragged ? 64 : 96) << 20);
+}
 
 // A table [vocab, hidden] with `tokens` of it: how the ids are dealt and where the order lies.
 struct Layout {
@@ -530,10 +640,22 @@ extern "C" int eg_embedding_bwd(const void* dout, const void* ids, int ids_64, v
     return by_width<scalar_t>(a.hidden, {dout, (const void*)dweight}, [&](auto vec, auto rag) -> int {
       using T = scalar_t;
       constexpr int V = decltype(vec)::value, W = 16 / (int)sizeof(T);
-      const int64_t packs = (hidden + V - 1) / V;
+      const int64_t packs = (hidden + V - 1) / V, bytes = vocab * hidden * (int64_t)sizeof(T);
       const int lanes = lanes_for(packs, kSumThreads), groups = kSumThreads / lanes;
       const int64_t columns = (packs + lanes - 1) / lanes;
       const int64_t sums = (l.pieces + groups - 1) / groups * columns;
+      if (few_tokens(tokens, vocab, bytes, accumulate, decltype(rag)::value)) {
+        const int wide = lanes_for(packs, kFewLanes);
+        const int64_t blocks = (packs + wide - 1) / wide, grid = blocks << l.shift;
+        if (check_grid(name, grid, kFewThreads)) return 1;
+        auto few = [&](auto id) {
+          EG_LAUNCH((embed_few_kernel<T, V, decltype(rag)::value, decltype(id)>), dim3((unsigned)grid),
+                    dim3(kFewThreads), 0, st, a, wide, (int)blocks);
+        };
+        if (ids_64) few(int64_t{});
+        else few(int{});
+        return check_launch(name);
+      }
       // the join in fours or twos of columns where a row's are aligned, zeros in whole packs (8191
       // tokens of [50257, 1538] fp16, a third of them one: 44 us in single columns, 40 in twos)
       const bool flat = aligned16(dweight);
@@ -542,7 +664,7 @@ extern "C" int eg_embedding_bwd(const void* dout, const void* ids, int ids_64, v
       const int parts = (int)std::min<int64_t>((hidden + span - 1) / span, kJoinParts);
       const int64_t joins = l.pieces > 1 ? (l.pieces - 1) * parts : 0;
       const int64_t chunk = (int64_t)kJoinThreads * kZeroPacks * (flat ? W : 1);
-      const int64_t bytes = vocab * hidden * (int64_t)sizeof(T), at_once = kSortThreads * kEarlyPacks * 16;
+      const int64_t at_once = kSortThreads * kEarlyPacks * 16;
       const int64_t early = accumulate || !flat ? 0 : std::min(early_bytes(tokens), bytes) / at_once;
       a.early = early * at_once;
       const int64_t zeros =

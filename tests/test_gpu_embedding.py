@@ -221,3 +221,63 @@ def test_a_captured_graph_replays_with_other_tokens():
         got = out.clone(), grad.clone()
         for x, y in zip(got, both_ways(weight, ids, dout)):
             assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", (BF16, F16, F32))
+@pytest.mark.parametrize("T", (1, 2, 9, 64, 255, 256, 257))
+def test_few_tokens(T, dtype):
+    """Around the limit of the single launch: runs over its pieces, buckets of many tokens."""
+    for V, H, how in ((1, 520, "flat"), (2, 2056, "flat"), (300, 33, "mixed"), (5000, 1100, "low"),
+                      (70000, 24, "strided"), (262144, 40, "flat"), (262145, 40, "low")):
+        print(f"\n[gpu-embedding] few {T} {V}x{H} {how} {dtype}", flush=True)
+        strided = how == "strided"  # in one bucket, whatever their number below 256 is
+        ids = tokens(T, 6).long() * 256 + 3 if strided else tokens(T, V, how, dtype=torch.int64)
+        weight, dout = normal(V, H, dtype=dtype), normal(T, H, dtype=dtype, seed=1)
+        _, grad = both_ways(weight, ids, dout, 0.75)
+        want, bound = embedding64(weight, ids, 0.75, -100, dout)[1]
+        assert_within("dweight", grad, want, bound)
+        assert torch.equal(grad, both_ways(weight, ids.int(), dout, 0.75)[1])
+        old = normal(V, H, dtype=dtype, seed=4)
+        _, saved = pair.embedding_forward_with_saved(weight, ids)
+        got = pair.embedding_backward_into(old.clone(), dout, saved, 0.75)
+        total = old.double() + want
+        room = bound + (2.0 ** -24 + torch.finfo(dtype).eps / 2) * total.abs()
+        used = torch.zeros(V, dtype=torch.bool, device="cuda")
+        used[ids[ids >= 0]] = True
+        assert_within("into", got[used], total[used], room[used])
+        assert torch.equal(got[~used], old[~used])
+
+
+def test_few_tokens_added_past_32_bit_offsets():
+    V, H = 540000, 4096  # 2.2e9 elements
+    grad = torch.zeros(V, H, dtype=BF16, device="cuda")
+    ids = torch.tensor([V - 1, 0, 525000, V - 1, 3], dtype=torch.int32, device="cuda")
+    dout = normal(5, H, dtype=BF16, seed=1)
+    saved = (ids, V, H, BF16)
+    pair.embedding_backward_into(grad, dout, saved)
+    assert torch.equal(grad[V - 1], (dout[0].float() + dout[3].float()).to(BF16))
+    for t in (1, 2, 4):
+        assert torch.equal(grad[int(ids[t])], dout[t])
+    assert int(torch.count_nonzero(grad)) == sum(
+        int(torch.count_nonzero(grad[v])) for v in (V - 1, 0, 525000, 3))
+
+
+def test_a_captured_graph_of_few_tokens():
+    T, V, H = 200, 128, 72
+    dout, ids, table = normal(T, H, dtype=BF16, seed=1), tokens(T, V), normal(V, H, dtype=BF16)
+    saved, into = (ids, V, H, BF16), table.clone()
+    pair.embedding_backward_into(into, dout, saved)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grad = pair.embedding_backward_from_saved(dout, saved)
+        pair.embedding_backward_into(into, dout, saved)
+    for seed, how in enumerate(("flat", "same", "mixed", "low")):
+        ids.copy_(tokens(T, V, how, seed))
+        dout.copy_(normal(T, H, dtype=BF16, seed=10 + seed))
+        into.copy_(table)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = grad.clone(), into.clone()
+        assert torch.equal(got[0], pair.embedding_backward_from_saved(dout, saved))
+        assert torch.equal(got[1], pair.embedding_backward_into(table.clone(), dout, saved))

@@ -541,9 +541,9 @@ int eg_embedding_fwd(const void* weight, const void* ids, int ids_64, void* out,
 size_t eg_embedding_workspace_bytes(int64_t tokens, int64_t vocab, int64_t hidden);
 
 /* Its gradient: dweight[v] = scale * sum of dout[t] over the tokens with ids[t] == v, fp32 sums in
- * an order that depends on the ids alone, one rounding; every row is written. accumulate: added
- * to dweight instead, where the rows of ids without a token are neither read nor written. The
- * workspace is 16-byte aligned. */
+ * an order that the ids, the sizes and the tensors' alignment fix, one rounding; every row is
+ * written. accumulate: added to dweight instead, where the rows of ids without a token are neither
+ * read nor written. The workspace is 16-byte aligned, dweight overlaps no input. */
 int eg_embedding_bwd(const void* dout, const void* ids, int ids_64, void* dweight,
                      void* workspace, int64_t tokens, int64_t vocab, int64_t hidden, float scale,
                      int64_t ignore_index, int accumulate, int dtype, void* stream);

@@ -281,3 +281,13 @@ def test_a_captured_graph_of_few_tokens():
         got = grad.clone(), into.clone()
         assert torch.equal(got[0], pair.embedding_backward_from_saved(dout, saved))
         assert torch.equal(got[1], pair.embedding_backward_into(table.clone(), dout, saved))
+
+
+@pytest.mark.parametrize("T,V,H", ((3, 5, 2 ** 20), (300, 5, 2 ** 20), (2, 3, 2 ** 20 - 1)))
+def test_the_widest_rows(T, V, H):
+    print(f"\n[gpu-embedding] widest {T} {V}x{H}", flush=True)
+    weight, dout, ids = normal(V, H, dtype=BF16), normal(T, H, dtype=BF16, seed=1), tokens(T, V - 1)
+    out, grad = both_ways(weight, ids, dout, 0.5)
+    (value, bound), (gvalue, gbound) = embedding64(weight, ids, 0.5, -100, dout)
+    assert_within("out", out, value, bound)
+    assert_within("dweight", grad, gvalue, gbound)

@@ -277,3 +277,21 @@ def test_two_graphs_with_a_workspace_each():
         torch.cuda.synchronize()
         for got, ref in zip(outs, want):
             assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
+
+
+@pytest.mark.parametrize("dtype", (BF16, F32))
+@pytest.mark.parametrize("T,H,KVH,D,pairs", ((3, 2, 1, 8192, 4096), (2, 1, 1, 8191, 4095),
+                                             (2, 65536, 1, 2, 1), (2, 300, 65536, 16, 4)))
+def test_the_widest_and_the_most_heads(T, H, KVH, D, pairs, dtype):
+    print(f"\n[gpu-norm-rotary] largest {T} {H}/{KVH} D={D} {dtype}", flush=True)
+    q, k, dq, dk = (make(T, h, D, dtype=dtype, seed=i) for i, h in enumerate((H, KVH, H, KVH)))
+    qw, kw = gain(D, dtype, 7), gain(D, dtype, 8)
+    pos, freqs = spots(T, 5000), turns(pairs)
+    for interleaved in (0, 1):
+        outs, saved = pair.norm_rotary_qk_forward_with_saved(q, k, qw, kw, pos, freqs, EPS, 1.0,
+                                                             interleaved)
+        grads = pair.norm_rotary_qk_backward_from_saved((dq, dk), saved, EPS, 1.0, interleaved)
+        for i, (x, w, dy) in enumerate(((q, qw, dq), (k, kw, dk))):
+            want = norm_rotary64(x, w, pos, freqs, EPS, 1.0, interleaved, dy)
+            for name, got in (("y", outs[i]), ("dx", grads[i]), ("dweight", grads[2 + i])):
+                assert_within(f"{'qk'[i]} {name}", got, *want[name])

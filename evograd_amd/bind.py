@@ -19,7 +19,8 @@ order, scalar defaults, gradient slots). One module-level
 ``torch.autograd.Function`` serves every bound pair; the pair and its plan ride
 into it as the first, non-tensor argument. Saved state is split into the tensor
 list autograd keeps (``save_for_backward``) and a mask of which positions held
-tensors, so the backward gets back exactly the tuple the forward built.
+tensors, so the backward gets back exactly the tuple the forward built. Gradients without a
+graph of their own can be differentiated once (``once.py``).
 """
 
 from __future__ import annotations
@@ -29,6 +30,7 @@ from dataclasses import dataclass
 
 import torch
 
+from .once import needs_tie, once, tie
 from .opdecl import Active, OpDecl
 
 _GENERIC = ("forward_with_saved", "backward_from_saved")
@@ -134,7 +136,7 @@ class _Binding:
     plan: CallPlan
     forward: object
     backward: object
-    scalars_for_backward: tuple   # scalar names the backward accepts
+    scalars_for_backward: tuple   # scalars the backward accepts: (name, argument index)
 
 
 class _PairFunction(torch.autograd.Function):
@@ -145,21 +147,23 @@ class _PairFunction(torch.autograd.Function):
         y, saved = binding.forward(*args)
         saved = tuple(saved) if isinstance(saved, (tuple, list)) else (saved,)
         mask = tuple(torch.is_tensor(item) for item in saved)
-        ctx.save_for_backward(*(item for item, is_t in zip(saved, mask) if is_t))
+        tensors = [item for item, is_t in zip(saved, mask) if is_t]
+        ties = (tie(),) if needs_tie(args, tensors, (y,)) else ()
+        ctx.save_for_backward(*tensors, *ties)
         ctx.plain = tuple(None if is_t else item for item, is_t in zip(saved, mask))
         ctx.mask = mask
         ctx.binding = binding
-        by_name = dict(zip(binding.plan.names, args))
-        ctx.scalars = {n: by_name[n] for n in binding.scalars_for_backward}
-        return y
+        ctx.scalars = {n: args[i] for n, i in binding.scalars_for_backward}
+        return (y, *ties) if ties else y
 
     @staticmethod
-    def backward(ctx, dy):
-        tensors = iter(ctx.saved_tensors)
+    def backward(ctx, dy, *_):
+        kept = ctx.saved_tensors
+        tensors = iter(kept)
         saved = tuple(next(tensors) if is_t else plain for is_t, plain in zip(ctx.mask, ctx.plain))
         binding = ctx.binding
         grads = binding.backward(dy.contiguous(), saved, **ctx.scalars)
-        return (None, *binding.plan.scatter(grads))
+        return (None, *binding.plan.scatter(once(binding.plan.op.name, grads, (dy, *kept))))
 
 
 def bind(op: OpDecl, module):
@@ -167,10 +171,12 @@ def bind(op: OpDecl, module):
     fwd, bwd = lookup_pair(op, module)
     plan = CallPlan.of(op)
     accepted = backward_inactive_kwargs(op, bwd, {})
-    binding = _Binding(plan, fwd, bwd, tuple(n for n in plan.scalar_names if n in accepted))
+    binding = _Binding(plan, fwd, bwd, tuple((n, plan.names.index(n)) for n in plan.scalar_names
+                                             if n in accepted))
 
     def call(*args, **kwargs):
-        return _PairFunction.apply(binding, *plan.arrange(args, kwargs).values())
+        out = _PairFunction.apply(binding, *plan.arrange(args, kwargs).values())
+        return out[0] if type(out) is tuple else out
 
     call.__name__ = call.__qualname__ = f"{op.name}_bound"
     call.plan = plan

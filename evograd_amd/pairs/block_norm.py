@@ -33,9 +33,9 @@ if not __package__:
         _sys.path.insert(0, _ROOT)
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from evograd_amd import _lib
+from evograd_amd.once import needs_tie, once, tie
 from evograd_amd.pairs._util import as_contiguous, check_same, tag, workspace
 
 _NONE, _CHANNEL, _ROW, _ELEMENT = range(4)
@@ -123,20 +123,24 @@ def block_norm_backward_from_saved(dout, saved, scale: float = 1.0):
 class BlockNorm(torch.autograd.Function):
     """``BlockNorm.apply(x, h, post_weight, gate, pre_weight, scale, eps)`` -> ``(s, y)``."""
 
+    @classmethod
+    def apply(cls, *args):
+        return super().apply(*args)[:2]
+
     @staticmethod
     def forward(ctx, x, h, post_weight, gate, pre_weight, scale=1.0, eps=1e-6):
         args = _prepare("BlockNorm", x, h, post_weight, gate, pre_weight)
         s, y = torch.empty_like(args[0]), torch.empty_like(args[0])
-        saved = _forward(s, y, *args, scale, eps)
+        saved = [t for t in _forward(s, y, *args, scale, eps) if t is not None]
+        ties = (tie(),) if needs_tie((x, h, post_weight, gate, pre_weight), saved, (s, y)) else ()
         ctx.has_gate = gate is not None
-        ctx.save_for_backward(*(t for t in saved if t is not None))
+        ctx.save_for_backward(*saved, *ties)
         ctx.scale = scale
-        return s, y
+        return (s, y, *ties)
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, ds, dy):
-        saved = ctx.saved_tensors
-        if not ctx.has_gate:
-            saved = (*saved[:3], None, *saved[3:])
-        return (*block_norm_backward_from_saved((ds, dy), saved, ctx.scale), None, None)
+    def backward(ctx, ds, dy, *_):
+        kept = ctx.saved_tensors
+        saved = kept[:6] if ctx.has_gate else (*kept[:3], None, *kept[3:5])
+        grads = block_norm_backward_from_saved((ds, dy), saved, ctx.scale)
+        return (*once("BlockNorm", grads, (ds, dy, *kept)), None, None)

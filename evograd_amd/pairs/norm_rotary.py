@@ -31,9 +31,9 @@ if not __package__:
 import struct
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from evograd_amd import _lib
+from evograd_amd.once import needs_tie, once, tie
 from evograd_amd.pairs._util import (MAX_HEAD_STRIDE, MAX_TOKEN_STRIDE, as_contiguous, check_same,
                                      head_rows, tag, workspace)
 from evograd_amd.pairs.rotary import _check as _check_positions
@@ -176,18 +176,22 @@ class NormRotaryQK(torch.autograd.Function):
     positions, freqs, eps, amplitude, interleaved)`` -> ``(q', k')``; positions and frequencies
     get no gradient, and the node can be differentiated once."""
 
+    @classmethod
+    def apply(cls, *args):
+        return super().apply(*args)[:2]
+
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, positions, freqs, eps=1e-6, amplitude=1.0,
                 interleaved=0):
         out, saved = norm_rotary_qk_forward_with_saved(q, k, q_weight, k_weight, positions, freqs,
                                                        eps, amplitude, interleaved)
-        ctx.save_for_backward(*saved)
+        ties = (tie(),) if needs_tie((q, k, q_weight, k_weight), saved, out) else ()
+        ctx.save_for_backward(*saved, *ties)
         ctx.scalars = (eps, amplitude, interleaved)
-        return out
+        return (*out, *ties)
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, dq_out, dk_out):
-        grads = norm_rotary_qk_backward_from_saved((dq_out, dk_out), ctx.saved_tensors,
-                                                   *ctx.scalars)
-        return (*grads, None, None, None, None, None)
+    def backward(ctx, dq_out, dk_out, *_):
+        kept = ctx.saved_tensors
+        grads = norm_rotary_qk_backward_from_saved((dq_out, dk_out), kept[:6], *ctx.scalars)
+        return (*once("NormRotaryQK", grads, (dq_out, dk_out, *kept)), None, None, None, None, None)

@@ -25,6 +25,7 @@ if not __package__:
 import torch
 
 from evograd_amd import _lib
+from evograd_amd.once import once
 from evograd_amd.pairs._util import as_contiguous, tag
 
 
@@ -89,7 +90,7 @@ def rope_qk_forward_with_saved(q: torch.Tensor, k: torch.Tensor, cos: torch.Tens
 
 class RopeQK(torch.autograd.Function):
     """The joint q/k pair as an autograd node: ``RopeQK.apply(q, k, cos, sin)`` ->
-    ``(q', k')``; the tables get no gradient."""
+    ``(q', k')``; the tables get no gradient, and the node can be differentiated once."""
 
     @staticmethod
     def forward(ctx, q, k, cos, sin):
@@ -99,8 +100,8 @@ class RopeQK(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dq_out, dk_out):
-        dq, dk = rope_qk_backward_from_saved((dq_out, dk_out), ctx.saved_tensors)
-        return dq, dk, None, None
+        grads = rope_qk_backward_from_saved((dq_out, dk_out), ctx.saved_tensors)
+        return (*once("RopeQK", grads, (dq_out, dk_out)), None, None)
 
 
 def rope_qk_backward_from_saved(grads, saved):

@@ -5,8 +5,8 @@ import torch
 
 from evograd_amd import _lib, decls
 from evograd_amd.bind import bind
-from evograd_amd.pairs import (cross_entropy, embedding, layernorm, norm_rotary, rmsnorm, rotary,
-                               softmax, topk_distillation)
+from evograd_amd.pairs import (block_norm, cross_entropy, embedding, layernorm, norm_rotary, rmsnorm,
+                               rope, rotary, softmax, topk_distillation)
 from tests import stub_pairs
 
 
@@ -116,3 +116,38 @@ def test_a_tie_holds_no_argument(no_kernels):
     y = bind(decls.LAYERNORM, layernorm)(part, torch.ones(8), torch.zeros(8))
     del part
     assert kept() is None and y.requires_grad
+
+
+def node(name, strided):
+    """Leaves, and a joint node's two outputs (RopeQK, RotaryQK, NormRotaryQK, BlockNorm)."""
+    shapes = {"BlockNorm": ((4, 8), (4, 8), (8,), (8,), (8,)),
+              "NormRotaryQK": ((4, 2, 8), (4, 1, 8), (8,), (8,)),
+              "RotaryQK": ((4, 2, 8), (4, 1, 8)), "RopeQK": ((1, 2, 4, 8), (1, 1, 4, 8))}[name]
+    leaves = [torch.zeros(s, requires_grad=True) for s in shapes]
+    args = [t.repeat_interleave(2, -1)[..., ::2] for t in leaves] if strided else leaves
+    if name == "BlockNorm":
+        return leaves, block_norm.BlockNorm.apply(*args, 1.0, 1e-6)
+    if name == "RopeQK":
+        return leaves, rope.RopeQK.apply(*args, torch.ones(4, 8), torch.ones(4, 8))
+    return leaves, getattr(norm_rotary if name[0] == "N" else rotary, name).apply(*args, POS, FREQ)
+
+
+@pytest.mark.parametrize("strided", (False, True))
+@pytest.mark.parametrize("name", ("BlockNorm", "NormRotaryQK", "RotaryQK", "RopeQK"))
+def test_joint_nodes_refuse_the_same(no_kernels, name, strided):
+    leaves, out = node(name, strided)
+    assert len(out) == 2
+    for constant in (False, True):  # upstream gradients
+        loss = sum((t if constant else t * t).sum() for t in out)
+        grads = torch.autograd.grad(loss, leaves, create_graph=True)
+        if constant and name in ("RotaryQK", "RopeQK"):  # linear: their gradients are constants
+            assert strided or not any(g.requires_grad for g in grads)
+            continue
+        for g in grads:
+            with pytest.raises(RuntimeError, match=f"{name}.*differentiate twice"):
+                torch.autograd.grad(g.sum() + leaves[0].sum(), leaves[0], retain_graph=True)
+            with pytest.raises(RuntimeError, match="differentiate twice"):
+                (g.sum() + leaves[0].sum()).backward(retain_graph=True)
+    leaves, out = node(name, strided)
+    (out[0].sum() + out[1].sum()).backward()
+    assert all(t.grad.shape == t.shape and not t.grad.requires_grad for t in leaves)

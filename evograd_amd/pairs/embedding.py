@@ -69,6 +69,9 @@ def _backward(name, dweight, dout, saved, scale, ignore_index):
                              f"{tuple(dweight.shape)} of {dweight.dtype}")
         if not dweight.is_contiguous():
             raise ValueError(f"{name}: dweight must be contiguous")
+        if dweight.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{name}: dweight requires gradients, and what is added in place has "
+                               "none; use torch.no_grad()")
     else:
         dweight = dout.new_empty((vocab, hidden))
     dout, ids = as_contiguous("dout", dout), as_contiguous("ids", ids)
@@ -77,6 +80,8 @@ def _backward(name, dweight, dout, saved, scale, ignore_index):
     _lib.call_on(dout, "eg_embedding_bwd", dout.data_ptr(), ids.data_ptr(),
                  ids.dtype == torch.int64, dweight.data_ptr(), ws.data_ptr(), ids.numel(), vocab,
                  hidden, scale, ignore_index, add, dtype, _lib.stream_of(dout))
+    if add:  # autograd sees a change through a pointer no other way
+        torch.autograd.graph.increment_version(dweight)
     return dweight
 
 
@@ -87,6 +92,8 @@ def embedding_backward_from_saved(dout: torch.Tensor, saved, scale: float = 1.0,
 
 def embedding_backward_into(dweight: torch.Tensor, dout: torch.Tensor, saved, scale: float = 1.0,
                             ignore_index: int = -100):
-    """``dweight += `` the gradient, in place; returns dweight."""
+    """``dweight += `` the gradient, in place; returns dweight, whose version moves on as in any
+    in-place operation. dweight overlaps neither dout nor the ids, and where gradients are
+    recorded it may not require any."""
     _lib.require_gpu("embedding_backward_into", dweight)
     return _backward("embedding_backward_into", dweight, dout, saved, scale, ignore_index)

@@ -236,3 +236,33 @@ def test_gradients_of_gradients_are_refused(no_kernels):
 def test_the_embedding_keeps_no_table(no_kernels):
     _, saved = embedding.embedding_forward_with_saved(W, IDS)
     assert saved[0] is IDS and saved[1:] == (6, 8, torch.float32)
+
+
+def test_a_gradient_added_in_place_is_a_change_that_autograd_sees(no_kernels):
+    """A node that saved the tensor before notices, and so does one that saved a view of it."""
+    dout, saved = torch.zeros(4, 8), (IDS, 6, 8, torch.float32)
+    flat = torch.zeros(48)
+    for held, target in ((flat, flat.view(6, 8)), (flat.view(6, 8), flat.view(6, 8))):
+        version = held._version
+        y = torch.zeros(held.shape, requires_grad=True) * held
+        assert embedding.embedding_backward_into(target, dout, saved) is target
+        assert held._version == version + 1
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+    version = dout._version
+    embedding.embedding_backward_from_saved(dout, saved)
+    assert dout._version == version
+
+
+def test_a_gradient_is_not_added_to_what_requires_gradients(no_kernels):
+    leaf, dout, saved = torch.zeros(6, 8, requires_grad=True), torch.zeros(4, 8), (IDS, 6, 8, torch.float32)
+    into = embedding.embedding_backward_into
+    for bad in (leaf, leaf * 1.0):
+        with pytest.raises(RuntimeError, match="requires gradients"):
+            into(bad, dout, saved)
+    with torch.no_grad():
+        assert into(leaf, dout, saved) is leaf
+    leaf.grad = torch.zeros(6, 8)
+    into(leaf.grad, dout, saved)
+    with torch.inference_mode():
+        into(torch.zeros(6, 8), dout, saved)

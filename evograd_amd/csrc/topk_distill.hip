@@ -48,7 +48,8 @@ constexpr int64_t kFewRows = 16;
 // / 256 threads: bf16 [8192, 128256] with one exponential 308 / 309 / 308, a squared one 330 / 309 /
 // 314, two 366 / 338 / 336, 16 rows 11.4 / 11.8 / 11.6; with 512 threads at 8 / 4 / 2 packs: 316 / 313
 // / 305, 328 / 315 / 308, 362 / 344 / 338.
-constexpr int kMostRow = 512, kUnroll = 2;
+// A narrower row takes the smallest workgroup that walks it in kRowSteps.
+constexpr int kMostRow = 512, kUnroll = 2, kRowSteps = 2;
 // The backward's workgroup (bf16 [8192, 128256], us: 512 threads 671, 256 655, 128 652 but 814 with 256
 // entries a row for 690, 256 of four packs 788).
 constexpr int kFlatBlock = 256, kFlatUnroll = 2, kFlatPer = kFlatBlock * kFlatUnroll;
@@ -543,8 +544,11 @@ extern "C" int eg_topk_distill_fwd(const void* logits, const int64_t* target, co
           constexpr int V = decltype(vec)::value;
           const int64_t packs = ((cols + V - 1) / V + a.splits - 1) / a.splits;
           RowLaunch<T, V, decltype(rag)::value, decltype(e)::value> row{a, st};
-          if (packs > kMostRow * rowwise::kUnroll) row.template go<kMostRow>();
-          else rowwise::pick_row_block(packs, row);
+          const int64_t threads = (packs + kUnroll * kRowSteps - 1) / (kUnroll * kRowSteps);
+          if (threads <= 64) row.template go<64>();
+          else if (threads <= 128) row.template go<128>();
+          else if (threads <= 256) row.template go<256>();
+          else row.template go<kMostRow>();
           return 0;
         });
       });

@@ -295,3 +295,48 @@ def test_the_widest_and_the_most_heads(T, H, KVH, D, pairs, dtype):
             want = norm_rotary64(x, w, pos, freqs, EPS, 1.0, interleaved, dy)
             for name, got in (("y", outs[i]), ("dx", grads[i]), ("dweight", grads[2 + i])):
                 assert_within(f"{'qk'[i]} {name}", got, *want[name])
+
+
+# Shapes whose walk takes several steps: tokens past those that the resident workgroups hold at once.
+@pytest.mark.parametrize("dtype", (BF16, F16, F32))
+@pytest.mark.parametrize("interleaved", (0, 1))
+@pytest.mark.parametrize("T,H,KVH,D,pairs", (
+    (40001, 4, 1, 64, 32),    # 8 or 16 tokens a workgroup
+    (4001, 16, 16, 128, 64),  # a token, 3 steps forward and 8 backward
+    (20003, 3, 2, 96, 24),    # columns that are not turned, lanes without columns
+    (40001, 12, 2, 64, 32),   # more than 64 MB: the streaming form
+    (70001, 1, 1, 10, 3),     # single columns
+    (9001, 40, 9, 64, 16),    # tokens that share workgroups of no whole number of them
+    (3001, 300, 2, 32, 8)))   # several workgroups a token
+def test_walks_of_several_steps(T, H, KVH, D, pairs, interleaved, dtype):
+    print(f"\n[gpu-norm-rotary] walk {T} {H}/{KVH} D={D} pairs={pairs} {interleaved} {dtype}", flush=True)
+    q, k, dq, dk = (make(T, h, D, dtype=dtype, seed=i) for i, h in enumerate((H, KVH, H, KVH)))
+    qw, kw = gain(D, dtype, 7), gain(D, dtype, 8)
+    pos, freqs = spots(T, 131072), turns(pairs)
+    outs, saved = pair.norm_rotary_qk_forward_with_saved(q, k, qw, kw, pos, freqs, EPS, 1.25, interleaved)
+    grads = pair.norm_rotary_qk_backward_from_saved((dq, dk), saved, EPS, 1.25, interleaved)
+    for i, (x, w, dy) in enumerate(((q, qw, dq), (k, kw, dk))):
+        want = norm_rotary64(x, w, pos, freqs, EPS, 1.25, interleaved, dy)
+        for name, got in (("y", outs[i]), ("dx", grads[i]), ("dweight", grads[2 + i])):
+            assert_within(f"{'qk'[i]} {name}", got, *want[name])
+    again = pair.norm_rotary_qk_backward_from_saved((dq, dk), saved, EPS, 1.25, interleaved)
+    for a, b in zip(grads, again):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", (BF16, F32))
+@pytest.mark.parametrize("interleaved", (0, 1))
+@pytest.mark.parametrize("T,H,KVH,D,pairs", ((2100, 2, 1, 514, 257), (3000, 1, 2, 130, 65),
+                                             (1500, 2, 3, 259, 65)))
+def test_a_wave_with_several_heads(T, H, KVH, D, pairs, interleaved, dtype):
+    """Heads of more than 64 lanes, more of them than the 2048 waves: q's and k's in one wave."""
+    print(f"\n[gpu-norm-rotary] wide {T} {H}/{KVH} D={D} pairs={pairs} {interleaved} {dtype}", flush=True)
+    q, k, dq, dk = (make(T, h, D, dtype=dtype, seed=i) for i, h in enumerate((H, KVH, H, KVH)))
+    qw, kw = gain(D, dtype, 7), gain(D, dtype, 8)
+    pos, freqs = spots(T, 131072), turns(pairs)
+    outs, saved = pair.norm_rotary_qk_forward_with_saved(q, k, qw, kw, pos, freqs, EPS, 0.75, interleaved)
+    grads = pair.norm_rotary_qk_backward_from_saved((dq, dk), saved, EPS, 0.75, interleaved)
+    for i, (x, w, dy) in enumerate(((q, qw, dq), (k, kw, dk))):
+        want = norm_rotary64(x, w, pos, freqs, EPS, 0.75, interleaved, dy)
+        for name, got in (("y", outs[i]), ("dx", grads[i]), ("dweight", grads[2 + i])):
+            assert_within(f"{'qk'[i]} {name}", got, *want[name])

@@ -286,3 +286,15 @@ def test_logits_past_32_bit_offsets():
     assert_within("loss", loss, *want[0])
     assert_within("dlogits", grad[rows - 2:], *want[1])
     assert not bool(grad[:rows - 2].any())
+
+
+@pytest.mark.parametrize("dtype", (BF16, F16, F32))
+@pytest.mark.parametrize("tau,soft,hard", ((1.5, 0.7, 0.3), (4.0, 1.0, 0.5), (0.5, 0.25, 1.0)))
+@pytest.mark.parametrize("rows,cols,K", (
+    (1, 1, 1), (2, 3, 2), (9, 64, 5), (33, 100, 100), (700, 40, 3), (17, 1000, 64), (3, 8192, 16),
+    (6, 8200, 300), (12, 20001, 33), (2, 70000, 1000), (1100, 8192, 9), (300, 4097, 40)))
+def test_two_exponentials_a_logit(rows, cols, K, tau, soft, hard, dtype):
+    """Temperatures other than 1 and 2 with hard labels: whole and ragged rows, in one part and in
+    several, of less than a workgroup and more."""
+    print(f"\n[gpu-distill] two {rows}x{cols} K={K} tau={tau} {soft}/{hard} {dtype}", flush=True)
+    check(make(rows, cols, K, dtype, seed=rows), tau, soft, hard, dloss=1024.0)

@@ -266,3 +266,53 @@ def test_a_gradient_is_not_added_to_what_requires_gradients(no_kernels):
     into(leaf.grad, dout, saved)
     with torch.inference_mode():
         into(torch.zeros(6, 8), dout, saved)
+
+
+def _short_form_cases():
+    """Tensors [4, 2, 8] of many steps, and broken ones, as norm_rotary may be given them."""
+    base = torch.zeros(4096)
+    for token in (0, 1, 8, 15, 16, 40, 1 << 22, (1 << 22) + 1):
+        for head in (0, 4, 8, 32, 1 << 40, (1 << 40) + 1):
+            for column in (1, 2):
+                yield torch.empty(3 * token + head + 7 * column + 1,
+                                  device="meta").as_strided((4, 2, 8), (token, head, column))
+    for shape in ((1, 2, 8), (4, 1, 8), (1, 1, 8), (4, 2, 1), (0, 2, 8), (4, 0, 8), (1, 1, 1)):
+        n = shape[0] * shape[1] * shape[2]
+        yield base[:n].view(shape)
+        if n:
+            for steps in ((0, 0, 0), (1, 1, 1), (3, 5, 7), (200, 30, 1), (1, 30, 1)):
+                yield base.as_strided(shape, steps)
+
+
+def test_norm_rotary_steps_are_those_of_the_strided_pairs():
+    """Its shorter form says what head_rows and strides_arg say, for every tensor."""
+    from evograd_amd.pairs._util import head_rows, strides_arg
+    for t in _short_form_cases():
+        (got, other), steps = norm_rotary._steps(t, t)
+        want = head_rows(t)
+        assert (got is t) == (want is t), (t.shape, t.stride())
+        assert got.stride() == want.stride() and got.shape == want.shape
+        assert steps == strides_arg(want, want), (t.shape, t.stride())
+
+
+def test_norm_rotary_takes_what_its_checks_take():
+    """The short look at the arguments never passes what the full one refuses, or the reverse."""
+    floats = (torch.float32, torch.float16, torch.bfloat16, torch.float64, torch.int32)
+    seen = set()
+    for shape in ((4, 2, 8), (4, 2, 7), (4, 8), (4, 2, 8, 1), (0, 2, 8)):
+        for dtype in floats:
+            x = torch.zeros(shape, dtype=dtype)
+            for weight in (torch.zeros(8, dtype=dtype), torch.zeros(7, dtype=dtype), torch.zeros(1, 8, dtype=dtype),
+                           torch.zeros(8, dtype=torch.float16)):
+                for pos in (POS, POS.long(), POS.float(), POS[:3], POS[:0], POS[:, None]):
+                    for freqs in (FREQ, FREQ.float(), FREQ[:3], FREQ[:0], FREQ[None], torch.ones(5).double()):
+                        try:
+                            norm_rotary._check("norm_rotary", x, weight, pos, freqs)
+                            _lib.dtype_tag(x.dtype)
+                            good = True
+                        except (TypeError, ValueError):
+                            good = False
+                        assert norm_rotary._fits(x, weight, pos, freqs) == good, (
+                            x.shape, dtype, weight.shape, weight.dtype, pos.shape, pos.dtype, freqs.shape)
+                        seen.add(good)
+    assert seen == {True, False}

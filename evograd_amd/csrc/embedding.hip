@@ -1,9 +1,11 @@
 // Embedding lookup with scaling, and its gradient by sorted tokens, for gfx950.
 //
 //   out[t] = scale * weight[ids[t]]
-//   dweight[v] = scale * sum of dout[t] over the tokens t with ids[t] == v, t ascending
-// in fp32, each output rounded once. A token equal to ignore_index gives a row of zeros, any
-// other one outside [0, vocab) a row of NaN; neither is used as an index or has a gradient.
+//   dweight[v] = scale * sum of dout[t] over the tokens t with ids[t] == v
+// in fp32, each output rounded once. An id's tokens are added in ascending pieces; the partial sums
+// of a run over many pieces are dealt to kJoinAdders adders and joined in their order. A token equal to
+// ignore_index gives a row of zeros, any other one outside [0, vocab) a row of NaN; neither is used
+// as an index or has a gradient.
 //
 // The gradient of few tokens is one launch (embed_few_kernel), that of more runs in three, both
 // without atomics on their sums:

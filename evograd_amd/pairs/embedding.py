@@ -4,13 +4,14 @@
     dweight[v] = scale * sum of dout[t] over the tokens t with ids[t] == v
 
 ``weight`` is [vocab, hidden], ``ids`` int32 or int64 of any shape, ``out`` [*ids.shape, hidden].
-Sums are fp32 in the tokens' order (the same bits every run), each result rounded once. A token
-equal to ``ignore_index`` gives a row of zeros; any other one outside [0, vocab) gives a row of
-NaN. Neither has a gradient. Saved state: ``(ids, vocab, hidden, dtype)``, and not the table.
+Sums are fp32, a token's rows piece by piece and then the pieces, in an order that the call fixes
+(the same bits every run); each result is rounded once. A token equal to ``ignore_index`` gives a
+row of zeros; any other one outside [0, vocab) gives a row of NaN. Neither has a gradient. Saved
+state: ``(ids, vocab, hidden, dtype)``, and not the table.
 
-``embedding_backward_into(dweight, dout, saved, ...)`` adds the gradient to one that is there
-(a table shared with the output projection): only the rows of the batch's own tokens are read and
-written, each rounded once.
+``embedding_backward_into(dweight, dout, saved, ...)`` adds the gradient to one that is there, of the
+table's shape and type (a table shared with the output projection): only the rows of the batch's
+own tokens are read and written, each rounded once.
 """
 
 from __future__ import annotations

@@ -13,11 +13,11 @@ the rows whose ``target`` (int64 [rows]) is not ``ignore_index``; the others are
 a zero gradient. Other targets are used by a hard label alone: with ``hard_weight`` 0 any of them
 will do.
 
-An entry with a negative id is none (a nucleus of fewer tokens), nor is one of value -inf; entries
-of the same token add up; a row without entries has a soft part of 0. An id of cols or more or a
-value of NaN or +inf makes the loss and the row's gradient NaN, and so does, with a hard label, a
-target outside [0, cols); neither is used as an index. With ``soft_weight`` 0 the entries are not
-looked at. Only the logits have a gradient:
+An entry with a negative id is none (a nucleus of fewer tokens), nor is one of value -inf at a
+column; entries of the same token add up; a row without entries has a soft part of 0. An id of cols
+or more, whatever its value, or a value of NaN or +inf makes the loss and the row's gradient NaN, and
+so does, with a hard label, a target outside [0, cols); neither is used as an index. With
+``soft_weight`` 0 the entries are not looked at. Only the logits have a gradient:
 
     dlogits = dloss / n * (hard_weight * (softmax(logits) - onehot(target))
                            + soft_weight * temperature * (q - sum of p at their tokens))

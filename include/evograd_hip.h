@@ -540,10 +540,12 @@ int eg_embedding_fwd(const void* weight, const void* ids, int ids_64, void* out,
  * fp32 partial rows per piece of 8 to 32 tokens. */
 size_t eg_embedding_workspace_bytes(int64_t tokens, int64_t vocab, int64_t hidden);
 
-/* Its gradient: dweight[v] = scale * sum of dout[t] over the tokens with ids[t] == v, fp32 sums in
- * an order that the ids, the sizes and the tensors' alignment fix, one rounding; every row is
- * written. accumulate: added to dweight instead, where the rows of ids without a token are neither
- * read nor written. The workspace is 16-byte aligned, dweight overlaps no input. */
+/* Its gradient: dweight[v] = scale * sum of dout[t] over the tokens with ids[t] == v, one rounding;
+ * every row is written. accumulate: added to dweight instead, where the rows of ids without a token
+ * are neither read nor written. Sums are fp32, piece by piece of an id's tokens and then of the
+ * pieces; the ids, the sizes, the type, the tensors' alignment and `accumulate` fix their order, so
+ * that the same call gives the same bits. The workspace is 16-byte aligned, dweight overlaps no
+ * input. */
 int eg_embedding_bwd(const void* dout, const void* ids, int ids_64, void* dweight,
                      void* workspace, int64_t tokens, int64_t vocab, int64_t hidden, float scale,
                      int64_t ignore_index, int accumulate, int dtype, void* stream);

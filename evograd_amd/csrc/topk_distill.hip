@@ -22,11 +22,12 @@
 // distill_finish_kernel does the rest of a row, whose work is a chain of short steps, in one wave;
 // distill_mean_kernel adds the rows; distill_bwd_kernel. bf16 [8192, 128256] with 64 entries at a
 // temperature of 2 with hard labels, a tenth of the rows ignored: 306 + 12 + 5 us forward (6.2
-// TB/s) and 684 backward (5.8 TB/s). With the finish at the end of the row's own workgroup the
-// forward took 597, as the streams of a CU's other workgroup do not fill it, and with the entries
-// loaded after the first barrier the backward 939. Rows that are no multiple of a pack: fp16 [2047,
-// 50257] 36 + 6 + 5 and 58; with the non-temporal hint on their loads 52 and 68, for unaligned packs
-// share cache lines.
+// TB/s) and 684 backward (5.8 TB/s), medians over whole steps; the figures below that compare variants
+// are least means of 20 launches of one kernel in a row, where this backward takes 655. With the
+// finish at the end of the row's own workgroup the forward took 597, as the streams of a CU's other
+// workgroup do not fill it, and with the entries loaded after the first barrier the backward 939. Rows
+// that are no multiple of a pack: fp16 [2047, 50257] 36 + 6 + 5 and 58; with the non-temporal hint on
+// their loads 52 and 68, for unaligned packs share cache lines.
 #include "rowwise.hpp"
 
 #include <algorithm>
@@ -48,10 +49,12 @@ constexpr int64_t kFewRows = 16;
 // / 256 threads: bf16 [8192, 128256] with one exponential 308 / 309 / 308, a squared one 330 / 309 /
 // 314, two 366 / 338 / 336, 16 rows 11.4 / 11.8 / 11.6; with 512 threads at 8 / 4 / 2 packs: 316 / 313
 // / 305, 328 / 315 / 308, 362 / 344 / 338.
-// A narrower row takes the smallest workgroup that walks it in kRowSteps.
+// A narrower row takes the smallest workgroup that walks it in kRowSteps (forward, us, in 1 / 2 / 4
+// steps: bf16 [8192, 4096] 33.6 / 30.0 / 29.6, [8192, 8192] 47.4 / 38.2 / 36.3, [4096, 1000] 15.2 / 15.1 /
+// 15.3, fp16 [3000, 2001] 15.0 / 14.6 / 14.5, fp32 [4096, 5000] 29.5 / 29.3 / 24.9).
 constexpr int kMostRow = 512, kUnroll = 2, kRowSteps = 2;
-// The backward's workgroup (bf16 [8192, 128256], us: 512 threads 671, 256 655, 128 652 but 814 with 256
-// entries a row for 690, 256 of four packs 788).
+// The backward's workgroup (bf16 [8192, 128256], a tenth of the rows ignored, us: 512 threads 671, 256
+// 655, 128 652 but 814 with 256 entries a row for 690, 256 of four packs 788).
 constexpr int kFlatBlock = 256, kFlatUnroll = 2, kFlatPer = kFlatBlock * kFlatUnroll;
 
 // The exponentials of a column: one of them (no hard label, no soft part or a temperature of 1),

@@ -321,8 +321,9 @@ __global__ __launch_bounds__(kMostThreads, kBackWaves) void norm_rotary_bwd_kern
 
 // Heads of more than 64 lanes' packs (single columns of wide heads): a wave per head, which reads
 // its columns again for every step and forms its own sines. Column sums lie in LDS, each
-// column with the lane that works on it. Bound by those sines: 2048 tokens, 8 heads of 514 bf16 42 + 90
-// us, of 130 with 65 pairs 19 + 38.
+// column with the lane that works on it. Bound by the loads, a column a lane and two waves a SIMD, and
+// not by the sines (8192 tokens, 8 heads of 513 bf16, forward: 65 pairs 179 us, 256 pairs 160): 2048
+// tokens, 8 heads of 514 42 + 90 us, of 130 with 65 pairs 19 + 38.
 
 template <typename T, bool INTER, bool BACK>
 __global__ __launch_bounds__(kWave) void norm_rotary_wide_kernel(HeadArgs a) {

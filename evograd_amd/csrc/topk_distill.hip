@@ -492,8 +492,9 @@ int check(const char* name, int64_t rows, int64_t cols, int64_t k, float tempera
     set_error("%s: size out of range (rows <= 2^22, cols <= 2^30, entries <= %d)", name, kMaxEntries);
     return 1;
   }
-  if (!(temperature > 0.f) || __builtin_isinf(temperature)) {
-    set_error("%s: temperature must be positive and finite", name);
+  // farther out its square or the logits' quotients leave fp32, and the loss would be NaN
+  if (!(temperature >= 0x1p-100f && temperature <= 0x1p60f)) {
+    set_error("%s: temperature must be positive, from 2^-100 to 2^60", name);
     return 1;
   }
   return 0;

@@ -1,7 +1,8 @@
 """Distillation from a teacher's top logits, beside the hard-label cross entropy, on gfx950.
 
 ``logits`` [rows, cols] are the student's, ``teacher_logits`` [rows, entries] the values a teacher
-gave its top tokens and ``teacher_ids`` [rows, entries] those tokens. Per row, at a temperature:
+gave its top tokens and ``teacher_ids`` [rows, entries] those tokens. Per row, at a temperature (from
+2^-100 to 2^60):
 
     p = softmax(teacher_logits / temperature) over the row's entries
     q = softmax(logits / temperature) over the whole vocabulary

@@ -589,8 +589,8 @@ size_t eg_topk_distill_workspace_bytes(int64_t rows, int64_t cols, int64_t entri
  * column all count, a row without entries has no soft part. With soft_weight != 0 an id >= cols or
  * a value of NaN or +inf, and with hard_weight != 0 a target outside [0, cols), makes the row's
  * loss and gradient NaN; with a weight of 0 entries or targets are not looked at. loss and
- * n_valid: one fp32 each. Saved: stats fp32 [rows, 4], probs fp32 [rows, entries]. tau > 0;
- * entries <= 1024, rows < 2^22, cols <= 2^30. */
+ * n_valid: one fp32 each. Saved: stats fp32 [rows, 4], probs fp32 [rows, entries]. 2^-100 <= tau
+ * <= 2^60, entries <= 1024, rows < 2^22, cols <= 2^30. */
 int eg_topk_distill_fwd(const void* logits, const int64_t* target, const void* teacher,
                         int teacher_dtype, const void* teacher_ids, int ids_64, float* loss,
                         float* stats, float* probs, float* n_valid, void* workspace, int64_t rows,

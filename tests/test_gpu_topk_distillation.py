@@ -298,3 +298,11 @@ def test_two_exponentials_a_logit(rows, cols, K, tau, soft, hard, dtype):
     several, of less than a workgroup and more."""
     print(f"\n[gpu-distill] two {rows}x{cols} K={K} tau={tau} {soft}/{hard} {dtype}", flush=True)
     check(make(rows, cols, K, dtype, seed=rows), tau, soft, hard, dloss=1024.0)
+
+
+@pytest.mark.parametrize("tau", (2.0 ** -100, 1e-6, 1e6, 2.0 ** 60))
+def test_the_ends_of_the_temperatures(tau):
+    """Nothing overflows on the way to the loss or its gradient."""
+    logits, target, teacher, ids = make(9, 200, 9, F32, ignore=0.0, cut=False)
+    loss, grad = step(logits, target, teacher, ids, tau, 1.0, 0.5)
+    assert bool(loss.isfinite()) and bool(grad.isfinite().all())

@@ -316,3 +316,15 @@ def test_norm_rotary_takes_what_its_checks_take():
                             x.shape, dtype, weight.shape, weight.dtype, pos.shape, pos.dtype, freqs.shape)
                         seen.add(good)
     assert seen == {True, False}
+
+
+@built
+@pytest.mark.parametrize("tau", (2.0 ** -101, 2.0 ** -149, 2.0 ** 61, 2.0 ** 127))
+def test_temperatures_whose_square_or_quotients_leave_fp32(tau):
+    """Refused before soft labels become NaN, whose factors grow infinite, or 0 times infinite."""
+    with pytest.raises(RuntimeError, match="temperature"):
+        _lib.call("eg_topk_distill_fwd", P, P, P, _lib.EG_F32, P, 0, P, P, P, P, P, 4, 9, 3, tau, 1.0, 0.0,
+                  -100, _lib.EG_F32, None)
+    with pytest.raises(RuntimeError, match="temperature"):
+        _lib.call("eg_topk_distill_bwd", P, P, P, P, 0, P, P, P, P, 4, 9, 3, tau, 1.0, 0.0, -100,
+                  _lib.EG_F32, None)

@@ -154,7 +154,7 @@ class _PairFunction(torch.autograd.Function):
         ctx.mask = mask
         ctx.binding = binding
         ctx.scalars = {n: args[i] for n, i in binding.scalars_for_backward}
-        return (y, *ties) if ties else y
+        return (y, *ties)
 
     @staticmethod
     def backward(ctx, dy, *_):
@@ -175,8 +175,7 @@ def bind(op: OpDecl, module):
                                              if n in accepted))
 
     def call(*args, **kwargs):
-        out = _PairFunction.apply(binding, *plan.arrange(args, kwargs).values())
-        return out[0] if type(out) is tuple else out
+        return _PairFunction.apply(binding, *plan.arrange(args, kwargs).values())[0]
 
     call.__name__ = call.__qualname__ = f"{op.name}_bound"
     call.plan = plan

@@ -151,3 +151,13 @@ def test_joint_nodes_refuse_the_same(no_kernels, name, strided):
     leaves, out = node(name, strided)
     (out[0].sum() + out[1].sum()).backward()
     assert all(t.grad.shape == t.shape and not t.grad.requires_grad for t in leaves)
+
+
+def test_what_a_pair_returns_is_what_a_call_returns():
+    """Also a pair's tuple of outputs, which no declaration has, without gradients."""
+    import types
+    both = types.SimpleNamespace(forward_with_saved=lambda x: ((x + 1, x + 2), (x,)),
+                                 backward_from_saved=lambda dy, saved: dy)
+    with torch.no_grad():
+        out = bind(decls.SOFTMAX, both)(torch.zeros(3))
+    assert isinstance(out, tuple) and out[0].tolist() == [1.0] * 3 and out[1].tolist() == [2.0] * 3
